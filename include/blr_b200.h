@@ -386,6 +386,50 @@ int blr_attention_decode(const void* q, int64_t ldq, const void* k_cache, const 
                          int64_t n_seq, int heads, int head_dim, int slots, int n_keys, float scale, int dtype,
                          void* out, int64_t ldo, void* scratch, size_t scratch_bytes, void* stream);
 
+/* ---- An 8-bit key / value cache and the attention over it.  No counterpart in the reference.
+ * Codes are (n_seq, kv_heads, slots, head_dim) bytes, int8 in [-127, 127] or e4m3, packed and 16-byte aligned; `block` slots of a head share one fp32
+ * scale, (n_seq, kv_heads, ceil(slots / block)): value = code * scale.  head_dim 64 or 128, block 16, 32, 64 or 128 (BLR_ERR_UNSUPPORTED else).
+ * start, n_new: device int64, one per sequence; a call's tokens of sequence s take slots start[s] .. start[s] + n_new[s] - 1 (n_new NULL: n_tok
+ * each).  Rows behind a sequence's n_new, and tokens whose slot is outside the cache, write nothing to it and leave zeros in an output.  16-bit tensors of
+ * `dtype`, rows 16-byte aligned, row strides multiples of 8; any of them, start and n_new too, may be written by the kernel directly ahead. */
+#define BLR_Q8_INT8 0
+#define BLR_Q8_E4M3 1
+typedef struct blr_q8_cache {
+  void* k;
+  void* v;
+  float* k_scale;
+  float* v_scale;
+  int64_t n_seq;
+  int kv_heads, slots, head_dim, block;
+  int code; /* BLR_Q8_INT8 | BLR_Q8_E4M3 */
+} blr_q8_cache;
+
+/* Rotary embedding and append.  q: n_seq * n_tok rows (sequence-major) of heads * head_dim values, k and v of kv_heads * head_dim.  The angle of a
+ * token is its slot's row of cos_table / sin_table ((>= slots, head_dim / 2) fp32, 16-byte aligned; pairs (i, i + head_dim / 2) rotate).  q_out: the
+ * rotated q.  Rotated k and v go to the cache as codes round(x (1 / s)), s = max(s_before, max|x| (1 / 127 or 1 / 448)) over the block's tokens, in fp32;
+ * s_before = 0 for a block that begins with this call, and where s grows over older tokens of the block their codes become round(code (s_before (1 / s))).  A scale below
+ * the smallest normal number is 0.  A block that a NaN or infinity is written to reads back as NaN. */
+int blr_rope_append_q8(const void* q, int64_t ldq, const void* k, int64_t ldk, const void* v, int64_t ldv,
+                       const float* cos_table, const float* sin_table, const int64_t* start, const int64_t* n_new, int64_t n_tok, int heads,
+                       int dtype, const blr_q8_cache* cache, void* q_out, int64_t ldo, void* stream);
+
+/* k_out, v_out (n_seq, kv_heads, slots, head_dim) = code * scale rounded to dtype; zeros from slot lengths[s] on (device int64, NULL: all slots). */
+int blr_cache_read_q8(const blr_q8_cache* cache, const int64_t* lengths, int dtype, void* k_out, void* v_out, void* stream);
+
+/* Causal attention of the newest tokens: row t < n_new[s] of sequence s sits at slot start[s] + t and sees slots 0 .. start[s] + t;
+ * out = softmax(scale * q . K^T) V.  heads a multiple of kv_heads: head h reads kv head h / (heads / kv_heads).  scratch:
+ * blr_attention_q8_scratch_bytes (may be 0), 16-byte aligned, nothing kept in it between calls. */
+size_t blr_attention_q8_scratch_bytes(const blr_q8_cache* cache, int64_t n_tok, int heads);
+int blr_attention_q8(const void* q, int64_t ldq, const blr_q8_cache* cache, const int64_t* start, const int64_t* n_new, int64_t n_tok, int heads,
+                     float scale, int dtype, void* out, int64_t ldo, void* scratch, size_t scratch_bytes, void* stream);
+
+/* Of each row of logits (row stride ld; kind 0 fp16, 1 bf16, 2 fp32): logprob[r] = log softmax(row)[ids[r]] (0 where ids[r] < 0: no token given; NaN
+ * where ids[r] >= vocab), entropy[r] of the softmax, and the `top` (0 .. 64, at most vocab) likeliest tokens by falling logit, ties by rising id: their
+ * log probabilities (rows, top) and ids (rows, top).  Logits of -inf have probability 0; a row of nothing else has log probabilities of -inf and entropy
+ * 0.  A row with a NaN or +inf has NaN for both (its tokens still in order, NaN first).  fp32 arithmetic and results.  No reference counterpart. */
+int blr_token_logprobs(const void* logits, int64_t ld, int64_t rows, int64_t vocab, int kind, const int64_t* ids, int top,
+                       float* logprob, float* entropy, float* top_logprob, int64_t* top_ids, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -31,6 +31,12 @@ class BlastProblem(C.Structure):
                 ("ldr", _i64), ("out", _vp), ("ldo", _i64)]
 
 
+class Q8CacheDesc(C.Structure):
+    """blr_q8_cache of include/blr_b200.h."""
+    _fields_ = [("k", _vp), ("v", _vp), ("k_scale", _vp), ("v_scale", _vp), ("n_seq", _i64), ("kv_heads", _int), ("slots", _int),
+                ("head_dim", _int), ("block", _int), ("code", _int)]
+
+
 ACT_NONE, ACT_SILU_MUL = 0, 1
 ACT_OUT = {None: 0, "gelu": 0x10, "gelu_tanh": 0x20}   # output activations of the fused call above 16 tokens
 
@@ -90,6 +96,11 @@ SIGNATURES = {
     "blr_rope_append": (_int, [_vp, _i64, _vp, _i64, _vp, _i64, _vp, _vp, _vp, _i64, _int, _int, _int, _int, _int, _vp, _vp, _vp]),
     "blr_attention_decode_scratch_bytes": (_sz, [_i64, _int, _int, _int]),
     "blr_attention_decode": (_int, [_vp, _i64, _vp, _vp, _i64, _int, _int, _int, _int, C.c_float, _int, _vp, _i64, _vp, _sz, _vp]),
+    "blr_rope_append_q8": (_int, [_vp, _i64, _vp, _i64, _vp, _i64, _vp, _vp, _vp, _vp, _i64, _int, _int, C.POINTER(Q8CacheDesc), _vp, _i64, _vp]),
+    "blr_cache_read_q8": (_int, [C.POINTER(Q8CacheDesc), _vp, _int, _vp, _vp, _vp]),
+    "blr_attention_q8_scratch_bytes": (_sz, [C.POINTER(Q8CacheDesc), _i64, _int]),
+    "blr_attention_q8": (_int, [_vp, _i64, C.POINTER(Q8CacheDesc), _vp, _vp, _i64, _int, C.c_float, _int, _vp, _i64, _vp, _sz, _vp]),
+    "blr_token_logprobs": (_int, [_vp, _i64, _i64, _i64, _int, _vp, _int, _vp, _vp, _vp, _vp, _vp]),
     "blr_quantize_sym": (_int, [_vp, _int, _i64, _i64, _int, _vp, _vp, _vp]),
     "blr_dequantize_sym": (_int, [_vp, _vp, _i64, _i64, _int, _i64, _int, _vp, _vp]),
 }

@@ -347,6 +347,28 @@ class LlamaLayer(nn.Module):
         (x,) = structured_multi([self.down_proj], g, x_mul=u, residual=x)
         return x
 
+    def forward_q8(self, x, tables, cache, start, n_new=None, kernels: bool = True):
+        """The layer on an 8-bit cache (ops.Q8Cache): x (B, T, d), the next T tokens of each sequence from slot start[b] on, of which the first n_new[b]
+        (None: all) are tokens.  kernels = False reads the cache back and leaves the attention to torch."""
+        from . import ops
+        B, T, d = x.shape
+        h = self.input_layernorm(x)
+        q, k, v = (t.view(B * T, d) for t in structured_multi([self.q_proj, self.k_proj, self.v_proj], h))
+        q = ops.rope_append_q8(q, k, v, tables[0], tables[1], start, cache, n_new)
+        if kernels:
+            a = ops.attention_q8(q, cache, start, n_new)
+        else:
+            slots = cache.k.shape[2]
+            last = start[:, None] + torch.arange(T, device=x.device)   # (slots behind a row's own are masked, and zeros where nobody wrote)
+            kc, vc = ops.cache_read_q8(cache, x.dtype, start + (T if n_new is None else n_new))
+            seen = torch.arange(slots, device=x.device) <= last[..., None]
+            a = F.scaled_dot_product_attention(q.view(B, T, self.heads, self.hd).transpose(1, 2), kc, vc, attn_mask=seen[:, None]).transpose(1, 2)
+        (x,) = structured_multi([self.o_proj], a.reshape(B, T, d), residual=x)
+        h = self.post_attention_layernorm(x)
+        g, u = structured_multi([self.gate_proj, self.up_proj], h)
+        (x,) = structured_multi([self.down_proj], g, x_mul=u, residual=x)
+        return x
+
     def forward(self, x, cos, sin, kc, vc, pos, causal: bool, tables=None):
         """x (B, T, d); kc, vc (B, H, S, hd) static cache; pos (T,) int64 cache slots of these tokens; cos, sin (T, hd/2)
         the angles of those slots.  causal: the T tokens are the whole sequence so far (prefill); else they attend to
@@ -378,10 +400,12 @@ class LlamaLayer(nn.Module):
 
 
 class LlamaDecoder(nn.Module):
-    """Decoder of the shape above with a static cache for `cache_len` positions and `batch` sequences."""
+    """Decoder of the shape above with a static cache for `cache_len` positions and `batch` sequences.  kv_cache "int8" or "e4m3": the cache in 8 bits with
+    a scale for each kv_block slots and head (ops.Q8Cache; CUDA, heads of 64 or 128), which a token attends to up to its own slot; sequences may then be
+    at different positions (`extend`).  None: in the activations' 16-bit type."""
 
     def __init__(self, shape: LlamaShape, method: str, batch: int, cache_len: int, device="cuda", dtype=torch.float16, seed=0,
-                 init_on_device: bool = False):
+                 init_on_device: bool = False, kv_cache: Optional[str] = None, kv_block: int = 16):
         super().__init__()
         g = torch.Generator(device=device if init_on_device else "cpu").manual_seed(seed)
         self.shape, self.method, self.batch, self.cache_len = shape, method, batch, cache_len
@@ -399,13 +423,35 @@ class LlamaDecoder(nn.Module):
         ang = torch.outer(torch.arange(cache_len, dtype=torch.float32), inv)
         self.register_buffer("cos", ang.cos().to(device), persistent=False)
         self.register_buffer("sin", ang.sin().to(device), persistent=False)
-        self.kcache = [torch.zeros(batch, shape.heads, cache_len, hd, device=device, dtype=dtype) for _ in range(shape.layers)]
-        self.vcache = [torch.zeros(batch, shape.heads, cache_len, hd, device=device, dtype=dtype) for _ in range(shape.layers)]
+        self.q8cache = None
+        if kv_cache is not None:
+            from . import ops
+            codes = {"int8": torch.int8, "e4m3": torch.float8_e4m3fn}.get(kv_cache)
+            if codes is None:
+                raise ValueError(f"unknown kv_cache {kv_cache!r}")
+            self.q8cache = [ops.q8_cache(batch, shape.heads, cache_len, hd, kv_block, codes, device) for _ in range(shape.layers)]
+        n16 = shape.layers if kv_cache is None else 0
+        self.kcache = [torch.zeros(batch, shape.heads, cache_len, hd, device=device, dtype=dtype) for _ in range(n16)]
+        self.vcache = [torch.zeros(batch, shape.heads, cache_len, hd, device=device, dtype=dtype) for _ in range(n16)]
 
     def structured_linears(self):
         return [m for layer in self.layers for m in layer.structured()]
 
+    def _hidden_q8(self, ids, start, n_new=None):
+        if ids.shape[1] > self.cache_len:
+            raise ValueError(f"{ids.shape[1]} tokens do not fit a cache of {self.cache_len} slots")
+        x, B = self.embed_tokens(ids), ids.shape[0]
+        for layer, cache in zip(self.layers, self.q8cache):
+            x = layer.forward_q8(x, (self.cos, self.sin), cache.first(B), start, n_new, self.fused_decode)
+        return x
+
     def _run(self, ids, pos, causal):
+        return self.lm_head(self.norm(self._hidden(ids, pos, causal)[:, -1]))
+
+    def _hidden(self, ids, pos, causal):
+        if self.q8cache is not None:
+            B = ids.shape[0]
+            return self._hidden_q8(ids, pos.new_zeros(B) if causal else pos if pos.numel() == B else pos.expand(B).contiguous())
         x = self.embed_tokens(ids)
         B = ids.shape[0]   # a smaller batch than the cache was built for uses the first B sequences' slots
         # one new token per sequence on the GPU with 16-bit activations takes the fused decode path
@@ -418,7 +464,7 @@ class LlamaDecoder(nn.Module):
         cos, sin = (None, None) if fused else (self.cos.index_select(0, pos), self.sin.index_select(0, pos))
         for i, layer in enumerate(self.layers):
             x = layer(x, cos, sin, self.kcache[i][:B], self.vcache[i][:B], pos, causal, tables)
-        return self.lm_head(self.norm(x[:, -1]))
+        return x
 
     @torch.no_grad()
     def prefill(self, ids: torch.Tensor) -> torch.Tensor:
@@ -429,8 +475,28 @@ class LlamaDecoder(nn.Module):
     @torch.no_grad()
     def decode_step(self, ids: torch.Tensor, pos: torch.Tensor) -> torch.Tensor:
         """ids (B, 1): one new token per sequence, written to cache slot pos (1,) and attending to the whole cache
-        (slots beyond the sequence's length must hold real keys: the benchmark decodes at a full cache)."""
+        (slots beyond the sequence's length must hold real keys: the benchmark decodes at a full cache).  On an 8-bit cache it attends to the slots up to
+        its own, and pos may be (B,), one for each sequence."""
         return self._run(ids, pos, False)
+
+    @torch.no_grad()
+    def extend(self, ids: torch.Tensor, start: torch.Tensor, n_new: Optional[torch.Tensor] = None) -> torch.Tensor:
+        """The next tokens of sequences at different positions, on an 8-bit cache: ids (B, T) go to slots start[b] .. (start (B,) int64), of each row the
+        first n_new[b] ((B,) int64; None: all).  Returns the logits behind each sequence's last new token (B, vocab); those of a sequence without a new
+        token mean nothing."""
+        if self.q8cache is None:
+            raise RuntimeError("extend needs a decoder with an 8-bit cache (kv_cache='int8' or 'e4m3')")
+        x = self._hidden_q8(ids, start, n_new)
+        last = x[:, -1] if n_new is None else x[torch.arange(ids.shape[0], device=ids.device), (n_new - 1).clamp(0, ids.shape[1] - 1)]
+        return self.lm_head(self.norm(last))
+
+    @torch.no_grad()
+    def score(self, ids: torch.Tensor, top: int = 0):
+        """How likely a text is: ids (B, T), a prefill of all of it; of each position but the last (log probability of the token that follows, entropy, log
+        probabilities of the `top` likeliest tokens, their ids), (B, T - 1) and (B, T - 1, top), as ops.token_logprobs gives them."""
+        from . import ops
+        x = self._hidden(ids, torch.arange(ids.shape[1], device=ids.device), True)
+        return ops.token_logprobs(self.lm_head(self.norm(x[:, :-1])), ids[:, 1:], top)
 
 
 # ------------------------------------------------------------------------------------------------ ViT-shaped encoder

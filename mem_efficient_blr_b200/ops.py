@@ -13,7 +13,7 @@ from __future__ import annotations
 import collections
 import threading
 import weakref
-from typing import Tuple
+from typing import NamedTuple, Tuple
 
 import torch
 
@@ -668,3 +668,126 @@ def attention_decode(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tens
                                      n_keys, float(scale) if scale else hd ** -0.5, L.dtype_code(q.dtype), out.data_ptr(),
                                      out.stride(0), scratch.data_ptr(), nbytes, L.stream_ptr(q.device)))
     return out
+
+
+# ----------------------------------------------------------------------------- 8-bit key / value cache
+class Q8Cache(NamedTuple):
+    """A layer's keys and values in 8 bits: codes (n_seq, kv_heads, slots, head_dim), int8 or float8_e4m3fn, and one fp32 scale for each `block` slots
+    of a head (n_seq, kv_heads, ceil(slots / block)); value = code * scale.  All contiguous; head_dim 64 or 128, block 16, 32, 64 or 128."""
+    k: torch.Tensor
+    v: torch.Tensor
+    k_scale: torch.Tensor
+    v_scale: torch.Tensor
+    block: int
+
+    def first(self, n_seq: int) -> "Q8Cache":
+        """The first n_seq sequences of the cache (views)."""
+        return Q8Cache(self.k[:n_seq], self.v[:n_seq], self.k_scale[:n_seq], self.v_scale[:n_seq], self.block)
+
+
+def q8_cache(n_seq: int, kv_heads: int, slots: int, head_dim: int, block: int = 16, dtype: torch.dtype = torch.int8, device="cuda") -> Q8Cache:
+    """An empty 8-bit cache (zeros)."""
+    assert dtype in _Q8_CODE and head_dim in (64, 128) and block in (16, 32, 64, 128), "8-bit caches: int8 or float8_e4m3fn, heads of 64 or 128, blocks of 16 to 128"
+    codes = lambda: torch.zeros(n_seq, kv_heads, slots, head_dim, dtype=dtype, device=device)   # noqa: E731
+    scale = lambda: torch.zeros(n_seq, kv_heads, -(-slots // block), dtype=torch.float32, device=device)   # noqa: E731
+    return Q8Cache(codes(), codes(), scale(), scale(), block)
+
+
+_Q8_CODE = {torch.int8: 0, torch.float8_e4m3fn: 1}
+
+
+def _no_grad(*ts: torch.Tensor) -> None:
+    if torch.is_grad_enabled() and any(t.requires_grad for t in ts):
+        raise RuntimeError("blr_b200: this operator has no derivative; call it under torch.no_grad() or on detached tensors")
+
+
+def _q8_desc(c: Q8Cache, x: torch.Tensor) -> "L.Q8CacheDesc":
+    _need_cuda(x, c.k, c.v, c.k_scale, c.v_scale)
+    assert c.k.dim() == 4 and c.v.shape == c.k.shape and c.v.dtype == c.k.dtype, "keys and values of an 8-bit cache are (n_seq, kv_heads, slots, head_dim) of one type"
+    assert c.k.dtype in _Q8_CODE, f"codes are int8 or float8_e4m3fn, got {c.k.dtype}"
+    n_seq, kv_heads, slots, hd = c.k.shape
+    assert c.k_scale.dtype == c.v_scale.dtype == torch.float32 and c.block > 0
+    assert tuple(c.k_scale.shape) == tuple(c.v_scale.shape) == (n_seq, kv_heads, -(-slots // c.block)), "one scale for each block of slots and head"
+    return L.Q8CacheDesc(c.k.data_ptr(), c.v.data_ptr(), c.k_scale.data_ptr(), c.v_scale.data_ptr(), n_seq, kv_heads, slots, hd, c.block, _Q8_CODE[c.k.dtype])
+
+
+def _per_sequence(t: torch.Tensor, x: torch.Tensor, n_seq: int, name: str) -> int:
+    assert t.dtype == torch.int64 and t.is_contiguous() and t.numel() == n_seq and t.device == x.device, \
+        f"{name} must be {n_seq} packed int64 values on the tensors' device"
+    return t.data_ptr()
+
+
+def rope_append_q8(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cos_table: torch.Tensor, sin_table: torch.Tensor, start: torch.Tensor,
+                   cache: Q8Cache, n_new=None) -> torch.Tensor:
+    """Rotary embedding and append to an 8-bit cache.  q (n_seq * n_tok, heads * head_dim), k and v (n_seq * n_tok, kv_heads * head_dim) 16-bit rows,
+    sequence-major; start (n_seq,) int64: the slot of each sequence's first token, n_new (n_seq,) int64 (None: all n_tok): how many of its rows are
+    tokens.  cos / sin tables (>= slots, head_dim / 2) fp32.  Returns the rotated q (zeros in rows that are no token) and writes codes and scales of the
+    rotated k and of v: a block's scale is the largest its tokens asked for since it was begun, and where it grows the codes that were there follow.
+    Tokens whose slot lies outside the cache write nothing."""
+    _no_grad(q, k, v)
+    d = _q8_desc(cache, q)
+    hd = d.head_dim
+    assert all(t.dim() == 2 for t in (q, k, v)) and q.dtype == k.dtype == v.dtype and q.device == k.device == v.device, "q, k, v are rows of one dtype and device"
+    rows = q.shape[0]
+    assert d.n_seq > 0 and rows % d.n_seq == 0 and k.shape == v.shape == (rows, d.kv_heads * hd) and q.shape[1] % hd == 0, "q, k, v: a row for each token of each sequence"
+    for t in (cos_table, sin_table):
+        assert t.dtype == torch.float32 and t.is_contiguous() and t.dim() == 2 and t.shape[0] >= d.slots and t.shape[1] == hd // 2 and t.device == q.device, \
+            "cos / sin tables are packed (slots, head_dim / 2) fp32"
+    q2, k2, v2 = (_rows16(t, t.shape[1]) for t in (q, k, v))
+    out = torch.empty((rows, q.shape[1]), dtype=q.dtype, device=q.device)
+    L.check(L.load().blr_rope_append_q8(q2.data_ptr(), q2.stride(0), k2.data_ptr(), k2.stride(0), v2.data_ptr(), v2.stride(0), cos_table.data_ptr(),
+                                        sin_table.data_ptr(), _per_sequence(start, q, d.n_seq, "start"),
+                                        None if n_new is None else _per_sequence(n_new, q, d.n_seq, "n_new"), rows // d.n_seq, q.shape[1] // hd,
+                                        L.dtype_code(q.dtype), d, out.data_ptr(), out.shape[1], L.stream_ptr(q.device)))
+    return out
+
+
+def cache_read_q8(cache: Q8Cache, dtype: torch.dtype, lengths=None) -> Tuple[torch.Tensor, torch.Tensor]:
+    """(keys, values) of an 8-bit cache in 16 bits, (n_seq, kv_heads, slots, head_dim): code * scale rounded once; zeros from slot lengths[s] of a sequence
+    on ((n_seq,) int64; None: all slots)."""
+    d = _q8_desc(cache, cache.k)
+    k, v = (torch.empty(cache.k.shape, dtype=dtype, device=cache.k.device) for _ in range(2))
+    L.check(L.load().blr_cache_read_q8(d, None if lengths is None else _per_sequence(lengths, cache.k, d.n_seq, "lengths"), L.dtype_code(dtype), k.data_ptr(),
+                                       v.data_ptr(), L.stream_ptr(cache.k.device)))
+    return k, v
+
+
+def attention_q8(q: torch.Tensor, cache: Q8Cache, start: torch.Tensor, n_new=None, scale: float = 0.0) -> torch.Tensor:
+    """Causal attention of each sequence's newest tokens over an 8-bit cache that holds them already: q (n_seq * n_tok, heads * head_dim) 16-bit rows,
+    sequence-major, heads a multiple of the cache's kv_heads; row t of sequence s sits at slot start[s] + t and sees the slots up to its own; rows from
+    n_new[s] on are no tokens and come out as zeros, as does a row that sees no slot.  scale defaults to head_dim ** -0.5.  Returns (rows, heads * head_dim)."""
+    _no_grad(q)
+    d = _q8_desc(cache, q)
+    assert q.dim() == 2 and d.n_seq > 0 and q.shape[0] % d.n_seq == 0 and q.shape[1] % (d.kv_heads * d.head_dim) == 0, "q: a row for each token of each sequence"
+    q2 = _rows16(q, q.shape[1])
+    lib, n_tok, heads = L.load(), q.shape[0] // d.n_seq, q.shape[1] // d.head_dim
+    out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+    nbytes = lib.blr_attention_q8_scratch_bytes(d, n_tok, heads)
+    scratch = torch.empty(nbytes, dtype=torch.uint8, device=q.device) if nbytes else None
+    L.check(lib.blr_attention_q8(q2.data_ptr(), q2.stride(0), d, _per_sequence(start, q, d.n_seq, "start"),
+                                 None if n_new is None else _per_sequence(n_new, q, d.n_seq, "n_new"), n_tok, heads, float(scale) if scale else d.head_dim ** -0.5,
+                                 L.dtype_code(q.dtype), out.data_ptr(), out.shape[1], None if scratch is None else scratch.data_ptr(), nbytes,
+                                 L.stream_ptr(q.device)))
+    return out
+
+
+def token_logprobs(logits: torch.Tensor, ids: torch.Tensor, top: int = 0) -> Tuple[torch.Tensor, torch.Tensor, torch.Tensor, torch.Tensor]:
+    """Of each row of logits (..., vocab), fp16, bf16 or fp32: (log probability of ids' token, entropy, log probabilities of the `top` likeliest tokens
+    (..., top), their ids), fp32 and int64.  ids (...) int64: a negative one stands for no token (0), one beyond the vocabulary gives NaN.  Ties go to the
+    lowest id; top <= 64."""
+    _no_grad(logits)
+    _need_cuda(logits)
+    assert logits.dim() >= 1 and ids.shape == logits.shape[:-1] and ids.dtype == torch.int64 and ids.device == logits.device, "ids: one int64 for each row of logits"
+    kind = {torch.float16: 0, torch.bfloat16: 1, torch.float32: 2}.get(logits.dtype)
+    assert kind is not None, f"expected float16, bfloat16 or float32 logits, got {logits.dtype}"
+    vocab, lead = logits.shape[-1], logits.shape[:-1]
+    x = logits if logits.dim() == 2 else logits.reshape(-1, vocab)
+    if x.stride(1) != 1 or (x.shape[0] > 1 and x.stride(0) < vocab):
+        x = x.contiguous()
+    rows, dev = x.shape[0], x.device
+    ids = ids.reshape(-1).contiguous()
+    lp, ent = (torch.empty(rows, dtype=torch.float32, device=dev) for _ in range(2))
+    tlp, tid = torch.empty((rows, top), dtype=torch.float32, device=dev), torch.empty((rows, top), dtype=torch.int64, device=dev)
+    L.check(L.load().blr_token_logprobs(x.data_ptr(), x.stride(0), rows, vocab, kind, ids.data_ptr(), top, lp.data_ptr(), ent.data_ptr(), tlp.data_ptr(),
+                                        tid.data_ptr(), L.stream_ptr(dev)))
+    return lp.view(lead), ent.view(lead), tlp.view(*lead, top), tid.view(*lead, top)

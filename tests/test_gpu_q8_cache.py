@@ -1,0 +1,508 @@
+"""The 8-bit key / value cache (append with rotary embedding, read back, attention) and the log probabilities of given tokens against plain
+implementations: codes and scales bit for bit against the formula in fp32 (each product and sum rounded by itself), the rest against 64 bits with tolerances
+that count roundings (half a step, eps / 2, each)."""
+import math
+
+import pytest
+import torch
+
+pytestmark = pytest.mark.gpu
+DEV = "cuda:0"
+TOP = {torch.int8: 127.0, torch.float8_e4m3fn: 448.0}
+I8, E4 = torch.int8, torch.float8_e4m3fn
+
+
+@pytest.fixture(scope="module")
+def ops():
+    if not torch.cuda.is_available():
+        pytest.skip("needs a CUDA device")
+    from mem_efficient_blr_b200 import ops as o
+    return o
+
+
+def _half(dtype):
+    return torch.finfo(dtype).eps / 2
+
+
+def _subnormal(dtype):
+    return torch.finfo(dtype).smallest_normal * torch.finfo(dtype).eps
+
+
+def _values(codes):
+    return codes.float() if codes.dtype == I8 else codes.to(torch.float32)
+
+
+def _coded(v, code):
+    v = torch.nan_to_num(v, nan=0.0)
+    return (v.round() if code == I8 else v).clamp(-TOP[code], TOP[code]).to(code)
+
+
+def _tables(slots, hd):
+    ang = torch.outer(torch.arange(slots, dtype=torch.float64), 10000.0 ** (-torch.arange(0, hd, 2, dtype=torch.float64) / hd))
+    return ang.cos().float(), ang.sin().float()
+
+
+def _rot(x, c, s):
+    a, b = x.chunk(2, dim=-1)
+    return torch.cat((a * c - b * s, b * c + a * s), dim=-1)
+
+
+def _write(codes, scale, x, s, start, block):
+    """x (n, hd) fp32 to slots start .. of one head's codes (slots, hd) and scale (blocks,), in place: the formula, block by block."""
+    slots, code = codes.shape[0], codes.dtype
+    first, end = max(start, 0), min(start + x.shape[0], slots)
+    if first >= end:
+        return
+    for j in range(first // block, (end - 1) // block + 1):
+        lo, hi = max(first, j * block), min(end, (j + 1) * block)
+        new = x[lo - start:hi - start]
+        big = new.abs().max()   # (a NaN stays one)
+        asked = big * torch.tensor(1.0 / TOP[code])
+        if asked < torch.finfo(torch.float32).tiny:
+            asked = torch.zeros(())
+        before = torch.zeros(()) if j * block >= first else scale[j].clone()
+        after = before if before.isnan() else torch.maximum(before, asked)
+        inv = 1.0 / after if after > 0 and not after.isinf() else torch.zeros(())
+        if not bool(after == before) and j * block < first:
+            old = slice(j * block, first)
+            codes[old] = _coded(_values(codes[old]) * (before * inv), code)
+        codes[lo:hi] = _coded(torch.where(inv == 0, torch.zeros(()), new * inv), code)
+        scale[j] = after
+
+
+def _cache(ops, B, KV, slots, hd, block, code, g, spread=1.0):
+    nb = -(-slots // block)
+    codes = lambda: _coded(torch.randn(B, KV, slots, hd, generator=g) * TOP[code] / 4, code)   # noqa: E731
+    scale = lambda: (torch.rand(B, KV, nb, generator=g) * spread + 0.3) * 4 / TOP[code]        # noqa: E731
+    return [codes(), codes(), scale(), scale()]
+
+
+def _on(ops, parts, block):
+    return ops.Q8Cache(*(t.to(DEV) for t in parts), block)
+
+
+APPENDS = [  # B, T, H, KV, hd, slots, block, starts, new
+    (1, 1, 1, 1, 64, 1, 16, [0], None),
+    (3, 1, 8, 2, 128, 33, 16, [0, 17, 32], None),
+    (2, 1, 4, 4, 64, 130, 128, [127, 128], None),
+    (1, 16, 2, 2, 128, 64, 16, [16], None),
+    (2, 19, 6, 3, 64, 45, 32, [26, 0], [19, 7]),
+    (4, 5, 4, 1, 128, 40, 64, [0, 33, 38, -2], [0, 5, 5, 5]),     # none; ordinary; past the end; before the beginning
+    (1, 300, 32, 8, 128, 301, 128, [1], None),
+    (2, 257, 5, 5, 64, 400, 16, [3, 100], [257, 256]),
+]
+
+
+@pytest.mark.parametrize("code", [I8, E4], ids=["int8", "e4m3"])
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("case", APPENDS, ids=[str(i) for i in range(len(APPENDS))])
+def test_append(ops, case, dtype, code):
+    B, T, H, KV, hd, slots, block, starts, new = case
+    g = torch.Generator().manual_seed(T + slots)
+    parts = _cache(ops, B, KV, slots, hd, block, code, g)
+    rn = lambda h: torch.randn(B * T, h * hd, generator=g).to(dtype)   # noqa: E731
+    q, k, v = rn(H), rn(KV), rn(KV)
+    cos, sin = _tables(slots, hd)
+    dev = _on(ops, parts, block)
+    out = ops.rope_append_q8(q.to(DEV), k.to(DEV), v.to(DEV), cos.to(DEV), sin.to(DEV), torch.tensor(starts, device=DEV), dev,
+                             None if new is None else torch.tensor(new, device=DEV))
+    torch.cuda.synchronize()
+    want = [t.clone() for t in parts]
+    want_q, room = torch.zeros(B, T, H, hd, dtype=torch.float64), torch.zeros(B, T, H, hd, dtype=torch.float64)
+    for b in range(B):
+        n = T if new is None else new[b]
+        for t in range(n):
+            at = starts[b] + t
+            if 0 <= at < slots:
+                x = q.view(B, T, H, hd)[b, t].double()
+                want_q[b, t] = _rot(x, cos[at].double(), sin[at].double())
+                room[b, t] = _rot(x.abs(), cos[at].abs().double(), -sin[at].abs().double()).abs()   # |a c| + |b s| of the first half, at least
+                room[b, t, :, hd // 2:] = (x[:, hd // 2:] * cos[at].double()).abs() + (x[:, :hd // 2] * sin[at].double()).abs()
+        slot = (torch.arange(n) + starts[b]).clamp(0, slots - 1)
+        for h in range(KV):
+            kh = _rot(k.view(B, T, KV, hd)[b, :n, h].float(), cos[slot], sin[slot])
+            _write(want[0][b, h], want[2][b, h], kh, sin, starts[b], block)
+            _write(want[1][b, h], want[3][b, h], v.view(B, T, KV, hd)[b, :n, h].float(), sin, starts[b], block)
+    got_q = out.cpu().double().view(B, T, H, hd)
+    # one rounding to 16 bits, three of fp32 ahead of it
+    tiny = _subnormal(dtype)
+    assert ((got_q - want_q).abs() <= _half(dtype) * want_q.abs() * 1.001 + 4 * 2.0 ** -24 * room + tiny).all()
+    for a, w in zip(dev[:4], want):
+        assert torch.equal(a.cpu().view(torch.uint8), w.view(torch.uint8))
+
+
+def test_a_block_filled_token_by_token(ops):
+    """Growing values: the scale grows at every token and older codes follow it; what comes out is off by half a step for each time, no more."""
+    B, H, hd, slots, block = 2, 3, 64, 48, 16
+    g = torch.Generator().manual_seed(5)
+    cos, sin = _tables(slots, hd)
+    cache = ops.q8_cache(B, H, slots, hd, block, I8, DEV)
+    want = [t.cpu().clone() for t in cache[:4]]
+    true = torch.zeros(B, H, slots, hd, dtype=torch.float64)
+    for t in range(slots):
+        q, k, v = ((torch.randn(B, H * hd, generator=g) * (1 + t % 16)).half() for _ in range(3))
+        ops.rope_append_q8(q.to(DEV), k.to(DEV), v.to(DEV), cos.to(DEV), sin.to(DEV), torch.full((B,), t, device=DEV), cache)
+        true[:, :, t] = v.view(B, H, hd).double()
+        for b in range(B):
+            for h in range(H):
+                _write(want[0][b, h], want[2][b, h], _rot(k.view(B, H, hd)[b, h:h + 1].float(), cos[t], sin[t]), None, t, block)
+                _write(want[1][b, h], want[3][b, h], v.view(B, H, hd)[b, h:h + 1].float(), None, t, block)
+    for a, w in zip(cache[:4], want):
+        assert torch.equal(a.cpu(), w)
+    _, vr = ops.cache_read_q8(cache, torch.float16)
+    step = cache.v_scale.cpu().double().repeat_interleave(block, -1)[..., None]
+    assert ((vr.cpu().double() - true).abs() <= (8.01 * step + _half(torch.float16) * true.abs())).all()   # 16 growths, each at most half a step of a smaller scale
+
+
+@pytest.mark.parametrize("code", [I8, E4], ids=["int8", "e4m3"])
+def test_append_of_values_that_are_no_numbers(ops, code):
+    """A NaN or an infinity makes its own block of its own head NaN, and nothing else; a block of values too small for a scale is zeros; a block begun
+    again is sound again."""
+    hd, slots, block = 64, 48, 16
+    cos, sin = _tables(slots, hd)
+    cache = ops.q8_cache(1, 2, slots, hd, block, code, DEV)
+    x = torch.ones(48, 2 * hd, dtype=torch.bfloat16)
+    x[3, 5], x[20, hd + 1] = math.nan, math.inf
+    x[32:] = 1e-38
+    put = lambda x, n, at: ops.rope_append_q8(x[:n].to(DEV), x[:n].to(DEV), x[:n].to(DEV), cos.to(DEV), sin.to(DEV), torch.tensor([at], device=DEV), cache)   # noqa: E731
+    put(x, 48, 0)
+    for t in ops.cache_read_q8(cache, torch.bfloat16):
+        t = t.cpu().float()
+        assert t[0, 0, :16].isnan().all() and t[0, 1, 16:32].isnan().all()
+        assert not t[0, 1, :16].isnan().any() and not t[0, 0, 16:32].isnan().any() and (t[0, :, 32:] == 0).all()
+    put(x[40:], 4, 4)     # into the middle of the bad block: still bad
+    assert ops.cache_read_q8(cache, torch.bfloat16)[1][0, 0, :16].isnan().all()
+    put(torch.ones_like(x), 16, 0)
+    assert (ops.cache_read_q8(cache, torch.bfloat16)[1][0, 0, :16] - 1).abs().max() <= (0.5 / 127 if code == I8 else 0) + _half(torch.bfloat16)
+
+
+@pytest.mark.parametrize("code", [I8, E4], ids=["int8", "e4m3"])
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("B,KV,hd,slots,block,lengths", [(1, 1, 64, 1, 16, None), (3, 2, 128, 77, 32, [0, 77, 50]), (2, 5, 64, 301, 128, [1000, -3])])
+def test_read(ops, B, KV, hd, slots, block, lengths, dtype, code):
+    g = torch.Generator().manual_seed(slots)
+    parts = _cache(ops, B, KV, slots, hd, block, code, g)
+    got = ops.cache_read_q8(_on(ops, parts, block), dtype, None if lengths is None else torch.tensor(lengths, device=DEV))
+    for codes, scale, o in zip(parts[:2], parts[2:], got):
+        want = _values(codes).double() * scale.double().repeat_interleave(block, -1)[..., :slots, None]
+        for b in range(B):
+            want[b, :, max(0, slots if lengths is None else lengths[b]):] = 0
+        tiny = _subnormal(dtype)
+        assert o.dtype == dtype and ((o.cpu().double() - want).abs() <= _half(dtype) * want.abs() * 1.001 + tiny).all()
+
+
+def _attention(q, parts, block, starts, new, scale):
+    """(out, allowance without the output's rounding) in 64 bits; q (B, T, H, hd).  Allowed: p is rounded to fp16 (half a step, 2^-12 of it; 2^-11 with what
+    the exponent's argument, up to 64 in fp32, and the sums of fp32 add) and below 2^-14 to multiples of 2^-24 of the largest value's scale, sixteen times that
+    where a larger scale came first; l is at least the sum taken against the true maximum."""
+    B, T, H, hd = q.shape
+    KV, slots = parts[0].shape[1:3]
+    k, v = (_values(c).double() * s.double().repeat_interleave(block, -1)[..., :slots, None] for c, s in ((parts[0], parts[2]), (parts[1], parts[3])))
+    out, room = torch.zeros(B, T, H, hd, dtype=torch.float64), torch.zeros(B, T, H, hd, dtype=torch.float64)
+    for b in range(B):
+        for t in range(T if new is None else max(0, min(T, new[b]))):
+            n = max(0, min(slots, starts[b] + t + 1))
+            if n == 0:
+                continue
+            for h in range(H):
+                kh, vh = k[b, h // (H // KV), :n], v[b, h // (H // KV), :n]
+                x = kh @ q[b, t, h].double() * scale
+                p = torch.exp(x - x.max())
+                l = p.sum()
+                out[b, t, h] = p @ vh / l
+                room[b, t, h] = 2.0 ** -11 * (p @ vh.abs()) / l + n * 2.0 ** -21 * vh.abs().max() / l
+    return out, room
+
+
+ATTENDS = [  # B, T, H, KV, hd, slots, block, starts, new
+    (1, 1, 1, 1, 64, 1, 16, [0], None),
+    (2, 1, 4, 2, 128, 17, 16, [16, 3], None),
+    (3, 1, 8, 8, 128, 600, 32, [599, 0, 255], None),
+    (2, 1, 8, 1, 64, 1100, 128, [1099, 64], None),
+    (4, 1, 4, 2, 64, 50, 16, [10, -1, 200, 49], [1, 1, 1, 0]),    # ordinary; sees nothing; past the end: all slots; no token
+    (1, 3, 14, 2, 128, 90, 64, [87], None),
+    (2, 5, 8, 2, 64, 700, 16, [300, 650], [5, 2]),
+    (1, 40, 4, 4, 128, 333, 16, [293], None),
+    (2, 70, 6, 2, 64, 300, 32, [0, 211], [70, 33]),
+    (1, 130, 2, 1, 128, 130, 16, [0], None),
+    (2, 150, 3, 3, 128, 420, 128, [1, 270], [0, 150]),
+    (1, 260, 4, 1, 64, 517, 64, [257], None),
+]
+
+
+@pytest.mark.parametrize("code", [I8, E4], ids=["int8", "e4m3"])
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("case", ATTENDS, ids=[str(i) for i in range(len(ATTENDS))])
+def test_attention(ops, case, dtype, code):
+    B, T, H, KV, hd, slots, block, starts, new = case
+    g = torch.Generator().manual_seed(slots + T)
+    parts = _cache(ops, B, KV, slots, hd, block, code, g)
+    q = (torch.randn(B, T, H, hd, generator=g) * 2).to(dtype)
+    args = (torch.tensor(starts, device=DEV), None if new is None else torch.tensor(new, device=DEV))
+    dirty = [t.clone() for t in parts]
+    for b in range(B):   # what nobody has written yet may be anything: the largest scales and NaN codes
+        end = max(0, min(slots, starts[b] + (T if new is None else new[b])))
+        for c, s in ((dirty[0], dirty[2]), (dirty[1], dirty[3])):
+            c.view(torch.uint8)[b, :, end:] = 0x7f
+            s[b, :, -(-end // block):] = math.nan
+    got = ops.attention_q8(q.view(B * T, H * hd).to(DEV), _on(ops, dirty, block), *args)
+    want, room = _attention(q, parts, block, starts, new, hd ** -0.5)
+    got = got.cpu().double().view(B, T, H, hd)
+    assert ((got - want).abs() <= _half(dtype) * want.abs() * 1.001 + room + _subnormal(dtype)).all()
+    again = ops.attention_q8(q.view(B * T, H * hd).to(DEV), _on(ops, parts, block), *args, scale=hd ** -0.5)
+    assert torch.equal(again.cpu().double().view(B, T, H, hd), got)   # the same sums in the same order
+
+
+@pytest.mark.parametrize("T", [1, 7, 160])
+def test_attention_of_uneven_values(ops, T):
+    """Scores that climb along the keys (the running maximum moves all the time), value scales from 1e-6 to 1e3 block by block, rows of q of very different
+    size, one of zeros: the same bounds hold."""
+    B, H, KV, hd, slots, block = 1, 4, 2, 128, 700, 16
+    g = torch.Generator().manual_seed(T)
+    parts = _cache(ops, B, KV, slots, hd, block, I8, g)
+    parts[2] *= torch.linspace(0.1, 3, parts[2].shape[2])
+    parts[3] = 10.0 ** (torch.rand(parts[3].shape, generator=g) * 9 - 6)
+    parts[3][:, :, 3] = 0
+    q = (torch.randn(B, T, H, hd, generator=g) * 10.0 ** (torch.arange(H) * 0.5 - 1.5)[:, None]).bfloat16()
+    q[:, :, 1] = 0
+    start = torch.tensor([slots - T], device=DEV)
+    got = ops.attention_q8(q.view(T, H * hd).to(DEV), _on(ops, parts, block), start).cpu().double().view(B, T, H, hd)
+    want, room = _attention(q, parts, block, [slots - T], None, hd ** -0.5)
+    assert ((got - want).abs() <= _half(torch.bfloat16) * want.abs() * 1.001 + room).all()
+
+
+@pytest.mark.parametrize("T,H,KV", [(3, 2, 2), (150, 2, 1)])
+def test_a_bad_block_reaches_only_the_rows_that_see_it(ops, T, H, KV):
+    hd, slots, block = 64, 300, 16
+    g = torch.Generator().manual_seed(1)
+    parts = _cache(ops, 1, KV, slots, hd, block, I8, g)
+    q = torch.randn(T, H * hd, generator=g).half()
+    start = 160 - T + 2   # slots 160 and 161, the block's first two, belong to the last two rows
+    for bad in (math.nan, math.inf):
+        for which in (2, 3):
+            spoilt = [t.clone() for t in parts]
+            spoilt[which][:, :, 10] = bad
+            out = ops.attention_q8(q.to(DEV), _on(ops, spoilt, block), torch.tensor([start], device=DEV)).cpu()
+            sound = ops.attention_q8(q.to(DEV), _on(ops, parts, block), torch.tensor([start], device=DEV)).cpu()
+            assert out[-2:].isnan().all() if bad != math.inf else not out[-2:].isfinite().all()
+            assert torch.equal(out[:-2], sound[:-2])
+
+
+def test_strides_and_streams(ops):
+    """q, k, v as columns of a fused projection's rows, and as views that the kernels do not take; a stream of its own."""
+    B, T, H, KV, hd, slots = 2, 6, 4, 2, 64, 40
+    g = torch.Generator().manual_seed(2)
+    wide = torch.randn(B * T, (H + 2 * KV) * hd, generator=g).half().to(DEV)
+    q, k, v = wide.split([H * hd, KV * hd, KV * hd], dim=1)
+    cos, sin = (t.to(DEV) for t in _tables(slots, hd))
+    start = torch.tensor([0, 30], device=DEV)
+
+    def both(q, k, v):
+        c = ops.q8_cache(B, KV, slots, hd, 16, I8, DEV)
+        r = ops.rope_append_q8(q, k, v, cos, sin, start, c)
+        return [r, ops.attention_q8(r, c, start), *c[:4]]
+
+    want = both(q.contiguous(), k.contiguous(), v.contiguous())
+    odd = torch.zeros(B * T, KV * hd + 3, dtype=torch.float16, device=DEV)[:, 3:]
+    odd.copy_(k)
+    s = torch.cuda.Stream()
+    s.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(s):
+        got = both(q, odd, v)
+    s.synchronize()
+    for a, b in zip(want, got):
+        assert torch.equal(a.view(torch.uint8), b.view(torch.uint8))
+
+
+def test_captured_and_replayed(ops):
+    """A graph of append and attention whose positions move by an in-place addition in the graph itself, against eager calls; two graphs of the same calls
+    replayed in turn on two streams share nothing."""
+    B, H, KV, hd, slots = 2, 4, 2, 128, 2048
+    cos, sin = (t.to(DEV) for t in _tables(slots, hd))
+    g = torch.Generator().manual_seed(3)
+    xs = [torch.randn(3, B, h * hd, generator=g).half().to(DEV) for h in (H, KV, KV)]
+
+    def make():
+        c = ops.q8_cache(B, KV, slots, hd, 16, I8, DEV)
+        start = torch.tensor([5, 1029], device=DEV)
+        return c, start, [x[0].clone() for x in xs]
+
+    def step(c, start, x):
+        r = ops.rope_append_q8(*x, cos, sin, start, c)
+        o = ops.attention_q8(r, c, start)
+        start.add_(1)
+        return o
+
+    eager = make()
+    want = []
+    for i in range(3):
+        for d, s in zip(eager[2], xs):
+            d.copy_(s[i])
+        want.append(step(*eager).clone())
+    graphs = []
+    for _ in range(2):
+        state = make()
+        st = torch.cuda.Stream()
+        st.wait_stream(torch.cuda.current_stream())
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.stream(st):
+            with torch.cuda.graph(graph, stream=st):
+                out = step(*state)
+        graphs.append((graph, st, state, out))
+    torch.cuda.synchronize()
+    for i in range(3):
+        for graph, st, state, out in graphs:
+            with torch.cuda.stream(st):
+                for d, s in zip(state[2], xs):
+                    d.copy_(s[i])
+                graph.replay()
+        torch.cuda.synchronize()
+        for graph, st, state, out in graphs:
+            assert torch.equal(out, want[i])
+
+
+def test_refusals_on_the_device(ops):
+    c = ops.q8_cache(1, 2, 32, 64, device=DEV)
+    cos, sin = (t.to(DEV) for t in _tables(32, 64))
+    x, start = torch.zeros(2, 128, dtype=torch.float16, device=DEV), torch.zeros(1, dtype=torch.int64, device=DEV)
+    bad = [lambda: ops.rope_append_q8(x, x[:1], x, cos, sin, start, c), lambda: ops.rope_append_q8(x, x, x.bfloat16(), cos, sin, start, c),
+           lambda: ops.rope_append_q8(x, x, x, cos[:31], sin[:31], start, c), lambda: ops.rope_append_q8(x, x, x, cos, sin.double(), start, c),
+           lambda: ops.rope_append_q8(x, x, x, cos, sin, start.int(), c), lambda: ops.rope_append_q8(x, x, x, cos, sin, start.expand(2), c),
+           lambda: ops.rope_append_q8(x, x, x, cos, sin, start.cpu(), c), lambda: ops.attention_q8(x[:, :64], c, start), lambda: ops.attention_q8(x.float(), c, start),
+           lambda: ops.attention_q8(x, c._replace(block=32), start), lambda: ops.attention_q8(x, c._replace(k=c.k.float()), start),
+           lambda: ops.attention_q8(x, c._replace(k=c.k.transpose(1, 2)), start), lambda: ops.attention_q8(x, c._replace(v_scale=c.v_scale.half()), start),
+           lambda: ops.cache_read_q8(c, torch.float32), lambda: ops.cache_read_q8(c, torch.float16, start.int()),
+           lambda: ops.token_logprobs(x, start), lambda: ops.token_logprobs(x.double(), start.expand(2)), lambda: ops.token_logprobs(x, start.expand(2).int())]
+    for call in bad:
+        with pytest.raises(AssertionError):
+            call()
+    with pytest.raises(RuntimeError, match="0 to 64"):
+        ops.token_logprobs(x, start.expand(2), 65)
+    with pytest.raises((AssertionError, RuntimeError)):
+        ops.attention_q8(x, ops.Q8Cache(*(t[..., :48].contiguous() for t in c[:2]), *c[2:4], 16), start)
+
+
+# ------------------------------------------------------------------------------------------------ log probabilities
+def _rows(rows, vocab, dtype, g, kind):
+    x = torch.randn(rows, vocab, generator=g) * 3
+    if kind == "masked":
+        x[torch.rand(rows, vocab, generator=g) < 0.7] = -math.inf
+        x[:, vocab // 2] = 1.0
+    elif kind == "equal":
+        x[:] = 0.25
+    elif kind == "lowest":   # places masked with the type's lowest number
+        x[:, 1:] = torch.finfo(dtype).min
+    elif kind == "large":
+        x = x * 1e4
+    elif kind == "steps":    # many ties
+        x = x.round()
+    return x.to(dtype)
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("rows,vocab,top,kind", [(1, 1, 1, ""), (1, 5, 5, ""), (3, 257, 64, ""), (4, 32000, 5, ""), (5, 1001, 8, "masked"), (2, 4096, 64, "equal"),
+                                                 (2, 333, 3, "lowest"), (3, 2048, 4, "large"), (37, 50257, 0, ""), (7, 20011, 20, "steps"), (300, 515, 2, ""),
+                                                 (2, 131072, 7, "steps"), (1, 151936, 33, "masked"), (160, 40000, 64, "equal")])
+def test_logprobs(ops, rows, vocab, top, kind, dtype):
+    g = torch.Generator().manual_seed(rows + vocab)
+    x = _rows(rows, vocab, dtype, g, kind)
+    ids = torch.randint(0, vocab, (rows,), generator=g)
+    lp, ent, tl, ti = (t.cpu() for t in ops.token_logprobs(x.to(DEV), ids.to(DEV), top))
+    d = x.double()
+    want = torch.log_softmax(d, -1)
+    far = d - d.amax(-1, keepdim=True)
+    log_s = far.exp().sum(-1, keepdim=True).log()
+    # S: e to 2^-21 and 2^-23 of its exponent's argument, sums over at most vocab / 256 + 64 terms in a row; then a difference of two fp32 numbers
+    rel_s = 2.0 ** -21 + (vocab / 256 + 64) * 2.0 ** -24
+    allow = rel_s + 2.0 ** -23 * (far.abs().nan_to_num(posinf=0) + log_s)
+    # (fp16 rows of "large" hold infinities: NaN in both)
+    ok = lambda got, ref, room: bool((((got.double() - ref).abs() <= room) | (got.double() == ref) | (got.isnan() & ref.isnan())).all())   # noqa: E731
+    assert ok(lp, want.gather(1, ids[:, None])[:, 0], allow.gather(1, ids[:, None])[:, 0])
+    e = torch.special.entr(want.exp()).sum(-1)
+    spread = (want.exp() * far.nan_to_num(neginf=0).abs()).sum(-1)   # sum p |x - M|: each term to rel_s and 2^-23 of its argument
+    assert ok(ent, e, rel_s * (1 + 2 * spread) + 2.0 ** -22 * (want.exp() * far.nan_to_num(neginf=0) ** 2).sum(-1) + 2.0 ** -23 * (log_s[:, 0] + spread))
+    order = x.float().sort(dim=-1, descending=True, stable=True).indices[:, :top]
+    assert tl.shape == ti.shape == (rows, top) and ti.dtype == torch.int64 and torch.equal(ti, order)
+    assert ok(tl, want.gather(1, order), allow.gather(1, order))
+
+
+def test_logprobs_of_rows_without_a_distribution(ops):
+    x = torch.zeros(6, 700)
+    x[0] = -math.inf
+    x[1, 3], x[1, 600] = math.nan, 5.0
+    x[2, 9], x[2, 8] = math.inf, 1.0
+    x[3, :] = -math.inf
+    x[3, 699] = -2.0
+    x[4, 100::2] = -0.0
+    for dtype in (torch.float16, torch.float32):
+        lp, ent, tl, ti = (t.cpu() for t in ops.token_logprobs(x.to(dtype).to(DEV), torch.tensor([1, 2, 9, 699, 700, -1], device=DEV), 3))
+        assert lp[0] == -math.inf and ent[0] == 0 and (tl[0] == -math.inf).all() and ti[0].tolist() == [0, 1, 2]
+        assert lp[1].isnan() and ent[1].isnan() and ti[1].tolist() == [3, 600, 0]
+        assert lp[2].isnan() and ent[2].isnan() and ti[2].tolist() == [9, 8, 0]
+        assert lp[3] == 0 and ent[3] == 0 and tl[3].tolist() == [0, -math.inf, -math.inf] and ti[3].tolist() == [699, 0, 1]
+        assert lp[4].isnan() and ti[4].tolist() == [0, 1, 2]     # an id beyond the vocabulary; -0 ties with 0
+        assert lp[5] == 0
+
+
+def test_logprobs_shapes_and_strides(ops):
+    g = torch.Generator().manual_seed(9)
+    x = torch.randn(3, 4, 1003, generator=g).half().to(DEV)
+    ids = torch.randint(0, 1000, (3, 4), generator=g).to(DEV)
+    want = ops.token_logprobs(x[..., :1000].contiguous(), ids, 4)
+    for got in (ops.token_logprobs(x[..., :1000], ids, 4), ops.token_logprobs(x[..., :1000].transpose(0, 1), ids.t(), 4)):
+        for a, b in zip(want, got):
+            assert a.shape[:2] == (3, 4) and torch.equal(a, b if b.shape[0] == 3 else b.transpose(0, 1))
+    one = ops.token_logprobs(x[0, 0, 1:1001], ids[0, 0])
+    assert one[0].shape == () and one[2].shape == (0,) and one[0].isfinite()
+    none = ops.token_logprobs(x[:0], ids[:0], 2)
+    assert none[0].shape == (0, 4) and none[3].shape == (0, 4, 2)
+
+
+# ------------------------------------------------------------------------------------------------ together, as a decoder uses them
+@pytest.mark.parametrize("code", ["int8", "e4m3"])
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+def test_decoder_on_an_8_bit_cache(ops, code, dtype):
+    from mem_efficient_blr_b200 import networks as nw
+    shape = nw.LlamaShape(layers=2, d=512, heads=8, ffn=1024, vocab=384, b=16, rank_attn=64, rank_mlp=96)
+    B, T, S = 3, 41, 64
+    ids = torch.randint(0, shape.vocab, (B, T), generator=torch.Generator().manual_seed(1)).to(DEV)
+    make = lambda **kw: nw.LlamaDecoder(shape, "blast", batch=B, cache_len=S, device=DEV, dtype=dtype, seed=3, **kw)   # noqa: E731
+    rel = lambda a, b: float((a.double() - b.double()).norm() / b.double().norm())   # noqa: E731
+    m, slow, plain = make(kv_cache=code), make(kv_cache=code, kv_block=32), make()
+    slow.fused_decode = False
+    a, c = m.prefill(ids[:, :T - 1]), plain.prefill(ids[:, :T - 1])
+    # quantising: a value is off by at most half a step, 1/254 of its block's largest (2^-4 of itself in e4m3), in both operands of both products of two layers
+    assert rel(a, c) < (0.1 if code == "e4m3" else 0.03)
+    step = m.decode_step(ids[:, T - 1:], torch.tensor([T - 1], device=DEV))
+    # the same tokens in pieces, sequences at different positions and a padded batch
+    n = torch.tensor([30, 17, 1], device=DEV)
+    p = make(kv_cache=code)
+    p.extend(ids[:, :30], torch.zeros(B, dtype=torch.int64, device=DEV), n)
+    idx = (n[:, None] + torch.arange(T - 1, device=DEV)).clamp(max=T - 1)
+    p.extend(ids.gather(1, idx), n, T - 1 - n)
+    piece = p.decode_step(ids[:, T - 1:], torch.full((B,), T - 1, device=DEV))
+    tol = 0.1 if code == "e4m3" else 0.03    # (a block's codes depend on how the block was filled)
+    assert rel(piece, step) < tol
+    # reading back and torch's attention, on blocks of 32
+    slow.prefill(ids[:, :T - 1])
+    assert rel(slow.decode_step(ids[:, T - 1:], torch.tensor([T - 1], device=DEV)), step) < tol
+    # scoring: the last position's distribution is the prefill's
+    lp, ent, tl, ti = m.score(ids, 3)
+    assert lp.shape == (B, T - 1) and tl.shape == (B, T - 1, 3)
+    want = torch.log_softmax(a.double(), -1)
+    assert (lp[:, -1].double() - want.gather(1, ids[:, -1:])[:, 0]).abs().max() < 0.05 and (lp <= 0).all() and (ent >= 0).all()
+    assert (plain.score(ids)[0] - lp).abs().mean() < (0.3 if code == "e4m3" else 0.1)
+
+
+def test_graphed_decode_on_an_8_bit_cache(ops):
+    from mem_efficient_blr_b200 import networks as nw
+    shape = nw.LlamaShape(layers=2, d=512, heads=8, ffn=1024, vocab=384, b=16, rank_attn=64, rank_mlp=96)
+    ids = torch.randint(0, shape.vocab, (2, 40), generator=torch.Generator().manual_seed(4)).to(DEV)
+    m = [nw.LlamaDecoder(shape, "blast_int8", batch=2, cache_len=48, device=DEV, seed=3, kv_cache="int8") for _ in range(2)]
+    for x in m:
+        x.prefill(ids[:, :36])
+    pos = torch.tensor([36], device=DEV)
+    step = nw.GraphedCall(m[0].decode_step, ids[:, 36:37].clone(), pos.clone())
+    for i in range(36, 40):
+        at = torch.tensor([i], device=DEV)
+        assert torch.equal(step(ids[:, i:i + 1], at), m[1].decode_step(ids[:, i:i + 1], at))
