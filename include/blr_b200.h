@@ -418,10 +418,11 @@ int blr_cache_read_q8(const blr_q8_cache* cache, const int64_t* lengths, int dty
 
 /* Causal attention of the newest tokens: row t < n_new[s] of sequence s sits at slot start[s] + t and sees slots 0 .. start[s] + t;
  * out = softmax(scale * q . K^T) V.  heads a multiple of kv_heads: head h reads kv head h / (heads / kv_heads).  scratch:
- * blr_attention_q8_scratch_bytes (may be 0), 16-byte aligned, nothing kept in it between calls. */
+ * blr_attention_q8_scratch_bytes (may be 0), 16-byte aligned, nothing kept in it between calls.  scale: a positive number.  ws: a workspace (NULL: none)
+ * whose status word tells of a device-side wait that ran out (blr_workspace_status); the rows concerned come out as NaN. */
 size_t blr_attention_q8_scratch_bytes(const blr_q8_cache* cache, int64_t n_tok, int heads);
 int blr_attention_q8(const void* q, int64_t ldq, const blr_q8_cache* cache, const int64_t* start, const int64_t* n_new, int64_t n_tok, int heads,
-                     float scale, int dtype, void* out, int64_t ldo, void* scratch, size_t scratch_bytes, void* stream);
+                     float scale, int dtype, void* out, int64_t ldo, void* scratch, size_t scratch_bytes, void* ws, void* stream);
 
 /* Of each row of logits (row stride ld; kind 0 fp16, 1 bf16, 2 fp32): logprob[r] = log softmax(row)[ids[r]] (0 where ids[r] < 0: no token given; NaN
  * where ids[r] >= vocab), entropy[r] of the softmax, and the `top` (0 .. 64, at most vocab) likeliest tokens by falling logit, ties by rising id: their

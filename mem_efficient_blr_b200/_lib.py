@@ -99,7 +99,7 @@ SIGNATURES = {
     "blr_rope_append_q8": (_int, [_vp, _i64, _vp, _i64, _vp, _i64, _vp, _vp, _vp, _vp, _i64, _int, _int, C.POINTER(Q8CacheDesc), _vp, _i64, _vp]),
     "blr_cache_read_q8": (_int, [C.POINTER(Q8CacheDesc), _vp, _int, _vp, _vp, _vp]),
     "blr_attention_q8_scratch_bytes": (_sz, [C.POINTER(Q8CacheDesc), _i64, _int]),
-    "blr_attention_q8": (_int, [_vp, _i64, C.POINTER(Q8CacheDesc), _vp, _vp, _i64, _int, C.c_float, _int, _vp, _i64, _vp, _sz, _vp]),
+    "blr_attention_q8": (_int, [_vp, _i64, C.POINTER(Q8CacheDesc), _vp, _vp, _i64, _int, C.c_float, _int, _vp, _i64, _vp, _sz, _vp, _vp]),
     "blr_token_logprobs": (_int, [_vp, _i64, _i64, _i64, _int, _vp, _int, _vp, _vp, _vp, _vp, _vp]),
     "blr_quantize_sym": (_int, [_vp, _int, _i64, _i64, _int, _vp, _vp, _vp]),
     "blr_dequantize_sym": (_int, [_vp, _vp, _i64, _i64, _int, _i64, _int, _vp, _vp]),

@@ -10,46 +10,18 @@
 // a small p is 2^-25 of the largest.
 // Bound by HBM on the codes (a key and its value are 2 hd bytes).  The keys of a row are shared out over the warps of a CTA and over up to kMaxSplits CTAs.
 #include "../../include/blr_b200.h"
-#include "q8.cuh"
+#include "q8_attention.h"
 #include "tmap.h"
 
 namespace blr {
 
 static constexpr int kQ8Warps = 8, kMaxSplits = 64;
 
-struct Q8AttnParams {
-  Q8View c;
-  const uint16_t* q;
-  uint16_t* out;
-  long long ldq, ldo;
-  const long long *start, *n_new;
-  float* part;
-  float scale_log2;
-  int T, H, G, rows, q_tiles, ns, bf16;
-};
-
-__device__ __forceinline__ float ex2(float x) {
-  float r;
-  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
-  return r;
-}
 __device__ __forceinline__ uint32_t transpose8x8(uint32_t a) {
   uint32_t d;
   asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(d) : "r"(a));
   return d;
 }
-__device__ __forceinline__ uint32_t pack_half2(float a, float b) {
-  const __half2 h = __floats2half2_rn(a, b);
-  return *reinterpret_cast<const uint32_t*>(&h);
-}
-
-// Slots that a row of token t sees.
-__device__ __forceinline__ int q8_seen(long long start, long long count, long long t, int slots) {
-  if (t >= count) return 0;
-  const long long n = start + t + 1;
-  return n <= 0 ? 0 : n > slots ? slots : (int)n;
-}
-
 template <int HD>
 struct Q8Keys {  // 16 keys of a warp: rows g and g + 8 of K, keys 2t, 2t + 1, 2t + 8, 2t + 9 of V
   uint32_t k[2][HD / 16], v[4][HD / 32];
@@ -92,8 +64,7 @@ __global__ void __launch_bounds__(32 * kQ8Warps) q8_attention_kernel(const __gri
   const int b = bh / p.c.kv_heads, h = bh - b * p.c.kv_heads, r0 = qt * kRows;
   asm volatile("griddepcontrol.wait;" ::: "memory");
   const long long start = p.start[b], count = p.n_new == nullptr ? p.T : min((long long)p.T, p.n_new[b]);
-  const int t_last = (min(r0 + kRows, p.rows) - 1) / p.G;
-  const int keys = (r0 / p.G) < count ? q8_seen(start, count, min((long long)t_last, count - 1), p.c.slots) : 0;
+  const int keys = q8_seen_by(p, start, count, r0, r0 + kRows);
   const int share = ((keys + p.ns - 1) / p.ns + 63) & ~63, k0 = min(keys, split * share), k1 = min(keys, k0 + share);
 
   // ---- the query rows as fp16 fragments, and what their dot products are to be multiplied with
@@ -128,8 +99,7 @@ __global__ void __launch_bounds__(32 * kQ8Warps) q8_attention_kernel(const __gri
     }
     most = max(most, __shfl_xor_sync(0xffffffffu, most, 1));
     most = max(most, __shfl_xor_sync(0xffffffffu, most, 2));
-    // bf16 rows: times the power of two that brings their largest value to 2^14
-    const int ex = (int)(most >> 23), up = p.bf16 && ex != 0 && ex != 255 ? min(268 - ex, 253) : 127;
+    const int up = q8_row_up(most, p.bf16);
     const float mul = __uint_as_float((uint32_t)up << 23), back = __uint_as_float((uint32_t)(254 - up) << 23);
 #pragma unroll
     for (int s = 0; s < kSteps; ++s) {
@@ -326,24 +296,25 @@ __global__ void __launch_bounds__(256) q8_combine_kernel(const __grid_constant__
     *reinterpret_cast<uint32_t*>(to + i) = p.bf16 ? q8_down2<true>(sum[i] * inv, sum[i + 1] * inv) : q8_down2<false>(sum[i] * inv, sum[i + 1] * inv);
 }
 
-// CTAs over which a row's keys are split: as many as fill the SMs, with at least 256 keys each.
-static int q8_splits(long long tiles, int slots) {
-  const long long room = 2ll * sm_count();
+// CTAs over which a row's keys are split: as many as fill the SMs, with at least 256 keys each (512 in the prompt kernel).
+static int q8_splits(long long tiles, int slots, bool prompt) {
+  const long long room = (prompt ? 1ll : 2ll) * sm_count(), least = prompt ? 512 : 256;
   long long ns = room / tiles;
-  if (ns > (slots + 255) / 256) ns = (slots + 255) / 256;
+  if (ns > (slots + least - 1) / least) ns = (slots + least - 1) / least;
   return ns < 1 ? 1 : ns > kMaxSplits ? kMaxSplits : (int)ns;
 }
 struct Q8Plan {
-  int nt, q_tiles, ns;
+  int nt, q_tiles, ns;  // nt: column tiles of 8 rows of the kernel here, 0: the prompt kernel
   long long rows, tiles;
 };
 static Q8Plan q8_plan(const blr_q8_cache* c, int64_t n_tok, int heads) {
   Q8Plan a = {};
   a.rows = n_tok * (heads / c->kv_heads);
-  a.nt = a.rows <= 8 ? 1 : 2;
-  a.q_tiles = (int)((a.rows + 8 * a.nt - 1) / (8 * a.nt));
+  a.nt = a.rows <= 8 ? 1 : a.rows <= 64 ? 2 : 0;
+  const int per = a.nt ? 8 * a.nt : kQ8PromptRows;
+  a.q_tiles = (int)((a.rows + per - 1) / per);
   a.tiles = c->n_seq * c->kv_heads * a.q_tiles;
-  a.ns = a.tiles > 0 ? q8_splits(a.tiles, c->slots) : 1;
+  a.ns = a.tiles > 0 ? q8_splits(a.tiles, c->slots, a.nt == 0) : 1;
   return a;
 }
 
@@ -375,7 +346,7 @@ size_t blr_attention_q8_scratch_bytes(const blr_q8_cache* cache, int64_t n_tok, 
 }
 
 int blr_attention_q8(const void* q, int64_t ldq, const blr_q8_cache* cache, const int64_t* start, const int64_t* n_new, int64_t n_tok, int heads,
-                     float scale, int dtype, void* out, int64_t ldo, void* scratch, size_t scratch_bytes, void* stream) {
+                     float scale, int dtype, void* out, int64_t ldo, void* scratch, size_t scratch_bytes, void* ws, void* stream) {
   Q8AttnParams p = {};
   int rc;
   if ((rc = q8_view(cache, &p.c))) return rc;
@@ -383,6 +354,7 @@ int blr_attention_q8(const void* q, int64_t ldq, const blr_q8_cache* cache, cons
   BLR_REQUIRE(heads > 0 && heads % cache->kv_heads == 0, BLR_ERR_ARG, "attention_q8: %d heads are no multiple of %d kv heads", heads, cache->kv_heads);
   BLR_REQUIRE(n_tok >= 0 && n_tok * (heads / cache->kv_heads) < (1ll << 30), BLR_ERR_SHAPE, "attention_q8: n_tok = %lld", (long long)n_tok);
   BLR_REQUIRE((ldq | ldo) % 8 == 0, BLR_ERR_ARG, "attention_q8: row strides must be multiples of 8");
+  BLR_REQUIRE(scale > 0.f && scale <= 3.0e38f, BLR_ERR_ARG, "attention_q8: the scale must be a positive number");
   if (cache->n_seq == 0 || n_tok == 0) return BLR_OK;
   BLR_REQUIRE(q && start && out, BLR_ERR_ARG, "null pointer");
   BLR_REQUIRE(((reinterpret_cast<uintptr_t>(q) | reinterpret_cast<uintptr_t>(out) | reinterpret_cast<uintptr_t>(scratch)) & 15) == 0, BLR_ERR_ARG,
@@ -397,11 +369,14 @@ int blr_attention_q8(const void* q, int64_t ldq, const blr_q8_cache* cache, cons
   p.part = static_cast<float*>(scratch);
   p.scale_log2 = scale * 1.4426950408889634f;
   p.T = (int)n_tok, p.H = heads, p.G = heads / cache->kv_heads, p.rows = (int)a.rows, p.q_tiles = a.q_tiles, p.ns = a.ns, p.bf16 = dtype == BLR_DTYPE_BF16;
+  p.n_bh = (int)(cache->n_seq * cache->kv_heads);
+  p.status = ws == nullptr ? nullptr : static_cast<unsigned*>(ws) + 255;
   const cudaStream_t st = static_cast<cudaStream_t>(stream);
   const dim3 grid((unsigned)(a.tiles * a.ns)), block(32 * kQ8Warps);
   auto go = [&](auto kernel) { return launch(kernel, grid, block, st, p); };
 #define BLR_Q8_ATTN(E4, HD) (a.nt == 1 ? go(q8_attention_kernel<E4, HD, 1>) : go(q8_attention_kernel<E4, HD, 2>))
-  if (cache->code == BLR_Q8_E4M3) rc = cache->head_dim == 128 ? BLR_Q8_ATTN(true, 128) : BLR_Q8_ATTN(true, 64);
+  if (a.nt == 0) rc = q8_launch_prompt(p, cache->head_dim, cache->code, st);
+  else if (cache->code == BLR_Q8_E4M3) rc = cache->head_dim == 128 ? BLR_Q8_ATTN(true, 128) : BLR_Q8_ATTN(true, 64);
   else rc = cache->head_dim == 128 ? BLR_Q8_ATTN(false, 128) : BLR_Q8_ATTN(false, 64);
 #undef BLR_Q8_ATTN
   if (rc || a.ns == 1) return rc;

@@ -1,0 +1,49 @@
+// Attention over an 8-bit cache: what its kernels share.  q8_attention.cu has the one for few rows and the entry point, q8_prompt.cu the one for many.
+#pragma once
+#include "q8.cuh"
+
+namespace blr {
+
+struct Q8AttnParams {
+  Q8View c;
+  const uint16_t* q;
+  uint16_t* out;
+  long long ldq, ldo;
+  const long long *start, *n_new;
+  float* part;       // ns > 1: of each (sequence, kv head, row, split) hd sums, the maximum that they are taken against, the sum of the weights, 2 free
+  unsigned* status;  // NULL, or where a wait that gave up is noted
+  float scale_log2;
+  int T, H, G, rows, q_tiles, ns, bf16, n_bh;
+};
+
+__device__ __forceinline__ float ex2(float x) {
+  float r;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+  return r;
+}
+__device__ __forceinline__ uint32_t pack_half2(float a, float b) {
+  const __half2 h = __floats2half2_rn(a, b);
+  return *reinterpret_cast<const uint32_t*>(&h);
+}
+// Slots that a row of token t sees.
+__device__ __forceinline__ int q8_seen(long long start, long long count, long long t, int slots) {
+  if (t >= count) return 0;
+  const long long n = start + t + 1;
+  return n <= 0 ? 0 : n > slots ? slots : (int)n;
+}
+// The slots that the last of rows [r0, r1) of a kv head sees: 0 where none of them is a token.
+__device__ __forceinline__ int q8_seen_by(const Q8AttnParams& p, long long start, long long count, int r0, int r1) {
+  r1 = min(r1, p.rows);
+  if (r0 >= r1 || r0 / p.G >= count) return 0;
+  return q8_seen(start, count, min((long long)((r1 - 1) / p.G), count - 1), p.c.slots);
+}
+// The power of two that brings a bf16 row whose largest value has these bits to 2^14, in fp16's range, as an exponent (127: 1); fp16 rows stay as they are.
+__device__ __forceinline__ int q8_row_up(uint32_t most, int bf16) {
+  const int ex = (int)(most >> 23);
+  return bf16 && ex != 0 && ex != 255 ? min(268 - ex, 253) : 127;
+}
+
+int q8_launch_prompt(const Q8AttnParams& p, int head_dim, int code, cudaStream_t stream);
+static constexpr int kQ8PromptRows = 256;  // rows of a CTA
+
+}  // namespace blr

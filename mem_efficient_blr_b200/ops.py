@@ -764,10 +764,10 @@ def attention_q8(q: torch.Tensor, cache: Q8Cache, start: torch.Tensor, n_new=Non
     out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
     nbytes = lib.blr_attention_q8_scratch_bytes(d, n_tok, heads)
     scratch = torch.empty(nbytes, dtype=torch.uint8, device=q.device) if nbytes else None
+    ws, st = _ws(q, 1, 0, 0)   # (its status word)
     L.check(lib.blr_attention_q8(q2.data_ptr(), q2.stride(0), d, _per_sequence(start, q, d.n_seq, "start"),
                                  None if n_new is None else _per_sequence(n_new, q, d.n_seq, "n_new"), n_tok, heads, float(scale) if scale else d.head_dim ** -0.5,
-                                 L.dtype_code(q.dtype), out.data_ptr(), out.shape[1], None if scratch is None else scratch.data_ptr(), nbytes,
-                                 L.stream_ptr(q.device)))
+                                 L.dtype_code(q.dtype), out.data_ptr(), out.shape[1], None if scratch is None else scratch.data_ptr(), nbytes, ws.data_ptr(), st))
     return out
 
 

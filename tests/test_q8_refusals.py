@@ -28,8 +28,8 @@ def _append(L, desc, q=P, ldq=256, n_tok=1, heads=4, dtype=0, ldo=256, start=P):
     return L.load().blr_rope_append_q8(q, ldq, P, 128, P, 128, P, P, start, None, n_tok, heads, dtype, desc, P, ldo, None)
 
 
-def _attend(L, desc, q=P, ldq=256, n_tok=1, heads=4, dtype=0, out=P, scratch=P, nbytes=1 << 30, start=P):
-    return L.load().blr_attention_q8(q, ldq, desc, start, None, n_tok, heads, 1.0, dtype, out, 256, scratch, nbytes, None)
+def _attend(L, desc, q=P, ldq=256, n_tok=1, heads=4, dtype=0, out=P, scratch=P, nbytes=1 << 30, start=P, scale=1.0):
+    return L.load().blr_attention_q8(q, ldq, desc, start, None, n_tok, heads, scale, dtype, out, 256, scratch, nbytes, None, None)
 
 
 @pytest.mark.parametrize("bad", [dict(head_dim=96), dict(head_dim=256), dict(block=8), dict(block=48), dict(block=256), dict(code=2), dict(kv_heads=0), dict(slots=0),
@@ -49,6 +49,7 @@ def test_arguments_of_the_cache_operators(L):
     assert _append(L, d, ldq=252) == ARG and _append(L, d, ldo=252) == ARG and _attend(L, d, ldq=252) == ARG
     assert _append(L, d, n_tok=-1) == ARG and _append(L, d, heads=0) == ARG
     assert _attend(L, d, heads=3) == ARG and _attend(L, d, heads=0) == ARG and _attend(L, d, n_tok=-1) == SHAPE
+    assert all(_attend(L, d, scale=s) == ARG for s in (0.0, -1.0, float("inf"), float("nan")))
     wide = _desc(L, n_seq=1, kv_heads=1, slots=100000, head_dim=128)
     need = lib.blr_attention_q8_scratch_bytes(wide, 1, 1)
     assert need > 0 and _attend(L, wide, heads=1, nbytes=need - 1) == WORKSPACE and _attend(L, wide, heads=1, scratch=None) == WORKSPACE
