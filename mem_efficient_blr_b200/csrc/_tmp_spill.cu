@@ -1,0 +1,513 @@
+// Causal attention of many rows over an 8-bit cache (q8.cuh) on tcgen05 / TMEM (sm_100a).  One CTA takes 256 rows of a kv head (tokens x query heads, token by
+// token) and walks the keys 128 at a time, warp-specialised:
+//   warps 0-3, 4-7  softmax of rows 0-127 and 128-255, a thread per row: S from TMEM, P back over it as fp16 pairs, O rescaled there when it has to be
+//   warps 8-11      widen the codes of the next keys and values to fp16 (exact) into shared memory, as tcgen05.mma reads them
+//   warps 12-15     one thread of the first issues the products: S = Q K^T (both from shared memory), O += P V (P from TMEM)
+// The scales stay out of the products: a group of 16 keys has one for its keys, which multiplies S in the exponent's argument, and one for its values, which
+// multiplies p by vs / R with R the largest of them so far (moved when it is 2^4 behind, like the maximum when it is 2^8 behind; see q8_attention.cu).
+// Order of the products: S0 S1 | PV0 S0 | PV1 S1 | ...: while the tensor cores do one half's PV and its next S, the other half's softmax runs.  P lies over S, so a
+// half's next S waits for its PV, in the same queue; a commit covers all products before it, so a softmax that has its S knows that its last PV is done.
+// Bounds: 2 x 2 x 512 cycles of tensor core and as many of ex2 (16 a cycle) for 256 x 128 scores of heads of 128.
+// All waits are bounded; a time-out is noted in *status, the rows of that CTA come out as NaN, and the kernel frees its TMEM and ends.
+#include <math_constants.h>
+
+#include "../../include/blr_b200.h"
+#include "q8_attention.h"
+#include "tmap.h"
+
+namespace blr {
+
+static constexpr int kPromptThreads = 512, kKeys = 128;
+// Registers of a thread at launch, and of the softmax warps (8), the widening ones (4) and the last four from then on: setmaxnreg waits for ever for registers that
+// the block was not launched with.
+static constexpr int kRegs = 128, kRegsSoftmax = 160, kRegsWiden = 136, kRegsIssue = 56;
+static_assert(8 * kRegsSoftmax + 4 * kRegsWiden + 4 * kRegsIssue <= kPromptThreads / 32 * kRegs, "more registers than the block has");
+
+__device__ __forceinline__ void tmem_ld32(uint32_t taddr, uint32_t (&r)[32]) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]),
+        "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]), "=r"(r[16]), "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]),
+        "=r"(r[23]), "=r"(r[24]), "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
+      : "r"(taddr)
+      : "memory");
+}
+__device__ __forceinline__ void tmem_ready(uint32_t (&r)[32]) {  // (uses of r stay behind the wait ahead of this)
+#pragma unroll
+  for (int i = 0; i < 32; i += 8)
+    asm volatile("" : "+r"(r[i]), "+r"(r[i + 1]), "+r"(r[i + 2]), "+r"(r[i + 3]), "+r"(r[i + 4]), "+r"(r[i + 5]), "+r"(r[i + 6]), "+r"(r[i + 7]));
+}
+__device__ __forceinline__ void tmem_st16(uint32_t taddr, const uint32_t (&r)[16]) {
+  asm volatile("tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16};" ::"r"(taddr), "r"(r[0]), "r"(r[1]),
+               "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]),
+               "r"(r[15])
+               : "memory");
+}
+__device__ __forceinline__ void sts128(uint32_t addr, uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
+  asm volatile("st.shared.v4.b32 [%0], {%1,%2,%3,%4};" ::"r"(addr), "r"(a), "r"(b), "r"(c), "r"(d) : "memory");
+}
+
+// Two floats of one 64-bit register: one instruction for both.
+__device__ __forceinline__ uint64_t pair(float a, float b) {
+  uint64_t r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
+  return r;
+}
+__device__ __forceinline__ void unpair(uint64_t v, float& a, float& b) { asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(v)); }
+__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
+  uint64_t r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+  return r;
+}
+__device__ __forceinline__ uint64_t mul2(uint64_t a, uint64_t b) {
+  uint64_t r;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+__device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
+  uint64_t r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+
+// What a CTA works on.  (Asked for anew where it is needed: kept in registers across the loops it would push others out of them.)
+struct Place {
+  int split, bh, b, h, r0;
+};
+__device__ __forceinline__ Place place_of(const Q8AttnParams& p) {
+  int cta;
+  asm volatile("mov.u32 %0, %%ctaid.x;" : "=r"(cta));
+  Place a;
+  const int tile = cta / p.ns;
+  a.split = cta - tile * p.ns;
+  a.bh = tile % p.n_bh;
+  a.r0 = (p.q_tiles - 1 - tile / p.n_bh) * kQ8PromptRows;  // the last rows have the most keys: their CTAs come first
+  a.b = a.bh / p.c.kv_heads;
+  a.h = a.bh - a.b * p.c.kv_heads;
+  return a;
+}
+
+// 128 rows of hd codes on their way to shared memory: a thread has 16 neighbouring codes of every (128 / kPasses)th row.
+template <int HD>
+struct Codes {
+  static constexpr int kChunks = HD / 16, kPasses = kChunks, kStep = 128 / kPasses;
+  uint4 w[kPasses];
+  __device__ __forceinline__ void load(const uint8_t* head, int key0, int last, int idx) {
+    const int c = idx % kChunks, row = idx / kChunks;
+    const uint8_t* const at = head + (long long)(key0 + row) * HD + 16 * c;
+    if (key0 + kKeys - 1 <= last) {
+#pragma unroll
+      for (int i = 0; i < kPasses; ++i) w[i] = *reinterpret_cast<const uint4*>(at + i * kStep * HD);
+    } else {
+#pragma unroll
+      for (int i = 0; i < kPasses; ++i) {  // (behind the last slot: anything, as long as it is read inside the cache; masked as keys, zeros as values)
+        const int over = max(0, key0 + row + i * kStep - last);
+        w[i] = *reinterpret_cast<const uint4*>(at + (i * kStep - over) * HD);
+      }
+    }
+  }
+  // Rows of 64 values, 128 bytes, swizzled as tcgen05.mma expects them; rows from `live` on become zeros.
+  template <bool E4M3>
+  __device__ __forceinline__ void store(uint32_t to, int live, int idx) const {
+    const int c = idx % kChunks, row0 = idx / kChunks, at = (c & 3) * 2, flip = HD == 128 ? c >> 2 : 0;
+#pragma unroll
+    for (int i = 0; i < kPasses; ++i) {
+      const int row = row0 + i * kStep;
+      const uint32_t ws[4] = {w[i].x, w[i].y, w[i].z, w[i].w};
+      uint32_t h[8];
+#pragma unroll
+      for (int n = 0; n < 4; ++n) {
+        const uint32_t b = q8_bias<E4M3>(ws[n]);
+        h[2 * n] = q8_half2<E4M3>(b, false), h[2 * n + 1] = q8_half2<E4M3>(b, true);
+      }
+      if (row >= live)
+#pragma unroll
+        for (int n = 0; n < 8; ++n) h[n] = 0;
+      const uint32_t base = to + (c >> 2) * 16384 + row * 128, x = base + (((at + flip) ^ (row & 7)) << 4), y = base + (((at + 1 - flip) ^ (row & 7)) << 4);
+      // (the lanes of a row write all its eight 16-byte places at once, so that no two meet in a bank)
+      if (flip) {
+        sts128(x, h[4], h[5], h[6], h[7]);
+        sts128(y, h[0], h[1], h[2], h[3]);
+      } else {
+        sts128(x, h[0], h[1], h[2], h[3]);
+        sts128(y, h[4], h[5], h[6], h[7]);
+      }
+    }
+  }
+};
+
+template <bool E4M3, int HD>
+__global__ void __launch_bounds__(kPromptThreads, 1) q8_prompt_kernel(const __grid_constant__ Q8AttnParams p) {
+  extern __shared__ __align__(1024) uint8_t prompt_raw[];
+  __shared__ __align__(16) float factors[4][20];
+  constexpr uint32_t kTile = 128 * HD * 2;
+  const uint32_t base = (smem_u32(prompt_raw) + 1023u) & ~1023u;
+  const uint32_t qs = base, ks = base + 2 * kTile, vs = base + 4 * kTile, bars = base + 6 * kTile;
+  const uint32_t kfull = bars, vfull = bars + 16, kempty = bars + 32, vempty = bars + 48, sfull = bars + 64, pfull = bars + 80, ofull = bars + 96, cfull = bars + 112;
+  uint32_t* const tmem_slot = reinterpret_cast<uint32_t*>(prompt_raw + (bars + 144 - smem_u32(prompt_raw)));
+  volatile int* const abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+  if (threadIdx.x == 0) {
+    *abort_flag = 0;
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(kfull + 8 * i, 4);
+      mbar_init(vfull + 8 * i, 4);
+      mbar_init(kempty + 8 * i, 1);
+      mbar_init(vempty + 8 * i, 1);
+      mbar_init(sfull + 8 * i, 1);
+      mbar_init(pfull + 8 * i, 4);
+      mbar_init(ofull + 8 * i, 1);
+    }
+    for (int i = 0; i < 4; ++i) mbar_init(cfull + 8 * i, 1);
+    mbar_init_fence();
+  }
+  if (warp == 12) tmem_alloc(smem_u32(tmem_slot), 512);
+
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  int keys, k0, n0, n1, lim = 0;
+  float factor = p.scale_log2;
+  const int wg = warp >> 2;
+  {
+    const Place at = place_of(p);
+    const long long start = p.start[at.b], count = p.n_new == nullptr ? p.T : min((long long)p.T, p.n_new[at.b]);
+    const int keys0 = q8_seen_by(p, start, count, at.r0, at.r0 + 128), keys1 = q8_seen_by(p, start, count, at.r0 + 128, at.r0 + 256);
+    keys = max(keys0, keys1);
+    const int share = ((keys + p.ns - 1) / p.ns + kKeys - 1) / kKeys * kKeys, k1 = min(keys, (at.split + 1) * share);
+    k0 = min(keys, at.split * share);
+    n0 = max(0, min(keys0, k1) - k0 + kKeys - 1) / kKeys;
+    n1 = max(0, min(keys1, k1) - k0 + kKeys - 1) / kKeys;
+
+  // ---- a softmax thread's row of q, as fp16
+  const int row_i = (int)threadIdx.x & 127, r = at.r0 + (int)threadIdx.x;
+  if (warp < 8) {
+    const bool live = r < p.rows && r / p.G < count;
+    const int tok = live ? r / p.G : 0;
+    const uint4* const row = reinterpret_cast<const uint4*>(p.q + ((long long)at.b * p.T + tok) * p.ldq + (long long)(at.h * p.G + (live ? r - tok * p.G : 0)) * HD);
+    float mul = 1.f;
+    if (live) lim = q8_seen(start, count, tok, p.c.slots);
+    if (live && p.bf16) {
+      uint32_t most = 0;
+#pragma unroll 4
+      for (int i = 0; i < HD / 8; ++i) {
+        const uint4 x = row[i];
+        const uint32_t ws[4] = {x.x, x.y, x.z, x.w};
+#pragma unroll
+        for (int n = 0; n < 4; ++n) most = max(most, max(ws[n] & 0x7fffu, (ws[n] >> 16) & 0x7fffu));
+      }
+      const int up = q8_row_up(most << 16, 1);
+      mul = __uint_as_float((uint32_t)up << 23);
+      factor *= __uint_as_float((uint32_t)(254 - up) << 23);
+    }
+    const uint32_t to = qs + wg * kTile + row_i * 128;
+#pragma unroll 4
+    for (int i = 0; i < HD / 8; ++i) {
+      const uint4 x = live ? row[i] : make_uint4(0, 0, 0, 0);
+      uint32_t ws[4] = {x.x, x.y, x.z, x.w};
+      if (p.bf16) {
+#pragma unroll
+        for (int n = 0; n < 4; ++n) {
+          const float2 f = q8_up2<true>(ws[n]);
+          ws[n] = pack_half2(f.x * mul, f.y * mul);
+        }
+      }
+      sts128(to + (i >> 3) * 16384 + (((i & 7) ^ (row_i & 7)) << 4), ws[0], ws[1], ws[2], ws[3]);
+    }
+    fence_proxy_async_smem();
+  }
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = *tmem_slot;
+  const int steps = max(n0, n1);
+
+  // (No spills in any of these: what shared memory leaves of L1 does not keep them, and a reload from L2 inside a loop costs more than anything that it saves.)
+  if (warp >= 12) {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kRegsIssue));
+    if (warp == 12 && elect_one()) {
+      const uint32_t id_s = umma_idesc(false, false, false, 128, kKeys), id_o = umma_idesc(false, false, true, 128, HD);
+      auto product_s = [&](int i, int j) {
+        uint32_t q_at = qs + i * kTile;
+        asm volatile("" : "+r"(q_at));  // (sixteen descriptors kept across the loop would be spilled)
+        const uint64_t a = umma_smem_desc(q_at, 16, 1024), k = umma_smem_desc(ks + (j & 1) * kTile, 16, 1024);
+#pragma unroll
+        for (int s = 0; s < HD / 16; ++s) umma_f16(tmem + 128 * i, a + (s >> 2) * 1024 + (s & 3) * 2, k + (s >> 2) * 1024 + (s & 3) * 2, id_s, s != 0);
+        umma_commit(sfull + 8 * i);
+      };
+      auto product_o = [&](int i, int j) {
+        const uint64_t v = umma_smem_desc(vs + (j & 1) * kTile, 16384, 1024);
+#pragma unroll
+        for (int s = 0; s < kKeys / 16; ++s) umma_f16_ts(tmem + 256 + 128 * i, tmem + 128 * i + 8 * s, v + 128 * s, id_o, (j | s) != 0);
+      };
+      bool ok = steps > 0 && mbar_wait(kfull, 0, abort_flag);
+      if (ok) {
+        tc_fence_after();
+        if (n0 > 0) product_s(0, 0);
+        if (n1 > 0) product_s(1, 0);
+        umma_commit(kempty);
+      }
+#pragma unroll 1
+      for (int j = 0; ok && j < steps; ++j) {
+        const uint32_t next = (j + 1) & 1;
+        if (j + 1 < steps && !mbar_wait(kfull + 8 * next, ((j + 1) >> 1) & 1, abort_flag)) { ok = false; break; }
+        if (!mbar_wait(vfull + 8 * (j & 1), (j >> 1) & 1, abort_flag)) { ok = false; break; }
+        // (written out: a loop around the products costs the elected thread hundreds of cycles a step)
+        if (j < n0) {
+          if (!mbar_wait(pfull, j & 1, abort_flag)) { ok = false; break; }
+          tc_fence_after();
+          product_o(0, j);
+          if (j + 1 < n0) product_s(0, j + 1);
+          else umma_commit(ofull);
+        }
+        if (j < n1) {
+          if (!mbar_wait(pfull + 8, j & 1, abort_flag)) { ok = false; break; }
+          tc_fence_after();
+          product_o(1, j);
+          if (j + 1 < n1) product_s(1, j + 1);
+          else umma_commit(ofull + 8);
+        }
+        umma_commit(vempty + 8 * (j & 1));
+        if (j + 1 < steps) umma_commit(kempty + 8 * next);
+      }
+    }
+    __syncwarp();
+  } else if (warp >= 8) {
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kRegsWiden));
+    const int idx = threadIdx.x & 127, last = p.c.slots - 1;
+    const Place at = place_of(p);
+    const uint8_t *const kh = p.c.k + (long long)at.bh * p.c.slots * HD, *const vh = p.c.v + (long long)at.bh * p.c.slots * HD;
+    // the first of these warps also prepares the steps' factors, four steps deep (a step's are free when the S of the step after it is done, and these
+    // warps are two steps ahead of that at most): of 8 groups of 16 keys ks and vs / R, and how R moved
+    const float* const scales = (lane < 8 ? p.c.k_scale : p.c.v_scale) + (long long)at.bh * p.c.n_blocks;
+    auto scale_at = [&](int j) { return scales[min((k0 + j * kKeys + 16 * (lane & 7)) >> p.c.block_log2, p.c.n_blocks - 1)]; };
+    float R = 0.f, inv_R = 0.f, next = warp == 8 && steps > 0 ? scale_at(0) : 0.f;
+    Codes<HD> kc, vc;
+    if (steps > 0) kc.load(kh, k0, last, idx), vc.load(vh, k0, last, idx);
+#pragma unroll 1
+    for (int j = 0; j < steps; ++j) {
+      const uint32_t s = j & 1, parity = ((j >> 1) & 1) ^ 1;
+      if (j >= 2 && !__all_sync(0xffffffffu, mbar_wait(kempty + 8 * s, parity, abort_flag))) break;
+      if (warp == 8) {
+        const float scale = next;
+        if (j + 1 < steps) next = scale_at(j + 1);
+        const float vmax = __uint_as_float(__reduce_max_sync(
+            0xffffffffu, lane >= 8 && k0 + j * kKeys + 16 * (lane & 7) < keys && scale <= 3.4e38f ? __float_as_uint(scale) : 0u));
+        float moved = 1.f;
+        if (vmax > 16.f * R) moved = R / vmax, R = vmax, inv_R = 1.f / vmax;
+        if (lane < 16) factors[j & 3][lane] = lane < 8 ? scale : scale * inv_R;
+        if (lane == 16) factors[j & 3][16] = moved;
+        if (lane == 17) factors[j & 3][17] = R;
+        __syncwarp();
+        if (lane == 0) mbar_arrive(cfull + 8 * (j & 3));
+      }
+      kc.template store<E4M3>(ks + s * kTile, 128, idx);
+      fence_proxy_async_smem();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(kfull + 8 * s);
+      if (j + 1 < steps) kc.load(kh, k0 + (j + 1) * kKeys, last, idx);
+      if (j >= 2 && !__all_sync(0xffffffffu, mbar_wait(vempty + 8 * s, parity, abort_flag))) break;
+      vc.template store<E4M3>(vs + s * kTile, keys - k0 - j * kKeys, idx);  // (slots that nobody wrote may hold anything)
+      fence_proxy_async_smem();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(vfull + 8 * s);
+      if (j + 1 < steps) vc.load(vh, k0 + (j + 1) * kKeys, last, idx);
+    }
+  } else {
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kRegsSoftmax));
+    const int n = wg ? n1 : n0;
+    const uint32_t lanes = (uint32_t)(32 * (warp & 3)) << 16, s_at = tmem + lanes + 128 * wg, o_at = tmem + lanes + 256 + 128 * wg;
+    float m = -INFINITY, l = 0.f, R = 0.f;
+    const int lim_all = __reduce_min_sync(0xffffffffu, lim);
+    bool ok = true;
+#pragma unroll 1
+    for (int j = 0; j < n; ++j) {
+      const int key0 = k0 + j * kKeys;
+      const bool part = key0 + kKeys > lim_all;  // some of the tile is masked for a row of the warp
+      if (!__all_sync(0xffffffffu, mbar_wait(cfull + 8 * (j & 3), (j >> 2) & 1, abort_flag))) { ok = false; break; }
+      const float* const fac = factors[j & 3];
+      float corr = fac[16];
+      const bool wider = corr != 1.f;
+      R = fac[17];
+      if (!__all_sync(0xffffffffu, mbar_wait(sfull + 8 * wg, j & 1, abort_flag))) { ok = false; break; }
+      tc_fence_after();
+      // 32 scores at a time; the next 32 are on their way while these are used
+      uint32_t x[2][32];
+      tmem_ld32(s_at, x[0]);
+#pragma unroll 1
+      for (int c = 0; c < 4; c += 2) {
+#pragma unroll
+        for (int u = 0; u < 2; ++u) {
+          const int cc = c + u;
+          const float2 kf = *reinterpret_cast<const float2*>(fac + 2 * cc), vf = *reinterpret_cast<const float2*>(fac + 8 + 2 * cc);
+          float cg[2] = {kf.x * factor, kf.y * factor}, fg[2] = {vf.x, vf.y};
+          tmem_ld_wait();
+          tmem_ready(x[u]);
+          if (u == 0 || c == 0) tmem_ld32(s_at + 32 * (cc + 1), x[u ^ 1]);
+          if (part) {
+            // masked scores are -inf and their weights 0: a group that is masked as a whole has factors of its own for that (its scales may be NaN), and a
+            // key scale of 0 makes way for a number that its scores vanish under
+            const int left = lim - key0 - 32 * cc;
+#pragma unroll
+            for (int g = 0; g < 2; ++g) {
+              if (16 * g >= left) cg[g] = 1.f, fg[g] = 0.f;
+              if (cg[g] == 0.f) cg[g] = 1e-37f;
+            }
+#pragma unroll
+            for (int i = 0; i < 32; ++i)
+              if (i >= left) x[u][i] = 0xff800000u;
+          }
+          float top[2] = {__uint_as_float(x[u][0]), __uint_as_float(x[u][16])};
+#pragma unroll
+          for (int i = 1; i < 16; ++i) top[0] = fmaxf(top[0], __uint_as_float(x[u][i])), top[1] = fmaxf(top[1], __uint_as_float(x[u][16 + i]));
+          const float mx = fmaxf(top[0] * cg[0], top[1] * cg[1]);
+          if (__any_sync(0xffffffffu, mx > m + 8.f) || (cc == 0 && (wider || j == 0))) {
+            // the maximum moves: what has been summed against the old one follows, P of this tile and O included
+            const float to = fmaxf(m, mx), down = to == -INFINITY ? 1.f : ex2(m - to);
+            m = to;
+            l *= down, corr *= down;
+#pragma unroll 1
+            for (int k = 0; k < cc; ++k) {
+              uint32_t y[16];
+              tmem_ld16(s_at + 16 * k, y);
+              tmem_ld_wait();
+              tmem_regs_ready(y);
+#pragma unroll
+              for (int i = 0; i < 16; ++i) {
+                const float2 f = q8_up2<false>(y[i]);
+                y[i] = pack_half2(f.x * down, f.y * down);
+              }
+              tmem_st16(s_at + 16 * k, y);
+            }
+            if (j > 0) {
+#pragma unroll 1
+              for (int k = 0; k < HD / 16; ++k) {
+                uint32_t o[16];
+                tmem_ld16(o_at + 16 * k, o);
+                tmem_ld_wait();
+                tmem_regs_ready(o);
+#pragma unroll
+                for (int i = 0; i < 16; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * corr);
+                tmem_st16(o_at + 16 * k, o);
+              }
+            }
+            corr = 1.f;
+          }
+          const float mu = m == -INFINITY ? 0.f : m;
+          const uint64_t neg = pair(-mu, -mu);
+          uint64_t sum[2] = {0, 0};
+          uint32_t y[16];
+#pragma unroll
+          for (int g = 0; g < 2; ++g) {
+            const uint64_t c2 = pair(cg[g], cg[g]), f2 = pair(fg[g], fg[g]);
+#pragma unroll
+            for (int i = 16 * g; i < 16 * g + 16; i += 2) {
+              float a, b, v, w;
+              unpair(fma2(pair(__uint_as_float(x[u][i]), __uint_as_float(x[u][i + 1])), c2, neg), a, b);
+              const uint64_t e = pair(ex2(a), ex2(b));
+              sum[g] = add2(sum[g], e);
+              unpair(mul2(e, f2), v, w);
+              y[i / 2] = pack_half2(v, w);
+            }
+          }
+          tmem_st16(s_at + 16 * cc, y);  // (over scores that have been read)
+          float a, b;
+          unpair(add2(sum[0], sum[1]), a, b);
+          l += a + b;
+        }
+      }
+      tmem_st_wait();
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(pfull + 8 * wg);
+    }
+    if (ok && n > 0 && !__all_sync(0xffffffffu, mbar_wait(ofull + 8 * wg, 0, abort_flag))) ok = false;
+    tc_fence_after();
+    const Place at = place_of(p);
+    const int r = at.r0 + (int)threadIdx.x;
+    const bool live = r < p.rows;
+    const float fin = !ok ? CUDART_NAN_F : p.ns > 1 ? R : l == 0.f ? 0.f : R / l;
+    const int tok = live ? r / p.G : 0;
+    uint16_t* const to = p.out + ((long long)at.b * p.T + tok) * p.ldo + (long long)(at.h * p.G + r - tok * p.G) * HD;
+    float* const to32 = p.part + (((long long)at.bh * p.rows + r) * p.ns + at.split) * (HD + 4);
+#pragma unroll 1
+    for (int c = 0; c < HD / 32; ++c) {
+      uint32_t x[32];
+      if (n > 0 && ok) {
+        tmem_ld32(o_at + 32 * c, x);
+        tmem_ld_wait();
+        tmem_ready(x);
+      } else {
+#pragma unroll
+        for (int i = 0; i < 32; ++i) x[i] = 0;
+      }
+      if (!live) continue;
+      if (ok && l == 0.f)  // (a row that sees nothing: zeros, whatever its products were)
+#pragma unroll
+        for (int i = 0; i < 32; ++i) x[i] = 0;
+      if (p.ns > 1) {
+#pragma unroll
+        for (int i = 0; i < 32; i += 4)
+          *reinterpret_cast<float4*>(to32 + 32 * c + i) = make_float4(__uint_as_float(x[i]) * fin, __uint_as_float(x[i + 1]) * fin,
+                                                                      __uint_as_float(x[i + 2]) * fin, __uint_as_float(x[i + 3]) * fin);
+      } else {
+#pragma unroll
+        for (int i = 0; i < 32; i += 8) {
+          uint32_t o[4];
+#pragma unroll
+          for (int z = 0; z < 4; ++z) {
+            const float u = __uint_as_float(x[i + 2 * z]) * fin, v = __uint_as_float(x[i + 2 * z + 1]) * fin;
+            o[z] = p.bf16 ? q8_down2<true>(u, v) : q8_down2<false>(u, v);
+          }
+          *reinterpret_cast<uint4*>(to + 32 * c + i) = make_uint4(o[0], o[1], o[2], o[3]);
+        }
+      }
+    }
+    if (live && p.ns > 1) to32[HD] = m, to32[HD + 1] = ok ? l : CUDART_NAN_F;
+  }
+  tc_fence_before();
+  __syncthreads();
+  if (*abort_flag) {
+    if (threadIdx.x == 0 && p.status) atomicExch(p.status, 1u);
+    for (int i = 0; i < 200; ++i) __nanosleep(1000);  // (products in flight end before their operands' memory is given back)
+  }
+  if (warp == 12) {
+    tc_fence_after();
+    tmem_dealloc(tmem, 512);
+  }
+}
+
+template <bool E4M3, int HD>
+static int launch_prompt(const Q8AttnParams& p, cudaStream_t stream) {
+  static bool configured[64] = {};
+  DeviceInfo di;
+  int rc;
+  if ((rc = device_info(&di))) return rc;
+  const int smem = 6 * 128 * HD * 2 + 1024 + 256 < 120 * 1024 ? 120 * 1024 : 6 * 128 * HD * 2 + 1024 + 256;  // one CTA per SM: a second one would only wait for TMEM
+  if (!configured[di.dev]) {
+    BLR_CUDA_OK(cudaFuncSetAttribute(q8_prompt_kernel<E4M3, HD>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
+    cudaFuncAttributes fa;
+    BLR_CUDA_OK(cudaFuncGetAttributes(&fa, q8_prompt_kernel<E4M3, HD>));
+    BLR_REQUIRE(fa.numRegs == kRegs, BLR_ERR_UNSUPPORTED, "the prompt kernel was built with %d registers, its split is made for %d", fa.numRegs, kRegs);
+    configured[di.dev] = true;
+  }
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((unsigned)((long long)p.n_bh * p.q_tiles * p.ns));
+  cfg.blockDim = dim3(kPromptThreads);
+  cfg.dynamicSmemBytes = (size_t)smem;
+  cfg.stream = stream;
+  cudaLaunchAttribute at[1];
+  at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  at[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = at;
+  cfg.numAttrs = 1;
+  BLR_CUDA_OK(cudaLaunchKernelEx(&cfg, q8_prompt_kernel<E4M3, HD>, p));
+  return BLR_OK;
+}
+
+int q8_launch_prompt(const Q8AttnParams& p, int head_dim, int code, cudaStream_t stream) {
+  if (code == BLR_Q8_E4M3) return head_dim == 128 ? launch_prompt<true, 128>(p, stream) : launch_prompt<true, 64>(p, stream);
+  return head_dim == 128 ? launch_prompt<false, 128>(p, stream) : launch_prompt<false, 64>(p, stream);
+}
+
+}  // namespace blr

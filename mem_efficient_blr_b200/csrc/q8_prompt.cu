@@ -2,7 +2,7 @@
 // token) and walks the keys 128 at a time, warp-specialised:
 //   warps 0-3, 4-7  softmax of rows 0-127 and 128-255, a thread per row: S from TMEM, P back over it as fp16 pairs, O rescaled there when it has to be
 //   warps 8-11      widen the codes of the next keys and values to fp16 (exact) into shared memory, as tcgen05.mma reads them
-//   warp 12         one thread issues the products: S = Q K^T (both from shared memory), O += P V (P from TMEM)
+//   warps 12-15     one thread of the first issues the products: S = Q K^T (both from shared memory), O += P V (P from TMEM)
 // The scales stay out of the products: a group of 16 keys has one for its keys, which multiplies S in the exponent's argument, and one for its values, which
 // multiplies p by vs / R with R the largest of them so far (moved when it is 2^4 behind, like the maximum when it is 2^8 behind; see q8_attention.cu).
 // Order of the products: S0 S1 | PV0 S0 | PV1 S1 | ...: while the tensor cores do one half's PV and its next S, the other half's softmax runs.  P lies over S, so a
@@ -17,7 +17,11 @@
 
 namespace blr {
 
-static constexpr int kPromptThreads = 416, kKeys = 128;
+static constexpr int kPromptThreads = 512, kKeys = 128;
+// Registers of a thread at launch, and of the softmax warps (8), the widening ones (4) and the last four from then on: setmaxnreg waits for ever for registers that
+// the block was not launched with.
+static constexpr int kRegs = 128, kRegsSoftmax = 176, kRegsWiden = 104, kRegsIssue = 56;
+static_assert(8 * kRegsSoftmax + 4 * kRegsWiden + 4 * kRegsIssue <= kPromptThreads / 32 * kRegs, "more registers than the block has");
 
 __device__ __forceinline__ void tmem_ld32(uint32_t taddr, uint32_t (&r)[32]) {
   asm volatile(
@@ -25,6 +29,13 @@ __device__ __forceinline__ void tmem_ld32(uint32_t taddr, uint32_t (&r)[32]) {
       : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]),
         "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]), "=r"(r[16]), "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]),
         "=r"(r[23]), "=r"(r[24]), "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
+      : "r"(taddr)
+      : "memory");
+}
+__device__ __forceinline__ void tmem_ld8(uint32_t taddr, uint32_t (&r)[8]) {  // (with its wait)
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x8.b32 {%0,%1,%2,%3,%4,%5,%6,%7}, [%8];\n\ttcgen05.wait::ld.sync.aligned;"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7])
       : "r"(taddr)
       : "memory");
 }
@@ -43,6 +54,114 @@ __device__ __forceinline__ void sts128(uint32_t addr, uint32_t a, uint32_t b, ui
   asm volatile("st.shared.v4.b32 [%0], {%1,%2,%3,%4};" ::"r"(addr), "r"(a), "r"(b), "r"(c), "r"(d) : "memory");
 }
 
+// Two floats of one 64-bit register: one instruction for both.
+__device__ __forceinline__ uint64_t pair(float a, float b) {
+  uint64_t r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
+  return r;
+}
+__device__ __forceinline__ void unpair(uint64_t v, float& a, float& b) { asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(v)); }
+__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
+  uint64_t r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+  return r;
+}
+__device__ __forceinline__ uint64_t mul2(uint64_t a, uint64_t b) {
+  uint64_t r;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+__device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
+  uint64_t r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+
+// Scores of 128 keys of a thread's row, from TMEM 32 at a time (the next 32 are on their way while these are used).
+__device__ __forceinline__ void mask32(uint32_t (&x)[32], int left) {
+#pragma unroll
+  for (int i = 0; i < 32; ++i)
+    if (i >= left) x[i] = 0xff800000u;
+}
+// The factors of 32 keys.  Masked scores are -inf and their weights 0: a group that is masked as a whole has factors of its own for that (its scales may be NaN), and
+// a key scale of 0 makes way for a number that its scores vanish under.
+__device__ __forceinline__ void factors32(uint32_t fac, int c, float factor, bool part, int left, float (&cg)[2], float (&fg)[2]) {
+  uint32_t k[2], v[2];
+  lds64(fac + 8 * c, k[0], k[1]);
+  lds64(fac + 32 + 8 * c, v[0], v[1]);
+#pragma unroll
+  for (int g = 0; g < 2; ++g) cg[g] = __uint_as_float(k[g]) * factor, fg[g] = __uint_as_float(v[g]);
+  if (part) {
+#pragma unroll
+    for (int g = 0; g < 2; ++g) {
+      if (16 * g >= left) cg[g] = 1.f, fg[g] = 0.f;
+      if (cg[g] == 0.f) cg[g] = 1e-37f;
+    }
+  }
+}
+// The maximum of a row's 128 scores, scaled:
+__device__ __forceinline__ float largest(const uint32_t (&x)[4][32], uint32_t fac, float factor, bool part, int left) {
+  float mx[2] = {-INFINITY, -INFINITY};
+#pragma unroll
+  for (int c = 0; c < 4; ++c) {
+    float cg[2], fg[2];
+    factors32(fac, c, factor, part, left - 32 * c, cg, fg);
+#pragma unroll
+    for (int g = 0; g < 2; ++g) {
+      float top = __uint_as_float(x[c][16 * g]);
+#pragma unroll
+      for (int i = 1; i < 16; ++i) top = fmaxf(top, __uint_as_float(x[c][16 * g + i]));
+      mx[g] = fmaxf(mx[g], top * cg[g]);
+    }
+  }
+  return fmaxf(mx[0], mx[1]);
+}
+// p = 2^(s - mu), and P = p vs / R as fp16 pairs over the scores in TMEM; returns the sum of p.
+__device__ __forceinline__ float weights(uint32_t s_at, const uint32_t (&x)[4][32], uint32_t fac, float factor, float mu, bool part, int left) {
+  uint64_t sum[2] = {0, 0};
+  const uint64_t neg = pair(-mu, -mu);
+#pragma unroll
+  for (int c = 0; c < 4; ++c) {
+    float cg[2], fg[2];
+    uint32_t y[16];
+    factors32(fac, c, factor, part, left - 32 * c, cg, fg);
+#pragma unroll
+    for (int g = 0; g < 2; ++g) {
+      const uint64_t c2 = pair(cg[g], cg[g]), f2 = pair(fg[g], fg[g]);
+#pragma unroll
+      for (int i = 16 * g; i < 16 * g + 16; i += 2) {
+        float a, b, v, w;
+        unpair(fma2(pair(__uint_as_float(x[c][i]), __uint_as_float(x[c][i + 1])), c2, neg), a, b);
+        const uint64_t e = pair(ex2(a), ex2(b));
+        sum[g] = add2(sum[g], e);
+        unpair(mul2(e, f2), v, w);
+        y[i / 2] = pack_half2(v, w);
+      }
+    }
+    tmem_st16(s_at + 16 * c, y);
+  }
+  float a, b;
+  unpair(add2(sum[0], sum[1]), a, b);
+  return a + b;
+}
+
+// What a CTA works on.  (Asked for anew where it is needed: kept in registers across the loops it would push others out of them.)
+struct Place {
+  int split, bh, b, h, r0;
+};
+__device__ __forceinline__ Place place_of(const Q8AttnParams& p) {
+  int cta;
+  asm volatile("mov.u32 %0, %%ctaid.x;" : "=r"(cta));
+  Place a;
+  const int tile = cta / p.ns;
+  a.split = cta - tile * p.ns;
+  a.bh = tile % p.n_bh;
+  a.r0 = (p.q_tiles - 1 - tile / p.n_bh) * kQ8PromptRows;  // the last rows have the most keys: their CTAs come first
+  a.b = a.bh / p.c.kv_heads;
+  a.h = a.bh - a.b * p.c.kv_heads;
+  return a;
+}
+
 // 128 rows of hd codes on their way to shared memory: a thread has 16 neighbouring codes of every (128 / kPasses)th row.
 template <int HD>
 struct Codes {
@@ -50,8 +169,17 @@ struct Codes {
   uint4 w[kPasses];
   __device__ __forceinline__ void load(const uint8_t* head, int key0, int last, int idx) {
     const int c = idx % kChunks, row = idx / kChunks;
+    const uint8_t* const at = head + (long long)(key0 + row) * HD + 16 * c;
+    if (key0 + kKeys - 1 <= last) {
 #pragma unroll
-    for (int i = 0; i < kPasses; ++i) w[i] = *reinterpret_cast<const uint4*>(head + (long long)min(key0 + row + i * kStep, last) * HD + 16 * c);
+      for (int i = 0; i < kPasses; ++i) w[i] = *reinterpret_cast<const uint4*>(at + i * kStep * HD);
+    } else {
+#pragma unroll
+      for (int i = 0; i < kPasses; ++i) {  // (behind the last slot: anything, as long as it is read inside the cache; masked as keys, zeros as values)
+        const int over = max(0, key0 + row + i * kStep - last);
+        w[i] = *reinterpret_cast<const uint4*>(at + (i * kStep - over) * HD);
+      }
+    }
   }
   // Rows of 64 values, 128 bytes, swizzled as tcgen05.mma expects them; rows from `live` on become zeros.
   template <bool E4M3>
@@ -86,12 +214,14 @@ struct Codes {
 template <bool E4M3, int HD>
 __global__ void __launch_bounds__(kPromptThreads, 1) q8_prompt_kernel(const __grid_constant__ Q8AttnParams p) {
   extern __shared__ __align__(1024) uint8_t prompt_raw[];
+  __shared__ __align__(16) float factors[4][20];
   constexpr uint32_t kTile = 128 * HD * 2;
   const uint32_t base = (smem_u32(prompt_raw) + 1023u) & ~1023u;
   const uint32_t qs = base, ks = base + 2 * kTile, vs = base + 4 * kTile, bars = base + 6 * kTile;
-  const uint32_t kfull = bars, vfull = bars + 16, kempty = bars + 32, vempty = bars + 48, sfull = bars + 64, pfull = bars + 80, ofull = bars + 96;
-  uint32_t* const tmem_slot = reinterpret_cast<uint32_t*>(prompt_raw + (bars + 112 - smem_u32(prompt_raw)));
-  volatile int* const abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
+  const uint32_t kfull = bars, vfull = bars + 16, kempty = bars + 32, vempty = bars + 48, sfull = bars + 64, pfull = bars + 80, ofull = bars + 96, cfull = bars + 112;
+  __shared__ uint32_t tmem_slot;
+  __shared__ volatile int aborted;
+  volatile int* const abort_flag = &aborted;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   if (threadIdx.x == 0) {
@@ -105,57 +235,51 @@ __global__ void __launch_bounds__(kPromptThreads, 1) q8_prompt_kernel(const __gr
       mbar_init(pfull + 8 * i, 4);
       mbar_init(ofull + 8 * i, 1);
     }
+    for (int i = 0; i < 4; ++i) mbar_init(cfull + 8 * i, 1);
     mbar_init_fence();
   }
-  if (warp == 12) tmem_alloc(smem_u32(tmem_slot), 512);
+  if (warp == 12) tmem_alloc(smem_u32(&tmem_slot), 512);
 
-  // the last rows have the most keys: their CTAs come first
-  const int split = blockIdx.x % p.ns, tile = blockIdx.x / p.ns, bh = tile % p.n_bh, r0 = (p.q_tiles - 1 - tile / p.n_bh) * kQ8PromptRows;
-  const int b = bh / p.c.kv_heads, h = bh - b * p.c.kv_heads;
   asm volatile("griddepcontrol.wait;" ::: "memory");
-  const long long start = p.start[b], count = p.n_new == nullptr ? p.T : min((long long)p.T, p.n_new[b]);
-  const int keys0 = q8_seen_by(p, start, count, r0, r0 + 128), keys1 = q8_seen_by(p, start, count, r0 + 128, r0 + 256), keys = max(keys0, keys1);
-  const int share = ((keys + p.ns - 1) / p.ns + kKeys - 1) / kKeys * kKeys, k0 = min(keys, split * share), k1 = min(keys, k0 + share);
-  auto steps_of = [&](int seen) { return max(0, min(seen, k1) - k0 + kKeys - 1) / kKeys; };
-  const int n0 = steps_of(keys0), n1 = steps_of(keys1), steps = max(n0, n1);
-  const long long head = (long long)bh * p.c.slots * HD;
+  int keys, k0, n0, n1, lim = 0;
+  float factor = p.scale_log2;
+  const int wg = warp >> 2;
+  {
+    const Place at = place_of(p);
+    const long long start = p.start[at.b], count = p.n_new == nullptr ? p.T : min((long long)p.T, p.n_new[at.b]);
+    const int keys0 = q8_seen_by(p, start, count, at.r0, at.r0 + 128), keys1 = q8_seen_by(p, start, count, at.r0 + 128, at.r0 + 256);
+    keys = max(keys0, keys1);
+    const int share = ((keys + p.ns - 1) / p.ns + kKeys - 1) / kKeys * kKeys, k1 = min(keys, (at.split + 1) * share);
+    k0 = min(keys, at.split * share);
+    n0 = max(0, min(keys0, k1) - k0 + kKeys - 1) / kKeys;
+    n1 = max(0, min(keys1, k1) - k0 + kKeys - 1) / kKeys;
 
   // ---- a softmax thread's row of q, as fp16
-  const int wg = warp >> 2, r = r0 + (int)threadIdx.x;
-  float factor = 0.f;
-  int lim = 0;
+  const int row_i = (int)threadIdx.x & 127, r = at.r0 + (int)threadIdx.x;
   if (warp < 8) {
-    uint4 x[HD / 8];
-    uint32_t most = 0;
     const bool live = r < p.rows && r / p.G < count;
-    if (live) {
-      const int tok = r / p.G;
-      const uint4* row = reinterpret_cast<const uint4*>(p.q + ((long long)b * p.T + tok) * p.ldq + (long long)(h * p.G + r - tok * p.G) * HD);
-#pragma unroll
-      for (int i = 0; i < HD / 8; ++i) x[i] = row[i];
-      lim = q8_seen(start, count, tok, p.c.slots);
-    } else {
-#pragma unroll
-      for (int i = 0; i < HD / 8; ++i) x[i] = make_uint4(0, 0, 0, 0);
-    }
+    const int tok = live ? r / p.G : 0;
+    const uint4* const row = reinterpret_cast<const uint4*>(p.q + ((long long)at.b * p.T + tok) * p.ldq + (long long)(at.h * p.G + (live ? r - tok * p.G : 0)) * HD);
     float mul = 1.f;
-    if (p.bf16) {
-#pragma unroll
+    if (live) lim = q8_seen(start, count, tok, p.c.slots);
+    if (live && p.bf16) {
+      uint32_t most = 0;
+#pragma unroll 4
       for (int i = 0; i < HD / 8; ++i) {
-        const uint32_t ws[4] = {x[i].x, x[i].y, x[i].z, x[i].w};
+        const uint4 x = row[i];
+        const uint32_t ws[4] = {x.x, x.y, x.z, x.w};
 #pragma unroll
         for (int n = 0; n < 4; ++n) most = max(most, max(ws[n] & 0x7fffu, (ws[n] >> 16) & 0x7fffu));
       }
       const int up = q8_row_up(most << 16, 1);
       mul = __uint_as_float((uint32_t)up << 23);
-      factor = __uint_as_float((uint32_t)(254 - up) << 23) * p.scale_log2;
-    } else {
-      factor = p.scale_log2;
+      factor *= __uint_as_float((uint32_t)(254 - up) << 23);
     }
-    const uint32_t to = qs + wg * kTile + (threadIdx.x & 127) * 128;
-#pragma unroll
+    const uint32_t to = qs + wg * kTile + row_i * 128;
+#pragma unroll 4
     for (int i = 0; i < HD / 8; ++i) {
-      uint32_t ws[4] = {x[i].x, x[i].y, x[i].z, x[i].w};
+      const uint4 x = live ? row[i] : make_uint4(0, 0, 0, 0);
+      uint32_t ws[4] = {x.x, x.y, x.z, x.w};
       if (p.bf16) {
 #pragma unroll
         for (int n = 0; n < 4; ++n) {
@@ -163,20 +287,26 @@ __global__ void __launch_bounds__(kPromptThreads, 1) q8_prompt_kernel(const __gr
           ws[n] = pack_half2(f.x * mul, f.y * mul);
         }
       }
-      sts128(to + (i >> 3) * 16384 + (((i & 7) ^ (threadIdx.x & 7)) << 4), ws[0], ws[1], ws[2], ws[3]);
+      sts128(to + (i >> 3) * 16384 + (((i & 7) ^ (row_i & 7)) << 4), ws[0], ws[1], ws[2], ws[3]);
     }
     fence_proxy_async_smem();
+  }
   }
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
-  const uint32_t tmem = *tmem_slot;
+  const uint32_t tmem = tmem_slot;
+  const int steps = max(n0, n1);
 
-  if (warp == 12) {
-    if (elect_one()) {
+  // (No spills in any of these: what shared memory leaves of L1 does not keep them, and a reload from L2 inside a loop costs more than anything that it saves.)
+  if (warp >= 12) {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kRegsIssue));
+    if (warp == 12 && elect_one()) {
       const uint32_t id_s = umma_idesc(false, false, false, 128, kKeys), id_o = umma_idesc(false, false, true, 128, HD);
       auto product_s = [&](int i, int j) {
-        const uint64_t a = umma_smem_desc(qs + i * kTile, 16, 1024), k = umma_smem_desc(ks + (j & 1) * kTile, 16, 1024);
+        uint32_t q_at = qs + i * kTile;
+        asm volatile("" : "+r"(q_at));  // (sixteen descriptors kept across the loop would be spilled)
+        const uint64_t a = umma_smem_desc(q_at, 16, 1024), k = umma_smem_desc(ks + (j & 1) * kTile, 16, 1024);
 #pragma unroll
         for (int s = 0; s < HD / 16; ++s) umma_f16(tmem + 128 * i, a + (s >> 2) * 1024 + (s & 3) * 2, k + (s >> 2) * 1024 + (s & 3) * 2, id_s, s != 0);
         umma_commit(sfull + 8 * i);
@@ -198,31 +328,55 @@ __global__ void __launch_bounds__(kPromptThreads, 1) q8_prompt_kernel(const __gr
         const uint32_t next = (j + 1) & 1;
         if (j + 1 < steps && !mbar_wait(kfull + 8 * next, ((j + 1) >> 1) & 1, abort_flag)) { ok = false; break; }
         if (!mbar_wait(vfull + 8 * (j & 1), (j >> 1) & 1, abort_flag)) { ok = false; break; }
-#pragma unroll 1
-        for (int i = 0; i < 2; ++i) {
-          const int n = i ? n1 : n0;
-          if (j >= n) continue;
-          if (!mbar_wait(pfull + 8 * i, j & 1, abort_flag)) { ok = false; break; }
+        // (written out: a loop around the products costs the elected thread hundreds of cycles a step)
+        if (j < n0) {
+          if (!mbar_wait(pfull, j & 1, abort_flag)) { ok = false; break; }
           tc_fence_after();
-          product_o(i, j);
-          if (j + 1 < n) product_s(i, j + 1);
-          else umma_commit(ofull + 8 * i);
+          product_o(0, j);
+          if (j + 1 < n0) product_s(0, j + 1);
+          else umma_commit(ofull);
         }
-        if (!ok) break;
+        if (j < n1) {
+          if (!mbar_wait(pfull + 8, j & 1, abort_flag)) { ok = false; break; }
+          tc_fence_after();
+          product_o(1, j);
+          if (j + 1 < n1) product_s(1, j + 1);
+          else umma_commit(ofull + 8);
+        }
         umma_commit(vempty + 8 * (j & 1));
         if (j + 1 < steps) umma_commit(kempty + 8 * next);
       }
     }
     __syncwarp();
   } else if (warp >= 8) {
-    const int idx = threadIdx.x - 256, last = p.c.slots - 1;
-    const uint8_t *kh = p.c.k + head, *vh = p.c.v + head;
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kRegsWiden));
+    const int idx = threadIdx.x & 127, last = p.c.slots - 1;
+    const Place at = place_of(p);
+    const uint8_t *const kh = p.c.k + (long long)at.bh * p.c.slots * HD, *const vh = p.c.v + (long long)at.bh * p.c.slots * HD;
+    // the first of these warps also prepares the steps' factors, four steps deep (a step's are free when the S of the step after it is done, and these
+    // warps are two steps ahead of that at most): of 8 groups of 16 keys ks and vs / R, and how R moved
+    const float* const scales = (lane < 8 ? p.c.k_scale : p.c.v_scale) + (long long)at.bh * p.c.n_blocks;
+    auto scale_at = [&](int j) { return scales[min((k0 + j * kKeys + 16 * (lane & 7)) >> p.c.block_log2, p.c.n_blocks - 1)]; };
+    float R = 0.f, inv_R = 0.f, next = warp == 8 && steps > 0 ? scale_at(0) : 0.f;
     Codes<HD> kc, vc;
     if (steps > 0) kc.load(kh, k0, last, idx), vc.load(vh, k0, last, idx);
 #pragma unroll 1
     for (int j = 0; j < steps; ++j) {
       const uint32_t s = j & 1, parity = ((j >> 1) & 1) ^ 1;
       if (j >= 2 && !__all_sync(0xffffffffu, mbar_wait(kempty + 8 * s, parity, abort_flag))) break;
+      if (warp == 8) {
+        const float scale = next;
+        if (j + 1 < steps) next = scale_at(j + 1);
+        const float vmax = __uint_as_float(__reduce_max_sync(
+            0xffffffffu, lane >= 8 && k0 + j * kKeys + 16 * (lane & 7) < keys && scale <= 3.4e38f ? __float_as_uint(scale) : 0u));
+        float moved = 1.f;
+        if (vmax > 16.f * R) moved = R / vmax, R = vmax, inv_R = 1.f / vmax;
+        if (lane < 16) factors[j & 3][lane] = lane < 8 ? scale : scale * inv_R;
+        if (lane == 16) factors[j & 3][16] = moved;
+        if (lane == 17) factors[j & 3][17] = R;
+        __syncwarp();
+        if (lane == 0) mbar_arrive(cfull + 8 * (j & 3));
+      }
       kc.template store<E4M3>(ks + s * kTile, 128, idx);
       fence_proxy_async_smem();
       __syncwarp();
@@ -236,88 +390,52 @@ __global__ void __launch_bounds__(kPromptThreads, 1) q8_prompt_kernel(const __gr
       if (j + 1 < steps) vc.load(vh, k0 + (j + 1) * kKeys, last, idx);
     }
   } else {
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kRegsSoftmax));
     const int n = wg ? n1 : n0;
     const uint32_t lanes = (uint32_t)(32 * (warp & 3)) << 16, s_at = tmem + lanes + 128 * wg, o_at = tmem + lanes + 256 + 128 * wg;
-    const float* const scales = (lane < 8 ? p.c.k_scale : p.c.v_scale) + (long long)bh * p.c.n_blocks;
-    float m = -INFINITY, l = 0.f, R = 0.f, inv_R = 0.f;
+    float m = -INFINITY, l = 0.f, R = 0.f;
+    const int lim_all = __reduce_min_sync(0xffffffffu, lim);
     bool ok = true;
 #pragma unroll 1
     for (int j = 0; j < n; ++j) {
-      const int key0 = k0 + j * kKeys, mine = key0 + 16 * (lane & 7);
-      const float scale = scales[min(mine >> p.c.block_log2, p.c.n_blocks - 1)];  // lanes 0-7: of the tile's groups of 16 keys, 8-15: of their values
-      const uint32_t vmax_bits = __reduce_max_sync(0xffffffffu, lane >= 8 && mine < keys && scale <= 3.4e38f ? __float_as_uint(scale) : 0u);
-      const float vmax = __uint_as_float(vmax_bits);
-      const bool part = key0 + kKeys > lim;  // some of the tile is masked
+      const int key0 = k0 + j * kKeys;
+      const bool part = key0 + kKeys > lim_all;  // some of the tile is masked for a row of the warp
+      if (!__all_sync(0xffffffffu, mbar_wait(cfull + 8 * (j & 3), (j >> 2) & 1, abort_flag))) { ok = false; break; }
+      const uint32_t fac = smem_u32(factors[j & 3]);
+      uint32_t vr[2];
+      lds64(fac + 64, vr[0], vr[1]);
+      float corr = __uint_as_float(vr[0]);
+      R = __uint_as_float(vr[1]);
       if (!__all_sync(0xffffffffu, mbar_wait(sfull + 8 * wg, j & 1, abort_flag))) { ok = false; break; }
       tc_fence_after();
-      float mx = -INFINITY;
+      uint32_t x[4][32];
 #pragma unroll
-      for (int c = 0; c < 4; ++c) {
-        uint32_t x[32];
-        tmem_ld32(s_at + 32 * c, x);
-        tmem_ld_wait();
-        tmem_ready(x);
+      for (int c = 0; c < 4; ++c) tmem_ld32(s_at + 32 * c, x[c]);
+      tmem_ld_wait();
 #pragma unroll
-        for (int g = 0; g < 2; ++g) {
-          float most = -INFINITY;
-          if (part) {
+      for (int c = 0; c < 4; ++c) tmem_ready(x[c]);
+      if (part) {
 #pragma unroll
-            for (int i = 0; i < 16; ++i) most = fmaxf(most, key0 + 32 * c + 16 * g + i < lim ? __uint_as_float(x[16 * g + i]) : -INFINITY);
-          } else {
-#pragma unroll
-            for (int i = 0; i < 16; ++i) most = fmaxf(most, __uint_as_float(x[16 * g + i]));
-          }
-          const float cg = __shfl_sync(0xffffffffu, scale, 2 * c + g) * factor;
-          if (most != -INFINITY) mx = fmaxf(mx, most * cg);
-        }
+        for (int c = 0; c < 4; ++c) mask32(x[c], lim - key0 - 32 * c);
       }
-      const bool wider = vmax > 16.f * R;
-      if (__any_sync(0xffffffffu, mx > m + 8.f) || wider) {
-        const float to = fmaxf(m, mx);
-        float corr = to == -INFINITY ? 1.f : ex2(m - to);
+      const float mx = largest(x, fac, factor, part, lim - key0);
+      if (__any_sync(0xffffffffu, mx > m + 8.f) || corr != 1.f) {
+        // the maximum moves: what has been summed against the old one follows
+        const float to = fmaxf(m, mx), down = to == -INFINITY ? 1.f : ex2(m - to);
         m = to;
-        l *= corr;
-        if (wider) corr *= R / vmax, R = vmax, inv_R = 1.f / vmax;
+        l *= down, corr *= down;
         if (j > 0) {
 #pragma unroll 1
-          for (int c = 0; c < HD / 32; ++c) {
-            uint32_t x[32];
-            tmem_ld32(o_at + 32 * c, x);
-            tmem_ld_wait();
-            tmem_ready(x);
-            uint32_t y[2][16];
+          for (int k = 0; k < HD / 8; ++k) {
+            uint32_t o[8];
+            tmem_ld8(o_at + 8 * k, o);
 #pragma unroll
-            for (int i = 0; i < 32; ++i) y[i >> 4][i & 15] = __float_as_uint(__uint_as_float(x[i]) * corr);
-            tmem_st16(o_at + 32 * c, y[0]);
-            tmem_st16(o_at + 32 * c + 16, y[1]);
+            for (int i = 0; i < 8; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * corr);
+            tmem_st8(o_at + 8 * k, o);
           }
         }
       }
-      const float mu = m == -INFINITY ? 0.f : m;
-#pragma unroll
-      for (int c = 0; c < 4; ++c) {
-        uint32_t x[32], y[16];
-        tmem_ld32(s_at + 32 * c, x);
-        tmem_ld_wait();
-        tmem_ready(x);
-#pragma unroll
-        for (int g = 0; g < 2; ++g) {
-          const float cg = __shfl_sync(0xffffffffu, scale, 2 * c + g) * factor, fg = __shfl_sync(0xffffffffu, scale, 8 + 2 * c + g) * inv_R;
-#pragma unroll
-          for (int i = 0; i < 16; i += 2) {
-            float e[2];
-#pragma unroll
-            for (int z = 0; z < 2; ++z) {
-              float v = ex2(fmaf(__uint_as_float(x[16 * g + i + z]), cg, -mu));
-              e[z] = v * fg;
-              if (part && key0 + 32 * c + 16 * g + i + z >= lim) v = e[z] = 0.f;  // (whatever lies there, a NaN or its scale's)
-              l += v;
-            }
-            y[8 * g + i / 2] = pack_half2(e[0], e[1]);
-          }
-        }
-        tmem_st16(s_at + 16 * c, y);  // (over scores that have been read)
-      }
+      l += weights(s_at, x, fac, factor, m == -INFINITY ? 0.f : m, part, lim - key0);
       tmem_st_wait();
       tc_fence_before();
       __syncwarp();
@@ -325,11 +443,13 @@ __global__ void __launch_bounds__(kPromptThreads, 1) q8_prompt_kernel(const __gr
     }
     if (ok && n > 0 && !__all_sync(0xffffffffu, mbar_wait(ofull + 8 * wg, 0, abort_flag))) ok = false;
     tc_fence_after();
+    const Place at = place_of(p);
+    const int r = at.r0 + (int)threadIdx.x;
     const bool live = r < p.rows;
     const float fin = !ok ? CUDART_NAN_F : p.ns > 1 ? R : l == 0.f ? 0.f : R / l;
     const int tok = live ? r / p.G : 0;
-    uint16_t* const to = p.out + ((long long)b * p.T + tok) * p.ldo + (long long)(h * p.G + r - tok * p.G) * HD;
-    float* const to32 = p.part + (((long long)bh * p.rows + r) * p.ns + split) * (HD + 4);
+    uint16_t* const to = p.out + ((long long)at.b * p.T + tok) * p.ldo + (long long)(at.h * p.G + r - tok * p.G) * HD;
+    float* const to32 = p.part + (((long long)at.bh * p.rows + r) * p.ns + at.split) * (HD + 4);
 #pragma unroll 1
     for (int c = 0; c < HD / 32; ++c) {
       uint32_t x[32];
@@ -383,13 +503,14 @@ static int launch_prompt(const Q8AttnParams& p, cudaStream_t stream) {
   DeviceInfo di;
   int rc;
   if ((rc = device_info(&di))) return rc;
+  const int smem = 6 * 128 * HD * 2 + 1024 + 256 < 120 * 1024 ? 120 * 1024 : 6 * 128 * HD * 2 + 1024 + 256;  // one CTA per SM: a second one would only wait for TMEM
   if (!configured[di.dev]) {
-    BLR_CUDA_OK(cudaFuncSetAttribute(q8_prompt_kernel<E4M3, HD>, cudaFuncAttributeMaxDynamicSharedMemorySize, di.max_smem_optin));
+    BLR_CUDA_OK(cudaFuncSetAttribute(q8_prompt_kernel<E4M3, HD>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
+    cudaFuncAttributes fa;
+    BLR_CUDA_OK(cudaFuncGetAttributes(&fa, q8_prompt_kernel<E4M3, HD>));
+    BLR_REQUIRE(fa.numRegs == kRegs, BLR_ERR_UNSUPPORTED, "the prompt kernel was built with %d registers, its split is made for %d", fa.numRegs, kRegs);
     configured[di.dev] = true;
   }
-  int smem = 6 * 128 * HD * 2 + 1024 + 256;
-  if (smem < 120 * 1024) smem = 120 * 1024;  // one CTA per SM: a second one would only wait for TMEM
-  BLR_REQUIRE(smem <= di.max_smem_optin, BLR_ERR_UNSUPPORTED, "device offers %d bytes of shared memory", di.max_smem_optin);
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3((unsigned)((long long)p.n_bh * p.q_tiles * p.ns));
   cfg.blockDim = dim3(kPromptThreads);
