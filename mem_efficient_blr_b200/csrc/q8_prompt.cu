@@ -145,6 +145,23 @@ __device__ __forceinline__ float weights(uint32_t s_at, const uint32_t (&x)[4][3
   return a + b;
 }
 
+// mbar_wait for the one thread that everything waits for: asking again and again, where a suspended try_wait has answered a thousand cycles late.
+__device__ __forceinline__ bool mbar_poll(uint32_t bar, uint32_t parity, volatile int* abort_flag) {
+  if (mbar_test_wait(bar, parity)) return true;
+  const long long t0 = clock64();
+  uint32_t spins = 0;
+  while (!mbar_test_wait(bar, parity)) {
+    if ((++spins & 0xff) == 0) {
+      if (*abort_flag) return false;
+      if (clock64() - t0 > kWaitBudgetCycles) {
+        *abort_flag = 1;
+        return false;
+      }
+    }
+  }
+  return true;
+}
+
 // What a CTA works on.  (Asked for anew where it is needed: kept in registers across the loops it would push others out of them.)
 struct Place {
   int split, bh, b, h, r0;
@@ -316,7 +333,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1) q8_prompt_kernel(const __gr
 #pragma unroll
         for (int s = 0; s < kKeys / 16; ++s) umma_f16_ts(tmem + 256 + 128 * i, tmem + 128 * i + 8 * s, v + 128 * s, id_o, (j | s) != 0);
       };
-      bool ok = steps > 0 && mbar_wait(kfull, 0, abort_flag);
+      bool ok = steps > 0 && mbar_poll(kfull, 0, abort_flag);
       if (ok) {
         tc_fence_after();
         if (n0 > 0) product_s(0, 0);
@@ -325,26 +342,27 @@ __global__ void __launch_bounds__(kPromptThreads, 1) q8_prompt_kernel(const __gr
       }
 #pragma unroll 1
       for (int j = 0; ok && j < steps; ++j) {
-        const uint32_t next = (j + 1) & 1;
-        if (j + 1 < steps && !mbar_wait(kfull + 8 * next, ((j + 1) >> 1) & 1, abort_flag)) { ok = false; break; }
-        if (!mbar_wait(vfull + 8 * (j & 1), (j >> 1) & 1, abort_flag)) { ok = false; break; }
+        const uint32_t s = j & 1;
         // (written out: a loop around the products costs the elected thread hundreds of cycles a step)
+        if (!mbar_poll(vfull + 8 * s, (j >> 1) & 1, abort_flag)) { ok = false; break; }
         if (j < n0) {
-          if (!mbar_wait(pfull, j & 1, abort_flag)) { ok = false; break; }
+          if (!mbar_poll(pfull, j & 1, abort_flag)) { ok = false; break; }
           tc_fence_after();
           product_o(0, j);
-          if (j + 1 < n0) product_s(0, j + 1);
-          else umma_commit(ofull);
+          if (j + 1 >= n0) umma_commit(ofull);
         }
+        if (j + 1 < steps && !mbar_poll(kfull + 8 * (s ^ 1), ((j + 1) >> 1) & 1, abort_flag)) { ok = false; break; }
+        tc_fence_after();
+        if (j + 1 < n0) product_s(0, j + 1);
         if (j < n1) {
-          if (!mbar_wait(pfull + 8, j & 1, abort_flag)) { ok = false; break; }
+          if (!mbar_poll(pfull + 8, j & 1, abort_flag)) { ok = false; break; }
           tc_fence_after();
           product_o(1, j);
-          if (j + 1 < n1) product_s(1, j + 1);
-          else umma_commit(ofull + 8);
+          if (j + 1 >= n1) umma_commit(ofull + 8);
         }
-        umma_commit(vempty + 8 * (j & 1));
-        if (j + 1 < steps) umma_commit(kempty + 8 * next);
+        umma_commit(vempty + 8 * s);
+        if (j + 1 < n1) product_s(1, j + 1);
+        if (j + 1 < steps) umma_commit(kempty + 8 * (s ^ 1));
       }
     }
     __syncwarp();
