@@ -1,22 +1,26 @@
 // Log probabilities of given tokens, entropy and likeliest tokens of rows of logits.
 //   M = max x,  S = sum e^(x - M),  log p(i) = (x_i - M) - log S,  H = log S - (sum e^(x - M) (x - M)) / S
-// Sums are fp32.  Order of the likeliest: falling value (NaN above everything, -0 equal to 0), ties by rising id.
+// Differences, exponentials and sums are fp32 (x - M is taken before it is scaled for ex2: M log2 e rounded once would be off by 2^-8 for logits of 10^4).
+// Order of the likeliest: falling value (NaN above everything, -0 equal to 0), ties by rising id.
+//
+// A cluster of 1 to 8 CTAs takes a row: each reads its part once into shared memory, keeping the maximum of what every thread reads, and works from there.
+// The smallest of the maxima of as many groups of threads as tokens are asked for is a number that at least so many values reach: only values that reach it
+// (some tens) are kept and ordered.  A list that overflows (rows of equal values) is made by one search for each token instead.
+// Bound by HBM (each logit once), closely followed by ex2 (16 a cycle and SM).
+#include <cooperative_groups.h>
 #include <math_constants.h>
 
 #include "../../include/blr_b200.h"
 #include "q8.cuh"
 #include "tmap.h"
 
+namespace cg = cooperative_groups;
+
 namespace blr {
 
-static constexpr int kLpThreads = 256, kLpMaxTop = 64;
+static constexpr int kLpThreads = 256, kLpWarps = kLpThreads / 32, kLpMaxTop = 64, kLpKept = 1024, kLpMaxPart = 200 * 1024;
+typedef unsigned long long Ranked;  // order_of(value) << 32 | ~id: larger is likelier
 
-template <int KIND>
-__device__ __forceinline__ float logit(const void* row, long long i) {
-  if constexpr (KIND == 0) return __half2float(static_cast<const __half*>(row)[i]);
-  else if constexpr (KIND == 1) return __bfloat162float(static_cast<const __nv_bfloat16*>(row)[i]);
-  else return static_cast<const float*>(row)[i];
-}
 // Whole numbers in the order of the values; 0 is below all of them.
 __device__ __forceinline__ uint32_t order_of(float x) {
   const uint32_t b = __float_as_uint(x + 0.f);
@@ -25,77 +29,280 @@ __device__ __forceinline__ uint32_t order_of(float x) {
 __device__ __forceinline__ float value_of(uint32_t o) {
   return __uint_as_float(o == 0xffffffffu ? 0x7fffffffu : o & 0x80000000u ? o & 0x7fffffffu : ~o);
 }
+__device__ __forceinline__ Ranked ranked(float x, int id) { return (Ranked)order_of(x) << 32 | (0xffffffffu - (uint32_t)id); }
+
+// 16 bytes of logits: kPer values.
+template <int KIND>
+struct Vec {
+  static constexpr int kPer = KIND == 2 ? 4 : 8;
+  __device__ __forceinline__ static void floats(const uint4& w, float (&f)[kPer]) {
+    const uint32_t ws[4] = {w.x, w.y, w.z, w.w};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      if constexpr (KIND == 2) {
+        f[i] = __uint_as_float(ws[i]);
+      } else {
+        const float2 v = q8_up2<KIND == 1>(ws[i]);
+        f[2 * i] = v.x, f[2 * i + 1] = v.y;
+      }
+    }
+  }
+  // the largest of them, a NaN before anything else
+  __device__ __forceinline__ static float most(const uint4& w) {
+    if constexpr (KIND == 2) {
+      const float a = __uint_as_float(w.x), b = __uint_as_float(w.y), c = __uint_as_float(w.z), d = __uint_as_float(w.w);
+      float r;
+      asm("{\n\t.reg .f32 t;\n\tmax.NaN.f32 t, %1, %2;\n\tmax.NaN.f32 t, t, %3;\n\tmax.NaN.f32 %0, t, %4;\n\t}" : "=f"(r) : "f"(a), "f"(b), "f"(c), "f"(d));
+      return r;
+    } else if constexpr (KIND == 1) {
+      const __nv_bfloat162* h = reinterpret_cast<const __nv_bfloat162*>(&w);
+      const __nv_bfloat162 m = __hmax2_nan(__hmax2_nan(h[0], h[1]), __hmax2_nan(h[2], h[3]));
+      return __bfloat162float(__hmax_nan(m.x, m.y));
+    } else {
+      const __half2* h = reinterpret_cast<const __half2*>(&w);
+      const __half2 m = __hmax2_nan(__hmax2_nan(h[0], h[1]), __hmax2_nan(h[2], h[3]));
+      return __half2float(__hmax_nan(m.x, m.y));
+    }
+  }
+};
+template <int KIND>
+__device__ __forceinline__ float logit(const void* row, long long i) {
+  if constexpr (KIND == 0) return __half2float(static_cast<const __half*>(row)[i]);
+  else if constexpr (KIND == 1) return __bfloat162float(static_cast<const __nv_bfloat16*>(row)[i]);
+  else return static_cast<const float*>(row)[i];
+}
+
+__device__ __forceinline__ float lp_ex2(float x) {
+  float r;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+  return r;
+}
+
+struct LpParams {
+  const void* logits;
+  long long ld;
+  const long long* ids;
+  float *logprob, *entropy, *top_lp;
+  long long* top_ids;
+  int vocab, top, part;  // part: vectors of a CTA
+};
+
+struct LpShared {
+  Ranked kept[kLpKept], best[kLpMaxTop], red[kLpWarps];
+  float edge[16], sums[2][kLpWarps], S, D;  // edge: values of the row ahead of its first whole vector and behind its last
+  uint32_t most, least, count;
+  uint32_t warp_most[kLpWarps], warp_least[kLpWarps];
+};
 
 template <int KIND>
-__global__ void __launch_bounds__(kLpThreads) token_logprobs_kernel(const void* logits, long long ld, int vocab, const long long* ids, int top,
-                                                                    float* logprob, float* entropy, float* top_lp, long long* top_ids) {
-  __shared__ unsigned long long red[kLpThreads / 32];
-  __shared__ float sums[2][kLpThreads / 32];
+__global__ void __launch_bounds__(kLpThreads) token_logprobs_kernel(const __grid_constant__ LpParams p) {
+  extern __shared__ __align__(16) uint4 part[];
+  __shared__ LpShared sh;
+  constexpr int kPer = Vec<KIND>::kPer, kSize = KIND == 2 ? 4 : 2;
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
-  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-  const long long r = blockIdx.x;
+  cg::cluster_group cluster = cg::this_cluster();
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, rank = cluster.block_rank(), n_cta = cluster.num_blocks();
+  const long long r = blockIdx.x / n_cta;
+  const char* const row = static_cast<const char*>(p.logits) + r * p.ld * kSize;
+  // whole vectors of the row, this CTA's of them, and the values around them (the first CTA's)
+  const int head = min(p.vocab, (int)((16 - (reinterpret_cast<uintptr_t>(row) & 15)) & 15) / kSize), vecs = (p.vocab - head) / kPer, tail = p.vocab - head - vecs * kPer;
+  const int v0 = min(vecs, rank * p.part), mine = min(vecs, v0 + p.part) - v0, id0 = head + v0 * kPer, edges = rank == 0 ? head + tail : 0;
+  auto edge_id = [&](int i) { return i < head ? i : p.vocab - tail + (i - head); };
+  if (tid == 0) sh.count = 0;
   asm volatile("griddepcontrol.wait;" ::: "memory");
-  const void* row = static_cast<const char*>(logits) + r * ld * (KIND == 2 ? 4 : 2);
-  // the largest of 64-bit numbers (order, ~id)
-  auto most = [&](unsigned long long v) {
+
+  // ---- the row into shared memory, and the largest value that each thread has seen (0: none)
+  uint32_t seen = 0;
+  {
+    const uint4* const from = reinterpret_cast<const uint4*>(row + (size_t)head * kSize) + v0;
+    constexpr int kAhead = 8;
+    for (int i0 = tid; i0 < mine; i0 += kAhead * kLpThreads) {
+      uint4 w[kAhead];
 #pragma unroll
-    for (int d = 16; d > 0; d >>= 1) v = max(v, __shfl_xor_sync(0xffffffffu, v, d));
-    __syncthreads();
-    if (lane == 0) red[warp] = v;
-    __syncthreads();
-    v = red[0];
-    for (int w = 1; w < kLpThreads / 32; ++w) v = max(v, red[w]);
-    return v;
-  };
-  uint32_t best = 0;
-  for (int i = tid; i < vocab; i += kLpThreads) best = max(best, order_of(logit<KIND>(row, i)));
-  const float M = value_of((uint32_t)most(best));
-  const bool finite = M <= 3.402823466e38f && M >= -3.402823466e38f;
+      for (int u = 0; u < kAhead; ++u)
+        if (i0 + u * kLpThreads < mine) w[u] = from[i0 + u * kLpThreads];
+#pragma unroll
+      for (int u = 0; u < kAhead; ++u)
+        if (i0 + u * kLpThreads < mine) {
+          part[i0 + u * kLpThreads] = w[u];
+          seen = max(seen, order_of(Vec<KIND>::most(w[u])));
+        }
+    }
+    if (tid < edges) {
+      const float x = logit<KIND>(row, edge_id(tid));
+      sh.edge[tid] = x;
+      seen = max(seen, order_of(x));
+    }
+  }
+  {
+    const uint32_t most = __reduce_max_sync(0xffffffffu, seen);
+    // groups of neighbouring threads: 8 (a warp each), 16, 32 or 64
+    uint32_t g = seen;
+    const int lanes = p.top <= 8 ? 32 : p.top <= 16 ? 16 : p.top <= 32 ? 8 : 4;
+    for (int d = 1; d < lanes; d <<= 1) g = max(g, __shfl_xor_sync(0xffffffffu, g, d));
+    const uint32_t least = __reduce_min_sync(0xffffffffu, g);
+    if (lane == 0) sh.warp_most[warp] = most, sh.warp_least[warp] = least;
+  }
+  __syncthreads();
+  if (tid == 0) {
+    uint32_t a = 0, b = 0xffffffffu;
+    for (int w = 0; w < kLpWarps; ++w) a = max(a, sh.warp_most[w]), b = min(b, sh.warp_least[w]);
+    sh.most = a, sh.least = b;
+  }
+  if (n_cta > 1) cluster.sync();
+  else __syncthreads();
+  uint32_t most = 0, least = 0;
+  for (int c = 0; c < n_cta; ++c) {
+    const LpShared* other = cluster.map_shared_rank(&sh, c);
+    most = max(most, other->most), least = max(least, other->least);
+  }
+  const float M = value_of(most), reach = value_of(least);
+  const bool finite = M <= 3.402823466e38f && M >= -3.402823466e38f, empty = M == -CUDART_INF_F;
+  const bool all = least == 0;  // (a group that saw nothing: keep everything)
+
+  // ---- the sums, and the values that reach the threshold
   float S = 0.f, D = 0.f;
-  for (int i = tid; finite && i < vocab; i += kLpThreads) {
-    const float d = logit<KIND>(row, i) - M, e = __expf(d);
+  auto keep = [&](float x, int id) {
+    const uint32_t at = atomicAdd(&sh.count, 1u);
+    if (at < kLpKept) sh.kept[at] = ranked(x, id);
+  };
+  auto add = [&](float x) {
+    const float d = fmaxf(x - M, -1e4f), e = lp_ex2(d * 1.4426950408889634f);  // (-inf: weight 0)
     S += e;
-    if (e > 0.f) D = fmaf(e, d, D);
+    D = fmaf(e, d, D);
+  };
+  if (finite) {
+    const bool list = p.top > 0;
+#pragma unroll 2
+    for (int i = tid; i < mine; i += kLpThreads) {
+      const uint4 w = part[i];
+      float f[kPer];
+      Vec<KIND>::floats(w, f);
+#pragma unroll
+      for (int k = 0; k < kPer; ++k) add(f[k]);
+      if (list && (all || Vec<KIND>::most(w) >= reach)) {
+#pragma unroll
+        for (int k = 0; k < kPer; ++k)
+          if (all || f[k] >= reach) keep(f[k], id0 + i * kPer + k);
+      }
+    }
+    if (tid < edges) {
+      const float x = sh.edge[tid];
+      add(x);
+      if (list && (all || x >= reach)) keep(x, edge_id(tid));
+    }
   }
 #pragma unroll
   for (int d = 16; d > 0; d >>= 1) S += __shfl_xor_sync(0xffffffffu, S, d), D += __shfl_xor_sync(0xffffffffu, D, d);
-  if (lane == 0) sums[0][warp] = S, sums[1][warp] = D;
+  if (lane == 0) sh.sums[0][warp] = S, sh.sums[1][warp] = D;
   __syncthreads();
-  S = D = 0.f;
-  for (int w = 0; w < kLpThreads / 32; ++w) S += sums[0][w], D += sums[1][w];
-  const float log_s = logf(S);
-  // (a row of -inf alone: every log probability -inf, entropy 0; a NaN or +inf: NaN)
-  const bool empty = M == -CUDART_INF_F;
-  auto lp = [&](float x) { return finite ? (x - M) - log_s : empty ? -CUDART_INF_F : CUDART_NAN_F; };
   if (tid == 0) {
-    const long long id = ids[r];
-    logprob[r] = id < 0 ? 0.f : id >= vocab ? CUDART_NAN_F : lp(logit<KIND>(row, id));
-    entropy[r] = finite ? log_s - D / S : empty ? 0.f : CUDART_NAN_F;
+    S = D = 0.f;
+    for (int w = 0; w < kLpWarps; ++w) S += sh.sums[0][w], D += sh.sums[1][w];
+    sh.S = S, sh.D = D;
   }
-  unsigned long long last = ~0ull;
-  for (int k = 0; k < top; ++k) {
-    unsigned long long v = 0;
-    for (int i = tid; i < vocab; i += kLpThreads) {
-      const unsigned long long c = (unsigned long long)order_of(logit<KIND>(row, i)) << 32 | (0xffffffffu - (uint32_t)i);
-      if (c < last) v = max(v, c);
+
+  // ---- this CTA's likeliest, in order (0: no more)
+  const int kept = (int)sh.count;
+  if (tid < kLpMaxTop) sh.best[tid] = 0;
+  __syncthreads();
+  if (finite && kept <= kLpKept) {
+    for (int i = tid; i < kept; i += kLpThreads) {
+      const Ranked v = sh.kept[i];
+      int before = 0;
+      for (int k = 0; k < kept; ++k) before += sh.kept[k] > v;
+      if (before < p.top) sh.best[before] = v;
     }
-    last = most(v);
-    if (tid == 0) top_lp[r * top + k] = lp(value_of((uint32_t)(last >> 32))), top_ids[r * top + k] = 0xffffffffu - (uint32_t)last;
+  } else {
+    Ranked last = ~0ull;
+    for (int k = 0; k < p.top && last != 0; ++k) {  // (too many equal ones, or a row with values that are no numbers: one search each)
+      Ranked v = 0;
+      auto look = [&](float x, int id) {
+        const Ranked c = ranked(x, id);
+        if (c < last) v = max(v, c);
+      };
+      for (int i = tid; i < mine; i += kLpThreads) {
+        float f[kPer];
+        Vec<KIND>::floats(part[i], f);
+#pragma unroll
+        for (int z = 0; z < kPer; ++z) look(f[z], id0 + i * kPer + z);
+      }
+      if (tid < edges) look(sh.edge[tid], edge_id(tid));
+#pragma unroll
+      for (int d = 16; d > 0; d >>= 1) v = max(v, __shfl_xor_sync(0xffffffffu, v, d));
+      if (lane == 0) sh.red[warp] = v;
+      __syncthreads();
+      v = sh.red[0];
+      for (int w = 1; w < kLpWarps; ++w) v = max(v, sh.red[w]);
+      if (tid == 0) sh.best[k] = v;
+      last = v;
+      __syncthreads();
+    }
   }
+  if (n_cta > 1) cluster.sync();
+  else __syncthreads();
+
+  // ---- the first CTA puts the row together
+  if (rank == 0) {
+    S = D = 0.f;
+    for (int c = 0; c < n_cta; ++c) {
+      const LpShared* other = cluster.map_shared_rank(&sh, c);
+      S += other->S, D += other->D;
+    }
+    const float log_s = logf(S);
+    // (a row of -inf alone: every log probability -inf, entropy 0; a NaN or +inf: NaN)
+    auto lp = [&](float x) { return finite ? (x - M) - log_s : empty ? -CUDART_INF_F : CUDART_NAN_F; };
+    if (tid == 0) {
+      const long long id = p.ids[r];
+      p.logprob[r] = id < 0 ? 0.f : id >= p.vocab ? CUDART_NAN_F : lp(logit<KIND>(row, id));
+      p.entropy[r] = finite ? log_s - D / S : empty ? 0.f : CUDART_NAN_F;
+    }
+    for (int i = tid; i < n_cta * p.top; i += kLpThreads) {
+      const int c = i / p.top, k = i - c * p.top;
+      const Ranked v = cluster.map_shared_rank(&sh, c)->best[k];
+      if (v == 0) continue;
+      int before = k;  // (lists are in order: a binary search in each of the others)
+      for (int o = 0; o < n_cta; ++o) {
+        if (o == c) continue;
+        const Ranked* list = cluster.map_shared_rank(&sh, o)->best;
+        int a = 0, z = p.top;
+        while (a < z) {
+          const int m = (a + z) >> 1;
+          if (list[m] > v) a = m + 1;
+          else z = m;
+        }
+        before += a;
+      }
+      if (before < p.top) p.top_lp[r * p.top + before] = lp(value_of((uint32_t)(v >> 32))), p.top_ids[r * p.top + before] = 0xffffffffu - (uint32_t)v;
+    }
+  }
+  if (n_cta > 1) cluster.sync();  // (a CTA's memory is there until the first one has read it)
 }
 
-template <typename K, typename... A>
-static int launch(K kern, dim3 grid, dim3 block, cudaStream_t st, A... args) {
+template <int KIND>
+static int launch_logprobs(const LpParams& p, int64_t rows, int ctas, int smem, cudaStream_t stream) {
+  static bool configured[64] = {};
+  DeviceInfo di;
+  int rc;
+  if ((rc = device_info(&di))) return rc;
+  if (!configured[di.dev]) {
+    BLR_CUDA_OK(cudaFuncSetAttribute(token_logprobs_kernel<KIND>, cudaFuncAttributeMaxDynamicSharedMemorySize, kLpMaxPart));
+    configured[di.dev] = true;
+  }
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = grid;
-  cfg.blockDim = block;
-  cfg.stream = st;
-  cudaLaunchAttribute at[1];
+  cfg.gridDim = dim3((unsigned)(rows * ctas));
+  cfg.blockDim = dim3(kLpThreads);
+  cfg.dynamicSmemBytes = (size_t)smem;
+  cfg.stream = stream;
+  cudaLaunchAttribute at[2];
   at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
   at[0].val.programmaticStreamSerializationAllowed = 1;
+  at[1].id = cudaLaunchAttributeClusterDimension;
+  at[1].val.clusterDim.x = (unsigned)ctas;
+  at[1].val.clusterDim.y = at[1].val.clusterDim.z = 1;
   cfg.attrs = at;
-  cfg.numAttrs = 1;
-  BLR_CUDA_OK(cudaLaunchKernelEx(&cfg, kern, args...));
+  cfg.numAttrs = 2;
+  BLR_CUDA_OK(cudaLaunchKernelEx(&cfg, token_logprobs_kernel<KIND>, p));
   return BLR_OK;
 }
 
@@ -108,17 +315,28 @@ extern "C" {
 int blr_token_logprobs(const void* logits, int64_t ld, int64_t rows, int64_t vocab, int kind, const int64_t* ids, int top, float* logprob,
                        float* entropy, float* top_logprob, int64_t* top_ids, void* stream) {
   BLR_REQUIRE(kind >= 0 && kind <= 2, BLR_ERR_ARG, "unknown kind of logits %d", kind);
-  BLR_REQUIRE(rows >= 0 && rows < (1ll << 31) && vocab > 0 && vocab < (1ll << 31) && (rows <= 1 || ld >= vocab), BLR_ERR_ARG,
-              "token_logprobs: %lld rows of %lld", (long long)rows, (long long)vocab);
+  const int64_t size = kind == 2 ? 4 : 2;
+  BLR_REQUIRE(rows >= 0 && rows < (1ll << 28) && vocab > 0 && (rows <= 1 || ld >= vocab), BLR_ERR_ARG, "token_logprobs: %lld rows of %lld", (long long)rows,
+              (long long)vocab);
+  BLR_REQUIRE(vocab * size <= 8ll * kLpMaxPart, BLR_ERR_UNSUPPORTED, "token_logprobs keeps a row in the shared memory of 8 SMs: at most %lld bytes, not %lld",
+              8ll * kLpMaxPart, (long long)(vocab * size));
   BLR_REQUIRE(top >= 0 && top <= kLpMaxTop && top <= vocab, BLR_ERR_ARG, "token_logprobs gives 0 to %d tokens (and no more than there are), not %d", kLpMaxTop, top);
   if (rows == 0) return BLR_OK;
   BLR_REQUIRE(logits && ids && logprob && entropy && (top == 0 || (top_logprob && top_ids)), BLR_ERR_ARG, "null pointer");
+  BLR_REQUIRE(reinterpret_cast<uintptr_t>(logits) % size == 0, BLR_ERR_ARG, "token_logprobs: logits must be aligned to their size");
+  // a row's part of at most 64 KB, so that three CTAs share an SM; few rows: over more CTAs, as long as each has 4 KB
+  int ctas = 1;
+  while (ctas < 8 && vocab * size > ctas * 65536ll) ctas *= 2;
+  while (ctas < 8 && rows * ctas < 2ll * sm_count() && vocab * size >= ctas * 8192ll) ctas *= 2;
+  LpParams p = {};
+  p.logits = logits, p.ld = ld, p.ids = reinterpret_cast<const long long*>(ids);
+  p.logprob = logprob, p.entropy = entropy, p.top_lp = top_logprob, p.top_ids = reinterpret_cast<long long*>(top_ids);
+  const int64_t per = 16 / size, vecs = vocab / per;  // (as many vectors as a row can have, however it is aligned)
+  p.vocab = (int)vocab, p.top = top, p.part = (int)((vecs + ctas - 1) / ctas);
+  if (p.part < 1) p.part = 1;
+  const int smem = p.part * 16;
   const cudaStream_t st = static_cast<cudaStream_t>(stream);
-  auto go = [&](auto kernel) {
-    return launch(kernel, dim3((unsigned)rows), dim3(kLpThreads), st, logits, (long long)ld, (int)vocab, reinterpret_cast<const long long*>(ids), top, logprob,
-                  entropy, top_logprob, reinterpret_cast<long long*>(top_ids));
-  };
-  return kind == 0 ? go(token_logprobs_kernel<0>) : kind == 1 ? go(token_logprobs_kernel<1>) : go(token_logprobs_kernel<2>);
+  return kind == 0 ? launch_logprobs<0>(p, rows, ctas, smem, st) : kind == 1 ? launch_logprobs<1>(p, rows, ctas, smem, st) : launch_logprobs<2>(p, rows, ctas, smem, st);
 }
 
 }  // extern "C"

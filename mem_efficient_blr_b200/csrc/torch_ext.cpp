@@ -863,7 +863,150 @@ PyObject* py_mlp(PyObject*, PyObject* const* a, Py_ssize_t na) {
   END_HANDLE_TH_ERRORS
 }
 
+// ops.Q8Cache, a tuple (k, v, k_scale, v_scale, block) of packed tensors on one device: what the library calls a cache.  What does not fit the
+// library's limits is left to it to refuse.
+struct Cache8 {
+  blr_q8_cache c = {};
+  const at::Tensor* k = nullptr;
+  bool take(PyObject* o) {
+    if (!PyTuple_Check(o) || PyTuple_GET_SIZE(o) != 5) return false;
+    const at::Tensor* t[4];
+    for (int i = 0; i < 4; ++i) {
+      t[i] = plain(PyTuple_GET_ITEM(o, i));
+      if (!t[i] || !t[i]->is_cuda() || t[i]->device() != t[0]->device() || !t[i]->is_contiguous()) return false;
+    }
+    k = t[0];
+    long block;
+    if (!take_ints(&PyTuple_GET_ITEM(o, 4), 1, &block) || block <= 0 || k->dim() != 4 || t[1]->sizes() != k->sizes()) return false;
+    const at::ScalarType dt = k->scalar_type();
+    if ((dt != at::kChar && dt != at::kFloat8_e4m3fn) || t[1]->scalar_type() != dt || t[2]->scalar_type() != at::kFloat || t[3]->scalar_type() != at::kFloat) return false;
+    const int64_t nb = (k->size(2) + block - 1) / block, size[3] = {k->size(0), k->size(1), nb};
+    if (t[2]->sizes() != at::IntArrayRef(size, 3) || t[3]->sizes() != at::IntArrayRef(size, 3) || k->size(2) > INT_MAX || block > INT_MAX) return false;
+    c.k = t[0]->data_ptr(), c.v = t[1]->data_ptr();
+    c.k_scale = static_cast<float*>(t[2]->data_ptr()), c.v_scale = static_cast<float*>(t[3]->data_ptr());
+    c.n_seq = k->size(0), c.kv_heads = (int)k->size(1), c.slots = (int)k->size(2), c.head_dim = (int)k->size(3), c.block = (int)block;
+    c.code = dt == at::kChar ? BLR_Q8_INT8 : BLR_Q8_E4M3;
+    return c.n_seq > 0 && c.kv_heads > 0 && c.head_dim > 0 && c.slots > 0;
+  }
+  // rows of q, of whole heads, for each of its sequences
+  bool rows_of(const Direct& d) const {
+    return d.x->dim() == 2 && k->device() == d.x->device() && d.n % c.n_seq == 0 && d.width % c.head_dim == 0;
+  }
+};
+
+// A number for each sequence, or (none_too) None: false when it is neither.
+bool per_sequence(const Direct& d, const Cache8& c, PyObject* o, bool none_too, const int64_t** p) {
+  *p = nullptr;
+  if (o == Py_None) return none_too;
+  const at::Tensor* t = d.factor(o, at::kLong);
+  if (!t || t->numel() != c.c.n_seq) return false;
+  *p = t->data_ptr<int64_t>();
+  return true;
+}
+
+// rope_append_q8(q, k, v, cos, sin, start, cache, n_new | None)
+PyObject* py_rope_append_q8(PyObject*, PyObject* const* a, Py_ssize_t na) {
+  HANDLE_TH_ERRORS
+  Direct d, dk, dv;
+  Cache8 c;
+  const int64_t *start, *n_new;
+  if (na != 8 || !d.take_x(a[0]) || !dk.take_x(a[1]) || !dv.take_x(a[2]) || !c.take(a[6]) || !c.rows_of(d)) BLR_NONE();
+  if (dk.dt != d.dt || dv.dt != d.dt || dk.dev != d.dev || dv.dev != d.dev || dk.x->dim() != 2 || dv.x->dim() != 2 || dk.n != d.n || dv.n != d.n ||
+      dk.width != (int64_t)c.c.kv_heads * c.c.head_dim || dv.width != dk.width)
+    BLR_NONE();
+  const at::Tensor *cs = d.factor(a[3], at::kFloat), *sn = d.factor(a[4], at::kFloat);
+  for (const at::Tensor* t : {cs, sn})
+    if (!t || t->dim() != 2 || t->size(0) < c.c.slots || t->size(1) != c.c.head_dim / 2) BLR_NONE();
+  if (!per_sequence(d, c, a[5], false, &start) || !per_sequence(d, c, a[7], true, &n_new) || records_grad({d.x, dk.x, dv.x})) BLR_NONE();
+  at::Tensor out = d.output(d.width);
+  void* o = out.data_ptr();
+  call_library([&] {
+    return blr_rope_append_q8(d.x->data_ptr(), d.ldx, dk.x->data_ptr(), dk.ldx, dv.x->data_ptr(), dv.ldx, cs->data_ptr<float>(), sn->data_ptr<float>(), start,
+                              n_new, d.n / c.c.n_seq, (int)(d.width / c.c.head_dim), d.code(), &c.c, o, d.width, d.st);
+  });
+  return THPVariable_Wrap(std::move(out));
+  END_HANDLE_TH_ERRORS
+}
+
+// attention_q8(q, cache, start, n_new | None, scale)
+PyObject* py_attention_q8(PyObject*, PyObject* const* a, Py_ssize_t na) {
+  HANDLE_TH_ERRORS
+  Direct d;
+  Cache8 c;
+  const int64_t *start, *n_new;
+  float scale;
+  if (na != 5 || !d.take_x(a[0]) || !c.take(a[1]) || !c.rows_of(d) || !per_sequence(d, c, a[2], false, &start) || !per_sequence(d, c, a[3], true, &n_new) ||
+      !take_eps(a[4], &scale) || d.width % ((int64_t)c.c.kv_heads * c.c.head_dim) != 0 || records_grad({d.x}))
+    BLR_NONE();
+  const int64_t n_tok = d.n / c.c.n_seq;
+  const int heads = (int)(d.width / c.c.head_dim);
+  if (scale == 0.f) scale = 1.f / std::sqrt((float)c.c.head_dim);
+  const size_t bytes = blr_attention_q8_scratch_bytes(&c.c, n_tok, heads);
+  at::Tensor out = d.output(d.width), part;
+  if (bytes > 0) part = at::detail::empty_cuda({(int64_t)bytes}, at::kByte, d.x->device(), c10::nullopt);
+  void *o = out.data_ptr(), *sp = bytes > 0 ? part.data_ptr() : nullptr;
+  call_library([&] {
+    return blr_attention_q8(d.x->data_ptr(), d.ldx, &c.c, start, n_new, n_tok, heads, scale, d.code(), o, d.width, sp, bytes, d.ws(0, 0).ptr, d.st);
+  });
+  return THPVariable_Wrap(std::move(out));
+  END_HANDLE_TH_ERRORS
+}
+
+// cache_read_q8(cache, bf16, lengths | None) -> (keys, values)
+PyObject* py_cache_read_q8(PyObject*, PyObject* const* a, Py_ssize_t na) {
+  HANDLE_TH_ERRORS
+  Direct d;
+  Cache8 c;
+  long bf16;
+  const int64_t* lengths;
+  if (na != 3 || !c.take(a[0]) || !take_ints(a + 1, 1, &bf16) || c10::impl::dispatch_mode_enabled() || at::impl::torch_function_mode_enabled()) BLR_NONE();
+  d.dev = c.k->device().index();
+  if (d.dev != c10::cuda::current_device() || !per_sequence(d, c, a[2], true, &lengths)) BLR_NONE();
+  d.st = at::cuda::getCurrentCUDAStream(d.dev).stream();
+  const at::ScalarType dt = bf16 ? at::kBFloat16 : at::kHalf;
+  at::Tensor k = at::detail::empty_cuda(c.k->sizes(), dt, c.k->device(), c10::nullopt), v = at::detail::empty_cuda(c.k->sizes(), dt, c.k->device(), c10::nullopt);
+  void *ko = k.data_ptr(), *vo = v.data_ptr();
+  call_library([&] { return blr_cache_read_q8(&c.c, lengths, bf16 ? BLR_DTYPE_BF16 : BLR_DTYPE_F16, ko, vo, d.st); });
+  PyObject* t = PyTuple_New(2);
+  if (t == nullptr) return nullptr;
+  PyTuple_SET_ITEM(t, 0, THPVariable_Wrap(std::move(k)));
+  PyTuple_SET_ITEM(t, 1, THPVariable_Wrap(std::move(v)));
+  return t;
+  END_HANDLE_TH_ERRORS
+}
+
+// token_logprobs(logits (rows, vocab), ids (rows), top) -> (log probabilities, entropies, those of the likeliest, their ids)
+PyObject* py_token_logprobs(PyObject*, PyObject* const* a, Py_ssize_t na) {
+  HANDLE_TH_ERRORS
+  long top;
+  if (na != 3 || c10::impl::dispatch_mode_enabled() || at::impl::torch_function_mode_enabled() || !take_ints(a + 2, 1, &top) || top < 0) BLR_NONE();
+  const at::Tensor *x = plain(a[0]), *ids = plain(a[1]);
+  if (!x || !ids || !x->is_cuda() || x->dim() != 2 || ids->dim() != 1 || ids->device() != x->device() || ids->scalar_type() != at::kLong || !ids->is_contiguous()) BLR_NONE();
+  const int64_t rows = x->size(0), vocab = x->size(1), ld = rows > 1 ? x->stride(0) : vocab;
+  const at::ScalarType dt = x->scalar_type();
+  if (rows == 0 || vocab == 0 || ids->size(0) != rows || x->stride(1) != 1 || ld < vocab || x->device().index() != c10::cuda::current_device() ||
+      (dt != at::kHalf && dt != at::kBFloat16 && dt != at::kFloat) || records_grad({x}))
+    BLR_NONE();
+  const cudaStream_t st = at::cuda::getCurrentCUDAStream(x->device().index()).stream();
+  auto make = [&](at::IntArrayRef size, at::ScalarType type) { return at::detail::empty_cuda(size, type, x->device(), c10::nullopt); };
+  at::Tensor out[4] = {make({rows}, at::kFloat), make({rows}, at::kFloat), make({rows, top}, at::kFloat), make({rows, top}, at::kLong)};
+  float *lp = out[0].data_ptr<float>(), *ent = out[1].data_ptr<float>(), *tl = out[2].data_ptr<float>();
+  int64_t* ti = out[3].data_ptr<int64_t>();
+  call_library([&] {
+    return blr_token_logprobs(x->data_ptr(), ld, rows, vocab, dt == at::kHalf ? 0 : dt == at::kBFloat16 ? 1 : 2, ids->data_ptr<int64_t>(), (int)top, lp, ent, tl, ti, st);
+  });
+  PyObject* t = PyTuple_New(4);
+  if (t == nullptr) return nullptr;
+  for (int i = 0; i < 4; ++i) PyTuple_SET_ITEM(t, i, THPVariable_Wrap(std::move(out[i])));
+  return t;
+  END_HANDLE_TH_ERRORS
+}
+
 PyMethodDef g_methods[] = {
+    {"rope_append_q8", (PyCFunction)(void*)py_rope_append_q8, METH_FASTCALL, nullptr},
+    {"attention_q8", (PyCFunction)(void*)py_attention_q8, METH_FASTCALL, nullptr},
+    {"cache_read_q8", (PyCFunction)(void*)py_cache_read_q8, METH_FASTCALL, nullptr},
+    {"token_logprobs", (PyCFunction)(void*)py_token_logprobs, METH_FASTCALL, nullptr},
     {"blast", (PyCFunction)(void*)py_blast, METH_FASTCALL, nullptr},
     {"blast_wq", (PyCFunction)(void*)py_blast_wq, METH_FASTCALL, nullptr},
     {"monarch", (PyCFunction)(void*)py_monarch, METH_FASTCALL, nullptr},

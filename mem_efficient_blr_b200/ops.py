@@ -724,6 +724,10 @@ def rope_append_q8(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cos_table:
     tokens.  cos / sin tables (>= slots, head_dim / 2) fp32.  Returns the rotated q (zeros in rows that are no token) and writes codes and scales of the
     rotated k and of v: a block's scale is the largest its tokens asked for since it was begun, and where it grows the codes that were there follow.
     Tokens whose slot lies outside the cache write nothing."""
+    dr = L.direct()
+    out = None if dr is None else dr.rope_append_q8(q, k, v, cos_table, sin_table, start, cache, n_new)
+    if out is not None:
+        return out
     _no_grad(q, k, v)
     d = _q8_desc(cache, q)
     hd = d.head_dim
@@ -745,6 +749,10 @@ def rope_append_q8(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cos_table:
 def cache_read_q8(cache: Q8Cache, dtype: torch.dtype, lengths=None) -> Tuple[torch.Tensor, torch.Tensor]:
     """(keys, values) of an 8-bit cache in 16 bits, (n_seq, kv_heads, slots, head_dim): code * scale rounded once; zeros from slot lengths[s] of a sequence
     on ((n_seq,) int64; None: all slots)."""
+    dr = L.direct()
+    out = None if dr is None or dtype not in (torch.float16, torch.bfloat16) else dr.cache_read_q8(cache, int(dtype == torch.bfloat16), lengths)
+    if out is not None:
+        return out
     d = _q8_desc(cache, cache.k)
     k, v = (torch.empty(cache.k.shape, dtype=dtype, device=cache.k.device) for _ in range(2))
     L.check(L.load().blr_cache_read_q8(d, None if lengths is None else _per_sequence(lengths, cache.k, d.n_seq, "lengths"), L.dtype_code(dtype), k.data_ptr(),
@@ -756,6 +764,10 @@ def attention_q8(q: torch.Tensor, cache: Q8Cache, start: torch.Tensor, n_new=Non
     """Causal attention of each sequence's newest tokens over an 8-bit cache that holds them already: q (n_seq * n_tok, heads * head_dim) 16-bit rows,
     sequence-major, heads a multiple of the cache's kv_heads; row t of sequence s sits at slot start[s] + t and sees the slots up to its own; rows from
     n_new[s] on are no tokens and come out as zeros, as does a row that sees no slot.  scale defaults to head_dim ** -0.5.  Returns (rows, heads * head_dim)."""
+    dr = L.direct()
+    out = None if dr is None else dr.attention_q8(q, cache, start, n_new, scale)
+    if out is not None:
+        return out
     _no_grad(q)
     d = _q8_desc(cache, q)
     assert q.dim() == 2 and d.n_seq > 0 and q.shape[0] % d.n_seq == 0 and q.shape[1] % (d.kv_heads * d.head_dim) == 0, "q: a row for each token of each sequence"
@@ -775,6 +787,10 @@ def token_logprobs(logits: torch.Tensor, ids: torch.Tensor, top: int = 0) -> Tup
     """Of each row of logits (..., vocab), fp16, bf16 or fp32: (log probability of ids' token, entropy, log probabilities of the `top` likeliest tokens
     (..., top), their ids), fp32 and int64.  ids (...) int64: a negative one stands for no token (0), one beyond the vocabulary gives NaN.  Ties go to the
     lowest id; top <= 64."""
+    dr = L.direct()
+    out = None if dr is None else dr.token_logprobs(logits, ids, top)
+    if out is not None:
+        return out
     _no_grad(logits)
     _need_cuda(logits)
     assert logits.dim() >= 1 and ids.shape == logits.shape[:-1] and ids.dtype == torch.int64 and ids.device == logits.device, "ids: one int64 for each row of logits"

@@ -192,8 +192,8 @@ def test_read(ops, B, KV, hd, slots, block, lengths, dtype, code):
 
 
 def _attention(q, parts, block, starts, new, scale):
-    """(out, allowance without the output's rounding) in 64 bits; q (B, T, H, hd).  Allowed: p is rounded to fp16 (half a step, 2^-12 of it; 2^-11 with what
-    the exponent's argument, up to 64 in fp32, and the sums of fp32 add) and below 2^-14 to multiples of 2^-24 of the largest value's scale, sixteen times that
+    """(out, allowance without the output's rounding) in 64 bits; q (B, T, H, hd).  Allowed: p is rounded to fp16 (half a step, at most 2^-11 of it, to either side;
+    what its exponent's argument and the sums of fp32 add is below 2^-16) and below 2^-14 to multiples of 2^-24 of the largest value's scale, sixteen times that
     where a larger scale came first; l is at least the sum taken against the true maximum."""
     B, T, H, hd = q.shape
     KV, slots = parts[0].shape[1:3]
@@ -451,7 +451,10 @@ def test_logprobs_shapes_and_strides(ops):
     want = ops.token_logprobs(x[..., :1000].contiguous(), ids, 4)
     for got in (ops.token_logprobs(x[..., :1000], ids, 4), ops.token_logprobs(x[..., :1000].transpose(0, 1), ids.t(), 4)):
         for a, b in zip(want, got):
-            assert a.shape[:2] == (3, 4) and torch.equal(a, b if b.shape[0] == 3 else b.transpose(0, 1))
+            b = b if b.shape[0] == 3 else b.transpose(0, 1)
+            # (the order of a row's sums goes by its alignment: each result is within rel_s + 2^-23 (|x - M| + log S) of the exact one, see test_logprobs, with
+            # |x - M| < 9 and log S < 8 here, so two are within twice that of each other)
+            assert a.shape[:2] == (3, 4) and a.shape == b.shape and (a - b).abs().max() <= (0 if a.dtype == torch.int64 else 2 * (2.0 ** -21 + 68 * 2.0 ** -24 + 17 * 2.0 ** -23))
     one = ops.token_logprobs(x[0, 0, 1:1001], ids[0, 0])
     assert one[0].shape == () and one[2].shape == (0,) and one[0].isfinite()
     none = ops.token_logprobs(x[:0], ids[:0], 2)
