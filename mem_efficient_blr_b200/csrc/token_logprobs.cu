@@ -18,7 +18,7 @@ namespace cg = cooperative_groups;
 
 namespace blr {
 
-static constexpr int kLpThreads = 256, kLpWarps = kLpThreads / 32, kLpMaxTop = 64, kLpKept = 1024, kLpMaxPart = 200 * 1024;
+static constexpr int kLpThreads = 512, kLpWarps = kLpThreads / 32, kLpMaxTop = 64, kLpKept = 1024, kLpMaxPart = 200 * 1024;
 typedef unsigned long long Ranked;  // order_of(value) << 32 | ~id: larger is likelier
 
 // Whole numbers in the order of the values; 0 is below all of them.
@@ -35,33 +35,37 @@ __device__ __forceinline__ Ranked ranked(float x, int id) { return (Ranked)order
 template <int KIND>
 struct Vec {
   static constexpr int kPer = KIND == 2 ? 4 : 8;
-  __device__ __forceinline__ static void floats(const uint4& w, float (&f)[kPer]) {
-    const uint32_t ws[4] = {w.x, w.y, w.z, w.w};
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      if constexpr (KIND == 2) {
-        f[i] = __uint_as_float(ws[i]);
-      } else {
-        const float2 v = q8_up2<KIND == 1>(ws[i]);
-        f[2 * i] = v.x, f[2 * i + 1] = v.y;
-      }
-    }
+  // their running maximum (16-bit values: of the odd and the even ones), a NaN before anything else
+  __device__ __forceinline__ static uint32_t larger(uint32_t a, uint32_t b) {
+    uint32_t r;
+    if constexpr (KIND == 0) asm("max.NaN.f16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
+    else if constexpr (KIND == 1) asm("max.NaN.bf16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
+    else asm("max.NaN.f32 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
+    return r;
   }
-  // the largest of them, a NaN before anything else
-  __device__ __forceinline__ static float most(const uint4& w) {
+  __device__ __forceinline__ static uint32_t largest(const uint4& w) { return larger(larger(w.x, w.y), larger(w.z, w.w)); }
+  static constexpr uint32_t kLowest = KIND == 0 ? 0xfc00fc00u : KIND == 1 ? 0xff80ff80u : 0xff800000u;  // -inf
+  __device__ __forceinline__ static float most(uint32_t m) {
+    if constexpr (KIND == 2) return __uint_as_float(m);
+    else return [](float2 v) { return v.x != v.x || v.x > v.y ? v.x : v.y; }(q8_up2<KIND == 1>(m));
+  }
+  __device__ __forceinline__ static float value(const uint4& w, int i) {
+    const uint32_t u = i < kPer / 2 ? i < kPer / 4 ? w.x : w.y : i < 3 * kPer / 4 ? w.z : w.w;
+    if constexpr (KIND == 2) return __uint_as_float(u);
+    else return [&](float2 v) { return i & 1 ? v.y : v.x; }(q8_up2<KIND == 1>(u));
+  }
+  // as pairs of floats, what is lower than -65504 (fp16) or -10^30 set to that: a weight of 0 is then one of a number
+  __device__ __forceinline__ static void pairs(const uint4& w, uint64_t (&f)[kPer / 2]) {
+    uint32_t ws[4] = {w.x, w.y, w.z, w.w};
     if constexpr (KIND == 2) {
-      const float a = __uint_as_float(w.x), b = __uint_as_float(w.y), c = __uint_as_float(w.z), d = __uint_as_float(w.w);
-      float r;
-      asm("{\n\t.reg .f32 t;\n\tmax.NaN.f32 t, %1, %2;\n\tmax.NaN.f32 t, t, %3;\n\tmax.NaN.f32 %0, t, %4;\n\t}" : "=f"(r) : "f"(a), "f"(b), "f"(c), "f"(d));
-      return r;
-    } else if constexpr (KIND == 1) {
-      const __nv_bfloat162* h = reinterpret_cast<const __nv_bfloat162*>(&w);
-      const __nv_bfloat162 m = __hmax2_nan(__hmax2_nan(h[0], h[1]), __hmax2_nan(h[2], h[3]));
-      return __bfloat162float(__hmax_nan(m.x, m.y));
+#pragma unroll
+      for (int i = 0; i < 2; ++i) f[i] = pair(fmaxf(__uint_as_float(ws[2 * i]), -1e30f), fmaxf(__uint_as_float(ws[2 * i + 1]), -1e30f));
     } else {
-      const __half2* h = reinterpret_cast<const __half2*>(&w);
-      const __half2 m = __hmax2_nan(__hmax2_nan(h[0], h[1]), __hmax2_nan(h[2], h[3]));
-      return __half2float(__hmax_nan(m.x, m.y));
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const float2 v = q8_up2<KIND == 1>(larger(ws[i], KIND == 0 ? 0xfbfffbffu : 0xf149f149u));
+        f[i] = pair(v.x, v.y);
+      }
     }
   }
 };
@@ -95,7 +99,7 @@ struct LpShared {
 };
 
 template <int KIND>
-__global__ void __launch_bounds__(kLpThreads) token_logprobs_kernel(const __grid_constant__ LpParams p) {
+__global__ void __launch_bounds__(kLpThreads, 3) token_logprobs_kernel(const __grid_constant__ LpParams p) {
   extern __shared__ __align__(16) uint4 part[];
   __shared__ LpShared sh;
   constexpr int kPer = Vec<KIND>::kPer, kSize = KIND == 2 ? 4 : 2;
@@ -115,7 +119,8 @@ __global__ void __launch_bounds__(kLpThreads) token_logprobs_kernel(const __grid
   uint32_t seen = 0;
   {
     const uint4* const from = reinterpret_cast<const uint4*>(row + (size_t)head * kSize) + v0;
-    constexpr int kAhead = 8;
+    constexpr int kAhead = 4;
+    uint32_t top = Vec<KIND>::kLowest;
     for (int i0 = tid; i0 < mine; i0 += kAhead * kLpThreads) {
       uint4 w[kAhead];
 #pragma unroll
@@ -125,9 +130,10 @@ __global__ void __launch_bounds__(kLpThreads) token_logprobs_kernel(const __grid
       for (int u = 0; u < kAhead; ++u)
         if (i0 + u * kLpThreads < mine) {
           part[i0 + u * kLpThreads] = w[u];
-          seen = max(seen, order_of(Vec<KIND>::most(w[u])));
+          top = Vec<KIND>::larger(top, Vec<KIND>::largest(w[u]));
         }
     }
+    if (tid < mine) seen = order_of(Vec<KIND>::most(top));
     if (tid < edges) {
       const float x = logit<KIND>(row, edge_id(tid));
       sh.edge[tid] = x;
@@ -136,9 +142,9 @@ __global__ void __launch_bounds__(kLpThreads) token_logprobs_kernel(const __grid
   }
   {
     const uint32_t most = __reduce_max_sync(0xffffffffu, seen);
-    // groups of neighbouring threads: 8 (a warp each), 16, 32 or 64
+    // groups of neighbouring threads: 16 (a warp each), 32 or 64
     uint32_t g = seen;
-    const int lanes = p.top <= 8 ? 32 : p.top <= 16 ? 16 : p.top <= 32 ? 8 : 4;
+    const int lanes = p.top <= kLpWarps ? 32 : p.top <= 2 * kLpWarps ? 16 : 8;
     for (int d = 1; d < lanes; d <<= 1) g = max(g, __shfl_xor_sync(0xffffffffu, g, d));
     const uint32_t least = __reduce_min_sync(0xffffffffu, g);
     if (lane == 0) sh.warp_most[warp] = most, sh.warp_least[warp] = least;
@@ -148,6 +154,23 @@ __global__ void __launch_bounds__(kLpThreads) token_logprobs_kernel(const __grid
     uint32_t a = 0, b = 0xffffffffu;
     for (int w = 0; w < kLpWarps; ++w) a = max(a, sh.warp_most[w]), b = min(b, sh.warp_least[w]);
     sh.most = a, sh.least = b;
+  }
+  if (p.top > 0) {
+    // at least as many threads as tokens are asked for have seen a value that reaches this minimum: the one that so many reach is closer
+    __syncthreads();
+    const uint32_t least = sh.least;
+    uint32_t* const list = reinterpret_cast<uint32_t*>(sh.kept);
+    if (seen >= least) list[atomicAdd(&sh.count, 1u)] = seen;
+    __syncthreads();
+    const int n = (int)sh.count;
+    if (least > 0 && tid < n) {
+      const uint32_t v = list[tid];
+      int before = 0;
+      for (int k = 0; k < n; ++k) before += list[k] > v || (list[k] == v && k < tid);
+      if (before == p.top - 1) sh.least = v;
+    }
+    __syncthreads();
+    if (tid == 0) sh.count = 0;
   }
   if (n_cta > 1) cluster.sync();
   else __syncthreads();
@@ -166,30 +189,44 @@ __global__ void __launch_bounds__(kLpThreads) token_logprobs_kernel(const __grid
     const uint32_t at = atomicAdd(&sh.count, 1u);
     if (at < kLpKept) sh.kept[at] = ranked(x, id);
   };
-  auto add = [&](float x) {
-    const float d = fmaxf(x - M, -1e4f), e = lp_ex2(d * 1.4426950408889634f);  // (-inf: weight 0)
-    S += e;
-    D = fmaf(e, d, D);
-  };
   if (finite) {
-    const bool list = p.top > 0;
+    uint64_t s2[2] = {0, 0}, d2[2] = {0, 0};
+    const uint64_t less = pair(-M, -M), log2e = pair(1.4426950408889634f, 1.4426950408889634f);
 #pragma unroll 2
     for (int i = tid; i < mine; i += kLpThreads) {
-      const uint4 w = part[i];
-      float f[kPer];
-      Vec<KIND>::floats(w, f);
+      uint64_t f[kPer / 2];
+      Vec<KIND>::pairs(part[i], f);
 #pragma unroll
-      for (int k = 0; k < kPer; ++k) add(f[k]);
-      if (list && (all || Vec<KIND>::most(w) >= reach)) {
-#pragma unroll
-        for (int k = 0; k < kPer; ++k)
-          if (all || f[k] >= reach) keep(f[k], id0 + i * kPer + k);
+      for (int k = 0; k < kPer / 2; ++k) {
+        const uint64_t d = add2(f[k], less);
+        float a, b;
+        unpair(mul2(d, log2e), a, b);
+        const uint64_t e = pair(lp_ex2(a), lp_ex2(b));
+        s2[k & 1] = add2(s2[k & 1], e);
+        d2[k & 1] = fma2(e, d, d2[k & 1]);
       }
     }
+    float a, b;
+    unpair(add2(s2[0], s2[1]), a, b);
+    S = a + b;
+    unpair(add2(d2[0], d2[1]), a, b);
+    D = a + b;
     if (tid < edges) {
-      const float x = sh.edge[tid];
-      add(x);
-      if (list && (all || x >= reach)) keep(x, edge_id(tid));
+      const float d = fmaxf(sh.edge[tid], -1e30f) - M, e = lp_ex2(d * 1.4426950408889634f);
+      S += e;
+      D = fmaf(e, d, D);
+    }
+    if (p.top > 0 && (all || seen >= least)) {  // (few threads)
+      for (int i = tid; i < mine; i += kLpThreads) {
+        const uint4 w = part[i];
+        if (!all && !(Vec<KIND>::most(Vec<KIND>::largest(w)) >= reach)) continue;
+#pragma unroll
+        for (int k = 0; k < kPer; ++k) {
+          const float x = Vec<KIND>::value(w, k);
+          if (all || x >= reach) keep(x, id0 + i * kPer + k);
+        }
+      }
+      if (tid < edges && (all || sh.edge[tid] >= reach)) keep(sh.edge[tid], edge_id(tid));
     }
   }
 #pragma unroll
@@ -222,10 +259,9 @@ __global__ void __launch_bounds__(kLpThreads) token_logprobs_kernel(const __grid
         if (c < last) v = max(v, c);
       };
       for (int i = tid; i < mine; i += kLpThreads) {
-        float f[kPer];
-        Vec<KIND>::floats(part[i], f);
+        const uint4 w = part[i];
 #pragma unroll
-        for (int z = 0; z < kPer; ++z) look(f[z], id0 + i * kPer + z);
+        for (int z = 0; z < kPer; ++z) look(Vec<KIND>::value(w, z), id0 + i * kPer + z);
       }
       if (tid < edges) look(sh.edge[tid], edge_id(tid));
 #pragma unroll
