@@ -15,49 +15,40 @@
 
 namespace blr {
 
-static constexpr int kQ8Warps = 8, kMaxSplits = 64;
+static constexpr int kMaxSplits = 64;
 
 __device__ __forceinline__ uint32_t transpose8x8(uint32_t a) {
   uint32_t d;
   asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(d) : "r"(a));
   return d;
 }
+// CTA (row tile, sequence and kv head, split): a warp takes every fourth group of 16 keys and brings them into a ring of its own, kFewStages groups deep, with
+// cp.async: no warp waits for another before the end.  A row's 16-byte pieces are written where the reads below meet no bank twice (heads of 64: twice for V).
+static constexpr int kFewWarps = 4, kFewThreads = 32 * kFewWarps, kFewStages = 3;
+
 template <int HD>
-struct Q8Keys {  // 16 keys of a warp: rows g and g + 8 of K, keys 2t, 2t + 1, 2t + 8, 2t + 9 of V
-  uint32_t k[2][HD / 16], v[4][HD / 32];
-  float ks, vs;
-};
-template <int HD>
-__device__ __forceinline__ void q8_load(Q8Keys<HD>& x, const Q8View& c, const uint8_t* kh, const uint8_t* vh, const float* ksh, const float* vsh, int j0, int g, int t) {
-  const int last = c.slots - 1;
-#pragma unroll
-  for (int i = 0; i < 2; ++i) {
-    const uint8_t* row = kh + (long long)min(j0 + 8 * i + g, last) * HD + 16 * t;
-#pragma unroll
-    for (int m = 0; m < HD / 64; ++m) {
-      const uint4 w = *reinterpret_cast<const uint4*>(row + 64 * m);
-      x.k[i][4 * m] = w.x, x.k[i][4 * m + 1] = w.y, x.k[i][4 * m + 2] = w.z, x.k[i][4 * m + 3] = w.w;
-    }
-  }
-#pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    const uint8_t* row = vh + (long long)min(j0 + 2 * t + (i & 1) + 8 * (i >> 1), last) * HD + (HD / 8) * g;
-    if constexpr (HD == 128) {
-      const uint4 w = *reinterpret_cast<const uint4*>(row);
-      x.v[i][0] = w.x, x.v[i][1] = w.y, x.v[i][2] = w.z, x.v[i][3] = w.w;
-    } else {
-      const uint2 w = *reinterpret_cast<const uint2*>(row);
-      x.v[i][0] = w.x, x.v[i][1] = w.y;
-    }
-  }
-  x.ks = ksh[j0 >> c.block_log2], x.vs = vsh[j0 >> c.block_log2];
+__host__ __device__ constexpr int few_ring_bytes() {  // (the warps' sums lie over it in the end)
+  constexpr int ring = kFewWarps * kFewStages * 32 * HD, sums = kFewWarps * 8 * (HD + 4) * 4;
+  return ring > sums ? ring : sums;
 }
+template <int HD, int NT>
+__host__ __device__ constexpr int few_smem_bytes() { return few_ring_bytes<HD>() + (NT > 2 ? NT * HD / 16 * 256 : 0); }
+
+__device__ __forceinline__ void cp_async16_cg(uint32_t to, const void* from) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(to), "l"(from) : "memory");
+}
+// Where the 16-byte piece c of row `row` of a group lies.
+template <int HD>
+__device__ __forceinline__ uint32_t few_place(int row, int c) { return row * HD + ((c ^ (HD == 128 ? row & 7 : (row >> 1) & 3)) << 4); }
 
 template <bool E4M3, int HD, int NT>
-__global__ void __launch_bounds__(32 * kQ8Warps) q8_attention_kernel(const __grid_constant__ Q8AttnParams p) {
-  constexpr int kSteps = HD / 16, kRows = 8 * NT, kPitch = HD + 4;
-  __shared__ float os[kQ8Warps][8][kPitch];
-  __shared__ float wm[kQ8Warps][kRows], wl[kQ8Warps][kRows];
+__global__ void __launch_bounds__(kFewThreads, NT == 1 ? 4 : NT == 2 ? 3 : 2) q8_attention_kernel(const __grid_constant__ Q8AttnParams p) {
+  constexpr int kSteps = HD / 16, kRows = 8 * NT, kPitch = HD + 4, kPieces = HD / 16;
+  constexpr bool kQShared = NT > 2;
+  extern __shared__ __align__(128) uint8_t ring[];
+  __shared__ float wm[kFewWarps][kRows], wl[kFewWarps][kRows];
+  float(*const os)[8][kPitch] = reinterpret_cast<float(*)[8][kPitch]>(ring);
+  uint2* const q_frag = reinterpret_cast<uint2*>(ring + few_ring_bytes<HD>());  // [tile][step][lane]
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
   const int split = blockIdx.x % p.ns, tile = blockIdx.x / p.ns, qt = tile % p.q_tiles, bh = tile / p.q_tiles;
@@ -65,201 +56,267 @@ __global__ void __launch_bounds__(32 * kQ8Warps) q8_attention_kernel(const __gri
   asm volatile("griddepcontrol.wait;" ::: "memory");
   const long long start = p.start[b], count = p.n_new == nullptr ? p.T : min((long long)p.T, p.n_new[b]);
   const int keys = q8_seen_by(p, start, count, r0, r0 + kRows);
-  const int share = ((keys + p.ns - 1) / p.ns + 63) & ~63, k0 = min(keys, split * share), k1 = min(keys, k0 + share);
+  const int share = ((keys + p.ns - 1) / p.ns + 16 * kFewWarps - 1) / (16 * kFewWarps) * (16 * kFewWarps), k0 = min(keys, split * share), k1 = min(keys, k0 + share);
+  // groups of this warp: 16 keys from first + 64 j on
+  const int first = k0 + 16 * warp, steps = first < k1 ? (k1 - first + 16 * kFewWarps - 1) / (16 * kFewWarps) : 0;
+  const uint32_t base = smem_u32(ring) + warp * kFewStages * 32 * HD;
+  const uint8_t *const kh = p.c.k + (long long)bh * p.c.slots * HD, *const vh = p.c.v + (long long)bh * p.c.slots * HD;
+  auto bring = [&](int j) {
+    if (j < steps) {
+      const uint32_t to = base + (j % kFewStages) * 32 * HD;
+      const int j0 = first + 16 * kFewWarps * j, c = lane % kPieces;
+#pragma unroll
+      for (int i = 0; i < kPieces / 2; ++i) {
+        const int row = lane / kPieces + i * (32 / kPieces);
+        const long long off = (long long)min(j0 + row, p.c.slots - 1) * HD + 16 * c;
+        cp_async16_cg(to + few_place<HD>(row, c), kh + off);
+        cp_async16_cg(to + 16 * HD + few_place<HD>(row, c), vh + off);
+      }
+    }
+    asm volatile("cp.async.commit_group;" ::: "memory");
+  };
+#pragma unroll
+  for (int j = 0; j < kFewStages - 1; ++j) bring(j);
 
-  // ---- the query rows as fp16 fragments, and what their dot products are to be multiplied with
-  uint32_t qf[NT][kSteps][2];
-  float factor[NT][2];
-  int lim[NT][2];
+  float o[NT][kSteps][4] = {}, m[NT][2], l[NT][2] = {}, R = 0.f, inv_R = 0.f;
+  {
+    // ---- the query rows as fp16 fragments, and what their dot products are to be multiplied with
+    uint32_t qf[kQShared ? 1 : NT][kSteps][2];
+    float factor[NT][2];
+    int lim[NT][2];
 #pragma unroll
-  for (int n = 0; n < NT; ++n) {
-    const int r = r0 + 8 * n + g;
-    float f[HD / 4];
-    uint32_t most = 0;
-    if (r < p.rows && r / p.G < count) {
-      const int tok = r / p.G;
-      const uint16_t* row = p.q + ((long long)b * p.T + tok) * p.ldq + (long long)(h * p.G + r - tok * p.G) * HD + 16 * t;
+    for (int n = 0; n < NT; ++n) {
+      const int r = r0 + 8 * n + g;
+      const bool live = r < p.rows && r / p.G < count;
+      const int tok = live ? r / p.G : 0;
+      const uint16_t* row = p.q + ((long long)b * p.T + tok) * p.ldq + (long long)(h * p.G + (live ? r - tok * p.G : 0)) * HD + (HD / 4) * t;
+      float f[HD / 4];
+      uint32_t most = 0;
 #pragma unroll
-      for (int m = 0; m < HD / 64; ++m) {
+      for (int w = 0; w < HD / 32; ++w) {
+        const uint4 x = live ? *reinterpret_cast<const uint4*>(row + 8 * w) : make_uint4(0, 0, 0, 0);
+        const uint32_t xs[4] = {x.x, x.y, x.z, x.w};
 #pragma unroll
-        for (int w = 0; w < 2; ++w) {
-          const uint4 x = *reinterpret_cast<const uint4*>(row + 64 * m + 8 * w);
-          const uint32_t xs[4] = {x.x, x.y, x.z, x.w};
+        for (int i = 0; i < 4; ++i) {
+          const float2 v = p.bf16 ? q8_up2<true>(xs[i]) : q8_up2<false>(xs[i]);
+          f[8 * w + 2 * i] = v.x, f[8 * w + 2 * i + 1] = v.y;
+          most = max(most, max(__float_as_uint(v.x) & 0x7fffffffu, __float_as_uint(v.y) & 0x7fffffffu));
+        }
+      }
+      most = max(most, __shfl_xor_sync(0xffffffffu, most, 1));
+      most = max(most, __shfl_xor_sync(0xffffffffu, most, 2));
+      const int up = q8_row_up(most, p.bf16);
+      const float mul = __uint_as_float((uint32_t)up << 23), back = __uint_as_float((uint32_t)(254 - up) << 23);
+#pragma unroll
+      for (int s = 0; s < kSteps; ++s) {
+        const uint32_t x = pack_half2(f[4 * s] * mul, f[4 * s + 1] * mul), y = pack_half2(f[4 * s + 2] * mul, f[4 * s + 3] * mul);
+        if constexpr (kQShared) {
+          if (warp == n % kFewWarps) q_frag[(n * kSteps + s) * 32 + lane] = make_uint2(x, y);
+        } else {
+          qf[n][s][0] = x, qf[n][s][1] = y;
+        }
+      }
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        factor[n][i] = __shfl_sync(0xffffffffu, back, 8 * t + 4 * i) * p.scale_log2;
+        const int rc = r0 + 8 * n + 2 * t + i;
+        lim[n][i] = rc < p.rows ? q8_seen(start, count, rc / p.G, p.c.slots) : 0;
+      }
+      m[n][0] = m[n][1] = -INFINITY;
+    }
+    if constexpr (kQShared) __syncthreads();
+    int lim_all = 0x7fffffff;  // keys below it are masked for no row of the warp
+#pragma unroll
+    for (int n = 0; n < NT; ++n) lim_all = min(lim_all, min(lim[n][0], lim[n][1]));
+    lim_all = __reduce_min_sync(0xffffffffu, lim_all);
+
+    const float *ksh = p.c.k_scale + (long long)bh * p.c.n_blocks, *vsh = p.c.v_scale + (long long)bh * p.c.n_blocks;
+    auto block_of = [&](int j) { return (first + 16 * kFewWarps * j) >> p.c.block_log2; };
+    float ks_next = steps > 0 ? ksh[block_of(0)] : 0.f, vs_next = steps > 0 ? vsh[block_of(0)] : 0.f;
+#pragma unroll 1
+    for (int j = 0; j < steps; ++j) {
+      const int j0 = first + 16 * kFewWarps * j;
+      const float ks = ks_next, vs = vs_next;
+      if (j + 1 < steps) ks_next = ksh[block_of(j + 1)], vs_next = vsh[block_of(j + 1)];
+      const uint32_t at = base + (j % kFewStages) * 32 * HD;
+      asm volatile("cp.async.wait_group %0;" ::"n"(kFewStages - 2) : "memory");
+      __syncwarp();  // (everybody's pieces are there, and everybody has done with the group before, whose place the next one takes)
+      bring(j + kFewStages - 1);
+      {
+        // ---- S^T: rows g and g + 8 of K, HD / 4 neighbouring dimensions of each
+        uint32_t kw[2][kSteps];
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+          const int row = 8 * i + g;
+          if constexpr (HD == 128) {
+            lds128(at + few_place<HD>(row, 2 * t), kw[i][0], kw[i][1], kw[i][2], kw[i][3]);
+            lds128(at + few_place<HD>(row, 2 * t + 1), kw[i][4], kw[i][5], kw[i][6], kw[i][7]);
+          } else {
+            lds128(at + few_place<HD>(row, t), kw[i][0], kw[i][1], kw[i][2], kw[i][3]);
+          }
+        }
+        float sc[NT][4] = {};
+#pragma unroll
+        for (int st = 0; st < kSteps; ++st) {
+          const uint32_t w0 = q8_bias<E4M3>(kw[0][st]), w1 = q8_bias<E4M3>(kw[1][st]);
+          const uint32_t a0 = q8_half2<E4M3>(w0, false), a1 = q8_half2<E4M3>(w1, false), a2 = q8_half2<E4M3>(w0, true), a3 = q8_half2<E4M3>(w1, true);
+#pragma unroll
+          for (int n = 0; n < NT; ++n) {
+            if constexpr (kQShared) {
+              const uint2 q = q_frag[(n * kSteps + st) * 32 + lane];
+              mma_16816<false>(sc[n], a0, a1, a2, a3, q.x, q.y);
+            } else {
+              mma_16816<false>(sc[n], a0, a1, a2, a3, qf[n][st][0], qf[n][st][1]);
+            }
+          }
+        }
+        // ---- V: keys 2t, 2t + 1, 2t + 8, 2t + 9, HD / 8 neighbouring dimensions of each
+        uint32_t vw[4][HD / 32];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const int row = 2 * t + (i & 1) + 8 * (i >> 1);
+          if constexpr (HD == 128) lds128(at + 16 * HD + few_place<HD>(row, g), vw[i][0], vw[i][1], vw[i][2], vw[i][3]);
+          else lds64(at + 16 * HD + few_place<HD>(row, g >> 1) + (g & 1) * 8, vw[i][0], vw[i][1]);
+        }
+        // ---- p
+        const bool part = j0 + 16 > lim_all;
+        bool behind = false;
+#pragma unroll
+        for (int n = 0; n < NT; ++n) {
+          const float c[2] = {factor[n][0] * ks, factor[n][1] * ks};
 #pragma unroll
           for (int i = 0; i < 4; ++i) {
-            const float2 v = p.bf16 ? q8_up2<true>(xs[i]) : q8_up2<false>(xs[i]);
-            f[16 * m + 8 * w + 2 * i] = v.x, f[16 * m + 8 * w + 2 * i + 1] = v.y;
-            most = max(most, max(__float_as_uint(v.x) & 0x7fffffffu, __float_as_uint(v.y) & 0x7fffffffu));
+            sc[n][i] *= c[i & 1];
+            if (part && j0 + g + 8 * (i >> 1) >= lim[n][i & 1]) sc[n][i] = -INFINITY;
+            behind |= sc[n][i] > m[n][i & 1] + 8.f;
+          }
+        }
+        if (__any_sync(0xffffffffu, behind)) {
+#pragma unroll
+          for (int n = 0; n < NT; ++n)
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+              float mx = fmaxf(sc[n][i], sc[n][i + 2]);
+#pragma unroll
+              for (int d = 4; d < 32; d <<= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, d));
+              mx = fmaxf(mx, m[n][i]);
+              const float corr = mx == -INFINITY ? 1.f : ex2(m[n][i] - mx);
+              m[n][i] = mx;
+              l[n][i] *= corr;
+#pragma unroll
+              for (int d = 0; d < kSteps; ++d) o[n][d][i] *= corr, o[n][d][i + 2] *= corr;
+            }
+        }
+        if (vs > 16.f * R && vs <= 3.4e38f) {
+          const float corr = R / vs;
+          R = vs, inv_R = 1.f / R;
+#pragma unroll
+          for (int n = 0; n < NT; ++n)
+#pragma unroll
+            for (int d = 0; d < kSteps; ++d)
+#pragma unroll
+              for (int i = 0; i < 4; ++i) o[n][d][i] *= corr;
+        }
+        const float f = vs * inv_R;
+        uint32_t pt[NT][2];
+#pragma unroll
+        for (int n = 0; n < NT; ++n) {
+          float e[4];
+          const float mu[2] = {m[n][0] == -INFINITY ? 0.f : m[n][0], m[n][1] == -INFINITY ? 0.f : m[n][1]};
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const float v = ex2(sc[n][i] - mu[i & 1]);
+            l[n][i & 1] += v;
+            e[i] = v * f;
+            if (part && j0 + g + 8 * (i >> 1) >= lim[n][i & 1]) e[i] = 0.f;  // (a masked place of a block that holds a NaN)
+          }
+          pt[n][0] = transpose8x8(pack_half2(e[0], e[1])), pt[n][1] = transpose8x8(pack_half2(e[2], e[3]));
+        }
+        if (j0 + 16 > keys) {  // (slots that nobody wrote may hold anything)
+#pragma unroll
+          for (int i = 0; i < 4; ++i)
+            if (j0 + 2 * t + (i & 1) + 8 * (i >> 1) >= keys)
+#pragma unroll
+              for (int w = 0; w < HD / 32; ++w) vw[i][w] = 0;
+        }
+        // ---- O^T
+#pragma unroll
+        for (int w = 0; w < HD / 32; ++w) {
+          uint32_t pr[2][2];  // [keys][bytes 0, 1 | 2, 3], interleaved by key
+#pragma unroll
+          for (int i = 0; i < 2; ++i) {
+            pr[i][0] = q8_bias<E4M3>(prmt(vw[2 * i][w], vw[2 * i + 1][w], 0x5140u));
+            pr[i][1] = q8_bias<E4M3>(prmt(vw[2 * i][w], vw[2 * i + 1][w], 0x7362u));
+          }
+#pragma unroll
+          for (int z = 0; z < 2; ++z) {
+            const uint32_t a0 = q8_half2<E4M3>(pr[0][z], false), a1 = q8_half2<E4M3>(pr[0][z], true);
+            const uint32_t a2 = q8_half2<E4M3>(pr[1][z], false), a3 = q8_half2<E4M3>(pr[1][z], true);
+#pragma unroll
+            for (int n = 0; n < NT; ++n) mma_16816<false>(o[n][2 * w + z], a0, a1, a2, a3, pt[n][0], pt[n][1]);
           }
         }
       }
-    } else {
-#pragma unroll
-      for (int i = 0; i < HD / 4; ++i) f[i] = 0.f;
     }
-    most = max(most, __shfl_xor_sync(0xffffffffu, most, 1));
-    most = max(most, __shfl_xor_sync(0xffffffffu, most, 2));
-    const int up = q8_row_up(most, p.bf16);
-    const float mul = __uint_as_float((uint32_t)up << 23), back = __uint_as_float((uint32_t)(254 - up) << 23);
-#pragma unroll
-    for (int s = 0; s < kSteps; ++s) {
-      qf[n][s][0] = pack_half2(f[4 * s] * mul, f[4 * s + 1] * mul);
-      qf[n][s][1] = pack_half2(f[4 * s + 2] * mul, f[4 * s + 3] * mul);
-    }
-#pragma unroll
-    for (int i = 0; i < 2; ++i) {
-      factor[n][i] = __shfl_sync(0xffffffffu, back, 8 * t + 4 * i) * p.scale_log2;
-      const int rc = r0 + 8 * n + 2 * t + i;
-      lim[n][i] = rc < p.rows ? q8_seen(start, count, rc / p.G, p.c.slots) : 0;
-    }
-  }
-
-  const long long base = (long long)bh * p.c.slots * HD;
-  const uint8_t *kh = p.c.k + base, *vh = p.c.v + base;
-  const float *ksh = p.c.k_scale + (long long)bh * p.c.n_blocks, *vsh = p.c.v_scale + (long long)bh * p.c.n_blocks;
-  float o[NT][kSteps][4] = {}, m[NT][2], mu[NT][2], l[NT][2] = {}, R = 0.f, inv_R = 0.f;
-#pragma unroll
-  for (int n = 0; n < NT; ++n) m[n][0] = m[n][1] = -INFINITY, mu[n][0] = mu[n][1] = 0.f;
-
-  Q8Keys<HD> next;
-  int j0 = k0 + 16 * warp;
-  if (j0 < k1) q8_load<HD>(next, p.c, kh, vh, ksh, vsh, j0, g, t);
-#pragma unroll 1
-  for (; j0 < k1; j0 += 16 * kQ8Warps) {
-    Q8Keys<HD> x = next;
-    if (j0 + 16 * kQ8Warps < k1) q8_load<HD>(next, p.c, kh, vh, ksh, vsh, j0 + 16 * kQ8Warps, g, t);
-    // ---- S^T
-    float s[NT][4] = {};
-#pragma unroll
-    for (int st = 0; st < kSteps; ++st) {
-      const uint32_t w0 = q8_bias<E4M3>(x.k[0][st]), w1 = q8_bias<E4M3>(x.k[1][st]);
-      const uint32_t a0 = q8_half2<E4M3>(w0, false), a1 = q8_half2<E4M3>(w1, false), a2 = q8_half2<E4M3>(w0, true), a3 = q8_half2<E4M3>(w1, true);
-#pragma unroll
-      for (int n = 0; n < NT; ++n) mma_16816<false>(s[n], a0, a1, a2, a3, qf[n][st][0], qf[n][st][1]);
-    }
-    // ---- p
-    bool behind = false;
+    asm volatile("cp.async.wait_all;" ::: "memory");
 #pragma unroll
     for (int n = 0; n < NT; ++n)
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        s[n][i] = j0 + g + 8 * (i >> 1) < lim[n][i & 1] ? s[n][i] * (factor[n][i & 1] * x.ks) : -INFINITY;
-        behind |= s[n][i] > m[n][i & 1] + 8.f;
-      }
-    if (__any_sync(0xffffffffu, behind)) {
-#pragma unroll
-      for (int n = 0; n < NT; ++n)
-#pragma unroll
-        for (int i = 0; i < 2; ++i) {
-          float mx = fmaxf(s[n][i], s[n][i + 2]);
-#pragma unroll
-          for (int d = 4; d < 32; d <<= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, d));
-          mx = fmaxf(mx, m[n][i]);
-          const float corr = mx == -INFINITY ? 1.f : ex2(m[n][i] - mx);
-          m[n][i] = mx, mu[n][i] = mx == -INFINITY ? 0.f : mx;
-          l[n][i] *= corr;
-#pragma unroll
-          for (int d = 0; d < kSteps; ++d) o[n][d][i] *= corr, o[n][d][i + 2] *= corr;
-        }
-    }
-    if (x.vs > 16.f * R && x.vs <= 3.4e38f) {
-      const float corr = R / x.vs;
-      R = x.vs, inv_R = 1.f / R;
-#pragma unroll
-      for (int n = 0; n < NT; ++n)
-#pragma unroll
-        for (int d = 0; d < kSteps; ++d)
-#pragma unroll
-          for (int i = 0; i < 4; ++i) o[n][d][i] *= corr;
-    }
-    const float f = x.vs * inv_R;
-    uint32_t pt[NT][2];
-#pragma unroll
-    for (int n = 0; n < NT; ++n) {
-      float e[4];
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const bool in = j0 + g + 8 * (i >> 1) < lim[n][i & 1];  // (a masked place of a block that holds a NaN stays 0)
-        const float v = ex2(s[n][i] - mu[n][i & 1]);
-        l[n][i & 1] += v;
-        e[i] = in ? v * f : 0.f;
-      }
-      pt[n][0] = transpose8x8(pack_half2(e[0], e[1])), pt[n][1] = transpose8x8(pack_half2(e[2], e[3]));
-    }
-    if (j0 + 16 > keys) {  // (slots that nobody wrote may hold anything)
-#pragma unroll
-      for (int i = 0; i < 4; ++i)
-        if (j0 + 2 * t + (i & 1) + 8 * (i >> 1) >= keys)
-#pragma unroll
-          for (int w = 0; w < HD / 32; ++w) x.v[i][w] = 0;
-    }
-    // ---- O^T
-#pragma unroll
-    for (int w = 0; w < HD / 32; ++w) {
-      uint32_t pr[2][2];  // [keys][bytes 0, 1 | 2, 3], interleaved by key
-#pragma unroll
       for (int i = 0; i < 2; ++i) {
-        pr[i][0] = q8_bias<E4M3>(prmt(x.v[2 * i][w], x.v[2 * i + 1][w], 0x5140u));
-        pr[i][1] = q8_bias<E4M3>(prmt(x.v[2 * i][w], x.v[2 * i + 1][w], 0x7362u));
-      }
 #pragma unroll
-      for (int z = 0; z < 2; ++z) {
-        const uint32_t a0 = q8_half2<E4M3>(pr[0][z], false), a1 = q8_half2<E4M3>(pr[0][z], true);
-        const uint32_t a2 = q8_half2<E4M3>(pr[1][z], false), a3 = q8_half2<E4M3>(pr[1][z], true);
-#pragma unroll
-        for (int n = 0; n < NT; ++n) mma_16816<false>(o[n][2 * w + z], a0, a1, a2, a3, pt[n][0], pt[n][1]);
+        for (int d = 4; d < 32; d <<= 1) l[n][i] += __shfl_xor_sync(0xffffffffu, l[n][i], d);
+        if (g == 0) wm[warp][8 * n + 2 * t + i] = m[n][i], wl[warp][8 * n + 2 * t + i] = l[n][i];
       }
-    }
   }
-
-  // ---- the warps' results meet
-#pragma unroll
-  for (int n = 0; n < NT; ++n)
-#pragma unroll
-    for (int i = 0; i < 2; ++i) {
-#pragma unroll
-      for (int d = 4; d < 32; d <<= 1) l[n][i] += __shfl_xor_sync(0xffffffffu, l[n][i], d);
-      if (g == 0) wm[warp][8 * n + 2 * t + i] = m[n][i], wl[warp][8 * n + 2 * t + i] = l[n][i];
-    }
+  // ---- the warps' results meet, over the ring
   __syncthreads();
 #pragma unroll
   for (int n = 0; n < NT; ++n) {
-    float M[2];
+    {
 #pragma unroll
-    for (int i = 0; i < 2; ++i) {
-      M[i] = -INFINITY;
-      for (int w = 0; w < kQ8Warps; ++w) M[i] = fmaxf(M[i], wm[w][8 * n + 2 * t + i]);
-      const float weight = m[n][i] == -INFINITY ? 0.f : ex2(m[n][i] - M[i]) * R;
+      for (int i = 0; i < 2; ++i) {
+        float M = -INFINITY;
+        for (int w = 0; w < kFewWarps; ++w) M = fmaxf(M, wm[w][8 * n + 2 * t + i]);
+        const float weight = m[n][i] == -INFINITY ? 0.f : ex2(m[n][i] - M) * R;
 #pragma unroll
-      for (int d = 0; d < kSteps; ++d)  // dimensions HD / 8 g + 2 d, + 1
-        *reinterpret_cast<float2*>(&os[warp][2 * t + i][(HD / 8) * g + 2 * d]) =
-            m[n][i] == -INFINITY ? make_float2(0.f, 0.f) : make_float2(o[n][d][i] * weight, o[n][d][i + 2] * weight);
+        for (int d = 0; d < kSteps; ++d)  // dimensions HD / 8 g + 2 d, + 1
+          *reinterpret_cast<float2*>(&os[warp][2 * t + i][(HD / 8) * g + 2 * d]) =
+              m[n][i] == -INFINITY ? make_float2(0.f, 0.f) : make_float2(o[n][d][i] * weight, o[n][d][i + 2] * weight);
+      }
     }
     __syncthreads();
-    constexpr int kPer = 8 * HD / (32 * kQ8Warps);  // values of a thread: 4 or 2 neighbours
-    const int row = threadIdx.x / (HD / kPer), d0 = (threadIdx.x - row * (HD / kPer)) * kPer, r = r0 + 8 * n + row;
-    float Mr = -INFINITY, Lr = 0.f, sum[kPer] = {};
-    for (int w = 0; w < kQ8Warps; ++w) Mr = fmaxf(Mr, wm[w][8 * n + row]);
-    for (int w = 0; w < kQ8Warps; ++w) {
-      if (wm[w][8 * n + row] != -INFINITY || wl[w][8 * n + row] != 0.f) Lr += wl[w][8 * n + row] * (Mr == -INFINITY ? 1.f : ex2(wm[w][8 * n + row] - Mr));
+    constexpr int kPer = 8 * HD / (32 * kFewWarps);  // values of a thread: 8 or 4 neighbours
+    {
+      const int row = threadIdx.x / (HD / kPer), d0 = (threadIdx.x - row * (HD / kPer)) * kPer, r = r0 + 8 * n + row;
+      float Mr = -INFINITY, Lr = 0.f, sum[kPer] = {};
+      for (int w = 0; w < kFewWarps; ++w) Mr = fmaxf(Mr, wm[w][8 * n + row]);
 #pragma unroll
-      for (int i = 0; i < kPer; ++i) sum[i] += os[w][row][d0 + i];
-    }
-    if (r < p.rows) {
-      const int tok = r / p.G;
-      if (p.ns == 1) {
-        const float inv = Lr == 0.f ? 0.f : 1.f / Lr;
-        uint16_t* to = p.out + ((long long)b * p.T + tok) * p.ldo + (long long)(h * p.G + r - tok * p.G) * HD + d0;
+      for (int w = 0; w < kFewWarps; ++w) {
+        if (wm[w][8 * n + row] != -INFINITY || wl[w][8 * n + row] != 0.f) Lr += wl[w][8 * n + row] * (Mr == -INFINITY ? 1.f : ex2(wm[w][8 * n + row] - Mr));
 #pragma unroll
-        for (int i = 0; i < kPer; i += 2)
-          *reinterpret_cast<uint32_t*>(to + i) = p.bf16 ? q8_down2<true>(sum[i] * inv, sum[i + 1] * inv) : q8_down2<false>(sum[i] * inv, sum[i + 1] * inv);
-      } else {
-        float* to = p.part + (((long long)bh * p.rows + r) * p.ns + split) * (HD + 4);
-        if (!(Lr == 0.f)) {
-#pragma unroll
-          for (int i = 0; i < kPer; ++i) to[d0 + i] = sum[i];
+        for (int i = 0; i < kPer; i += 4) {
+          const float4 x = *reinterpret_cast<const float4*>(&os[w][row][d0 + i]);
+          sum[i] += x.x, sum[i + 1] += x.y, sum[i + 2] += x.z, sum[i + 3] += x.w;
         }
-        if (d0 == 0) to[HD] = Mr, to[HD + 1] = Lr;
+      }
+      if (r < p.rows) {
+        const int tok = r / p.G;
+        if (p.ns == 1) {
+          const float inv = Lr == 0.f ? 0.f : 1.f / Lr;
+          uint16_t* to = p.out + ((long long)b * p.T + tok) * p.ldo + (long long)(h * p.G + r - tok * p.G) * HD + d0;
+          uint32_t x[kPer / 2];
+#pragma unroll
+          for (int i = 0; i < kPer; i += 2) x[i / 2] = p.bf16 ? q8_down2<true>(sum[i] * inv, sum[i + 1] * inv) : q8_down2<false>(sum[i] * inv, sum[i + 1] * inv);
+          if constexpr (kPer == 8) *reinterpret_cast<uint4*>(to) = make_uint4(x[0], x[1], x[2], x[3]);
+          else *reinterpret_cast<uint2*>(to) = make_uint2(x[0], x[1]);
+        } else {
+          float* to = p.part + (((long long)bh * p.rows + r) * p.ns + split) * (HD + 4);
+          if (!(Lr == 0.f)) {
+#pragma unroll
+            for (int i = 0; i < kPer; i += 4) *reinterpret_cast<float4*>(to + d0 + i) = make_float4(sum[i], sum[i + 1], sum[i + 2], sum[i + 3]);
+          }
+          if (d0 == 0) to[HD] = Mr, to[HD + 1] = Lr;
+        }
       }
     }
     __syncthreads();
@@ -310,7 +367,7 @@ struct Q8Plan {
 static Q8Plan q8_plan(const blr_q8_cache* c, int64_t n_tok, int heads) {
   Q8Plan a = {};
   a.rows = n_tok * (heads / c->kv_heads);
-  a.nt = a.rows <= 8 ? 1 : a.rows <= 64 ? 2 : 0;
+  a.nt = a.rows <= 8 ? 1 : a.rows <= 16 ? 2 : a.rows <= 64 ? 4 : 0;
   const int per = a.nt ? 8 * a.nt : kQ8PromptRows;
   a.q_tiles = (int)((a.rows + per - 1) / per);
   a.tiles = c->n_seq * c->kv_heads * a.q_tiles;
@@ -319,10 +376,11 @@ static Q8Plan q8_plan(const blr_q8_cache* c, int64_t n_tok, int heads) {
 }
 
 template <typename K, typename... A>
-static int launch(K kern, dim3 grid, dim3 block, cudaStream_t st, A... args) {
+static int launch(K kern, dim3 grid, dim3 block, size_t smem, cudaStream_t st, A... args) {
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = grid;
   cfg.blockDim = block;
+  cfg.dynamicSmemBytes = smem;
   cfg.stream = st;
   cudaLaunchAttribute at[1];
   at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
@@ -331,6 +389,20 @@ static int launch(K kern, dim3 grid, dim3 block, cudaStream_t st, A... args) {
   cfg.numAttrs = 1;
   BLR_CUDA_OK(cudaLaunchKernelEx(&cfg, kern, args...));
   return BLR_OK;
+}
+
+template <bool E4M3, int HD, int NT>
+static int launch_few(const Q8AttnParams& p, long long ctas, cudaStream_t st) {
+  static bool configured[64] = {};
+  constexpr int smem = few_smem_bytes<HD, NT>();
+  DeviceInfo di;
+  int rc;
+  if ((rc = device_info(&di))) return rc;
+  if (!configured[di.dev]) {
+    BLR_CUDA_OK(cudaFuncSetAttribute(q8_attention_kernel<E4M3, HD, NT>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
+    configured[di.dev] = true;
+  }
+  return launch(q8_attention_kernel<E4M3, HD, NT>, dim3((unsigned)ctas), dim3(kFewThreads), smem, st, p);
 }
 
 }  // namespace blr
@@ -372,17 +444,20 @@ int blr_attention_q8(const void* q, int64_t ldq, const blr_q8_cache* cache, cons
   p.n_bh = (int)(cache->n_seq * cache->kv_heads);
   p.status = ws == nullptr ? nullptr : static_cast<unsigned*>(ws) + 255;
   const cudaStream_t st = static_cast<cudaStream_t>(stream);
-  const dim3 grid((unsigned)(a.tiles * a.ns)), block(32 * kQ8Warps);
-  auto go = [&](auto kernel) { return launch(kernel, grid, block, st, p); };
-#define BLR_Q8_ATTN(E4, HD) (a.nt == 1 ? go(q8_attention_kernel<E4, HD, 1>) : go(q8_attention_kernel<E4, HD, 2>))
-  if (a.nt == 0) rc = q8_launch_prompt(p, cache->head_dim, cache->code, st);
-  else if (cache->code == BLR_Q8_E4M3) rc = cache->head_dim == 128 ? BLR_Q8_ATTN(true, 128) : BLR_Q8_ATTN(true, 64);
-  else rc = cache->head_dim == 128 ? BLR_Q8_ATTN(false, 128) : BLR_Q8_ATTN(false, 64);
+  if (a.nt == 0) {
+    rc = q8_launch_prompt(p, cache->head_dim, cache->code, st);
+  } else {
+    const long long ctas = a.tiles * a.ns;
+#define BLR_Q8_ATTN(E4, HD) \
+  (a.nt == 1 ? launch_few<E4, HD, 1>(p, ctas, st) : a.nt == 2 ? launch_few<E4, HD, 2>(p, ctas, st) : launch_few<E4, HD, 4>(p, ctas, st))
+    if (cache->code == BLR_Q8_E4M3) rc = cache->head_dim == 128 ? BLR_Q8_ATTN(true, 128) : BLR_Q8_ATTN(true, 64);
+    else rc = cache->head_dim == 128 ? BLR_Q8_ATTN(false, 128) : BLR_Q8_ATTN(false, 64);
 #undef BLR_Q8_ATTN
+  }
   if (rc || a.ns == 1) return rc;
   const long long total = cache->n_seq * cache->kv_heads * a.rows;
   const dim3 cgrid((unsigned)((total + 7) / 8));
-  return cache->head_dim == 128 ? launch(q8_combine_kernel<128>, cgrid, dim3(256), st, p, total) : launch(q8_combine_kernel<64>, cgrid, dim3(256), st, p, total);
+  return cache->head_dim == 128 ? launch(q8_combine_kernel<128>, cgrid, dim3(256), 0, st, p, total) : launch(q8_combine_kernel<64>, cgrid, dim3(256), 0, st, p, total);
 }
 
 }  // extern "C"
