@@ -51,12 +51,33 @@ __global__ void __launch_bounds__(kFewThreads, NT == 1 ? 4 : NT == 2 ? 3 : 2) q8
   uint2* const q_frag = reinterpret_cast<uint2*>(ring + few_ring_bytes<HD>());  // [tile][step][lane]
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
-  const int split = blockIdx.x % p.ns, tile = blockIdx.x / p.ns, qt = tile % p.q_tiles, bh = tile / p.q_tiles;
+  const int tiles = p.n_bh * p.q_tiles, split = blockIdx.x / tiles, tile = blockIdx.x - split * tiles, qt = tile % p.q_tiles, bh = tile / p.q_tiles;
   const int b = bh / p.c.kv_heads, h = bh - b * p.c.kv_heads, r0 = qt * kRows;
   asm volatile("griddepcontrol.wait;" ::: "memory");
   const long long start = p.start[b], count = p.n_new == nullptr ? p.T : min((long long)p.T, p.n_new[b]);
   const int keys = q8_seen_by(p, start, count, r0, r0 + kRows);
-  const int share = ((keys + p.ns - 1) / p.ns + 16 * kFewWarps - 1) / (16 * kFewWarps) * (16 * kFewWarps), k0 = min(keys, split * share), k1 = min(keys, k0 + share);
+  int share = keys;
+  if (p.ns > 1 && p.n_seq == 1) {
+    share = ((keys + p.ns - 1) / p.ns + 16 * kFewWarps - 1) / (16 * kFewWarps) * (16 * kFewWarps);
+  } else if (p.ns > 1) {
+    // as many keys for every CTA, whatever its sequence's length: all of them over the CTAs that the SMs hold, but a sequence has no more than ns CTAs
+    float total = 0.f;
+    for (int i = lane; i < p.n_seq; i += 32) {
+      const long long n = p.n_new == nullptr ? p.T : min((long long)p.T, p.n_new[i]);
+      total += (float)q8_seen_by(p, p.start[i], n, 0, p.rows);
+    }
+#pragma unroll
+    for (int d = 16; d > 0; d >>= 1) total += __shfl_xor_sync(0xffffffffu, total, d);
+    const float even = total * (float)(p.c.kv_heads * p.q_tiles) / (float)p.room;
+    const int n = max(1, min(p.ns, (int)((float)keys / fmaxf(even, 1.f))));  // (rounded down: all of them together are no more than the SMs hold)
+    share = ((keys + n - 1) / n + 16 * kFewWarps - 1) / (16 * kFewWarps) * (16 * kFewWarps);
+  }
+  const int k0 = (int)min((long long)keys, (long long)split * share), k1 = min(keys, k0 + min(share, keys - k0));
+  if (p.ns > 1 && k0 >= k1) {  // no keys for this CTA: its rows say so
+    if (threadIdx.x < kRows && r0 + threadIdx.x < p.rows)
+      *reinterpret_cast<float2*>(p.part + (((long long)bh * p.rows + r0 + threadIdx.x) * p.ns + split) * (HD + 4) + HD) = make_float2(-INFINITY, 0.f);
+    return;
+  }
   // groups of this warp: 16 keys from first + 64 j on
   const int first = k0 + 16 * warp, steps = first < k1 ? (k1 - first + 16 * kFewWarps - 1) / (16 * kFewWarps) : 0;
   const uint32_t base = smem_u32(ring) + warp * kFewStages * 32 * HD;
@@ -77,6 +98,9 @@ __global__ void __launch_bounds__(kFewThreads, NT == 1 ? 4 : NT == 2 ? 3 : 2) q8
   };
 #pragma unroll
   for (int j = 0; j < kFewStages - 1; ++j) bring(j);
+  const float *ksh = p.c.k_scale + (long long)bh * p.c.n_blocks, *vsh = p.c.v_scale + (long long)bh * p.c.n_blocks;
+  auto block_of = [&](int j) { return (first + 16 * kFewWarps * j) >> p.c.block_log2; };
+  float ks_next = steps > 0 ? ksh[block_of(0)] : 0.f, vs_next = steps > 0 ? vsh[block_of(0)] : 0.f;
 
   float o[NT][kSteps][4] = {}, m[NT][2], l[NT][2] = {}, R = 0.f, inv_R = 0.f;
   {
@@ -130,9 +154,6 @@ __global__ void __launch_bounds__(kFewThreads, NT == 1 ? 4 : NT == 2 ? 3 : 2) q8
     for (int n = 0; n < NT; ++n) lim_all = min(lim_all, min(lim[n][0], lim[n][1]));
     lim_all = __reduce_min_sync(0xffffffffu, lim_all);
 
-    const float *ksh = p.c.k_scale + (long long)bh * p.c.n_blocks, *vsh = p.c.v_scale + (long long)bh * p.c.n_blocks;
-    auto block_of = [&](int j) { return (first + 16 * kFewWarps * j) >> p.c.block_log2; };
-    float ks_next = steps > 0 ? ksh[block_of(0)] : 0.f, vs_next = steps > 0 ? vsh[block_of(0)] : 0.f;
 #pragma unroll 1
     for (int j = 0; j < steps; ++j) {
       const int j0 = first + 16 * kFewWarps * j;
@@ -300,9 +321,9 @@ __global__ void __launch_bounds__(kFewThreads, NT == 1 ? 4 : NT == 2 ? 3 : 2) q8
         }
       }
       if (r < p.rows) {
-        const int tok = r / p.G;
         if (p.ns == 1) {
           const float inv = Lr == 0.f ? 0.f : 1.f / Lr;
+          const int tok = r / p.G;
           uint16_t* to = p.out + ((long long)b * p.T + tok) * p.ldo + (long long)(h * p.G + r - tok * p.G) * HD + d0;
           uint32_t x[kPer / 2];
 #pragma unroll
@@ -332,18 +353,36 @@ __global__ void __launch_bounds__(256) q8_combine_kernel(const __grid_constant__
   const long long row = (long long)blockIdx.x * 8 + (threadIdx.x >> 5);
   if (row >= total) return;
   const float* from = p.part + row * p.ns * (HD + 4);
-  float M = -INFINITY, L = 0.f, sum[HD / 32] = {};
-  for (int s = lane; s < p.ns; s += 32) M = fmaxf(M, from[s * (HD + 4) + HD]);
+  // lane s has the weight of splits s and s + 32
+  float w[2], M = -INFINITY, L = 0.f, sum[HD / 32] = {};
+  float2 ml[2];
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    ml[i] = lane + 32 * i < p.ns ? *reinterpret_cast<const float2*>(from + (lane + 32 * i) * (HD + 4) + HD) : make_float2(-INFINITY, 0.f);
+    M = fmaxf(M, ml[i].x);
+  }
 #pragma unroll
   for (int d = 16; d > 0; d >>= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, d));
-  for (int s = 0; s < p.ns; ++s) {
-    const float* x = from + s * (HD + 4);
-    const float ls = x[HD + 1];
-    if (ls == 0.f) continue;
-    const float w = M == -INFINITY ? 1.f : ex2(x[HD] - M);
-    L += ls * w;
 #pragma unroll
-    for (int i = 0; i < HD / 32; ++i) sum[i] += x[(HD / 32) * lane + i] * w;
+  for (int i = 0; i < 2; ++i) {
+    w[i] = ml[i].y == 0.f ? 0.f : M == -INFINITY || ml[i].y != ml[i].y ? 1.f : ex2(ml[i].x - M);
+    L += ml[i].y == 0.f ? 0.f : ml[i].y * w[i];
+  }
+#pragma unroll
+  for (int d = 16; d > 0; d >>= 1) L += __shfl_xor_sync(0xffffffffu, L, d);
+#pragma unroll 8
+  for (int s = 0; s < p.ns; ++s) {
+    const float ws = __shfl_sync(0xffffffffu, s < 32 ? w[0] : w[1], s & 31);
+    float x[HD / 32];
+    if constexpr (HD == 128) {
+      const float4 v = *reinterpret_cast<const float4*>(from + s * (HD + 4) + 4 * lane);
+      x[0] = v.x, x[1] = v.y, x[2] = v.z, x[3] = v.w;
+    } else {
+      const float2 v = *reinterpret_cast<const float2*>(from + s * (HD + 4) + 2 * lane);
+      x[0] = v.x, x[1] = v.y;
+    }
+#pragma unroll
+    for (int i = 0; i < HD / 32; ++i) sum[i] += ws == 0.f ? 0.f : x[i] * ws;  // (a split without keys has left its sums as they were)
   }
   const float inv = L == 0.f ? 0.f : 1.f / L;
   const long long bh = row / p.rows, r = row - bh * p.rows, b = bh / p.c.kv_heads, h = bh - b * p.c.kv_heads, tok = r / p.G;
@@ -353,25 +392,27 @@ __global__ void __launch_bounds__(256) q8_combine_kernel(const __grid_constant__
     *reinterpret_cast<uint32_t*>(to + i) = p.bf16 ? q8_down2<true>(sum[i] * inv, sum[i + 1] * inv) : q8_down2<false>(sum[i] * inv, sum[i + 1] * inv);
 }
 
-// CTAs over which a row's keys are split: as many as fill the SMs, with at least 256 keys each (512 in the prompt kernel).
-static int q8_splits(long long tiles, int slots, bool prompt) {
-  const long long room = (prompt ? 1ll : 2ll) * sm_count(), least = prompt ? 512 : 256;
-  long long ns = room / tiles;
-  if (ns > (slots + least - 1) / least) ns = (slots + least - 1) / least;
-  return ns < 1 ? 1 : ns > kMaxSplits ? kMaxSplits : (int)ns;
-}
 struct Q8Plan {
-  int nt, q_tiles, ns;  // nt: column tiles of 8 rows of the kernel here, 0: the prompt kernel
+  int nt, q_tiles, ns, room;  // nt: column tiles of 8 rows of the kernel here, 0: the prompt kernel; ns: CTAs that may share a row tile's keys
   long long rows, tiles;
 };
+// Few row tiles share their keys out over more CTAs, as many as the SMs hold at a time (4, 3, 2 or 1 of a kind); a second kernel sums the parts.  The host does not
+// know the sequences' lengths: a tile may have half as many CTAs again as its even share, and the kernel here shares by the
+// lengths.  Up to 512 slots a second launch (3 us) costs more than it saves (1 sequence x 32 heads x 300 keys: 2 CTAs a head TODO us, one TODO).
 static Q8Plan q8_plan(const blr_q8_cache* c, int64_t n_tok, int heads) {
   Q8Plan a = {};
   a.rows = n_tok * (heads / c->kv_heads);
-  a.nt = a.rows <= 8 ? 1 : a.rows <= 16 ? 2 : a.rows <= 64 ? 4 : 0;
+  a.nt = a.rows <= 8 ? 1 : a.rows <= 16 ? 2 : a.rows <= 32 ? 4 : 0;
   const int per = a.nt ? 8 * a.nt : kQ8PromptRows;
   a.q_tiles = (int)((a.rows + per - 1) / per);
   a.tiles = c->n_seq * c->kv_heads * a.q_tiles;
-  a.ns = a.tiles > 0 ? q8_splits(a.tiles, c->slots, a.nt == 0) : 1;
+  a.room = (a.nt == 1 ? 4 : a.nt == 2 ? 3 : a.nt == 4 ? 2 : 1) * sm_count();
+  long long ns = a.tiles > 0 ? a.room / a.tiles : 1;
+  const long long least = a.nt ? 128 : 512, most = (c->slots + least - 1) / least;  // keys of a CTA
+  if (a.nt && ns > 1 && c->n_seq > 1) ns += ns / 2;
+  if (c->slots <= 512) ns = 1;
+  if (ns > most) ns = most;
+  a.ns = ns < 1 ? 1 : ns > kMaxSplits ? kMaxSplits : (int)ns;
   return a;
 }
 
@@ -441,7 +482,7 @@ int blr_attention_q8(const void* q, int64_t ldq, const blr_q8_cache* cache, cons
   p.part = static_cast<float*>(scratch);
   p.scale_log2 = scale * 1.4426950408889634f;
   p.T = (int)n_tok, p.H = heads, p.G = heads / cache->kv_heads, p.rows = (int)a.rows, p.q_tiles = a.q_tiles, p.ns = a.ns, p.bf16 = dtype == BLR_DTYPE_BF16;
-  p.n_bh = (int)(cache->n_seq * cache->kv_heads);
+  p.n_bh = (int)(cache->n_seq * cache->kv_heads), p.n_seq = (int)cache->n_seq, p.room = a.room;
   p.status = ws == nullptr ? nullptr : static_cast<unsigned*>(ws) + 255;
   const cudaStream_t st = static_cast<cudaStream_t>(stream);
   if (a.nt == 0) {

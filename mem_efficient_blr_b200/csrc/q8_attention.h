@@ -13,7 +13,8 @@ struct Q8AttnParams {
   float* part;       // ns > 1: of each (sequence, kv head, row, split) hd sums, the maximum that they are taken against, the sum of the weights, 2 free
   unsigned* status;  // NULL, or where a wait that gave up is noted
   float scale_log2;
-  int T, H, G, rows, q_tiles, ns, bf16, n_bh;
+  int T, H, G, rows, q_tiles, ns, bf16, n_bh, n_seq;
+  int room;  // CTAs that the SMs hold
 };
 
 __device__ __forceinline__ float ex2(float x) {
