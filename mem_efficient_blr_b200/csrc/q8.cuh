@@ -41,7 +41,7 @@ __device__ __forceinline__ void q8_floats(uint32_t w, float (&f)[4]) {
   const float2 x = __half22float2(*reinterpret_cast<const __half2*>(&lo)), y = __half22float2(*reinterpret_cast<const __half2*>(&hi));
   f[0] = x.x, f[1] = x.y, f[2] = y.x, f[3] = y.y;
 }
-// Four numbers in a code's range (or beyond it by a rounding) as codes, to nearest even.
+// Four numbers in a code's range (or beyond it by less than half a step) as codes, to nearest even.
 template <bool E4M3>
 __device__ __forceinline__ uint32_t q8_codes(const float (&f)[4]) {
   if constexpr (E4M3) {
@@ -53,7 +53,7 @@ __device__ __forceinline__ uint32_t q8_codes(const float (&f)[4]) {
     uint32_t b[4];
 #pragma unroll
     for (int i = 0; i < 4; ++i)  // 1.5 * 2^23 + x is rounded to a whole number, whose last byte is x's
-      b[i] = __float_as_uint(__fadd_rn(fminf(fmaxf(f[i], -127.f), 127.f), 12582912.f));
+      b[i] = __float_as_uint(__fadd_rn(f[i], 12582912.f));
     return prmt(prmt(b[0], b[1], 0x0040u), prmt(b[2], b[3], 0x0040u), 0x5410u);
   }
 }

@@ -41,7 +41,7 @@ struct AppendParams {
   long long ldq, ldk, ldv, ldo;
   const float *cos_t, *sin_t;
   const long long *start, *n_new;
-  long long n_seq, units;  // units: blocks to look at, over sequences, heads, keys and values
+  uint32_t rows, units;  // units: blocks to look at, over sequences, heads, keys and values
   int T, H, blocks_per, q_heads, q_parts;
   unsigned unit_ctas;
 };
@@ -95,22 +95,31 @@ __device__ __forceinline__ void store_codes(uint8_t* row, int e, const float (&a
   }
 }
 
-// CTAs [0, unit_ctas): a warp has 16 slots of a block of one head's keys or values, a block's warps meet over its maximum; heads run fastest, so that the
+__device__ __forceinline__ float max_nan(float a, float b) {
+  float r;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+  return r;
+}
+
+// CTAs [0, unit_ctas): a warp has 8 slots of a block of one head's keys or values, a block's warps meet over its maximum; heads run fastest, so that the
 // warps of a CTA share their tokens' angles and read neighbouring parts of a row.  The rest: a warp rotates q_heads heads of a row of q.
-// Bound by HBM; a value is read once and held in registers between the maximum and its code.
+// Bound by HBM; a value is read once and held in registers between the maximum and its code.  (16 slots a warp: 110 registers, half the warps; a prompt of
+// 2048 tokens x 32 heads TODO us against TODO.)
+static constexpr int kAppendWarps = 16, kAppendThreads = 32 * kAppendWarps, kSlotsLog2 = 3, kSteps = 2;  // kSteps: of 4 slots
+
 template <bool BF16, bool E4M3, int E>
-__global__ void __launch_bounds__(256) rope_append_q8_kernel(const __grid_constant__ AppendParams p) {
-  __shared__ uint32_t most[8];
+__global__ void __launch_bounds__(kAppendThreads, 2) rope_append_q8_kernel(const __grid_constant__ AppendParams p) {
+  __shared__ uint32_t most[kAppendWarps];
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   constexpr int hd = 16 * E;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, sub = lane >> 3, e = lane & 7;
   asm volatile("griddepcontrol.wait;" ::: "memory");
   if (blockIdx.x >= p.unit_ctas) {
-    const long long item = (long long)(blockIdx.x - p.unit_ctas) * 8 + warp, r = item / p.q_parts;
-    const int h0 = (int)(item - r * p.q_parts) * p.q_heads;
-    if (r >= p.n_seq * p.T) return;
-    const long long b = r / p.T, t = r - b * p.T;
-    const long long slot = p.start[b] + t;
+    // (32 bits: the divisions of 64 took a quarter of the instructions)
+    const uint32_t item = (blockIdx.x - p.unit_ctas) * kAppendWarps + warp, row = item / (uint32_t)p.q_parts, b = row / (uint32_t)p.T, t = row - b * p.T;
+    const int h0 = (int)(item - row * p.q_parts) * p.q_heads;
+    if (row >= p.rows) return;
+    const long long r = row, slot = p.start[b] + t;
     const bool live = (p.n_new == nullptr || t < p.n_new[b]) && slot >= 0 && slot < p.c.slots;
     float c[E] = {}, s[E] = {};
     if (live) {
@@ -135,26 +144,25 @@ __global__ void __launch_bounds__(256) rope_append_q8_kernel(const __grid_consta
     }
     return;
   }
-  // ---- 16 slots of a block
-  const int wl = p.c.block_log2 - 4, per_cta = 8 >> wl, w = warp & ((1 << wl) - 1);
-  const long long unit = (long long)blockIdx.x * per_cta + (warp >> wl);
+  // ---- 8 slots of a block
+  const int wl = p.c.block_log2 - kSlotsLog2, per_cta = kAppendWarps >> wl, w = warp & ((1 << wl) - 1);
+  const uint32_t unit = blockIdx.x * per_cta + (warp >> wl);
   const bool mine = unit < p.units;
-  long long u = mine ? unit : 0;
-  const int h = (int)(u % p.c.kv_heads);
-  u /= p.c.kv_heads;
-  const bool is_v = u & 1;
-  u >>= 1;
-  const int j = (int)(u % p.blocks_per);
-  const long long b = u / p.blocks_per;
+  uint32_t u = mine ? unit : 0, v = u / (uint32_t)p.c.kv_heads;
+  const int h = (int)(u - v * p.c.kv_heads);
+  const bool is_v = v & 1;
+  v >>= 1;
+  const long long b = v / (uint32_t)p.blocks_per;
+  const int j = (int)(v - (uint32_t)b * p.blocks_per);
   const long long start = p.start[b], count = p.n_new == nullptr ? p.T : max(0ll, min((long long)p.T, p.n_new[b]));
   const long long first = max(start, 0ll), end = min(start + count, (long long)p.c.slots);  // the new slots
-  const long long block = (first >> p.c.block_log2) + j, s0 = (block << p.c.block_log2) + 16 * w;
+  const long long block = (first >> p.c.block_log2) + j, s0 = (block << p.c.block_log2) + (w << kSlotsLog2);
   const bool touched = mine && first < end && (block << p.c.block_log2) < end;  // (the same for all warps of a block)
-  float x[4][E], y[4][E];
-  uint32_t top = 0;
+  float x[kSteps][E], y[kSteps][E];
+  float big = 0.f;  // (max.NaN: a block with a NaN has it for its maximum, and reads back as NaN throughout)
   const long long head = b * p.c.kv_heads + h;
 #pragma unroll
-  for (int i = 0; i < 4; ++i) {
+  for (int i = 0; i < kSteps; ++i) {
     const long long slot = s0 + 4 * i + sub;
     if (touched && slot >= first && slot < end) {
       const long long r = b * p.T + (slot - start);
@@ -168,11 +176,10 @@ __global__ void __launch_bounds__(256) rope_append_q8_kernel(const __grid_consta
         rotate<E>(x[i], y[i], c, s);
       }
 #pragma unroll
-      for (int z = 0; z < E; ++z)  // as bits, where a NaN is above everything: a block with one reads back as NaN throughout
-        top = max(top, max(__float_as_uint(x[i][z]) & 0x7fffffffu, __float_as_uint(y[i][z]) & 0x7fffffffu));
+      for (int z = 0; z < E; ++z) big = max_nan(big, fabsf(x[i][z])), big = max_nan(big, fabsf(y[i][z]));
     }
   }
-  top = __reduce_max_sync(0xffffffffu, top);
+  uint32_t top = __reduce_max_sync(0xffffffffu, __float_as_uint(big) & 0x7fffffffu);
   if (lane == 0) most[warp] = top;
   __syncthreads();
   if (!touched) return;
@@ -187,12 +194,16 @@ __global__ void __launch_bounds__(256) rope_append_q8_kernel(const __grid_consta
   const bool grown = __float_as_uint(after) > __float_as_uint(before);
   const float ratio = __fmul_rn(before, inverse);
 #pragma unroll
-  for (int i = 0; i < 4; ++i) {
+  for (int i = 0; i < kSteps; ++i) {
     const long long slot = s0 + 4 * i + sub;
     uint8_t* const row = codes + (4 * i + sub) * hd;
     if (slot >= first && slot < end) {
 #pragma unroll
-      for (int z = 0; z < E; ++z) x[i][z] = inverse == 0.f ? 0.f : __fmul_rn(x[i][z], inverse), y[i][z] = inverse == 0.f ? 0.f : __fmul_rn(y[i][z], inverse);
+      for (int z = 0; z < E; ++z) x[i][z] = __fmul_rn(x[i][z], inverse), y[i][z] = __fmul_rn(y[i][z], inverse);
+      if (inverse == 0.f) {  // (what is no number has code 0)
+#pragma unroll
+        for (int z = 0; z < E; ++z) x[i][z] = y[i][z] = 0.f;
+      }
       store_codes<E4M3, E>(row, e, x[i], y[i]);
     } else if (grown && slot < first) {
 #pragma unroll
@@ -210,7 +221,7 @@ __global__ void __launch_bounds__(256) rope_append_q8_kernel(const __grid_consta
     }
   }
   // (every warp of the block has read the old scale by now only if they meet again)
-  if (wl > 0) asm volatile("bar.sync %0, %1;" ::"r"(1 + (warp >> wl)), "r"(32 << wl) : "memory");
+  asm volatile("bar.sync %0, %1;" ::"r"(1 + (warp >> wl)), "r"(32 << wl) : "memory");
   if (w == 0 && lane == 0) *scale = after;
 }
 
@@ -281,23 +292,23 @@ int blr_rope_append_q8(const void* q, int64_t ldq, const void* k, int64_t ldk, c
   p.ldq = ldq, p.ldk = ldk, p.ldv = ldv, p.ldo = ldo;
   p.cos_t = cos_table, p.sin_t = sin_table;
   p.start = reinterpret_cast<const long long*>(start), p.n_new = reinterpret_cast<const long long*>(n_new);
-  p.n_seq = cache->n_seq, p.T = (int)n_tok, p.H = heads;
+  p.T = (int)n_tok, p.H = heads;
   // T neighbouring slots lie in at most this many blocks
   p.blocks_per = (int)(((n_tok + cache->block - 2) >> p.c.block_log2) + 1);
-  p.units = p.n_seq * p.blocks_per * 2 * p.c.kv_heads;
-  const int per_cta = 8 >> (p.c.block_log2 - 4);
-  const long long unit_ctas = (p.units + per_cta - 1) / per_cta;
-  // a row's heads by as few warps as leave every SM its eight
-  const long long rows = p.n_seq * n_tok;
+  const long long units = cache->n_seq * p.blocks_per * 2 * p.c.kv_heads, rows = cache->n_seq * n_tok;
+  const int per_cta = kAppendWarps >> (p.c.block_log2 - kSlotsLog2);
+  const long long unit_ctas = (units + per_cta - 1) / per_cta;
+  // a row's heads by as few warps as leave every SM its sixteen
   p.q_heads = 4;
   while (p.q_heads < 16 && rows * ((heads + 2 * p.q_heads - 1) / (2 * p.q_heads)) >= 16ll * sm_count()) p.q_heads *= 2;
   p.q_parts = (heads + p.q_heads - 1) / p.q_heads;
-  const long long ctas = unit_ctas + (rows * p.q_parts + 7) / 8;
-  BLR_REQUIRE(ctas < (1ll << 31), BLR_ERR_SHAPE, "too many tokens");
+  const long long ctas = unit_ctas + (rows * p.q_parts + kAppendWarps - 1) / kAppendWarps;
+  BLR_REQUIRE(ctas < (1ll << 31) / kAppendWarps && units < (1ll << 31) && rows * p.q_parts < (1ll << 31) - kAppendWarps, BLR_ERR_SHAPE, "too many tokens");
+  p.units = (uint32_t)units, p.rows = (uint32_t)rows;
   p.unit_ctas = (unsigned)unit_ctas;
   const cudaStream_t st = static_cast<cudaStream_t>(stream);
   const bool bf = dtype == BLR_DTYPE_BF16, e4 = cache->code == BLR_Q8_E4M3;
-  auto go = [&](auto kernel) { return launch(kernel, dim3((unsigned)ctas), dim3(256), st, p); };
+  auto go = [&](auto kernel) { return launch(kernel, dim3((unsigned)ctas), dim3(kAppendThreads), st, p); };
   if (cache->head_dim == 128)
     return bf ? (e4 ? go(rope_append_q8_kernel<true, true, 8>) : go(rope_append_q8_kernel<true, false, 8>))
               : (e4 ? go(rope_append_q8_kernel<false, true, 8>) : go(rope_append_q8_kernel<false, false, 8>));
