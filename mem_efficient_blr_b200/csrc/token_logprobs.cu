@@ -1,6 +1,7 @@
 // Log probabilities of given tokens, entropy and likeliest tokens of rows of logits.
 //   M = max x,  S = sum e^(x - M),  log p(i) = (x_i - M) - log S,  H = log S - (sum e^(x - M) (x - M)) / S
-// Differences, exponentials and sums are fp32 (x - M is taken before it is scaled for ex2: M log2 e rounded once would be off by 2^-8 for logits of 10^4).
+// in fp32, with one multiply-add ahead of ex2: t = x c - m for c = log2 e and m = M c rounded, which is (x - M) c + d with the same d = M c - m for the whole row, found
+// exactly by a multiply-add.  So sum 2^t = 2^d S, log S = log sum 2^t - d log 2, and H = log sum 2^t - log 2 (sum 2^t t) / sum 2^t, where d has dropped out.
 // Order of the likeliest: falling value (NaN above everything, -0 equal to 0), ties by rising id.
 //
 // A cluster of 1 to 8 CTAs takes a row: each reads its part once into shared memory, keeping the maximum of what every thread reads, and works from there.
@@ -54,17 +55,16 @@ struct Vec {
     if constexpr (KIND == 2) return __uint_as_float(u);
     else return [&](float2 v) { return i & 1 ? v.y : v.x; }(q8_up2<KIND == 1>(u));
   }
-  // as pairs of floats, what is lower than -65504 (fp16) or -10^30 set to that: a weight of 0 is then one of a number
-  __device__ __forceinline__ static void pairs(const uint4& w, uint64_t (&f)[kPer / 2]) {
-    uint32_t ws[4] = {w.x, w.y, w.z, w.w};
-    if constexpr (KIND == 2) {
+  // as floats, what is lower than -65504 (fp16) or -10^30 set to that: a weight of 0 is then one of a number
+  __device__ __forceinline__ static void floats(const uint4& w, float (&f)[kPer]) {
+    const uint32_t ws[4] = {w.x, w.y, w.z, w.w};
 #pragma unroll
-      for (int i = 0; i < 2; ++i) f[i] = pair(fmaxf(__uint_as_float(ws[2 * i]), -1e30f), fmaxf(__uint_as_float(ws[2 * i + 1]), -1e30f));
-    } else {
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
+    for (int i = 0; i < 4; ++i) {
+      if constexpr (KIND == 2) {
+        f[i] = fmaxf(__uint_as_float(ws[i]), -1e30f);
+      } else {
         const float2 v = q8_up2<KIND == 1>(larger(ws[i], KIND == 0 ? 0xfbfffbffu : 0xf149f149u));
-        f[i] = pair(v.x, v.y);
+        f[2 * i] = v.x, f[2 * i + 1] = v.y;
       }
     }
   }
@@ -82,6 +82,27 @@ __device__ __forceinline__ float lp_ex2(float x) {
   return r;
 }
 
+// Of the largest values that up to 64 groups of threads have seen, the `top`-th (by one warp): at least so many of a row's values reach it, and seldom many more.
+// 0: there are fewer.
+__device__ __forceinline__ uint32_t reached_by(const uint32_t* group, int groups, int top, int lane) {
+  uint32_t found = 0;
+  for (int i = lane; i < groups; i += 32) {
+    const uint32_t v = group[i];
+    int ahead = 0;
+    for (int k = 0; k < groups; ++k) ahead += group[k] > v || (group[k] == v && k < i);
+    if (ahead == top - 1) found = v;
+  }
+  return __reduce_max_sync(0xffffffffu, found);
+}
+// The groups of a CTA's warps: a warp each, or a half or a quarter of one; the first thread of each leaves what its group has seen.
+__device__ __forceinline__ int leave_group(uint32_t seen, uint32_t* group, int warps, int top, int warp, int lane) {
+  const int parts = top <= warps ? 1 : top <= 2 * warps ? 2 : 4;
+  uint32_t g = seen;
+  for (int d = 1; d < 32 / parts; d <<= 1) g = max(g, __shfl_xor_sync(0xffffffffu, g, d));
+  if (lane % (32 / parts) == 0) group[warp * parts + lane / (32 / parts)] = g;
+  return warps * parts;
+}
+
 struct LpParams {
   const void* logits;
   long long ld;
@@ -95,7 +116,7 @@ struct LpShared {
   Ranked kept[kLpKept], best[kLpMaxTop], red[kLpWarps];
   float edge[16], sums[2][kLpWarps], S, D;  // edge: values of the row ahead of its first whole vector and behind its last
   uint32_t most, least, count;
-  uint32_t warp_most[kLpWarps], warp_least[kLpWarps];
+  uint32_t group[64];
 };
 
 template <int KIND>
@@ -115,24 +136,36 @@ __global__ void __launch_bounds__(kLpThreads, 3) token_logprobs_kernel(const __g
   if (tid == 0) sh.count = 0;
   asm volatile("griddepcontrol.wait;" ::: "memory");
 
+  const bool writes = rank == 0 && tid == kLpThreads - 1;  // (its loads are on their way long before they are used)
+  const long long id = writes ? p.ids[r] : -1;
+
   // ---- the row into shared memory, and the largest value that each thread has seen (0: none)
   uint32_t seen = 0;
   {
     const uint4* const from = reinterpret_cast<const uint4*>(row + (size_t)head * kSize) + v0;
     constexpr int kAhead = 4;
     uint32_t top = Vec<KIND>::kLowest;
-    for (int i0 = tid; i0 < mine; i0 += kAhead * kLpThreads) {
+    int i = tid;
+    for (; i + (kAhead - 1) * kLpThreads < mine; i += kAhead * kLpThreads) {
       uint4 w[kAhead];
 #pragma unroll
-      for (int u = 0; u < kAhead; ++u)
-        if (i0 + u * kLpThreads < mine) w[u] = from[i0 + u * kLpThreads];
+      for (int u = 0; u < kAhead; ++u) w[u] = from[i + u * kLpThreads];
 #pragma unroll
-      for (int u = 0; u < kAhead; ++u)
-        if (i0 + u * kLpThreads < mine) {
-          part[i0 + u * kLpThreads] = w[u];
-          top = Vec<KIND>::larger(top, Vec<KIND>::largest(w[u]));
-        }
+      for (int u = 0; u < kAhead; ++u) {
+        part[i + u * kLpThreads] = w[u];
+        top = Vec<KIND>::larger(top, Vec<KIND>::largest(w[u]));
+      }
     }
+    uint4 w[kAhead - 1];
+#pragma unroll
+    for (int u = 0; u < kAhead - 1; ++u)
+      if (i + u * kLpThreads < mine) w[u] = from[i + u * kLpThreads];
+#pragma unroll
+    for (int u = 0; u < kAhead - 1; ++u)
+      if (i + u * kLpThreads < mine) {
+        part[i + u * kLpThreads] = w[u];
+        top = Vec<KIND>::larger(top, Vec<KIND>::largest(w[u]));
+      }
     if (tid < mine) seen = order_of(Vec<KIND>::most(top));
     if (tid < edges) {
       const float x = logit<KIND>(row, edge_id(tid));
@@ -140,82 +173,58 @@ __global__ void __launch_bounds__(kLpThreads, 3) token_logprobs_kernel(const __g
       seen = max(seen, order_of(x));
     }
   }
-  {
-    const uint32_t most = __reduce_max_sync(0xffffffffu, seen);
-    // groups of neighbouring threads: 16 (a warp each), 32 or 64
-    uint32_t g = seen;
-    const int lanes = p.top <= kLpWarps ? 32 : p.top <= 2 * kLpWarps ? 16 : 8;
-    for (int d = 1; d < lanes; d <<= 1) g = max(g, __shfl_xor_sync(0xffffffffu, g, d));
-    const uint32_t least = __reduce_min_sync(0xffffffffu, g);
-    if (lane == 0) sh.warp_most[warp] = most, sh.warp_least[warp] = least;
-  }
+  const float given = id >= 0 && id < p.vocab ? logit<KIND>(row, id) : 0.f;
+  const int groups = leave_group(seen, sh.group, kLpWarps, p.top, warp, lane);
   __syncthreads();
-  if (tid == 0) {
-    uint32_t a = 0, b = 0xffffffffu;
-    for (int w = 0; w < kLpWarps; ++w) a = max(a, sh.warp_most[w]), b = min(b, sh.warp_least[w]);
-    sh.most = a, sh.least = b;
-  }
-  if (p.top > 0) {
-    // at least as many threads as tokens are asked for have seen a value that reaches this minimum: the one that so many reach is closer
-    __syncthreads();
-    const uint32_t least = sh.least;
-    uint32_t* const list = reinterpret_cast<uint32_t*>(sh.kept);
-    if (seen >= least) list[atomicAdd(&sh.count, 1u)] = seen;
-    __syncthreads();
-    const int n = (int)sh.count;
-    if (least > 0 && tid < n) {
-      const uint32_t v = list[tid];
-      int before = 0;
-      for (int k = 0; k < n; ++k) before += list[k] > v || (list[k] == v && k < tid);
-      if (before == p.top - 1) sh.least = v;
-    }
-    __syncthreads();
-    if (tid == 0) sh.count = 0;
+  if (warp == 0) {
+    uint32_t most = 0;
+    for (int i = lane; i < groups; i += 32) most = max(most, sh.group[i]);
+    most = __reduce_max_sync(0xffffffffu, most);
+    const uint32_t least = p.top > 0 ? reached_by(sh.group, groups, p.top, lane) : 0u;
+    if (lane == 0) sh.most = most, sh.least = least;
   }
   if (n_cta > 1) cluster.sync();
   else __syncthreads();
   uint32_t most = 0, least = 0;
-  for (int c = 0; c < n_cta; ++c) {
-    const LpShared* other = cluster.map_shared_rank(&sh, c);
+  for (int o = 0; o < n_cta; ++o) {
+    const LpShared* other = cluster.map_shared_rank(&sh, o);
     most = max(most, other->most), least = max(least, other->least);
   }
   const float M = value_of(most), reach = value_of(least);
   const bool finite = M <= 3.402823466e38f && M >= -3.402823466e38f, empty = M == -CUDART_INF_F;
-  const bool all = least == 0;  // (a group that saw nothing: keep everything)
+  const bool all = least == 0;  // (too few groups have seen anything: keep everything)
 
   // ---- the sums, and the values that reach the threshold
+  // (beyond 10^37, where M log2 e may be infinite, numbers that differ are at least 2^99 apart: c = 1 gives the same weights, 1 and 0)
+  const bool far = fabsf(M) > 1e37f;
+  const float c = far ? 1.f : 1.4426950408889634f, m = M * c;
   float S = 0.f, D = 0.f;
   auto keep = [&](float x, int id) {
     const uint32_t at = atomicAdd(&sh.count, 1u);
     if (at < kLpKept) sh.kept[at] = ranked(x, id);
   };
   if (finite) {
-    uint64_t s2[2] = {0, 0}, d2[2] = {0, 0};
-    const uint64_t less = pair(-M, -M), log2e = pair(1.4426950408889634f, 1.4426950408889634f);
-#pragma unroll 2
-    for (int i = tid; i < mine; i += kLpThreads) {
-      uint64_t f[kPer / 2];
-      Vec<KIND>::pairs(part[i], f);
+    float s2[2] = {0.f, 0.f}, d2[2] = {0.f, 0.f};
+    auto add = [&](float x, int k) {
+      const float t = fmaf(x, c, -m), e = lp_ex2(t);
+      s2[k] += e;
+      d2[k] = fmaf(e, t, d2[k]);
+    };
+    int i = tid;
+    auto vec = [&](const uint4& w) {
+      float f[kPer];
+      Vec<KIND>::floats(w, f);
 #pragma unroll
-      for (int k = 0; k < kPer / 2; ++k) {
-        const uint64_t d = add2(f[k], less);
-        float a, b;
-        unpair(mul2(d, log2e), a, b);
-        const uint64_t e = pair(lp_ex2(a), lp_ex2(b));
-        s2[k & 1] = add2(s2[k & 1], e);
-        d2[k & 1] = fma2(e, d, d2[k & 1]);
-      }
+      for (int k = 0; k < kPer; ++k) add(f[k], k & 1);
+    };
+    for (; i + kLpThreads < mine; i += 2 * kLpThreads) {
+      const uint4 w = part[i], v = part[i + kLpThreads];
+      vec(w);
+      vec(v);
     }
-    float a, b;
-    unpair(add2(s2[0], s2[1]), a, b);
-    S = a + b;
-    unpair(add2(d2[0], d2[1]), a, b);
-    D = a + b;
-    if (tid < edges) {
-      const float d = fmaxf(sh.edge[tid], -1e30f) - M, e = lp_ex2(d * 1.4426950408889634f);
-      S += e;
-      D = fmaf(e, d, D);
-    }
+    if (i < mine) vec(part[i]);
+    if (tid < edges) add(fmaxf(sh.edge[tid], -1e30f), 0);
+    S = s2[0] + s2[1], D = d2[0] + d2[1];
     if (p.top > 0 && (all || seen >= least)) {  // (few threads)
       for (int i = tid; i < mine; i += kLpThreads) {
         const uint4 w = part[i];
@@ -233,10 +242,11 @@ __global__ void __launch_bounds__(kLpThreads, 3) token_logprobs_kernel(const __g
   for (int d = 16; d > 0; d >>= 1) S += __shfl_xor_sync(0xffffffffu, S, d), D += __shfl_xor_sync(0xffffffffu, D, d);
   if (lane == 0) sh.sums[0][warp] = S, sh.sums[1][warp] = D;
   __syncthreads();
-  if (tid == 0) {
-    S = D = 0.f;
-    for (int w = 0; w < kLpWarps; ++w) S += sh.sums[0][w], D += sh.sums[1][w];
-    sh.S = S, sh.D = D;
+  if (warp == 0) {
+    S = lane < kLpWarps ? sh.sums[0][lane] : 0.f, D = lane < kLpWarps ? sh.sums[1][lane] : 0.f;
+#pragma unroll
+    for (int d = 16; d > 0; d >>= 1) S += __shfl_xor_sync(0xffffffffu, S, d), D += __shfl_xor_sync(0xffffffffu, D, d);
+    if (lane == 0) sh.S = S, sh.D = D;
   }
 
   // ---- this CTA's likeliest, in order (0: no more)
@@ -281,25 +291,24 @@ __global__ void __launch_bounds__(kLpThreads, 3) token_logprobs_kernel(const __g
   // ---- the first CTA puts the row together
   if (rank == 0) {
     S = D = 0.f;
-    for (int c = 0; c < n_cta; ++c) {
-      const LpShared* other = cluster.map_shared_rank(&sh, c);
+    for (int o = 0; o < n_cta; ++o) {
+      const LpShared* other = cluster.map_shared_rank(&sh, o);
       S += other->S, D += other->D;
     }
-    const float log_s = logf(S);
+    const float log_sum = logf(S), log_s = log_sum - fmaf(M, c, -m) * 0.69314718055994531f;
     // (a row of -inf alone: every log probability -inf, entropy 0; a NaN or +inf: NaN)
     auto lp = [&](float x) { return finite ? (x - M) - log_s : empty ? -CUDART_INF_F : CUDART_NAN_F; };
-    if (tid == 0) {
-      const long long id = p.ids[r];
-      p.logprob[r] = id < 0 ? 0.f : id >= p.vocab ? CUDART_NAN_F : lp(logit<KIND>(row, id));
-      p.entropy[r] = finite ? log_s - D / S : empty ? 0.f : CUDART_NAN_F;
+    if (writes) {
+      p.logprob[r] = id < 0 ? 0.f : id >= p.vocab ? CUDART_NAN_F : lp(given);
+      p.entropy[r] = finite ? log_sum - D / S * (far ? 1.f : 0.69314718055994531f) : empty ? 0.f : CUDART_NAN_F;
     }
     for (int i = tid; i < n_cta * p.top; i += kLpThreads) {
-      const int c = i / p.top, k = i - c * p.top;
-      const Ranked v = cluster.map_shared_rank(&sh, c)->best[k];
+      const int from = i / p.top, k = i - from * p.top;
+      const Ranked v = cluster.map_shared_rank(&sh, from)->best[k];
       if (v == 0) continue;
       int before = k;  // (lists are in order: a binary search in each of the others)
       for (int o = 0; o < n_cta; ++o) {
-        if (o == c) continue;
+        if (o == from) continue;
         const Ranked* list = cluster.map_shared_rank(&sh, o)->best;
         int a = 0, z = p.top;
         while (a < z) {

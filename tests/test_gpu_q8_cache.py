@@ -402,7 +402,9 @@ def _rows(rows, vocab, dtype, g, kind):
 @pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16, torch.float32])
 @pytest.mark.parametrize("rows,vocab,top,kind", [(1, 1, 1, ""), (1, 5, 5, ""), (3, 257, 64, ""), (4, 32000, 5, ""), (5, 1001, 8, "masked"), (2, 4096, 64, "equal"),
                                                  (2, 333, 3, "lowest"), (3, 2048, 4, "large"), (37, 50257, 0, ""), (7, 20011, 20, "steps"), (300, 515, 2, ""),
-                                                 (2, 131072, 7, "steps"), (1, 151936, 33, "masked"), (160, 40000, 64, "equal")])
+                                                 (2, 131072, 7, "steps"), (1, 151936, 33, "masked"), (160, 40000, 64, "equal"),
+                                                 # (many rows of 16 to 64 KB)
+                                                 (311, 9001, 8, ""), (300, 20000, 64, "masked"), (602, 15011, 33, "steps"), (296, 16000, 40, "equal"), (299, 8300, 0, "lowest")])
 def test_logprobs(ops, rows, vocab, top, kind, dtype):
     g = torch.Generator().manual_seed(rows + vocab)
     x = _rows(rows, vocab, dtype, g, kind)
@@ -426,8 +428,11 @@ def test_logprobs(ops, rows, vocab, top, kind, dtype):
     assert ok(tl, want.gather(1, order), allow.gather(1, order))
 
 
-def test_logprobs_of_rows_without_a_distribution(ops):
-    x = torch.zeros(6, 700)
+@pytest.mark.parametrize("many", [1, 60])   # (60 times six rows of 9000: the kernel for many rows)
+def test_logprobs_of_rows_without_a_distribution(ops, many):
+    x = torch.zeros(6, 700 if many == 1 else 9000)
+    if many > 1:
+        x[:, 700:] = -math.inf
     x[0] = -math.inf
     x[1, 3], x[1, 600] = math.nan, 5.0
     x[2, 9], x[2, 8] = math.inf, 1.0
@@ -435,7 +440,10 @@ def test_logprobs_of_rows_without_a_distribution(ops):
     x[3, 699] = -2.0
     x[4, 100::2] = -0.0
     for dtype in (torch.float16, torch.float32):
-        lp, ent, tl, ti = (t.cpu() for t in ops.token_logprobs(x.to(dtype).to(DEV), torch.tensor([1, 2, 9, 699, 700, -1], device=DEV), 3))
+        ids = torch.tensor([1, 2, 9, 699, x.shape[1], -1], device=DEV)
+        every = [t.cpu() for t in ops.token_logprobs(x.to(dtype).to(DEV).repeat(many, 1), ids.repeat(many), 3)]
+        lp, ent, tl, ti = (t[-6:] for t in every)
+        assert all(torch.equal(t[:6].nan_to_num(7.0), t[-6:].nan_to_num(7.0)) for t in every)
         assert lp[0] == -math.inf and ent[0] == 0 and (tl[0] == -math.inf).all() and ti[0].tolist() == [0, 1, 2]
         assert lp[1].isnan() and ent[1].isnan() and ti[1].tolist() == [3, 600, 0]
         assert lp[2].isnan() and ent[2].isnan() and ti[2].tolist() == [9, 8, 0]
