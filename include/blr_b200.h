@@ -388,7 +388,7 @@ int blr_attention_decode(const void* q, int64_t ldq, const void* k_cache, const 
 
 /* ---- An 8-bit key / value cache and the attention over it.  No counterpart in the reference.
  * Codes are (n_seq, kv_heads, slots, head_dim) bytes, int8 in [-127, 127] or e4m3, packed and 16-byte aligned; `block` slots of a head share one fp32
- * scale, (n_seq, kv_heads, ceil(slots / block)): value = code * scale.  head_dim 64 or 128, block 16, 32, 64 or 128 (BLR_ERR_UNSUPPORTED else).
+ * scale that is not negative, (n_seq, kv_heads, ceil(slots / block)): value = code * scale.  head_dim 64 or 128, block 16, 32, 64 or 128 (BLR_ERR_UNSUPPORTED else).
  * start, n_new: device int64, one per sequence; a call's tokens of sequence s take slots start[s] .. start[s] + n_new[s] - 1 (n_new NULL: n_tok
  * each).  Rows behind a sequence's n_new, and tokens whose slot is outside the cache, write nothing to it and leave zeros in an output.  16-bit tensors of
  * `dtype`, rows 16-byte aligned, row strides multiples of 8; any of them, start and n_new too, may be written by the kernel directly ahead. */
@@ -427,7 +427,8 @@ int blr_attention_q8(const void* q, int64_t ldq, const blr_q8_cache* cache, cons
 /* Of each row of logits (row stride ld; kind 0 fp16, 1 bf16, 2 fp32): logprob[r] = log softmax(row)[ids[r]] (0 where ids[r] < 0: no token given; NaN
  * where ids[r] >= vocab), entropy[r] of the softmax, and the `top` (0 .. 64, at most vocab) likeliest tokens by falling logit, ties by rising id: their
  * log probabilities (rows, top) and ids (rows, top).  Logits of -inf have probability 0; a row of nothing else has log probabilities of -inf and entropy
- * 0.  A row with a NaN or +inf has NaN for both (its tokens still in order, NaN first).  fp32 arithmetic and results.  No reference counterpart. */
+ * 0.  A row with a NaN or +inf has NaN for both (its tokens still in order, NaN first).  fp32 arithmetic and results; the order of a row's sums goes by its
+ * alignment and by how many rows there are.  A row is at most 1600 KB (BLR_ERR_UNSUPPORTED above).  No reference counterpart. */
 int blr_token_logprobs(const void* logits, int64_t ld, int64_t rows, int64_t vocab, int kind, const int64_t* ids, int top,
                        float* logprob, float* entropy, float* top_logprob, int64_t* top_ids, void* stream);
 

@@ -288,6 +288,45 @@ def test_a_bad_block_reaches_only_the_rows_that_see_it(ops, T, H, KV):
             assert torch.equal(out[:-2], sound[:-2])
 
 
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("T,H", [(2, 4), (90, 2)])
+def test_a_row_of_q_that_is_no_number_stays_alone(ops, T, H, dtype):
+    g = torch.Generator().manual_seed(6)
+    parts = _cache(ops, 1, H, 200, 128, 32, I8, g)
+    q = torch.randn(T, H, 128, generator=g).to(dtype)
+    call = lambda q: ops.attention_q8(q.view(T, -1).to(DEV), _on(ops, parts, 32), torch.tensor([200 - T], device=DEV)).cpu().view(T, H, 128)   # noqa: E731
+    sound = call(q)
+    q[1, 1, 7], q[0, 0, 3] = math.nan, math.inf
+    got = call(q)
+    assert got[1, 1].isnan().all() and not got[0, 0].isfinite().all()
+    got[1, 1], got[0, 0] = sound[1, 1], sound[0, 0]
+    assert torch.equal(got, sound)
+
+
+@pytest.mark.parametrize("T", [1, 70])
+def test_a_cache_beyond_32_bit_offsets(ops, T):
+    """5 GB of codes for the keys and as many for the values: the last 16 slots are written, everything before them has scale 0, so that its keys score 0 and
+    its values are 0: out = sum p v / (n + sum p) over the last slots."""
+    hd, slots, block = 128, 40_000_016, 16
+    cache = ops.q8_cache(1, 1, slots, hd, block, I8, DEV)
+    cos, sin = torch.ones(1, hd // 2, device=DEV), torch.zeros(1, hd // 2, device=DEV)   # (angles of 0: nothing turns)
+    g = torch.Generator().manual_seed(8)
+    new = slots - 16 - (T - 16 if T > 16 else 0)
+    k, v, q = (torch.randn(T, hd, generator=g).bfloat16() for _ in range(3))
+    tables = (cos.expand(slots, -1).contiguous(), sin.expand(slots, -1).contiguous())
+    start = torch.tensor([new], device=DEV)
+    r = ops.rope_append_q8(q.to(DEV), k.to(DEV), v.to(DEV), *tables, start, cache)
+    assert torch.equal(r.cpu(), q)
+    got = ops.attention_q8(r, cache, start).cpu().double()
+    del tables
+    kq, vq = (c[0, 0, new:new + T].cpu().double() * sc[0, 0, new // block:].cpu().double().repeat_interleave(block)[new % block:][:T, None]
+              for c, sc in ((cache.k, cache.k_scale), (cache.v, cache.v_scale)))
+    x = (q.double() @ kq.T * hd ** -0.5 + math.log(1e6)).exp().tril()   # (weights times 10^6, for the sake of the sums here)
+    total = 1e6 * new + x.sum(1, keepdim=True)
+    # the output's rounding, p's (2^-11), and 2^-19 for sums of up to 2^25 fp32 terms, most of them equal to 1, over some hundred threads
+    assert ((got - x @ vq / total).abs() <= (2.0 ** -8 + 2.0 ** -19) * (x @ vq / total).abs() * 1.001 + 2.0 ** -11 * (x @ vq.abs() / total)).all()
+
+
 def test_strides_and_streams(ops):
     """q, k, v as columns of a fused projection's rows, and as views that the kernels do not take; a stream of its own."""
     B, T, H, KV, hd, slots = 2, 6, 4, 2, 64, 40

@@ -64,6 +64,7 @@ def test_arguments_of_the_log_probabilities(L):
     call = lambda logits=P, ld=100, rows=2, vocab=100, kind=0, ids=P, top=3, tl=P: f(logits, ld, rows, vocab, kind, ids, top, P, P, tl, P, None)   # noqa: E731
     assert call(kind=3) == ARG and call(ld=99) == ARG and call(vocab=0) == ARG and call(rows=-1) == ARG
     assert call(top=65) == ARG and call(top=-1) == ARG and call(vocab=2, top=3) == ARG
+    assert call(vocab=900000, ld=900000) == UNSUPPORTED and call(vocab=450000, ld=450000, kind=2) == UNSUPPORTED and call(logits=P + 1) == ARG
     assert call(logits=None) == ARG and call(ids=None) == ARG and call(tl=None) == ARG
     assert call(rows=0, logits=None) == 0
 
