@@ -394,8 +394,10 @@ __global__ void __launch_bounds__(256) q8_combine_kernel(const __grid_constant__
 
 struct Q8Plan {
   int nt, q_tiles, ns, room;  // nt: column tiles of 8 rows of the kernel here, 0: the prompt kernel; ns: CTAs that may share a row tile's keys
-  long long rows, tiles;
+  long long rows, tiles, wide_tiles;  // wide_tiles: of 128 slots of a head, whose codes are widened ahead (0: not)
 };
+static constexpr int kWideFrom = 4;  // row tiles of a kv head from which its codes are widened ahead
+static constexpr long long kWideBytes = 256ll << 20;  // room that widened codes may take
 // Few row tiles share their keys out over more CTAs, as many as the SMs hold at a time (4, 3, 2 or 1 of a kind); a second kernel sums the parts.  The host does not
 // know the sequences' lengths: a tile may have half as many CTAs again as its even share, and the kernel here shares by the
 // lengths.  Up to 512 slots a second launch (3 us) costs more than it saves (1 sequence x 32 heads x 300 keys: 2 CTAs a head TODO us, one TODO).
@@ -413,8 +415,11 @@ static Q8Plan q8_plan(const blr_q8_cache* c, int64_t n_tok, int heads) {
   if (c->slots <= 512) ns = 1;
   if (ns > most) ns = most;
   a.ns = ns < 1 ? 1 : ns > kMaxSplits ? kMaxSplits : (int)ns;
+  const long long wide = (c->slots + 127) / 128;
+  if (a.nt == 0 && a.q_tiles >= kWideFrom && c->n_seq * c->kv_heads * wide * 512 * c->head_dim <= kWideBytes) a.wide_tiles = wide;
   return a;
 }
+static size_t q8_wide_bytes(const Q8Plan& a, const blr_q8_cache* c) { return (size_t)(c->n_seq * c->kv_heads * a.wide_tiles) * 512 * c->head_dim; }
 
 template <typename K, typename... A>
 static int launch(K kern, dim3 grid, dim3 block, size_t smem, cudaStream_t st, A... args) {
@@ -455,7 +460,7 @@ extern "C" {
 size_t blr_attention_q8_scratch_bytes(const blr_q8_cache* cache, int64_t n_tok, int heads) {
   if (!cache || cache->n_seq <= 0 || cache->kv_heads <= 0 || cache->slots <= 0 || n_tok <= 0 || heads <= 0 || heads % cache->kv_heads != 0) return 0;
   const Q8Plan a = q8_plan(cache, n_tok, heads);
-  return a.ns > 1 ? (size_t)cache->n_seq * cache->kv_heads * a.rows * a.ns * (cache->head_dim + 4) * sizeof(float) : 0;
+  return q8_wide_bytes(a, cache) + (a.ns > 1 ? (size_t)cache->n_seq * cache->kv_heads * a.rows * a.ns * (cache->head_dim + 4) * sizeof(float) : 0);
 }
 
 int blr_attention_q8(const void* q, int64_t ldq, const blr_q8_cache* cache, const int64_t* start, const int64_t* n_new, int64_t n_tok, int heads,
@@ -479,7 +484,8 @@ int blr_attention_q8(const void* q, int64_t ldq, const blr_q8_cache* cache, cons
   p.q = static_cast<const uint16_t*>(q), p.out = static_cast<uint16_t*>(out);
   p.ldq = ldq, p.ldo = ldo;
   p.start = reinterpret_cast<const long long*>(start), p.n_new = reinterpret_cast<const long long*>(n_new);
-  p.part = static_cast<float*>(scratch);
+  p.wide = a.wide_tiles > 0 ? static_cast<uint8_t*>(scratch) : nullptr, p.wide_tiles = (int)a.wide_tiles;
+  p.part = reinterpret_cast<float*>(static_cast<uint8_t*>(scratch) + q8_wide_bytes(a, cache));
   p.scale_log2 = scale * 1.4426950408889634f;
   p.T = (int)n_tok, p.H = heads, p.G = heads / cache->kv_heads, p.rows = (int)a.rows, p.q_tiles = a.q_tiles, p.ns = a.ns, p.bf16 = dtype == BLR_DTYPE_BF16;
   p.n_bh = (int)(cache->n_seq * cache->kv_heads), p.n_seq = (int)cache->n_seq, p.room = a.room;

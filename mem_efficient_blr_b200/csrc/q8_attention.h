@@ -11,10 +11,11 @@ struct Q8AttnParams {
   long long ldq, ldo;
   const long long *start, *n_new;
   float* part;       // ns > 1: of each (sequence, kv head, row, split) hd sums, the maximum that they are taken against, the sum of the weights, 2 free
+  uint8_t* wide;     // NULL, or room for the codes as fp16: of each (sequence, kv head, 128 slots) a tile of keys and one of values
   unsigned* status;  // NULL, or where a wait that gave up is noted
   float scale_log2;
   int T, H, G, rows, q_tiles, ns, bf16, n_bh, n_seq;
-  int room;  // CTAs that the SMs hold
+  int room, wide_tiles;  // CTAs that the SMs hold; tiles of a head
 };
 
 __device__ __forceinline__ float ex2(float x) {

@@ -17,11 +17,14 @@
 
 namespace blr {
 
-static constexpr int kPromptThreads = 512, kKeys = 128;
-// Registers of a thread at launch, and of the softmax warps (8), the widening ones (4) and the last four from then on: setmaxnreg waits for ever for registers that
-// the block was not launched with.
-static constexpr int kRegs = 128, kRegsSoftmax = 176, kRegsWiden = 104, kRegsIssue = 56;
-static_assert(8 * kRegsSoftmax + 4 * kRegsWiden + 4 * kRegsIssue <= kPromptThreads / 32 * kRegs, "more registers than the block has");
+static constexpr int kKeys = 128;
+// Threads, and registers of a thread at launch and from then on of the softmax warps (8), the widening ones (4, none where the codes have been widened) and the last
+// four: setmaxnreg waits for ever for registers that the block was not launched with.
+template <bool WIDE>
+struct Split {
+  static constexpr int kThreads = WIDE ? 384 : 512, kLaunch = WIDE ? 168 : 128, kSoftmax = WIDE ? 216 : 176, kWiden = 104, kIssue = 56;
+  static_assert(8 * kSoftmax + (WIDE ? 0 : 4 * kWiden) + 4 * kIssue <= kThreads / 32 * kLaunch, "more registers than the block has");
+};
 
 __device__ __forceinline__ void tmem_ld32(uint32_t taddr, uint32_t (&r)[32]) {
   asm volatile(
@@ -205,8 +208,9 @@ struct Codes {
   }
 };
 
-template <bool E4M3, int HD>
-__global__ void __launch_bounds__(kPromptThreads, 1) q8_prompt_kernel(const __grid_constant__ Q8AttnParams p) {
+template <bool E4M3, int HD, bool WIDE>
+__global__ void __launch_bounds__(Split<WIDE>::kThreads, 1) q8_prompt_kernel(const __grid_constant__ Q8AttnParams p) {
+  constexpr int kLast = WIDE ? 8 : 12;  // the first of the last four warps
   extern __shared__ __align__(1024) uint8_t prompt_raw[];
   __shared__ __align__(16) float factors[4][20];
   constexpr uint32_t kTile = 128 * HD * 2;
@@ -221,8 +225,8 @@ __global__ void __launch_bounds__(kPromptThreads, 1) q8_prompt_kernel(const __gr
   if (threadIdx.x == 0) {
     *abort_flag = 0;
     for (int i = 0; i < 2; ++i) {
-      mbar_init(kfull + 8 * i, 4);
-      mbar_init(vfull + 8 * i, 4);
+      mbar_init(kfull + 8 * i, WIDE ? 1 : 4);
+      mbar_init(vfull + 8 * i, WIDE ? 1 : 4);
       mbar_init(kempty + 8 * i, 1);
       mbar_init(vempty + 8 * i, 1);
       mbar_init(sfull + 8 * i, 1);
@@ -232,7 +236,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1) q8_prompt_kernel(const __gr
     for (int i = 0; i < 4; ++i) mbar_init(cfull + 8 * i, 1);
     mbar_init_fence();
   }
-  if (warp == 12) tmem_alloc(smem_u32(&tmem_slot), 512);
+  if (warp == kLast) tmem_alloc(smem_u32(&tmem_slot), 512);
 
   asm volatile("griddepcontrol.wait;" ::: "memory");
   int keys, k0, n0, n1, lim = 0;
@@ -293,9 +297,53 @@ __global__ void __launch_bounds__(kPromptThreads, 1) q8_prompt_kernel(const __gr
   const int steps = max(n0, n1);
 
   // (No spills in any of these: what shared memory leaves of L1 does not keep them, and a reload from L2 inside a loop costs more than anything that it saves.)
-  if (warp >= 12) {
-    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kRegsIssue));
-    if (warp == 12 && elect_one()) {
+  // A step's factors: of 8 groups of 16 keys ks and vs / R, and how R moved.  One warp makes them, four steps deep (a step's are free when the S of the step after it
+  // is done, and that warp is two steps ahead of that at most).
+  float R_made = 0.f, inv_R = 0.f, next_scale = 0.f;
+  auto scale_at = [&](int j) {
+    const float* const scales = (lane < 8 ? p.c.k_scale : p.c.v_scale) + (long long)place_of(p).bh * p.c.n_blocks;
+    return scales[min((k0 + j * kKeys + 16 * (lane & 7)) >> p.c.block_log2, p.c.n_blocks - 1)];
+  };
+  auto make_factors = [&](int j) {
+    const float scale = next_scale;
+    if (j + 1 < steps) next_scale = scale_at(j + 1);
+    const float vmax = __uint_as_float(
+        __reduce_max_sync(0xffffffffu, lane >= 8 && k0 + j * kKeys + 16 * (lane & 7) < keys && scale <= 3.4e38f ? __float_as_uint(scale) : 0u));
+    float moved = 1.f;
+    if (vmax > 16.f * R_made) moved = R_made / vmax, R_made = vmax, inv_R = 1.f / vmax;
+    if (lane < 16) factors[j & 3][lane] = lane < 8 ? scale : scale * inv_R;
+    if (lane == 16) factors[j & 3][16] = moved;
+    if (lane == 17) factors[j & 3][17] = R_made;
+    __syncwarp();
+    if (lane == 0) mbar_arrive(cfull + 8 * (j & 3));
+  };
+  if (warp >= kLast) {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(Split<WIDE>::kIssue));
+    if (WIDE && warp == kLast + 1) {
+      // tiles of widened keys and values as they are to lie in shared memory
+      if (elect_one()) {
+        const uint8_t* const from = p.wide + ((long long)place_of(p).bh * p.wide_tiles + k0 / kKeys) * 2 * kTile;
+#pragma unroll 1
+        for (int j = 0; j < steps; ++j) {
+          const uint32_t s = j & 1, parity = ((j >> 1) & 1) ^ 1;
+          if (j >= 2 && !mbar_wait(kempty + 8 * s, parity, abort_flag)) break;
+          mbar_arrive_expect_tx(kfull + 8 * s, kTile);
+          bulk_load(ks + s * kTile, from + (long long)j * 2 * kTile, kTile, kfull + 8 * s);
+          if (j >= 2 && !mbar_wait(vempty + 8 * s, parity, abort_flag)) break;
+          mbar_arrive_expect_tx(vfull + 8 * s, kTile);
+          bulk_load(vs + s * kTile, from + (long long)j * 2 * kTile + kTile, kTile, vfull + 8 * s);
+        }
+      }
+      __syncwarp();
+    } else if (WIDE && warp == kLast + 2) {
+      if (steps > 0) next_scale = scale_at(0);
+#pragma unroll 1
+      for (int j = 0; j < steps; ++j) {
+        if (j >= 2 && !__all_sync(0xffffffffu, mbar_wait(kempty + 8 * (j & 1), ((j >> 1) & 1) ^ 1, abort_flag))) break;
+        make_factors(j);
+      }
+    }
+    if (warp == kLast && elect_one()) {
       const uint32_t id_s = umma_idesc(false, false, false, 128, kKeys), id_o = umma_idesc(false, false, true, 128, HD);
       auto product_s = [&](int i, int j) {
         uint32_t q_at = qs + i * kTile;
@@ -343,35 +391,19 @@ __global__ void __launch_bounds__(kPromptThreads, 1) q8_prompt_kernel(const __gr
       }
     }
     __syncwarp();
-  } else if (warp >= 8) {
-    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kRegsWiden));
+  } else if (!WIDE && warp >= 8) {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(Split<WIDE>::kWiden));
     const int idx = threadIdx.x & 127, last = p.c.slots - 1;
-    const Place at = place_of(p);
-    const uint8_t *const kh = p.c.k + (long long)at.bh * p.c.slots * HD, *const vh = p.c.v + (long long)at.bh * p.c.slots * HD;
-    // the first of these warps also prepares the steps' factors, four steps deep (a step's are free when the S of the step after it is done, and these
-    // warps are two steps ahead of that at most): of 8 groups of 16 keys ks and vs / R, and how R moved
-    const float* const scales = (lane < 8 ? p.c.k_scale : p.c.v_scale) + (long long)at.bh * p.c.n_blocks;
-    auto scale_at = [&](int j) { return scales[min((k0 + j * kKeys + 16 * (lane & 7)) >> p.c.block_log2, p.c.n_blocks - 1)]; };
-    float R = 0.f, inv_R = 0.f, next = warp == 8 && steps > 0 ? scale_at(0) : 0.f;
+    const long long head = (long long)place_of(p).bh * p.c.slots * HD;
+    const uint8_t *const kh = p.c.k + head, *const vh = p.c.v + head;
+    if (warp == 8 && steps > 0) next_scale = scale_at(0);
     Codes<HD> kc, vc;
     if (steps > 0) kc.load(kh, k0, last, idx), vc.load(vh, k0, last, idx);
 #pragma unroll 1
     for (int j = 0; j < steps; ++j) {
       const uint32_t s = j & 1, parity = ((j >> 1) & 1) ^ 1;
       if (j >= 2 && !__all_sync(0xffffffffu, mbar_wait(kempty + 8 * s, parity, abort_flag))) break;
-      if (warp == 8) {
-        const float scale = next;
-        if (j + 1 < steps) next = scale_at(j + 1);
-        const float vmax = __uint_as_float(__reduce_max_sync(
-            0xffffffffu, lane >= 8 && k0 + j * kKeys + 16 * (lane & 7) < keys && scale <= 3.4e38f ? __float_as_uint(scale) : 0u));
-        float moved = 1.f;
-        if (vmax > 16.f * R) moved = R / vmax, R = vmax, inv_R = 1.f / vmax;
-        if (lane < 16) factors[j & 3][lane] = lane < 8 ? scale : scale * inv_R;
-        if (lane == 16) factors[j & 3][16] = moved;
-        if (lane == 17) factors[j & 3][17] = R;
-        __syncwarp();
-        if (lane == 0) mbar_arrive(cfull + 8 * (j & 3));
-      }
+      if (warp == 8) make_factors(j);
       kc.template store<E4M3>(ks + s * kTile, 128, idx);
       fence_proxy_async_smem();
       __syncwarp();
@@ -385,7 +417,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1) q8_prompt_kernel(const __gr
       if (j + 1 < steps) vc.load(vh, k0 + (j + 1) * kKeys, last, idx);
     }
   } else {
-    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kRegsSoftmax));
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(Split<WIDE>::kSoftmax));
     const int n = wg ? n1 : n0;
     const uint32_t lanes = (uint32_t)(32 * (warp & 3)) << 16, s_at = tmem + lanes + 128 * wg, o_at = tmem + lanes + 256 + 128 * wg;
     float m = -INFINITY, l = 0.f, R = 0.f;
@@ -486,29 +518,48 @@ __global__ void __launch_bounds__(kPromptThreads, 1) q8_prompt_kernel(const __gr
     if (threadIdx.x == 0 && p.status) atomicExch(p.status, 1u);
     for (int i = 0; i < 200; ++i) __nanosleep(1000);  // (products in flight end before their operands' memory is given back)
   }
-  if (warp == 12) {
+  if (warp == kLast) {
     tc_fence_after();
     tmem_dealloc(tmem, 512);
   }
 }
 
+// The codes of 128 slots of a head as fp16, in the very order that a tile has in shared memory; zeros behind a sequence's last slot.  Where a tile of keys is read by
+// several CTAs it is widened once like this, instead of by each: 2 bytes a code written and read through L2.
 template <bool E4M3, int HD>
-static int launch_prompt(const Q8AttnParams& p, cudaStream_t stream) {
-  static bool configured[64] = {};
-  DeviceInfo di;
-  int rc;
-  if ((rc = device_info(&di))) return rc;
-  const int smem = 6 * 128 * HD * 2 + 1024 + 256 < 120 * 1024 ? 120 * 1024 : 6 * 128 * HD * 2 + 1024 + 256;  // one CTA per SM: a second one would only wait for TMEM
-  if (!configured[di.dev]) {
-    BLR_CUDA_OK(cudaFuncSetAttribute(q8_prompt_kernel<E4M3, HD>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
-    cudaFuncAttributes fa;
-    BLR_CUDA_OK(cudaFuncGetAttributes(&fa, q8_prompt_kernel<E4M3, HD>));
-    BLR_REQUIRE(fa.numRegs == kRegs, BLR_ERR_UNSUPPORTED, "the prompt kernel was built with %d registers, its split is made for %d", fa.numRegs, kRegs);
-    configured[di.dev] = true;
+__global__ void __launch_bounds__(256) q8_widen_kernel(const __grid_constant__ Q8AttnParams p) {
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  constexpr int kChunks = HD / 16;
+  const int tile = blockIdx.x % p.wide_tiles, bh = blockIdx.x / p.wide_tiles, b = bh / p.c.kv_heads, key0 = tile * kKeys;
+  const long long count = p.n_new == nullptr ? p.T : min((long long)p.T, p.n_new[b]);
+  const int keys = q8_seen_by(p, p.start[b], count, 0, p.rows);
+  if (key0 >= keys) return;
+  uint8_t* const to = p.wide + ((long long)bh * p.wide_tiles + tile) * 2 * (128 * HD * 2);
+#pragma unroll
+  for (int i = threadIdx.x; i < 2 * 128 * kChunks; i += 256) {
+    const int which = i / (128 * kChunks), at = i - which * (128 * kChunks), row = at / kChunks, c = at - row * kChunks;
+    uint4 w = make_uint4(0, 0, 0, 0);
+    const bool live = key0 + row < keys;
+    if (live) w = *reinterpret_cast<const uint4*>((which ? p.c.v : p.c.k) + ((long long)bh * p.c.slots + key0 + row) * HD + 16 * c);
+    const uint32_t ws[4] = {w.x, w.y, w.z, w.w};
+    uint32_t h[8];
+#pragma unroll
+    for (int n = 0; n < 4; ++n) {
+      const uint32_t v = q8_bias<E4M3>(ws[n]);
+      h[2 * n] = live ? q8_half2<E4M3>(v, false) : 0u, h[2 * n + 1] = live ? q8_half2<E4M3>(v, true) : 0u;
+    }
+    uint8_t* const line = to + which * (128 * HD * 2) + (c >> 2) * 16384 + row * 128;
+    *reinterpret_cast<uint4*>(line + ((((c & 3) * 2) ^ (row & 7)) << 4)) = make_uint4(h[0], h[1], h[2], h[3]);
+    *reinterpret_cast<uint4*>(line + ((((c & 3) * 2 + 1) ^ (row & 7)) << 4)) = make_uint4(h[4], h[5], h[6], h[7]);
   }
+}
+
+template <typename K>
+static int launch(K kernel, long long ctas, int threads, int smem, const Q8AttnParams& p, cudaStream_t stream) {
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3((unsigned)((long long)p.n_bh * p.q_tiles * p.ns));
-  cfg.blockDim = dim3(kPromptThreads);
+  cfg.gridDim = dim3((unsigned)ctas);
+  cfg.blockDim = dim3((unsigned)threads);
   cfg.dynamicSmemBytes = (size_t)smem;
   cfg.stream = stream;
   cudaLaunchAttribute at[1];
@@ -516,13 +567,40 @@ static int launch_prompt(const Q8AttnParams& p, cudaStream_t stream) {
   at[0].val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = at;
   cfg.numAttrs = 1;
-  BLR_CUDA_OK(cudaLaunchKernelEx(&cfg, q8_prompt_kernel<E4M3, HD>, p));
+  BLR_CUDA_OK(cudaLaunchKernelEx(&cfg, kernel, p));
   return BLR_OK;
 }
 
+template <bool E4M3, int HD, bool WIDE>
+static int launch_prompt(const Q8AttnParams& p, cudaStream_t stream) {
+  static bool configured[64] = {};
+  DeviceInfo di;
+  int rc;
+  if ((rc = device_info(&di))) return rc;
+  const int smem = 6 * 128 * HD * 2 + 1024 + 256 < 120 * 1024 ? 120 * 1024 : 6 * 128 * HD * 2 + 1024 + 256;  // one CTA per SM: a second one would only wait for TMEM
+  if (!configured[di.dev]) {
+    BLR_CUDA_OK(cudaFuncSetAttribute(q8_prompt_kernel<E4M3, HD, WIDE>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
+    cudaFuncAttributes fa;
+    BLR_CUDA_OK(cudaFuncGetAttributes(&fa, q8_prompt_kernel<E4M3, HD, WIDE>));
+    BLR_REQUIRE(fa.numRegs == Split<WIDE>::kLaunch, BLR_ERR_UNSUPPORTED, "the prompt kernel was built with %d registers, its split is made for %d", fa.numRegs,
+                Split<WIDE>::kLaunch);
+    configured[di.dev] = true;
+  }
+  return launch(q8_prompt_kernel<E4M3, HD, WIDE>, (long long)p.n_bh * p.q_tiles * p.ns, Split<WIDE>::kThreads, smem, p, stream);
+}
+
 int q8_launch_prompt(const Q8AttnParams& p, int head_dim, int code, cudaStream_t stream) {
-  if (code == BLR_Q8_E4M3) return head_dim == 128 ? launch_prompt<true, 128>(p, stream) : launch_prompt<true, 64>(p, stream);
-  return head_dim == 128 ? launch_prompt<false, 128>(p, stream) : launch_prompt<false, 64>(p, stream);
+  const bool e4 = code == BLR_Q8_E4M3;
+  if (p.wide == nullptr) {
+    if (head_dim == 128) return e4 ? launch_prompt<true, 128, false>(p, stream) : launch_prompt<false, 128, false>(p, stream);
+    return e4 ? launch_prompt<true, 64, false>(p, stream) : launch_prompt<false, 64, false>(p, stream);
+  }
+  const long long tiles = (long long)p.n_bh * p.wide_tiles;
+  int rc;
+  if (head_dim == 128) rc = e4 ? launch(q8_widen_kernel<true, 128>, tiles, 256, 0, p, stream) : launch(q8_widen_kernel<false, 128>, tiles, 256, 0, p, stream);
+  else rc = e4 ? launch(q8_widen_kernel<true, 64>, tiles, 256, 0, p, stream) : launch(q8_widen_kernel<false, 64>, tiles, 256, 0, p, stream);
+  if (rc) return rc;
+  return head_dim == 128 ? launch_prompt<false, 128, true>(p, stream) : launch_prompt<false, 64, true>(p, stream);
 }
 
 }  // namespace blr

@@ -227,6 +227,8 @@ ATTENDS = [  # B, T, H, KV, hd, slots, block, starts, new
     (1, 130, 2, 1, 128, 130, 16, [0], None),
     (2, 150, 3, 3, 128, 420, 128, [1, 270], [0, 150]),
     (1, 260, 4, 1, 64, 517, 64, [257], None),
+    (2, 410, 4, 2, 128, 900, 32, [490, 100], [410, 77]),          # (codes widened ahead)
+    (3, 520, 2, 1, 64, 523, 16, [3, -7, 0], [520, 520, 0]),
 ]
 
 
