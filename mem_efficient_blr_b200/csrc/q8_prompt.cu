@@ -4,7 +4,8 @@
 //   warps 8-11      widen the codes of the next keys and values to fp16 (exact) into shared memory, as tcgen05.mma reads them
 //   warps 12-15     one thread of the first issues the products: S = Q K^T (both from shared memory), O += P V (P from TMEM)
 // The scales stay out of the products: a group of 16 keys has one for its keys, which multiplies S in the exponent's argument, and one for its values, which
-// multiplies p by vs / R with R the largest of them so far (moved when it is 2^4 behind, like the maximum when it is 2^8 behind; see q8_attention.cu).
+// multiplies p by vs / R with R the largest of them so far (moved when it is 2^4 behind, like the maximum when a tile's sum of p comes to 2^11; see
+// q8_attention.cu).
 // Order of the products: S0 S1 | PV0 S0 | PV1 S1 | ...: while the tensor cores do one half's PV and its next S, the other half's softmax runs.  P lies over S, so a
 // half's next S waits for its PV, in the same queue; a commit covers all products before it, so a softmax that has its S knows that its last PV is done.
 // Bounds: 2 x 2 x 512 cycles of tensor core and as many of ex2 (16 a cycle) for 256 x 128 scores of heads of 128.
@@ -445,24 +446,29 @@ __global__ void __launch_bounds__(Split<WIDE>::kThreads, 1) q8_prompt_kernel(con
 #pragma unroll
         for (int c = 0; c < 4; ++c) mask32(x[c], lim - key0 - 32 * c);
       }
-      const float mx = largest(x, fac, factor, part, lim - key0);
-      if (__any_sync(0xffffffffu, mx > m + 8.f) || corr != 1.f) {
-        // the maximum moves: what has been summed against the old one follows
-        const float to = fmaxf(m, mx), down = to == -INFINITY ? 1.f : ex2(m - to);
-        m = to;
-        l *= down, corr *= down;
-        if (j > 0) {
+      // against the maximum so far, which is seldom left behind: a sum above 2^11 tells of it (P, up to 16 times as large, is still a half then), and all is done once more
+      float total;
 #pragma unroll 1
-          for (int k = 0; k < HD / 8; ++k) {
-            uint32_t o[8];
-            tmem_ld8(o_at + 8 * k, o);
+      for (bool moved = j == 0 || corr != 1.f;; moved = true) {
+        if (moved) {
+          const float to = fmaxf(m, largest(x, fac, factor, part, lim - key0)), down = to == -INFINITY ? 1.f : ex2(m - to);
+          m = to;
+          l *= down, corr *= down;
+          if (j > 0) {
+#pragma unroll 1
+            for (int k = 0; k < HD / 8; ++k) {
+              uint32_t o[8];
+              tmem_ld8(o_at + 8 * k, o);
 #pragma unroll
-            for (int i = 0; i < 8; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * corr);
-            tmem_st8(o_at + 8 * k, o);
+              for (int i = 0; i < 8; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * corr);
+              tmem_st8(o_at + 8 * k, o);
+            }
           }
         }
+        total = weights(s_at, x, fac, factor, m == -INFINITY ? 0.f : m, part, lim - key0);
+        if (moved || !__any_sync(0xffffffffu, total > 2048.f)) break;
       }
-      l += weights(s_at, x, fac, factor, m == -INFINITY ? 0.f : m, part, lim - key0);
+      l += total;
       tmem_st_wait();
       tc_fence_before();
       __syncwarp();
