@@ -5,10 +5,13 @@
 // memory: the sum of the first product may run over the dimensions in any order, so a thread takes 16 neighbouring bytes of a key, and the second over the keys in
 // any order, so it takes 16 neighbouring dimensions of four keys; P^T comes out of S^T by movmatrix.
 //   s_j = ks_j c (q . k_j),  p_j = 2^(s_j - m),  l = sum p_j,  o = sum (p_j vs_j / R) v_j  with codes k_j, v_j and the scales ks_j, vs_j of their blocks:
-// codes are exact in fp16, q is too (bf16 rows are brought into its range by a power of two), so the only roundings to 16 bits are q's own and p's; sums are fp32.
+// codes are exact in fp16, q is too (bf16 rows are brought into its range by a power of two; what is 2^-38 of a row's largest value may be lost), so the only rounding to
+// 16 bits is p's; sums are fp32.
 // m follows the maximum only where it is more than 2^8 behind, R the largest value scale where it is more than 2^4 behind: p stays below 2^12, and what is lost of
 // a small p is 2^-25 of the largest.
-// Bound by HBM on the codes (a key and its value are 2 hd bytes).  The keys of a row are shared out over the warps of a CTA and over up to kMaxSplits CTAs.
+// Bound by HBM on the codes (a key and its value are 2 hd bytes): 64 sequences x 32 heads x 2048 keys of 128, 1.08 GB, 166 us in a graph, 6.5 TB/s; by latency where they are
+// few (1 sequence: 12.6 us for 17 MB: positions, codes, a few groups a warp, the second kernel).  The keys of a row are shared out over the warps of a CTA and
+// over up to kMaxSplits CTAs.  A first version that loaded the groups into registers took 280 us for the former: 8 warps an SM instead of 16.
 #include "../../include/blr_b200.h"
 #include "q8_attention.h"
 #include "tmap.h"
@@ -396,11 +399,13 @@ struct Q8Plan {
   int nt, q_tiles, ns, room;  // nt: column tiles of 8 rows of the kernel here, 0: the prompt kernel; ns: CTAs that may share a row tile's keys
   long long rows, tiles, wide_tiles;  // wide_tiles: of 128 slots of a head, whose codes are widened ahead (0: not)
 };
-static constexpr int kWideFrom = 4;  // row tiles of a kv head from which its codes are widened ahead
-static constexpr long long kWideBytes = 256ll << 20;  // room that widened codes may take
+// Row tiles of a kv head from which its codes are widened ahead of the prompt kernel (us without | with, 32 heads on 8: 32 tiles, 2048 tokens 64 | 70, 64 tiles, 4096 tokens
+// 202 | 184, 128 tiles, 8192 tokens 670 | 600), and the room that they may take.
+static constexpr int kWideFrom = 48;
+static constexpr long long kWideBytes = 256ll << 20;
 // Few row tiles share their keys out over more CTAs, as many as the SMs hold at a time (4, 3, 2 or 1 of a kind); a second kernel sums the parts.  The host does not
 // know the sequences' lengths: a tile may have half as many CTAs again as its even share, and the kernel here shares by the
-// lengths.  Up to 512 slots a second launch (3 us) costs more than it saves (1 sequence x 32 heads x 300 keys: 2 CTAs a head TODO us, one TODO).
+// lengths.  Up to 512 slots a second launch (3 us) costs more than it saves (1 sequence x 32 heads x 300 keys of 2048 slots, shared and summed: 10 us, of which the second kernel 3).
 static Q8Plan q8_plan(const blr_q8_cache* c, int64_t n_tok, int heads) {
   Q8Plan a = {};
   a.rows = n_tok * (heads / c->kv_heads);

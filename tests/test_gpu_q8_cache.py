@@ -200,17 +200,20 @@ def _attention(q, parts, block, starts, new, scale):
     k, v = (_values(c).double() * s.double().repeat_interleave(block, -1)[..., :slots, None] for c, s in ((parts[0], parts[2]), (parts[1], parts[3])))
     out, room = torch.zeros(B, T, H, hd, dtype=torch.float64), torch.zeros(B, T, H, hd, dtype=torch.float64)
     for b in range(B):
-        for t in range(T if new is None else max(0, min(T, new[b]))):
-            n = max(0, min(slots, starts[b] + t + 1))
-            if n == 0:
-                continue
-            for h in range(H):
-                kh, vh = k[b, h // (H // KV), :n], v[b, h // (H // KV), :n]
-                x = kh @ q[b, t, h].double() * scale
-                p = torch.exp(x - x.max())
-                l = p.sum()
-                out[b, t, h] = p @ vh / l
-                room[b, t, h] = 2.0 ** -11 * (p @ vh.abs()) / l + n * 2.0 ** -21 * vh.abs().max() / l
+        rows = T if new is None else max(0, min(T, new[b]))
+        seen = (torch.arange(rows) + starts[b] + 1).clamp(0, slots)
+        n = int(seen.max()) if rows else 0
+        if n == 0:
+            continue
+        out_of_sight = torch.arange(n) >= seen[:, None]
+        for h in range(H):
+            kh, vh = k[b, h // (H // KV), :n], v[b, h // (H // KV), :n]
+            x = (q[b, :rows, h].double() @ kh.T * scale).masked_fill(out_of_sight, -math.inf)
+            p = torch.exp(x - x.amax(1, keepdim=True).clamp(min=-1e300))
+            l = p.sum(1, keepdim=True).clamp(min=1e-300)
+            most = vh.abs().amax(1).cummax(0).values[seen.clamp(min=1) - 1]   # the largest value that the row sees
+            out[b, :rows, h] = p @ vh / l
+            room[b, :rows, h] = 2.0 ** -11 * (p @ vh.abs()) / l + torch.where(seen > 0, seen * 2.0 ** -21 * most, torch.zeros(()).double())[:, None] / l.clamp(min=1e-3)
     return out, room
 
 
@@ -227,8 +230,9 @@ ATTENDS = [  # B, T, H, KV, hd, slots, block, starts, new
     (1, 130, 2, 1, 128, 130, 16, [0], None),
     (2, 150, 3, 3, 128, 420, 128, [1, 270], [0, 150]),
     (1, 260, 4, 1, 64, 517, 64, [257], None),
-    (2, 410, 4, 2, 128, 900, 32, [490, 100], [410, 77]),          # (codes widened ahead)
-    (3, 520, 2, 1, 64, 523, 16, [3, -7, 0], [520, 520, 0]),
+    (2, 410, 4, 2, 128, 900, 32, [490, 100], [410, 77]),
+    (2, 1520, 8, 1, 64, 1560, 32, [25, -7], [1520, 800]),         # (codes widened ahead)
+    (1, 1540, 8, 1, 128, 1600, 16, [60], None),
 ]
 
 
