@@ -55,15 +55,14 @@ struct Vec {
     if constexpr (KIND == 2) return __uint_as_float(u);
     else return [&](float2 v) { return i & 1 ? v.y : v.x; }(q8_up2<KIND == 1>(u));
   }
-  // as floats, what is lower than -65504 (fp16) or -10^30 set to that: a weight of 0 is then one of a number
   __device__ __forceinline__ static void floats(const uint4& w, float (&f)[kPer]) {
     const uint32_t ws[4] = {w.x, w.y, w.z, w.w};
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
       if constexpr (KIND == 2) {
-        f[i] = fmaxf(__uint_as_float(ws[i]), -1e30f);
+        f[i] = __uint_as_float(ws[i]);
       } else {
-        const float2 v = q8_up2<KIND == 1>(larger(ws[i], KIND == 0 ? 0xfbfffbffu : 0xf149f149u));
+        const float2 v = q8_up2<KIND == 1>(ws[i]);
         f[2 * i] = v.x, f[2 * i + 1] = v.y;
       }
     }
@@ -195,7 +194,7 @@ __global__ void __launch_bounds__(kLpThreads, 3) token_logprobs_kernel(const __g
   const bool all = least == 0;  // (too few groups have seen anything: keep everything)
 
   // ---- the sums, and the values that reach the threshold
-  // (beyond 10^37, where M log2 e may be infinite, numbers that differ are at least 2^99 apart: c = 1 gives the same weights, 1 and 0)
+  // (beyond 10^37, where M log2 e may be infinite, numbers that differ are at least 2^99 apart: c = 1 gives the same weights, 1 and 0; a row of the type's lowest number is one)
   const bool far = fabsf(M) > 1e37f;
   const float c = far ? 1.f : 1.4426950408889634f, m = M * c;
   float S = 0.f, D = 0.f;
@@ -206,7 +205,7 @@ __global__ void __launch_bounds__(kLpThreads, 3) token_logprobs_kernel(const __g
   if (finite) {
     float s2[2] = {0.f, 0.f}, d2[2] = {0.f, 0.f};
     auto add = [&](float x, int k) {
-      const float t = fmaf(x, c, -m), e = lp_ex2(t);
+      const float t = fmaxf(fmaf(x, c, -m), -1e30f), e = lp_ex2(t);  // (-inf: a weight of 0, and of a number)
       s2[k] += e;
       d2[k] = fmaf(e, t, d2[k]);
     };
@@ -223,7 +222,7 @@ __global__ void __launch_bounds__(kLpThreads, 3) token_logprobs_kernel(const __g
       vec(v);
     }
     if (i < mine) vec(part[i]);
-    if (tid < edges) add(fmaxf(sh.edge[tid], -1e30f), 0);
+    if (tid < edges) add(sh.edge[tid], 0);
     S = s2[0] + s2[1], D = d2[0] + d2[1];
     if (p.top > 0 && (all || seen >= least)) {  // (few threads)
       for (int i = tid; i < mine; i += kLpThreads) {

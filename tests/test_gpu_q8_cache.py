@@ -437,6 +437,11 @@ def _rows(rows, vocab, dtype, g, kind):
         x[:] = 0.25
     elif kind == "lowest":   # places masked with the type's lowest number
         x[:, 1:] = torch.finfo(dtype).min
+    elif kind == "all lowest":   # a row that is masked as a whole in that way is an even distribution
+        x[:] = torch.finfo(dtype).min
+        x[1:, ::3] = 0
+    elif kind == "ends":
+        x[:, 1], x[:, vocab // 2], x[1:, 3] = torch.finfo(dtype).min, -math.inf, torch.finfo(dtype).max
     elif kind == "large":
         x = x * 1e4
     elif kind == "steps":    # many ties
@@ -449,7 +454,7 @@ def _rows(rows, vocab, dtype, g, kind):
                                                  (2, 333, 3, "lowest"), (3, 2048, 4, "large"), (37, 50257, 0, ""), (7, 20011, 20, "steps"), (300, 515, 2, ""),
                                                  (2, 131072, 7, "steps"), (1, 151936, 33, "masked"), (160, 40000, 64, "equal"),
                                                  # (many rows of 16 to 64 KB)
-                                                 (311, 9001, 8, ""), (300, 20000, 64, "masked"), (602, 15011, 33, "steps"), (296, 16000, 40, "equal"), (299, 8300, 0, "lowest")])
+                                                 (311, 9001, 8, ""), (300, 20000, 64, "masked"), (602, 15011, 33, "steps"), (296, 16000, 40, "equal"), (299, 8300, 0, "lowest"), (2, 1030, 4, "all lowest"), (3, 40003, 9, "ends")])
 def test_logprobs(ops, rows, vocab, top, kind, dtype):
     g = torch.Generator().manual_seed(rows + vocab)
     x = _rows(rows, vocab, dtype, g, kind)
