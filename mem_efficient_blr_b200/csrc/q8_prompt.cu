@@ -11,7 +11,8 @@
 // Bounds: 2 x 2 x 512 cycles of tensor core and as many of ex2 (16 a cycle) for 256 x 128 scores of heads of 128.  A step takes some 4000 (8192 tokens, 32 heads on 8: 600 us,
 // 917 TFLOP/s): each half's chain of softmax (2400: S from TMEM, 128 ex2 a thread at 14 cycles) and products (1250 from P to the next S) is what it waits for; the
 // two halves' chains overlap, but TMEM has no room for a second S of each.  Tried without gain: part of ex2 as a polynomial on the FMA pipe (1/8: 617 us, 3/8: 623), four
-// softmax warpgroups of half a tile's width each (771), vs / R in the exponent instead of a multiplication (610), scores read twice instead of held (697).
+// softmax warpgroups of half a tile's width each (771), vs / R in the exponent instead of a multiplication (610), scores read twice instead of held (697),
+// steps of 64 keys with two places for each half's S (616: S reads both its operands for 64 columns, 768 cycles a step, and the two halves fall into step).
 // All waits are bounded; a time-out is noted in *status, the rows of that CTA come out as NaN, and the kernel frees its TMEM and ends.
 #include <math_constants.h>
 
