@@ -89,7 +89,10 @@ def build_torch_ext(force: bool = False, verbose: bool = False) -> str:
     ce.load(name="_blr_torch", sources=[os.path.join(CSRC, "torch_ext.cpp")], extra_cflags=["-O2", "-std=c++17"],
             extra_include_paths=[os.path.join(HERE, "..", "include")], extra_ldflags=[f"-L{HERE}", "-lblr_b200"],
             build_directory=bdir, with_cuda=True, is_python_module=False, verbose=verbose)
-    shutil.copyfile(os.path.join(bdir, "_blr_torch.so"), EXT)
+    # (a file of its own, then renamed: written over in place, a process that has the extension loaded loses its relocated pages and crashes at the next call)
+    fresh = f"{EXT}.{os.getpid()}"
+    shutil.copyfile(os.path.join(bdir, "_blr_torch.so"), fresh)
+    os.replace(fresh, EXT)
     return EXT
 
 
