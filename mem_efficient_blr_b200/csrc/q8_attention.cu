@@ -399,9 +399,9 @@ struct Q8Plan {
   int nt, q_tiles, ns, room;  // nt: column tiles of 8 rows of the kernel here, 0: the prompt kernel; ns: CTAs that may share a row tile's keys
   long long rows, tiles, wide_tiles;  // wide_tiles: of 128 slots of a head, whose codes are widened ahead (0: not)
 };
-// Row tiles of a kv head from which its codes are widened ahead of the prompt kernel (us without | with, 32 heads on 8: 32 tiles, 2048 tokens 64 | 70, 64 tiles, 4096 tokens
-// 202 | 184, 128 tiles, 8192 tokens 670 | 600), and the room that they may take.
-static constexpr int kWideFrom = 48;
+// Row tiles of a kv head from which its codes are widened ahead of the prompt kernel (us without | with, 32 heads on 8: 32 tiles, 2048 tokens 59 | 68, 40 tiles, 2560 tokens
+// 93 | 91, 64 tiles, 4096 tokens 187 | 180, 128 tiles, 8192 tokens 637 | 557), and the room that they may take.
+static constexpr int kWideFrom = 40;
 static constexpr long long kWideBytes = 256ll << 20;
 // Few row tiles share their keys out over more CTAs, as many as the SMs hold at a time (4, 3, 2 or 1 of a kind); a second kernel sums the parts.  The host does not
 // know the sequences' lengths: a tile may have half as many CTAs again as its even share, and the kernel here shares by the

@@ -1,18 +1,20 @@
 // Causal attention of many rows over an 8-bit cache (q8.cuh) on tcgen05 / TMEM (sm_100a).  One CTA takes 256 rows of a kv head (tokens x query heads, token by
-// token) and walks the keys 128 at a time, warp-specialised:
+// token) and walks the keys in tiles of 128, warp-specialised:
 //   warps 0-3, 4-7  softmax of rows 0-127 and 128-255, a thread per row: S from TMEM, P back over it as fp16 pairs, O rescaled there when it has to be
 //   warps 8-11      widen the codes of the next keys and values to fp16 (exact) into shared memory, as tcgen05.mma reads them
 //   warps 12-15     one thread of the first issues the products: S = Q K^T (both from shared memory), O += P V (P from TMEM)
 // The scales stay out of the products: a group of 16 keys has one for its keys, which multiplies S in the exponent's argument, and one for its values, which
 // multiplies p by vs / R with R the largest of them so far (moved when it is 2^4 behind, like the maximum when a tile's sum of p comes to 2^11; see
 // q8_attention.cu).
-// Order of the products: S0 S1 | PV0 S0 | PV1 S1 | ...: while the tensor cores do one half's PV and its next S, the other half's softmax runs.  P lies over S, so a
-// half's next S waits for its PV, in the same queue; a commit covers all products before it, so a softmax that has its S knows that its last PV is done.
-// Bounds: 2 x 2 x 512 cycles of tensor core and as many of ex2 (16 a cycle) for 256 x 128 scores of heads of 128.  A step takes some 4000 (8192 tokens, 32 heads on 8: 600 us,
-// 917 TFLOP/s): each half's chain of softmax (2400: S from TMEM, 128 ex2 a thread at 14 cycles) and products (1250 from P to the next S) is what it waits for; the
-// two halves' chains overlap, but TMEM has no room for a second S of each.  Tried without gain: part of ex2 as a polynomial on the FMA pipe (1/8: 617 us, 3/8: 623), four
-// softmax warpgroups of half a tile's width each (771), vs / R in the exponent instead of a multiplication (610), scores read twice instead of held (697),
-// steps of 64 keys with two places for each half's S (616: S reads both its operands for 64 columns, 768 cycles a step, and the two halves fall into step).
+// A step is half a tile, 64 keys, and a half's S alternates between two places of TMEM: S0 S0 S1 S1 first, then PV0 S0 | PV1 S1 | ... with the S two steps ahead of the PV, into
+// the place that the PV's P has left (P lies over the S that it was made of; one queue, so in order).  Neither half waits for the other's softmax, or for its own scores.
+// O is rescaled, seldom, when the last PV is known to be done.
+// Bounds, a step of 256 x 64 scores of heads of 128: 1280 cycles of tensor core (2 x 256 for PV, 2 x 384 for S, which reads both operands from shared memory for 64 columns)
+// and 1024 of ex2 (16 a cycle).  It takes 2150: the softmaxes of both halves share the schedulers for 1520 from scores in registers to P in TMEM, and spend 640 on barriers,
+// factors and TMEM's latency.  8192 tokens, 32 heads on 8: 592 us, 928 TFLOP/s.  (Steps of 128 keys, which leave no room for a second S: 600, and 3 x 257 tokens over up to 6001
+// keys of heads of 64 71 instead of 67.  All ex2 left out: 12 % less time.  With the next scores loaded between the two halves of a step's: 610.)  Tried on steps of 128 without
+// gain: part of ex2 as a polynomial on the FMA pipe (1/8: 617 us, 3/8: 623), four softmax warpgroups of half a tile's width each (771), vs / R in the exponent instead of a
+// multiplication (610), scores read twice instead of held (697).
 // All waits are bounded; a time-out is noted in *status, the rows of that CTA come out as NaN, and the kernel frees its TMEM and ends.
 #include <math_constants.h>
 
@@ -22,7 +24,7 @@
 
 namespace blr {
 
-static constexpr int kKeys = 128;
+static constexpr int kKeys = 128, kStepKeys = 64;
 // Threads, and registers of a thread at launch and from then on of the softmax warps (8), the widening ones (4, none where the codes have been widened) and the last
 // four: setmaxnreg waits for ever for registers that the block was not launched with.
 template <bool WIDE>
@@ -84,11 +86,11 @@ __device__ __forceinline__ void factors32(uint32_t fac, int c, float factor, boo
     }
   }
 }
-// The maximum of a row's 128 scores, scaled:
-__device__ __forceinline__ float largest(const uint32_t (&x)[4][32], uint32_t fac, float factor, bool part, int left) {
+// The maximum of 64 scores of a row, scaled:
+__device__ __forceinline__ float largest(const uint32_t (&x)[2][32], uint32_t fac, float factor, bool part, int left) {
   float mx[2] = {-INFINITY, -INFINITY};
 #pragma unroll
-  for (int c = 0; c < 4; ++c) {
+  for (int c = 0; c < 2; ++c) {
     float cg[2], fg[2];
     factors32(fac, c, factor, part, left - 32 * c, cg, fg);
 #pragma unroll
@@ -102,11 +104,11 @@ __device__ __forceinline__ float largest(const uint32_t (&x)[4][32], uint32_t fa
   return fmaxf(mx[0], mx[1]);
 }
 // p = 2^(s - mu), and P = p vs / R as fp16 pairs over the scores in TMEM; returns the sum of p.
-__device__ __forceinline__ float weights(uint32_t s_at, const uint32_t (&x)[4][32], uint32_t fac, float factor, float mu, bool part, int left) {
+__device__ __forceinline__ float weights(uint32_t s_at, const uint32_t (&x)[2][32], uint32_t fac, float factor, float mu, bool part, int left) {
   uint64_t sum[2] = {0, 0};
   const uint64_t neg = pair(-mu, -mu);
 #pragma unroll
-  for (int c = 0; c < 4; ++c) {
+  for (int c = 0; c < 2; ++c) {
     float cg[2], fg[2];
     uint32_t y[16];
     factors32(fac, c, factor, part, left - 32 * c, cg, fg);
@@ -221,7 +223,7 @@ __global__ void __launch_bounds__(Split<WIDE>::kThreads, 1) q8_prompt_kernel(con
   constexpr uint32_t kTile = 128 * HD * 2;
   const uint32_t base = (smem_u32(prompt_raw) + 1023u) & ~1023u;
   const uint32_t qs = base, ks = base + 2 * kTile, vs = base + 4 * kTile, bars = base + 6 * kTile;
-  const uint32_t kfull = bars, vfull = bars + 16, kempty = bars + 32, vempty = bars + 48, sfull = bars + 64, pfull = bars + 80, ofull = bars + 96, cfull = bars + 112;
+  const uint32_t kfull = bars, vfull = bars + 16, kempty = bars + 32, vempty = bars + 48, sfull = bars + 64, pfull = bars + 96, done = bars + 128, cfull = bars + 160;  // sfull, pfull, done: [half][place]
   __shared__ uint32_t tmem_slot;
   __shared__ volatile int aborted;
   volatile int* const abort_flag = &aborted;
@@ -234,11 +236,13 @@ __global__ void __launch_bounds__(Split<WIDE>::kThreads, 1) q8_prompt_kernel(con
       mbar_init(vfull + 8 * i, WIDE ? 1 : 4);
       mbar_init(kempty + 8 * i, 1);
       mbar_init(vempty + 8 * i, 1);
+    }
+    for (int i = 0; i < 4; ++i) {
       mbar_init(sfull + 8 * i, 1);
       mbar_init(pfull + 8 * i, 4);
-      mbar_init(ofull + 8 * i, 1);
+      mbar_init(done + 8 * i, 1);
+      mbar_init(cfull + 8 * i, 1);
     }
-    for (int i = 0; i < 4; ++i) mbar_init(cfull + 8 * i, 1);
     mbar_init_fence();
   }
   if (warp == kLast) tmem_alloc(smem_u32(&tmem_slot), 512);
@@ -254,8 +258,8 @@ __global__ void __launch_bounds__(Split<WIDE>::kThreads, 1) q8_prompt_kernel(con
     keys = max(keys0, keys1);
     const int share = ((keys + p.ns - 1) / p.ns + kKeys - 1) / kKeys * kKeys, k1 = min(keys, (at.split + 1) * share);
     k0 = min(keys, at.split * share);
-    n0 = max(0, min(keys0, k1) - k0 + kKeys - 1) / kKeys;
-    n1 = max(0, min(keys1, k1) - k0 + kKeys - 1) / kKeys;
+    n0 = max(0, min(keys0, k1) - k0 + kStepKeys - 1) / kStepKeys;
+    n1 = max(0, min(keys1, k1) - k0 + kStepKeys - 1) / kStepKeys;
 
   // ---- a softmax thread's row of q, as fp16
   const int row_i = (int)threadIdx.x & 127, r = at.r0 + (int)threadIdx.x;
@@ -299,7 +303,7 @@ __global__ void __launch_bounds__(Split<WIDE>::kThreads, 1) q8_prompt_kernel(con
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem = tmem_slot;
-  const int steps = max(n0, n1);
+  const int halves = max(n0, n1), steps = (halves + 1) / 2;  // (n0, n1, halves: of 64 keys; steps: tiles of 128)
 
   // (No spills in any of these: what shared memory leaves of L1 does not keep them, and a reload from L2 inside a loop costs more than anything that it saves.)
   // A step's factors: of 8 groups of 16 keys ks and vs / R, and how R moved.  One warp makes them, four steps deep (a step's are free when the S of the step after it
@@ -349,50 +353,56 @@ __global__ void __launch_bounds__(Split<WIDE>::kThreads, 1) q8_prompt_kernel(con
       }
     }
     if (warp == kLast && elect_one()) {
-      const uint32_t id_s = umma_idesc(false, false, false, 128, kKeys), id_o = umma_idesc(false, false, true, 128, HD);
-      auto product_s = [&](int i, int j) {
+      const uint32_t id_s = umma_idesc(false, false, false, 128, kStepKeys), id_o = umma_idesc(false, false, true, 128, HD);
+      auto product_s = [&](int i, int u) {
         uint32_t q_at = qs + i * kTile;
         asm volatile("" : "+r"(q_at));  // (sixteen descriptors kept across the loop would be spilled)
-        const uint64_t a = umma_smem_desc(q_at, 16, 1024), k = umma_smem_desc(ks + (j & 1) * kTile, 16, 1024);
+        const uint64_t a = umma_smem_desc(q_at, 16, 1024), k = umma_smem_desc(ks + ((u >> 1) & 1) * kTile + (u & 1) * 8192, 16, 1024);
+        const uint32_t to = tmem + 128 * i + 64 * (u & 1);
 #pragma unroll
-        for (int s = 0; s < HD / 16; ++s) umma_f16(tmem + 128 * i, a + (s >> 2) * 1024 + (s & 3) * 2, k + (s >> 2) * 1024 + (s & 3) * 2, id_s, s != 0);
-        umma_commit(sfull + 8 * i);
+        for (int s = 0; s < HD / 16; ++s) umma_f16(to, a + (s >> 2) * 1024 + (s & 3) * 2, k + (s >> 2) * 1024 + (s & 3) * 2, id_s, s != 0);
+        umma_commit(sfull + 16 * i + 8 * (u & 1));
       };
-      auto product_o = [&](int i, int j) {
-        const uint64_t v = umma_smem_desc(vs + (j & 1) * kTile, 16384, 1024);
+      auto product_o = [&](int i, int u) {
+        const uint64_t v = umma_smem_desc(vs + ((u >> 1) & 1) * kTile + (u & 1) * 8192, 16384, 1024);
+        const uint32_t from = tmem + 128 * i + 64 * (u & 1);
 #pragma unroll
-        for (int s = 0; s < kKeys / 16; ++s) umma_f16_ts(tmem + 256 + 128 * i, tmem + 128 * i + 8 * s, v + 128 * s, id_o, (j | s) != 0);
+        for (int s = 0; s < kStepKeys / 16; ++s) umma_f16_ts(tmem + 256 + 128 * i, from + 8 * s, v + 128 * s, id_o, (u | s) != 0);
+        umma_commit(done + 16 * i + 8 * (u & 1));  // (one for each place: behind the last P two products may be under way, and a barrier's parity tells two phases apart, not three)
       };
-      bool ok = steps > 0 && mbar_poll(kfull, 0, abort_flag);
+      bool ok = halves > 0 && mbar_poll(kfull, 0, abort_flag);
       if (ok) {
         tc_fence_after();
         if (n0 > 0) product_s(0, 0);
+        if (n0 > 1) product_s(0, 1);
         if (n1 > 0) product_s(1, 0);
+        if (n1 > 1) product_s(1, 1);
         umma_commit(kempty);
       }
 #pragma unroll 1
-      for (int j = 0; ok && j < steps; ++j) {
-        const uint32_t s = j & 1;
+      for (int u = 0; ok && u < halves; ++u) {
+        const int j = u >> 1, next = u + 2;
         // (written out: a loop around the products costs the elected thread hundreds of cycles a step)
-        if (!mbar_poll(vfull + 8 * s, (j >> 1) & 1, abort_flag)) { ok = false; break; }
-        if (j < n0) {
-          if (!mbar_poll(pfull, j & 1, abort_flag)) { ok = false; break; }
-          tc_fence_after();
-          product_o(0, j);
-          if (j + 1 >= n0) umma_commit(ofull);
+        if ((u & 1) == 0) {
+          if (!mbar_poll(vfull + 8 * (j & 1), (j >> 1) & 1, abort_flag)) { ok = false; break; }
+          if (next < halves && !mbar_poll(kfull + 8 * ((j + 1) & 1), ((j + 1) >> 1) & 1, abort_flag)) { ok = false; break; }
         }
-        if (j + 1 < steps && !mbar_poll(kfull + 8 * (s ^ 1), ((j + 1) >> 1) & 1, abort_flag)) { ok = false; break; }
-        tc_fence_after();
-        if (j + 1 < n0) product_s(0, j + 1);
-        if (j < n1) {
-          if (!mbar_poll(pfull + 8, j & 1, abort_flag)) { ok = false; break; }
+        if (u < n0) {
+          if (!mbar_poll(pfull + 8 * (u & 1), j & 1, abort_flag)) { ok = false; break; }
           tc_fence_after();
-          product_o(1, j);
-          if (j + 1 >= n1) umma_commit(ofull + 8);
+          product_o(0, u);
+          if (next < n0) product_s(0, next);
         }
-        umma_commit(vempty + 8 * s);
-        if (j + 1 < n1) product_s(1, j + 1);
-        if (j + 1 < steps) umma_commit(kempty + 8 * (s ^ 1));
+        if (u < n1) {
+          if (!mbar_poll(pfull + 16 + 8 * (u & 1), j & 1, abort_flag)) { ok = false; break; }
+          tc_fence_after();
+          product_o(1, u);
+          if (next < n1) product_s(1, next);
+        }
+        if (u & 1) {
+          if (next < halves) umma_commit(kempty + 8 * ((j + 1) & 1));
+          umma_commit(vempty + 8 * (j & 1));
+        }
       }
     }
     __syncwarp();
@@ -424,41 +434,44 @@ __global__ void __launch_bounds__(Split<WIDE>::kThreads, 1) q8_prompt_kernel(con
   } else {
     asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(Split<WIDE>::kSoftmax));
     const int n = wg ? n1 : n0;
-    const uint32_t lanes = (uint32_t)(32 * (warp & 3)) << 16, s_at = tmem + lanes + 128 * wg, o_at = tmem + lanes + 256 + 128 * wg;
+    const uint32_t lanes = (uint32_t)(32 * (warp & 3)) << 16, o_at = tmem + lanes + 256 + 128 * wg;
     float m = -INFINITY, l = 0.f, R = 0.f;
     const int lim_all = __reduce_min_sync(0xffffffffu, lim);
     bool ok = true;
 #pragma unroll 1
-    for (int j = 0; j < n; ++j) {
-      const int key0 = k0 + j * kKeys;
-      const bool part = key0 + kKeys > lim_all;  // some of the tile is masked for a row of the warp
-      if (!__all_sync(0xffffffffu, mbar_wait(cfull + 8 * (j & 3), (j >> 2) & 1, abort_flag))) { ok = false; break; }
-      const uint32_t fac = smem_u32(factors[j & 3]);
+    for (int u = 0; u < n; ++u) {
+      const int j = u >> 1, key0 = k0 + u * kStepKeys;
+      const uint32_t s_at = tmem + lanes + 128 * wg + 64 * (u & 1);
+      const bool part = key0 + kStepKeys > lim_all;  // some of these keys are masked for a row of the warp
+      if ((u & 1) == 0 && !__all_sync(0xffffffffu, mbar_wait(cfull + 8 * (j & 3), (j >> 2) & 1, abort_flag))) { ok = false; break; }
+      const uint32_t tile = smem_u32(factors[j & 3]), fac = tile + 16 * (u & 1);  // (of the step's four groups; those of their values 32 bytes behind)
       uint32_t vr[2];
-      lds64(fac + 64, vr[0], vr[1]);
-      float corr = __uint_as_float(vr[0]);
+      lds64(tile + 64, vr[0], vr[1]);
+      float corr = u & 1 ? 1.f : __uint_as_float(vr[0]);
       R = __uint_as_float(vr[1]);
-      if (!__all_sync(0xffffffffu, mbar_wait(sfull + 8 * wg, j & 1, abort_flag))) { ok = false; break; }
+      if (!__all_sync(0xffffffffu, mbar_wait(sfull + 16 * wg + 8 * (u & 1), j & 1, abort_flag))) { ok = false; break; }
       tc_fence_after();
-      uint32_t x[4][32];
-#pragma unroll
-      for (int c = 0; c < 4; ++c) tmem_ld32(s_at + 32 * c, x[c]);
+      uint32_t x[2][32];
+      tmem_ld32(s_at, x[0]);
+      tmem_ld32(s_at + 32, x[1]);
       tmem_ld_wait();
-#pragma unroll
-      for (int c = 0; c < 4; ++c) tmem_ready(x[c]);
+      tmem_ready(x[0]);
+      tmem_ready(x[1]);
       if (part) {
-#pragma unroll
-        for (int c = 0; c < 4; ++c) mask32(x[c], lim - key0 - 32 * c);
+        mask32(x[0], lim - key0);
+        mask32(x[1], lim - key0 - 32);
       }
       // against the maximum so far, which is seldom left behind: a sum above 2^11 tells of it (P, up to 16 times as large, is still a half then), and all is done once more
-      float total;
+      float total = 0.f;
 #pragma unroll 1
-      for (bool moved = j == 0 || corr != 1.f;; moved = true) {
+      for (bool moved = u == 0 || corr != 1.f;; moved = true) {
         if (moved) {
           const float to = fmaxf(m, largest(x, fac, factor, part, lim - key0)), down = to == -INFINITY ? 1.f : ex2(m - to);
           m = to;
           l *= down, corr *= down;
-          if (j > 0) {
+          if (u > 0) {
+            if (!__all_sync(0xffffffffu, mbar_wait(done + 16 * wg + 8 * ((u - 1) & 1), ((u - 1) >> 1) & 1, abort_flag))) { ok = false; break; }
+            tc_fence_after();
 #pragma unroll 1
             for (int k = 0; k < HD / 8; ++k) {
               uint32_t o[8];
@@ -472,13 +485,14 @@ __global__ void __launch_bounds__(Split<WIDE>::kThreads, 1) q8_prompt_kernel(con
         total = weights(s_at, x, fac, factor, m == -INFINITY ? 0.f : m, part, lim - key0);
         if (moved || !__any_sync(0xffffffffu, total > 2048.f)) break;
       }
+      if (!ok) break;
       l += total;
       tmem_st_wait();
       tc_fence_before();
       __syncwarp();
-      if (lane == 0) mbar_arrive(pfull + 8 * wg);
+      if (lane == 0) mbar_arrive(pfull + 16 * wg + 8 * (u & 1));
     }
-    if (ok && n > 0 && !__all_sync(0xffffffffu, mbar_wait(ofull + 8 * wg, 0, abort_flag))) ok = false;
+    if (ok && n > 0 && !__all_sync(0xffffffffu, mbar_wait(done + 16 * wg + 8 * ((n - 1) & 1), ((n - 1) >> 1) & 1, abort_flag))) ok = false;
     tc_fence_after();
     const Place at = place_of(p);
     const int r = at.r0 + (int)threadIdx.x;
