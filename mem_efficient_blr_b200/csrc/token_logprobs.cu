@@ -19,7 +19,7 @@ namespace cg = cooperative_groups;
 
 namespace blr {
 
-static constexpr int kLpThreads = 512, kLpWarps = kLpThreads / 32, kLpMaxTop = 64, kLpKept = 1024, kLpMaxPart = 200 * 1024;
+static constexpr int kLpMaxTop = 64, kLpGroups = 128, kLpMaxPart = 200 * 1024;
 typedef unsigned long long Ranked;  // order_of(value) << 32 | ~id: larger is likelier
 
 // Whole numbers in the order of the values; 0 is below all of them.
@@ -81,7 +81,7 @@ __device__ __forceinline__ float lp_ex2(float x) {
   return r;
 }
 
-// Of the largest values that up to 64 groups of threads have seen, the `top`-th (by one warp): at least so many of a row's values reach it, and seldom many more.
+// Of the largest values that groups of threads have seen, the `top`-th (by one warp): at least so many of a row's values reach it, and seldom many more.
 // 0: there are fewer.
 __device__ __forceinline__ uint32_t reached_by(const uint32_t* group, int groups, int top, int lane) {
   uint32_t found = 0;
@@ -93,13 +93,16 @@ __device__ __forceinline__ uint32_t reached_by(const uint32_t* group, int groups
   }
   return __reduce_max_sync(0xffffffffu, found);
 }
-// The groups of a CTA's warps: a warp each, or a half or a quarter of one; the first thread of each leaves what its group has seen.
-__device__ __forceinline__ int leave_group(uint32_t seen, uint32_t* group, int warps, int top, int warp, int lane) {
-  const int parts = top <= warps ? 1 : top <= 2 * warps ? 2 : 4;
+// The groups of a CTA's warps, a warp each or equal parts of one: as few as make a group that has seen something for each token asked for, twice as many in a CTA of few warps,
+// which has less room for what reaches the threshold.  The first thread of each leaves what its group has seen.
+template <int WARPS>
+__device__ __forceinline__ int leave_group(uint32_t seen, uint32_t* group, int vectors, int top, int warp, int lane) {
+  int parts = 1;
+  while (parts < 32 && parts * WARPS < kLpGroups && (min(vectors, 32 * WARPS) * parts + 31) / 32 < (WARPS == 16 ? top : 2 * top)) parts *= 2;
   uint32_t g = seen;
   for (int d = 1; d < 32 / parts; d <<= 1) g = max(g, __shfl_xor_sync(0xffffffffu, g, d));
   if (lane % (32 / parts) == 0) group[warp * parts + lane / (32 / parts)] = g;
-  return warps * parts;
+  return WARPS * parts;
 }
 
 struct LpParams {
@@ -111,17 +114,22 @@ struct LpParams {
   int vocab, top, part;  // part: vectors of a CTA
 };
 
+// What a CTA of THREADS threads keeps beside its part of the row; kKept: room for values that reach the threshold.
+template <int THREADS>
 struct LpShared {
-  Ranked kept[kLpKept], best[kLpMaxTop], red[kLpWarps];
-  float edge[16], sums[2][kLpWarps], S, D;  // edge: values of the row ahead of its first whole vector and behind its last
+  static constexpr int kWarps = THREADS / 32, kKept = THREADS == 512 ? 1024 : 4 * THREADS;
+  Ranked kept[kKept], best[kLpMaxTop], red[kWarps];
+  float edge[16], sums[2][kWarps], S, D;  // edge: values of the row ahead of its first whole vector and behind its last
   uint32_t most, least, count;
-  uint32_t group[64];
+  uint32_t group[kLpGroups];
 };
 
-template <int KIND>
-__global__ void __launch_bounds__(kLpThreads, 3) token_logprobs_kernel(const __grid_constant__ LpParams p) {
+template <int KIND, int THREADS>
+__global__ void __launch_bounds__(THREADS, THREADS == 512 ? 3 : 1536 / THREADS < 32 ? 1536 / THREADS : 32) token_logprobs_kernel(const __grid_constant__ LpParams p) {
   extern __shared__ __align__(16) uint4 part[];
-  __shared__ LpShared sh;
+  typedef LpShared<THREADS> Shared;
+  constexpr int kLpThreads = THREADS, kLpWarps = Shared::kWarps, kLpKept = Shared::kKept;
+  __shared__ Shared sh;
   constexpr int kPer = Vec<KIND>::kPer, kSize = KIND == 2 ? 4 : 2;
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   cg::cluster_group cluster = cg::this_cluster();
@@ -173,7 +181,7 @@ __global__ void __launch_bounds__(kLpThreads, 3) token_logprobs_kernel(const __g
     }
   }
   const float given = id >= 0 && id < p.vocab ? logit<KIND>(row, id) : 0.f;
-  const int groups = leave_group(seen, sh.group, kLpWarps, p.top, warp, lane);
+  const int groups = leave_group<kLpWarps>(seen, sh.group, mine, p.top, warp, lane);
   __syncthreads();
   if (warp == 0) {
     uint32_t most = 0;
@@ -186,7 +194,7 @@ __global__ void __launch_bounds__(kLpThreads, 3) token_logprobs_kernel(const __g
   else __syncthreads();
   uint32_t most = 0, least = 0;
   for (int o = 0; o < n_cta; ++o) {
-    const LpShared* other = cluster.map_shared_rank(&sh, o);
+    const Shared* other = cluster.map_shared_rank(&sh, o);
     most = max(most, other->most), least = max(least, other->least);
   }
   const float M = value_of(most), reach = value_of(least);
@@ -250,7 +258,7 @@ __global__ void __launch_bounds__(kLpThreads, 3) token_logprobs_kernel(const __g
 
   // ---- this CTA's likeliest, in order (0: no more)
   const int kept = (int)sh.count;
-  if (tid < kLpMaxTop) sh.best[tid] = 0;
+  for (int i = tid; i < kLpMaxTop; i += kLpThreads) sh.best[i] = 0;
   __syncthreads();
   if (finite && kept <= kLpKept) {
     for (int i = tid; i < kept; i += kLpThreads) {
@@ -291,7 +299,7 @@ __global__ void __launch_bounds__(kLpThreads, 3) token_logprobs_kernel(const __g
   if (rank == 0) {
     S = D = 0.f;
     for (int o = 0; o < n_cta; ++o) {
-      const LpShared* other = cluster.map_shared_rank(&sh, o);
+      const Shared* other = cluster.map_shared_rank(&sh, o);
       S += other->S, D += other->D;
     }
     const float log_sum = logf(S), log_s = log_sum - fmaf(M, c, -m) * 0.69314718055994531f;
@@ -323,19 +331,19 @@ __global__ void __launch_bounds__(kLpThreads, 3) token_logprobs_kernel(const __g
   if (n_cta > 1) cluster.sync();  // (a CTA's memory is there until the first one has read it)
 }
 
-template <int KIND>
+template <int KIND, int THREADS>
 static int launch_logprobs(const LpParams& p, int64_t rows, int ctas, int smem, cudaStream_t stream) {
   static bool configured[64] = {};
   DeviceInfo di;
   int rc;
   if ((rc = device_info(&di))) return rc;
   if (!configured[di.dev]) {
-    BLR_CUDA_OK(cudaFuncSetAttribute(token_logprobs_kernel<KIND>, cudaFuncAttributeMaxDynamicSharedMemorySize, kLpMaxPart));
+    BLR_CUDA_OK(cudaFuncSetAttribute(token_logprobs_kernel<KIND, THREADS>, cudaFuncAttributeMaxDynamicSharedMemorySize, kLpMaxPart));
     configured[di.dev] = true;
   }
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3((unsigned)(rows * ctas));
-  cfg.blockDim = dim3(kLpThreads);
+  cfg.blockDim = dim3(THREADS);
   cfg.dynamicSmemBytes = (size_t)smem;
   cfg.stream = stream;
   cudaLaunchAttribute at[2];
@@ -346,9 +354,14 @@ static int launch_logprobs(const LpParams& p, int64_t rows, int ctas, int smem, 
   at[1].val.clusterDim.y = at[1].val.clusterDim.z = 1;
   cfg.attrs = at;
   cfg.numAttrs = 2;
-  BLR_CUDA_OK(cudaLaunchKernelEx(&cfg, token_logprobs_kernel<KIND>, p));
+  BLR_CUDA_OK(cudaLaunchKernelEx(&cfg, token_logprobs_kernel<KIND, THREADS>, p));
   return BLR_OK;
 }
+
+// Rows of at most so many vectors of 16 bytes that one CTA takes whole: a warp's, four warps'.  (4000 rows, us with 512 | 128 | 32 threads: 300 values of fp16 and 20 alternatives
+// 150 | 40 | 22, 300 of fp32 144 | 37 | 21, 500 of fp32 235 | 22 | 24; 2000 of fp16 and 5 alternatives 45 | 20 | 32, 8000 of fp32 70 | 62 | 97.)  A warp has 32 groups at most for its
+// threshold: for more alternatives four take the row (300 of fp16, 64 alternatives 151 | 99 | 180).
+static constexpr int kWarpVecs = 96, kWarpTop = 32, kFourWarpVecs = 2048;
 
 }  // namespace blr
 
@@ -380,7 +393,12 @@ int blr_token_logprobs(const void* logits, int64_t ld, int64_t rows, int64_t voc
   if (p.part < 1) p.part = 1;
   const int smem = p.part * 16;
   const cudaStream_t st = static_cast<cudaStream_t>(stream);
-  return kind == 0 ? launch_logprobs<0>(p, rows, ctas, smem, st) : kind == 1 ? launch_logprobs<1>(p, rows, ctas, smem, st) : launch_logprobs<2>(p, rows, ctas, smem, st);
+#define BLR_LP(THREADS) \
+  (kind == 0 ? launch_logprobs<0, THREADS>(p, rows, ctas, smem, st) : kind == 1 ? launch_logprobs<1, THREADS>(p, rows, ctas, smem, st) : launch_logprobs<2, THREADS>(p, rows, ctas, smem, st))
+  if (ctas == 1 && p.part <= kWarpVecs && top <= kWarpTop) return BLR_LP(32);
+  if (ctas == 1 && p.part <= kFourWarpVecs) return BLR_LP(128);
+  return BLR_LP(512);
+#undef BLR_LP
 }
 
 }  // extern "C"

@@ -478,6 +478,28 @@ def test_logprobs(ops, rows, vocab, top, kind, dtype):
     assert ok(tl, want.gather(1, order), allow.gather(1, order))
 
 
+# Rows short enough for one or four warps (up to 96 and 2048 vectors of 16 bytes), around both limits, and more alternatives than a warp has threads.  At most 2048 x 8 values
+# for 128 threads with two sums each, 64 terms in a row, or 96 x 8 for 32, 12 (and 8 more for the joining): fewer than the vocab / 256 + 64 that test_logprobs allows.
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("rows,vocab,top,kind", [(700, 300, 20, ""), (33, 20, 20, "steps"), (301, 97, 32, "masked"), (40, 300, 33, ""), (40, 300, 64, "masked"), (50, 768, 9, "equal"),
+                                                 (50, 776, 32, ""), (50, 384, 32, "steps"), (50, 388, 5, "lowest"), (2, 300, 4, "all lowest"), (5, 500, 7, "ends"),
+                                                 (310, 4111, 20, "masked"), (300, 8191, 64, ""), (300, 8192, 64, "equal"), (298, 8200, 64, "steps"), (297, 16384, 20, "large"),
+                                                 (297, 16399, 20, "")])
+def test_logprobs_of_short_rows(ops, rows, vocab, top, kind, dtype):
+    test_logprobs(ops, rows, vocab, top, kind, dtype)
+
+
+@pytest.mark.parametrize("vocab,top", [(12, 12), (300, 8), (300, 40)])
+def test_logprobs_of_short_rows_with_a_nan_or_infinity(ops, vocab, top):
+    x = torch.randn(4, vocab, generator=torch.Generator().manual_seed(vocab))
+    x[0, 7], x[1, 11], x[2, :] = math.nan, math.inf, -math.inf
+    lp, ent, tl, ti = (t.cpu() for t in ops.token_logprobs(x.half().to(DEV), torch.tensor([1, 2, 3, 4], device=DEV), top))
+    assert lp[:2].isnan().all() and ent[:2].isnan().all() and ti[0, 0] == 7 and ti[1, 0] == 11
+    assert lp[2] == -math.inf and ent[2] == 0 and ti[2].tolist() == list(range(top))
+    assert torch.equal(ti[3], x[3].half().float().sort(descending=True, stable=True).indices[:top]) and lp[3].isfinite()
+    assert torch.equal(ti[0, 1:], x[0].half().float().nan_to_num(-math.inf).sort(descending=True, stable=True).indices[:top - 1])
+
+
 @pytest.mark.parametrize("many", [1, 60])   # (60 times six rows of 9000: the kernel for many rows)
 def test_logprobs_of_rows_without_a_distribution(ops, many):
     x = torch.zeros(6, 700 if many == 1 else 9000)
