@@ -6,7 +6,8 @@
 //
 // A cluster of 1 to 8 CTAs takes a row: each reads its part once into shared memory, keeping the maximum of what every thread reads, and works from there.
 // The smallest of the maxima of as many groups of threads as tokens are asked for is a number that at least so many values reach: only values that reach it
-// (some tens) are kept and ordered.  A list that overflows (rows of equal values) is made by one search for each token instead.
+// (some tens) are kept and ordered.  A list that overflows is made anew of those above that number and the first of those that equal it (2047 rows of 32000 bf16 with 3 tokens
+// that are not ruled out, 8 alternatives: 89 us, by one search for each token 497); one that overflows again by searches.
 // Bound by HBM (each logit once), closely followed by ex2 (16 a cycle and SM).
 #include <cooperative_groups.h>
 #include <math_constants.h>
@@ -236,6 +237,7 @@ __global__ void __launch_bounds__(THREADS, THREADS == 512 ? 3 : 1536 / THREADS <
       for (int i = tid; i < mine; i += kLpThreads) {
         const uint4 w = part[i];
         if (!all && !(Vec<KIND>::most(Vec<KIND>::largest(w)) >= reach)) continue;
+        if (*(volatile uint32_t*)&sh.count > kLpKept) break;  // (too many: made anew below)
 #pragma unroll
         for (int k = 0; k < kPer; ++k) {
           const float x = Vec<KIND>::value(w, k);
@@ -257,9 +259,43 @@ __global__ void __launch_bounds__(THREADS, THREADS == 512 ? 3 : 1536 / THREADS <
   }
 
   // ---- this CTA's likeliest, in order (0: no more)
-  const int kept = (int)sh.count;
+  int kept = (int)sh.count;
   for (int i = tid; i < kLpMaxTop; i += kLpThreads) sh.best[i] = 0;
   __syncthreads();
+  if (finite && !all && kept > kLpKept) {
+    // Many values are equal to the threshold (tokens that are ruled out, where fewer are left than asked for): those above it, and by rising id those on it until there are enough.
+    if (tid == 0) sh.count = 0;
+    __syncthreads();
+    for (int i = tid; i < mine; i += kLpThreads) {
+      const uint4 w = part[i];
+      if (!(Vec<KIND>::most(Vec<KIND>::largest(w)) > reach)) continue;
+#pragma unroll
+      for (int k = 0; k < kPer; ++k) {
+        const float x = Vec<KIND>::value(w, k);
+        if (x > reach) keep(x, id0 + i * kPer + k);
+      }
+    }
+    if (tid < edges && sh.edge[tid] > reach) keep(sh.edge[tid], edge_id(tid));
+    if (warp == 0) {
+      int found = 0;
+      auto look = [&](bool there, float x, int id) {
+        const bool on = there && x == reach;
+        if (on) keep(x, id);
+        found += __popc(__ballot_sync(0xffffffffu, on));
+      };
+      const int ahead = min(edges, head);
+      look(lane < ahead, lane < ahead ? sh.edge[lane] : 0.f, lane);
+      for (int i0 = 0; i0 < mine && found < p.top; i0 += 32) {
+        const int i = i0 + lane;
+        const uint4 w = i < mine ? part[i] : make_uint4(0, 0, 0, 0);
+#pragma unroll
+        for (int k = 0; k < kPer; ++k) look(i < mine, Vec<KIND>::value(w, k), id0 + i * kPer + k);
+      }
+      if (found < p.top) look(ahead + lane < edges, ahead + lane < edges ? sh.edge[ahead + lane] : 0.f, edge_id(ahead + lane));
+    }
+    __syncthreads();
+    kept = (int)sh.count;
+  }
   if (finite && kept <= kLpKept) {
     for (int i = tid; i < kept; i += kLpThreads) {
       const Ranked v = sh.kept[i];
@@ -269,7 +305,7 @@ __global__ void __launch_bounds__(THREADS, THREADS == 512 ? 3 : 1536 / THREADS <
     }
   } else {
     Ranked last = ~0ull;
-    for (int k = 0; k < p.top && last != 0; ++k) {  // (too many equal ones, or a row with values that are no numbers: one search each)
+    for (int k = 0; k < p.top && last != 0; ++k) {  // (too many all the same, or a row with values that are no numbers: one search each)
       Ranked v = 0;
       auto look = [&](float x, int id) {
         const Ranked c = ranked(x, id);

@@ -489,6 +489,33 @@ def test_logprobs_of_short_rows(ops, rows, vocab, top, kind, dtype):
     test_logprobs(ops, rows, vocab, top, kind, dtype)
 
 
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("rows,vocab,left,top,ruled_out", [(3, 32001, 3, 8, "inf"), (300, 32000, 3, 64, "inf"), (2, 32003, 70, 64, "lowest"), (300, 9001, 5, 20, "lowest"), (9, 2000, 0, 7, "lowest"),
+                                                           (300, 4099, 1, 33, "inf"), (5, 700, 2, 20, "inf"), (301, 9000, 2, 40, "below"), (2, 700, 2, 20, "below")])
+def test_logprobs_with_few_tokens_left(ops, rows, vocab, left, top, ruled_out, dtype):
+    g = torch.Generator().manual_seed(vocab)
+    low = torch.finfo(dtype).min
+    x = torch.full((rows, vocab), -math.inf if ruled_out == "inf" else low)
+    if ruled_out == "below":   # (numbers below the one that most have, at the front and among them)
+        x[:, :] = -2.0
+        x[:, :top] = -math.inf
+        x[:, 100::3] = low
+    at = torch.rand(rows, vocab, generator=g).argsort(-1)[:, :left]
+    x.scatter_(1, at, torch.randn(rows, left, generator=g))
+    x = x.to(dtype)
+    ids = at[:, 0].contiguous() if left else torch.zeros(rows, dtype=torch.int64)
+    lp, ent, tl, ti = (t.cpu() for t in ops.token_logprobs(x.to(DEV), ids.to(DEV), top))
+    order = x.float().sort(dim=-1, descending=True, stable=True).indices[:, :top]
+    assert torch.equal(ti, order)
+    d = x.double()
+    want = torch.log_softmax(d, -1)
+    far = (d - d.amax(-1, keepdim=True)).abs()
+    allow = 2.0 ** -21 + (vocab / 256 + 64) * 2.0 ** -24 + 2.0 ** -23 * (far + math.log(vocab))   # (as test_logprobs has it; log S is at most log vocab)
+    for got, ref, room in ((tl, want.gather(1, order), allow.gather(1, order)), (lp, want.gather(1, ids[:, None])[:, 0], allow.gather(1, ids[:, None])[:, 0])):
+        assert bool((((got.double() - ref).abs() <= room) | (got.double() == ref) | ((got == -math.inf) & (ref < -3.4e38))).all())   # (fp32: the lowest less M may pass the range)
+    assert ent.isfinite().all()
+
+
 @pytest.mark.parametrize("vocab,top", [(12, 12), (300, 8), (300, 40)])
 def test_logprobs_of_short_rows_with_a_nan_or_infinity(ops, vocab, top):
     x = torch.randn(4, vocab, generator=torch.Generator().manual_seed(vocab))
