@@ -11,7 +11,7 @@
 // O is rescaled, seldom, when the last PV is known to be done.
 // Bounds, a step of 256 x 64 scores of heads of 128: 1280 cycles of tensor core (2 x 256 for PV, 2 x 384 for S, which reads both operands from shared memory for 64 columns)
 // and 1024 of ex2 (16 a cycle).  It takes 2150: the softmaxes of both halves share the schedulers for 1520 from scores in registers to P in TMEM, and spend 640 on barriers,
-// factors and TMEM's latency.  8192 tokens, 32 heads on 8: 592 us, 928 TFLOP/s.  (Steps of 128 keys, which leave no room for a second S: 600, and 3 x 257 tokens over up to 6001
+// factors and TMEM's latency.  8192 tokens, 32 heads on 8: 592 us, 928 TFLOP/s.  (Steps of 128 keys, which leave no room for a second S: 600; back to back 571 against 561; and 3 x 257 tokens over up to 6001
 // keys of heads of 64 71 instead of 67.  All ex2 left out: 12 % less time.  With the next scores loaded between the two halves of a step's: 610.)  Tried on steps of 128 without
 // gain: part of ex2 as a polynomial on the FMA pipe (1/8: 617 us, 3/8: 623), four softmax warpgroups of half a tile's width each (771), vs / R in the exponent instead of a
 // multiplication (610), scores read twice instead of held (697).
