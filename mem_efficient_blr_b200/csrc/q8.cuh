@@ -74,6 +74,12 @@ __device__ __forceinline__ uint32_t q8_down2(float a, float b) {
   }
 }
 
+__device__ __forceinline__ float ex2(float x) {
+  float r;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+  return r;
+}
+
 // Two floats of one 64-bit register: one instruction for both.
 __device__ __forceinline__ uint64_t pair(float a, float b) {
   uint64_t r;

@@ -1,7 +1,8 @@
 // Log probabilities of given tokens, entropy and likeliest tokens of rows of logits.
 //   M = max x,  S = sum e^(x - M),  log p(i) = (x_i - M) - log S,  H = log S - (sum e^(x - M) (x - M)) / S
-// in fp32, with one multiply-add ahead of ex2: t = x c - m for c = log2 e and m = M c rounded, which is (x - M) c + d with the same d = M c - m for the whole row, found
-// exactly by a multiply-add.  So sum 2^t = 2^d S, log S = log sum 2^t - d log 2, and H = log sum 2^t - log 2 (sum 2^t t) / sum 2^t, where d has dropped out.
+// in fp32: e^(x - M) = 2^t for t = (x - M) log2 e, and H = log S - log 2 (sum 2^t t) / S.  The difference comes first: it is all that counts, and is exact for
+// values next to M however far from 0 they lie (a row that is masked throughout with -1e10, say), where a product of M would be off by any number.  It costs nothing,
+// since pairs of values share an instruction (add, mul, add, fma for two, beside two ex2 and two clamps).
 // Order of the likeliest: falling value (NaN above everything, -0 equal to 0), ties by rising id.
 //
 // A cluster of 1 to 8 CTAs takes a row: each reads its part once into shared memory, keeping the maximum of what every thread reads, and works from there.
@@ -74,12 +75,6 @@ __device__ __forceinline__ float logit(const void* row, long long i) {
   if constexpr (KIND == 0) return __half2float(static_cast<const __half*>(row)[i]);
   else if constexpr (KIND == 1) return __bfloat162float(static_cast<const __nv_bfloat16*>(row)[i]);
   else return static_cast<const float*>(row)[i];
-}
-
-__device__ __forceinline__ float lp_ex2(float x) {
-  float r;
-  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
-  return r;
 }
 
 // Of the largest values that groups of threads have seen, the `top`-th (by one warp): at least so many of a row's values reach it, and seldom many more.
@@ -203,27 +198,28 @@ __global__ void __launch_bounds__(THREADS, THREADS == 512 ? 3 : 1536 / THREADS <
   const bool all = least == 0;  // (too few groups have seen anything: keep everything)
 
   // ---- the sums, and the values that reach the threshold
-  // (beyond 10^37, where M log2 e may be infinite, numbers that differ are at least 2^99 apart: c = 1 gives the same weights, 1 and 0; a row of the type's lowest number is one)
-  const bool far = fabsf(M) > 1e37f;
-  const float c = far ? 1.f : 1.4426950408889634f, m = M * c;
   float S = 0.f, D = 0.f;
   auto keep = [&](float x, int id) {
     const uint32_t at = atomicAdd(&sh.count, 1u);
     if (at < kLpKept) sh.kept[at] = ranked(x, id);
   };
   if (finite) {
-    float s2[2] = {0.f, 0.f}, d2[2] = {0.f, 0.f};
-    auto add = [&](float x, int k) {
-      const float t = fmaxf(fmaf(x, c, -m), -1e30f), e = lp_ex2(t);  // (-inf: a weight of 0, and of a number)
-      s2[k] += e;
-      d2[k] = fmaf(e, t, d2[k]);
+    const uint64_t low = pair(-M, -M), log2e = pair(1.4426950408889634f, 1.4426950408889634f);
+    uint64_t s2 = 0, d2 = 0;
+    auto add = [&](float x, float y) {
+      float t[2];
+      unpair(mul2(add2(pair(x, y), low), log2e), t[0], t[1]);
+      t[0] = fmaxf(t[0], -1e30f), t[1] = fmaxf(t[1], -1e30f);  // (-inf: a weight of 0, and of a number)
+      const uint64_t e = pair(ex2(t[0]), ex2(t[1]));
+      s2 = add2(s2, e);
+      d2 = fma2(e, pair(t[0], t[1]), d2);
     };
     int i = tid;
     auto vec = [&](const uint4& w) {
       float f[kPer];
       Vec<KIND>::floats(w, f);
 #pragma unroll
-      for (int k = 0; k < kPer; ++k) add(f[k], k & 1);
+      for (int k = 0; k < kPer; k += 2) add(f[k], f[k + 1]);
     };
     for (; i + kLpThreads < mine; i += 2 * kLpThreads) {
       const uint4 w = part[i], v = part[i + kLpThreads];
@@ -231,8 +227,10 @@ __global__ void __launch_bounds__(THREADS, THREADS == 512 ? 3 : 1536 / THREADS <
       vec(v);
     }
     if (i < mine) vec(part[i]);
-    if (tid < edges) add(sh.edge[tid], 0);
-    S = s2[0] + s2[1], D = d2[0] + d2[1];
+    if (tid < edges) add(sh.edge[tid], -CUDART_INF_F);
+    float odd;
+    unpair(s2, S, odd), S += odd;
+    unpair(d2, D, odd), D += odd;
     if (p.top > 0 && (all || seen >= least)) {  // (few threads)
       for (int i = tid; i < mine; i += kLpThreads) {
         const uint4 w = part[i];
@@ -338,12 +336,12 @@ __global__ void __launch_bounds__(THREADS, THREADS == 512 ? 3 : 1536 / THREADS <
       const Shared* other = cluster.map_shared_rank(&sh, o);
       S += other->S, D += other->D;
     }
-    const float log_sum = logf(S), log_s = log_sum - fmaf(M, c, -m) * 0.69314718055994531f;
+    const float log_s = logf(S);
     // (a row of -inf alone: every log probability -inf, entropy 0; a NaN or +inf: NaN)
     auto lp = [&](float x) { return finite ? (x - M) - log_s : empty ? -CUDART_INF_F : CUDART_NAN_F; };
     if (writes) {
       p.logprob[r] = id < 0 ? 0.f : id >= p.vocab ? CUDART_NAN_F : lp(given);
-      p.entropy[r] = finite ? log_sum - D / S * (far ? 1.f : 0.69314718055994531f) : empty ? 0.f : CUDART_NAN_F;
+      p.entropy[r] = finite ? log_s - D / S * 0.69314718055994531f : empty ? 0.f : CUDART_NAN_F;
     }
     for (int i = tid; i < n_cta * p.top; i += kLpThreads) {
       const int from = i / p.top, k = i - from * p.top;
