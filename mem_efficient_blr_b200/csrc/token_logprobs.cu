@@ -24,13 +24,14 @@ namespace blr {
 static constexpr int kLpMaxTop = 64, kLpGroups = 128, kLpMaxPart = 200 * 1024;
 typedef unsigned long long Ranked;  // order_of(value) << 32 | ~id: larger is likelier
 
-// Whole numbers in the order of the values; 0 is below all of them.
+// Whole numbers in the order of the values; 0 is below all of them, and 0xffffffff, with which a search begins, above: a NaN, which comes first, is one less.
+static constexpr uint32_t kOrderOfNan = 0xfffffffeu;
 __device__ __forceinline__ uint32_t order_of(float x) {
   const uint32_t b = __float_as_uint(x + 0.f);
-  return x != x ? 0xffffffffu : b & 0x80000000u ? ~b : b | 0x80000000u;
+  return x != x ? kOrderOfNan : b & 0x80000000u ? ~b : b | 0x80000000u;
 }
 __device__ __forceinline__ float value_of(uint32_t o) {
-  return __uint_as_float(o == 0xffffffffu ? 0x7fffffffu : o & 0x80000000u ? o & 0x7fffffffu : ~o);
+  return __uint_as_float(o == kOrderOfNan ? 0x7fffffffu : o & 0x80000000u ? o & 0x7fffffffu : ~o);
 }
 __device__ __forceinline__ Ranked ranked(float x, int id) { return (Ranked)order_of(x) << 32 | (0xffffffffu - (uint32_t)id); }
 
