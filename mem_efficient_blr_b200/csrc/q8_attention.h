@@ -40,6 +40,27 @@ __device__ __forceinline__ int q8_row_up(uint32_t most, int bf16) {
   return bf16 && ex != 0 && ex != 255 ? min(268 - ex, 253) : 127;
 }
 
+
+// A row's weights are taken against two references of its own: p = 2^(s - m), and P = p vs D, rounded to fp16, for the product with the codes, so that O = D sum p v.
+// m is a whole number, the largest score rounded up when it was last moved; D = 2^-d brings the largest p vs to between 2^2 and 2^4 when it is moved.  Both are moved
+// where the row's own keys ask for it, so that what it does not see has no part in any of its bits, and both by powers of two, so that nothing but P is rounded:
+// a weight loses 2^-11 of itself, or 2^-27 of the row's heaviest where it is next to nothing beside that one.
+static constexpr float kQ8Lift = 4.f;
+// A whole number above log2 of a block's scale; -inf where it is 0 (or next to it) or no number: such a block moves nothing.
+__device__ __forceinline__ float q8_above(float scale) {
+  const uint32_t e = (__float_as_uint(scale) >> 23) & 0xff;
+  return e == 0 || e == 255 ? -INFINITY : (float)e - 126.f;
+}
+__device__ __forceinline__ float q8_exponent(float D) { return 127.f - (float)(int)(__float_as_uint(D) >> 23); }  // d
+__device__ __forceinline__ float q8_unit(float D) { return __uint_as_float((254u << 23) - __float_as_uint(D)); }                  // 2^d
+// To m = `to`, the heaviest of the new keys at 2^heavy against it.  l is to be multiplied with `down`, O with `corr`.
+__device__ __forceinline__ void q8_move(float to, float heavy, float& m, float& D, float& down, float& corr) {
+  const float keep = q8_exponent(D) + (m - to), next = fmaxf(fmaxf(keep, heavy - kQ8Lift), -126.f);
+  down = ex2(m - to), corr = ex2(keep - next);
+  m = to;
+  D = __uint_as_float((uint32_t)(127 - (int)next) << 23);
+}
+
 int q8_launch_prompt(const Q8AttnParams& p, int head_dim, int code, cudaStream_t stream);
 static constexpr int kQ8PromptRows = 256;  // rows of a CTA
 

@@ -3,9 +3,8 @@
 //   warps 0-3, 4-7  softmax of rows 0-127 and 128-255, a thread per row: S from TMEM, P back over it as fp16 pairs, O rescaled there when it has to be
 //   warps 8-11      widen the codes of the next keys and values to fp16 (exact) into shared memory, as tcgen05.mma reads them
 //   warps 12-15     one thread of the first issues the products: S = Q K^T (both from shared memory), O += P V (P from TMEM)
-// The scales stay out of the products: a group of 16 keys has one for its keys, which multiplies S in the exponent's argument, and one for its values, which
-// multiplies p by vs / R with R the largest of them so far (moved when it is 2^4 behind, like the maximum when a tile's sum of p comes to 2^11; see
-// q8_attention.cu).
+// The scales stay out of the products: a group of 16 keys has one for its keys, which multiplies S in the exponent's argument, and one for its values, which multiplies p.
+// A thread keeps its row's references for both (q8_attention.h) and moves them when a step's sum of p, or that times the largest factor, has outgrown them.
 // A step is half a tile, 64 keys, and a half's S alternates between two places of TMEM: S0 S0 S1 S1 first, then PV0 S0 | PV1 S1 | ... with the S two steps ahead of the PV, into
 // the place that the PV's P has left (P lies over the S that it was made of; one queue, so in order).  Neither half waits for the other's softmax, or for its own scores.
 // O is rescaled, seldom, when the last PV is known to be done.
@@ -64,20 +63,27 @@ __device__ __forceinline__ void sts128(uint32_t addr, uint32_t a, uint32_t b, ui
   asm volatile("st.shared.v4.b32 [%0], {%1,%2,%3,%4};" ::"r"(addr), "r"(a), "r"(b), "r"(c), "r"(d) : "memory");
 }
 
-// Scores of 128 keys of a thread's row, from TMEM 32 at a time (the next 32 are on their way while these are used).
+// A thread has the 64 scores of its row for a step in registers, x, in four groups of 16 keys.
 __device__ __forceinline__ void mask32(uint32_t (&x)[32], int left) {
 #pragma unroll
   for (int i = 0; i < 32; ++i)
     if (i >= left) x[i] = 0xff800000u;
 }
-// The factors of 32 keys.  Masked scores are -inf and their weights 0: a group that is masked as a whole has factors of its own for that (its scales may be NaN), and
-// a key scale of 0 makes way for a number that its scores vanish under.
-__device__ __forceinline__ void factors32(uint32_t fac, int c, float factor, bool part, int left, float (&cg)[2], float (&fg)[2]) {
-  uint32_t k[2], v[2];
-  lds64(fac + 8 * c, k[0], k[1]);
-  lds64(fac + 32 + 8 * c, v[0], v[1]);
+__device__ __forceinline__ float min_nan(float a, float b) {
+  float r;
+  asm("min.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+  return r;
+}
+// The factors of two groups: cg of their scores, fg of their weights.  Masked scores are -inf and their weights 0: a group that is masked as a whole has factors of its own for
+// that (its scales may be NaN), and a key scale of 0 makes way for a number that its scores vanish under.
+__device__ __forceinline__ void factors32(uint32_t fac, int c, float factor, float D, bool part, int left, float (&cg)[2], float (&fg)[2]) {
+  uint64_t k, v;
+  asm volatile("ld.shared.b64 %0, [%1];" : "=l"(k) : "r"(fac + 8 * c) : "memory");
+  asm volatile("ld.shared.b64 %0, [%1];" : "=l"(v) : "r"(fac + 32 + 8 * c) : "memory");
+  unpair(mul2(k, pair(factor, factor)), cg[0], cg[1]);
+  unpair(mul2(v, pair(D, D)), fg[0], fg[1]);
 #pragma unroll
-  for (int g = 0; g < 2; ++g) cg[g] = __uint_as_float(k[g]) * factor, fg[g] = __uint_as_float(v[g]);
+  for (int g = 0; g < 2; ++g) fg[g] = min_nan(fg[g], 3.402823466e38f);  // (a finite scale: no 0 times infinity)
   if (part) {
 #pragma unroll
     for (int g = 0; g < 2; ++g) {
@@ -86,32 +92,41 @@ __device__ __forceinline__ void factors32(uint32_t fac, int c, float factor, boo
     }
   }
 }
-// The maximum of 64 scores of a row, scaled:
-__device__ __forceinline__ float largest(const uint32_t (&x)[2][32], uint32_t fac, float factor, bool part, int left) {
-  float mx[2] = {-INFINITY, -INFINITY};
+// Moves a row's references to the maxima of its groups (q8_attention.h).
+__device__ __forceinline__ void move_to(const uint32_t (&x)[2][32], uint32_t fac, float factor, bool part, int left, float& m, float& D, float& down, float& corr) {
+  float peak[4], to = m;
 #pragma unroll
   for (int c = 0; c < 2; ++c) {
     float cg[2], fg[2];
-    factors32(fac, c, factor, part, left - 32 * c, cg, fg);
+    factors32(fac, c, factor, D, part, left - 32 * c, cg, fg);
 #pragma unroll
     for (int g = 0; g < 2; ++g) {
       float top = __uint_as_float(x[c][16 * g]);
 #pragma unroll
       for (int i = 1; i < 16; ++i) top = fmaxf(top, __uint_as_float(x[c][16 * g + i]));
-      mx[g] = fmaxf(mx[g], top * cg[g]);
+      peak[2 * c + g] = ceilf(top * cg[g]);
+      to = fmaxf(to, peak[2 * c + g]);
     }
   }
-  return fmaxf(mx[0], mx[1]);
+  if (to == -INFINITY) return;
+  uint32_t vs[4];
+  lds128(fac + 32, vs[0], vs[1], vs[2], vs[3]);
+  float heavy = -INFINITY;
+#pragma unroll
+  for (int g = 0; g < 4; ++g) heavy = fmaxf(heavy, peak[g] - to + q8_above(__uint_as_float(vs[g])));
+  q8_move(to, heavy, m, D, down, corr);
 }
-// p = 2^(s - mu), and P = p vs / R as fp16 pairs over the scores in TMEM; returns the sum of p.
-__device__ __forceinline__ float weights(uint32_t s_at, const uint32_t (&x)[2][32], uint32_t fac, float factor, float mu, bool part, int left) {
+// p = 2^(s - mu), and P = p vs D as fp16 pairs over the scores in TMEM; returns the sum of p, and the largest of the factors vs D.
+__device__ __forceinline__ float weights(uint32_t s_at, const uint32_t (&x)[2][32], uint32_t fac, float factor, float D, float mu, bool part, int left, float& most) {
   uint64_t sum[2] = {0, 0};
   const uint64_t neg = pair(-mu, -mu);
+  most = 0.f;
 #pragma unroll
   for (int c = 0; c < 2; ++c) {
     float cg[2], fg[2];
     uint32_t y[16];
-    factors32(fac, c, factor, part, left - 32 * c, cg, fg);
+    factors32(fac, c, factor, D, part, left - 32 * c, cg, fg);
+    most = fmaxf(most, fmaxf(fg[0], fg[1]));
 #pragma unroll
     for (int g = 0; g < 2; ++g) {
       const uint64_t c2 = pair(cg[g], cg[g]), f2 = pair(fg[g], fg[g]);
@@ -219,7 +234,7 @@ template <bool E4M3, int HD, bool WIDE>
 __global__ void __launch_bounds__(Split<WIDE>::kThreads, 1) q8_prompt_kernel(const __grid_constant__ Q8AttnParams p) {
   constexpr int kLast = WIDE ? 8 : 12;  // the first of the last four warps
   extern __shared__ __align__(1024) uint8_t prompt_raw[];
-  __shared__ __align__(16) float factors[4][20];
+  __shared__ __align__(16) float factors[4][16];
   constexpr uint32_t kTile = 128 * HD * 2;
   const uint32_t base = (smem_u32(prompt_raw) + 1023u) & ~1023u;
   const uint32_t qs = base, ks = base + 2 * kTile, vs = base + 4 * kTile, bars = base + 6 * kTile;
@@ -306,9 +321,9 @@ __global__ void __launch_bounds__(Split<WIDE>::kThreads, 1) q8_prompt_kernel(con
   const int halves = max(n0, n1), steps = (halves + 1) / 2;  // (n0, n1, halves: of 64 keys; steps: tiles of 128)
 
   // (No spills in any of these: what shared memory leaves of L1 does not keep them, and a reload from L2 inside a loop costs more than anything that it saves.)
-  // A step's factors: of 8 groups of 16 keys ks and vs / R, and how R moved.  One warp makes them, four steps deep (a step's are free when the S of the step after it
+  // A step's factors: ks and vs of 8 groups of 16 keys (an infinite vs as a NaN).  One warp brings them, four steps deep (a step's are free when the S of the step after it
   // is done, and that warp is two steps ahead of that at most).
-  float R_made = 0.f, inv_R = 0.f, next_scale = 0.f;
+  float next_scale = 0.f;
   auto scale_at = [&](int j) {
     const float* const scales = (lane < 8 ? p.c.k_scale : p.c.v_scale) + (long long)place_of(p).bh * p.c.n_blocks;
     return scales[min((k0 + j * kKeys + 16 * (lane & 7)) >> p.c.block_log2, p.c.n_blocks - 1)];
@@ -316,13 +331,7 @@ __global__ void __launch_bounds__(Split<WIDE>::kThreads, 1) q8_prompt_kernel(con
   auto make_factors = [&](int j) {
     const float scale = next_scale;
     if (j + 1 < steps) next_scale = scale_at(j + 1);
-    const float vmax = __uint_as_float(
-        __reduce_max_sync(0xffffffffu, lane >= 8 && k0 + j * kKeys + 16 * (lane & 7) < keys && scale <= 3.4e38f ? __float_as_uint(scale) : 0u));
-    float moved = 1.f;
-    if (vmax > 16.f * R_made) moved = R_made / vmax, R_made = vmax, inv_R = 1.f / vmax;
-    if (lane < 16) factors[j & 3][lane] = lane < 8 ? scale : scale * inv_R;
-    if (lane == 16) factors[j & 3][16] = moved;
-    if (lane == 17) factors[j & 3][17] = R_made;
+    if (lane < 16) factors[j & 3][lane] = lane < 8 || scale <= 3.402823466e38f ? scale : CUDART_NAN_F;
     __syncwarp();
     if (lane == 0) mbar_arrive(cfull + 8 * (j & 3));
   };
@@ -435,7 +444,7 @@ __global__ void __launch_bounds__(Split<WIDE>::kThreads, 1) q8_prompt_kernel(con
     asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(Split<WIDE>::kSoftmax));
     const int n = wg ? n1 : n0;
     const uint32_t lanes = (uint32_t)(32 * (warp & 3)) << 16, o_at = tmem + lanes + 256 + 128 * wg;
-    float m = -INFINITY, l = 0.f, R = 0.f;
+    float m = -INFINITY, l = 0.f, D = 1.f;
     const int lim_all = __reduce_min_sync(0xffffffffu, lim);
     bool ok = true;
 #pragma unroll 1
@@ -444,11 +453,7 @@ __global__ void __launch_bounds__(Split<WIDE>::kThreads, 1) q8_prompt_kernel(con
       const uint32_t s_at = tmem + lanes + 128 * wg + 64 * (u & 1);
       const bool part = key0 + kStepKeys > lim_all;  // some of these keys are masked for a row of the warp
       if ((u & 1) == 0 && !__all_sync(0xffffffffu, mbar_wait(cfull + 8 * (j & 3), (j >> 2) & 1, abort_flag))) { ok = false; break; }
-      const uint32_t tile = smem_u32(factors[j & 3]), fac = tile + 16 * (u & 1);  // (of the step's four groups; those of their values 32 bytes behind)
-      uint32_t vr[2];
-      lds64(tile + 64, vr[0], vr[1]);
-      float corr = u & 1 ? 1.f : __uint_as_float(vr[0]);
-      R = __uint_as_float(vr[1]);
+      const uint32_t fac = smem_u32(factors[j & 3]) + 16 * (u & 1);  // (of the step's four groups; those of their values 32 bytes behind)
       if (!__all_sync(0xffffffffu, mbar_wait(sfull + 16 * wg + 8 * (u & 1), j & 1, abort_flag))) { ok = false; break; }
       tc_fence_after();
       uint32_t x[2][32];
@@ -461,15 +466,17 @@ __global__ void __launch_bounds__(Split<WIDE>::kThreads, 1) q8_prompt_kernel(con
         mask32(x[0], lim - key0);
         mask32(x[1], lim - key0 - 32);
       }
-      // against the maximum so far, which is seldom left behind: a sum above 2^11 tells of it (P, up to 16 times as large, is still a half then), and all is done once more
+      // against the references so far, which are seldom left behind: a sum above 2^11, or one that may bring a P above 2^15, tells of it, and all is done once more.  The rows that
+      // ask for it move theirs, the others come out as they were.
       float total = 0.f;
+      bool ask = m == -INFINITY && lim > key0;  // (a row's first keys)
 #pragma unroll 1
-      for (bool moved = u == 0 || corr != 1.f;; moved = true) {
+      for (bool moved = __any_sync(0xffffffffu, ask);; moved = true) {
         if (moved) {
-          const float to = fmaxf(m, largest(x, fac, factor, part, lim - key0)), down = to == -INFINITY ? 1.f : ex2(m - to);
-          m = to;
-          l *= down, corr *= down;
-          if (u > 0) {
+          float down = 1.f, corr = 1.f;
+          if (ask) move_to(x, fac, factor, part, lim - key0, m, D, down, corr);
+          l *= down;
+          if (u > 0 && __any_sync(0xffffffffu, corr != 1.f)) {
             if (!__all_sync(0xffffffffu, mbar_wait(done + 16 * wg + 8 * ((u - 1) & 1), ((u - 1) >> 1) & 1, abort_flag))) { ok = false; break; }
             tc_fence_after();
 #pragma unroll 1
@@ -482,8 +489,10 @@ __global__ void __launch_bounds__(Split<WIDE>::kThreads, 1) q8_prompt_kernel(con
             }
           }
         }
-        total = weights(s_at, x, fac, factor, m == -INFINITY ? 0.f : m, part, lim - key0);
-        if (moved || !__any_sync(0xffffffffu, total > 2048.f)) break;
+        float most;
+        total = weights(s_at, x, fac, factor, D, m == -INFINITY ? 0.f : m, part, lim - key0, most);
+        ask = total > 2048.f || total * most > 32768.f;
+        if (moved || !__any_sync(0xffffffffu, ask)) break;
       }
       if (!ok) break;
       l += total;
@@ -497,7 +506,7 @@ __global__ void __launch_bounds__(Split<WIDE>::kThreads, 1) q8_prompt_kernel(con
     const Place at = place_of(p);
     const int r = at.r0 + (int)threadIdx.x;
     const bool live = r < p.rows;
-    const float fin = !ok ? CUDART_NAN_F : p.ns > 1 ? R : l == 0.f ? 0.f : R / l;
+    const float fin = !ok ? CUDART_NAN_F : p.ns > 1 ? 1.f : l == 0.f ? 0.f : 1.f / l, unit = q8_unit(D);
     const int tok = live ? r / p.G : 0;
     uint16_t* const to = p.out + ((long long)at.b * p.T + tok) * p.ldo + (long long)(at.h * p.G + r - tok * p.G) * HD;
     float* const to32 = p.part + (((long long)at.bh * p.rows + r) * p.ns + at.split) * (HD + 4);
@@ -513,21 +522,20 @@ __global__ void __launch_bounds__(Split<WIDE>::kThreads, 1) q8_prompt_kernel(con
         for (int i = 0; i < 32; ++i) x[i] = 0;
       }
       if (!live) continue;
-      if (ok && l == 0.f)  // (a row that sees nothing: zeros, whatever its products were)
 #pragma unroll
-        for (int i = 0; i < 32; ++i) x[i] = 0;
+      for (int i = 0; i < 32; ++i)  // (a row that sees nothing: zeros, whatever its products were)
+        x[i] = ok && l == 0.f ? 0u : __float_as_uint(__uint_as_float(x[i]) * fin * unit);
       if (p.ns > 1) {
 #pragma unroll
         for (int i = 0; i < 32; i += 4)
-          *reinterpret_cast<float4*>(to32 + 32 * c + i) = make_float4(__uint_as_float(x[i]) * fin, __uint_as_float(x[i + 1]) * fin,
-                                                                      __uint_as_float(x[i + 2]) * fin, __uint_as_float(x[i + 3]) * fin);
+          *reinterpret_cast<float4*>(to32 + 32 * c + i) = make_float4(__uint_as_float(x[i]), __uint_as_float(x[i + 1]), __uint_as_float(x[i + 2]), __uint_as_float(x[i + 3]));
       } else {
 #pragma unroll
         for (int i = 0; i < 32; i += 8) {
           uint32_t o[4];
 #pragma unroll
           for (int z = 0; z < 4; ++z) {
-            const float u = __uint_as_float(x[i + 2 * z]) * fin, v = __uint_as_float(x[i + 2 * z + 1]) * fin;
+            const float u = __uint_as_float(x[i + 2 * z]), v = __uint_as_float(x[i + 2 * z + 1]);
             o[z] = p.bf16 ? q8_down2<true>(u, v) : q8_down2<false>(u, v);
           }
           *reinterpret_cast<uint4*>(to + 32 * c + i) = make_uint4(o[0], o[1], o[2], o[3]);
