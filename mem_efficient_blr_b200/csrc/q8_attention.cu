@@ -4,11 +4,11 @@
 // mma.sync (keys, then dimensions, as the 16 rows, 8 query rows as the columns), so that one query row costs what eight do and no operand is transposed in
 // memory: the sum of the first product may run over the dimensions in any order, so a thread takes 16 neighbouring bytes of a key, and the second over the keys in
 // any order, so it takes 16 neighbouring dimensions of four keys; P^T comes out of S^T by movmatrix.
-//   s_j = ks_j c (q . k_j),  p_j = 2^(s_j - m),  l = sum p_j,  o = sum (p_j vs_j / R) v_j  with codes k_j, v_j and the scales ks_j, vs_j of their blocks:
+//   s_j = ks_j c (q . k_j),  p_j = 2^(s_j - m),  l = sum p_j,  o = sum (p_j vs_j D) v_j  with codes k_j, v_j, the scales ks_j, vs_j of their blocks, and the row's own
+// references m and D (q8_attention.h):
 // codes are exact in fp16, q is too (bf16 rows are brought into its range by a power of two; what is 2^-38 of a row's largest value may be lost), so the only rounding to
-// 16 bits is p's; sums are fp32.
-// m follows the maximum only where it is more than 2^8 behind, R the largest value scale where it is more than 2^4 behind: p stays below 2^12, and what is lost of
-// a small p is 2^-25 of the largest.
+// 16 bits is that of p_j vs_j D; sums are fp32.
+// m follows the maximum only where it is more than 2^8 behind, D the heaviest p vs only where it has outgrown 2^15.
 // Bound by HBM on the codes (a key and its value are 2 hd bytes): 64 sequences x 32 heads x 2048 keys of 128, 1.08 GB, 166 us in a graph, 6.5 TB/s; by latency where they are
 // few (1 sequence: 12.6 us for 17 MB: positions, codes, a few groups a warp, the second kernel).  The keys of a row are shared out over the warps of a CTA and
 // over up to kMaxSplits CTAs.  A first version that loaded the groups into registers took 280 us for the former: 8 warps an SM instead of 16.
@@ -49,7 +49,7 @@ __global__ void __launch_bounds__(kFewThreads, NT == 1 ? 4 : NT == 2 ? 3 : 2) q8
   constexpr int kSteps = HD / 16, kRows = 8 * NT, kPitch = HD + 4, kPieces = HD / 16;
   constexpr bool kQShared = NT > 2;
   extern __shared__ __align__(128) uint8_t ring[];
-  __shared__ float wm[kFewWarps][kRows], wl[kFewWarps][kRows];
+  __shared__ float wm[kFewWarps][kRows], wl[kFewWarps][kRows], wu[kFewWarps][kRows];
   float(*const os)[8][kPitch] = reinterpret_cast<float(*)[8][kPitch]>(ring);
   uint2* const q_frag = reinterpret_cast<uint2*>(ring + few_ring_bytes<HD>());  // [tile][step][lane]
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
@@ -105,7 +105,7 @@ __global__ void __launch_bounds__(kFewThreads, NT == 1 ? 4 : NT == 2 ? 3 : 2) q8
   auto block_of = [&](int j) { return (first + 16 * kFewWarps * j) >> p.c.block_log2; };
   float ks_next = steps > 0 ? ksh[block_of(0)] : 0.f, vs_next = steps > 0 ? vsh[block_of(0)] : 0.f;
 
-  float o[NT][kSteps][4] = {}, m[NT][2], l[NT][2] = {}, R = 0.f, inv_R = 0.f;
+  float o[NT][kSteps][4] = {}, m[NT][2], l[NT][2] = {}, D[NT][2], safe = INFINITY;  // safe: value scales up to it bring no row's P beyond 2^15 as long as its p is at most 2^8
   {
     // ---- the query rows as fp16 fragments, and what their dot products are to be multiplied with
     uint32_t qf[kQShared ? 1 : NT][kSteps][2];
@@ -149,7 +149,7 @@ __global__ void __launch_bounds__(kFewThreads, NT == 1 ? 4 : NT == 2 ? 3 : 2) q8
         const int rc = r0 + 8 * n + 2 * t + i;
         lim[n][i] = rc < p.rows ? q8_seen(start, count, rc / p.G, p.c.slots) : 0;
       }
-      m[n][0] = m[n][1] = -INFINITY;
+      m[n][0] = m[n][1] = -INFINITY, D[n][0] = D[n][1] = 1.f;
     }
     if constexpr (kQShared) __syncthreads();
     int lim_all = 0x7fffffff;  // keys below it are masked for no row of the warp
@@ -204,54 +204,60 @@ __global__ void __launch_bounds__(kFewThreads, NT == 1 ? 4 : NT == 2 ? 3 : 2) q8
         }
         // ---- p
         const bool part = j0 + 16 > lim_all;
-        bool behind = false;
+        uint32_t behind = vs > safe ? (1u << NT) - 1 : 0;  // a bit for each tile of rows
 #pragma unroll
         for (int n = 0; n < NT; ++n) {
           const float c[2] = {factor[n][0] * ks, factor[n][1] * ks};
+          bool up = false;
 #pragma unroll
           for (int i = 0; i < 4; ++i) {
             sc[n][i] *= c[i & 1];
             if (part && j0 + g + 8 * (i >> 1) >= lim[n][i & 1]) sc[n][i] = -INFINITY;
-            behind |= sc[n][i] > m[n][i & 1] + 8.f;
+            up |= sc[n][i] > m[n][i & 1] + 8.f;
           }
+          behind |= up ? 1u << n : 0;
         }
-        if (__any_sync(0xffffffffu, behind)) {
+        if (__any_sync(0xffffffffu, behind != 0)) {
+          if (NT > 1) behind = __reduce_or_sync(0xffffffffu, behind);
+          float least = INFINITY;  // of the rows' 2^d
 #pragma unroll
-          for (int n = 0; n < NT; ++n)
+          for (int n = 0; n < NT; ++n) {
+            if (NT == 1 || (behind >> n & 1)) {
 #pragma unroll
-            for (int i = 0; i < 2; ++i) {
-              float mx = fmaxf(sc[n][i], sc[n][i + 2]);
+              for (int i = 0; i < 2; ++i) {
+                float mx = fmaxf(sc[n][i], sc[n][i + 2]);
 #pragma unroll
-              for (int d = 4; d < 32; d <<= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, d));
-              mx = fmaxf(mx, m[n][i]);
-              const float corr = mx == -INFINITY ? 1.f : ex2(m[n][i] - mx);
-              m[n][i] = mx;
-              l[n][i] *= corr;
+                for (int d = 4; d < 32; d <<= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, d));
+                // a row that the new keys do not ask stays as it is; a factor vs D that no fp32 holds asks too, as long as the row sees the block
+                const float f = vs <= 3.402823466e38f ? vs * D[n][i] : 0.f, peak = ceilf(mx);
+                const bool ask = mx > m[n][i] + 8.f || ex2(mx - m[n][i]) * f > 32768.f || (f > 3.402823466e38f && mx != -INFINITY);
+                const float to = ask ? fmaxf(m[n][i], peak) : m[n][i];
+                float to_m = m[n][i], to_D = D[n][i], down, corr;
+                q8_move(to, fmaxf(peak - to, -123.f) + q8_above(vs), to_m, to_D, down, corr);
+                if (!ask) to_D = D[n][i], down = corr = 1.f;
+                m[n][i] = to, D[n][i] = to_D;
+                l[n][i] *= down;
 #pragma unroll
-              for (int d = 0; d < kSteps; ++d) o[n][d][i] *= corr, o[n][d][i + 2] *= corr;
+                for (int d = 0; d < kSteps; ++d) o[n][d][i] *= corr, o[n][d][i + 2] *= corr;
+              }
             }
+#pragma unroll
+            for (int i = 0; i < 2; ++i)
+              if (m[n][i] != -INFINITY) least = fminf(least, q8_unit(D[n][i]));
+          }
+          safe = 128.f * __uint_as_float(__reduce_min_sync(0xffffffffu, __float_as_uint(least)));
         }
-        if (vs > 16.f * R && vs <= 3.4e38f) {
-          const float corr = R / vs;
-          R = vs, inv_R = 1.f / R;
-#pragma unroll
-          for (int n = 0; n < NT; ++n)
-#pragma unroll
-            for (int d = 0; d < kSteps; ++d)
-#pragma unroll
-              for (int i = 0; i < 4; ++i) o[n][d][i] *= corr;
-        }
-        const float f = vs * inv_R;
         uint32_t pt[NT][2];
 #pragma unroll
         for (int n = 0; n < NT; ++n) {
           float e[4];
           const float mu[2] = {m[n][0] == -INFINITY ? 0.f : m[n][0], m[n][1] == -INFINITY ? 0.f : m[n][1]};
+          const float f[2] = {vs * D[n][0], vs * D[n][1]};
 #pragma unroll
           for (int i = 0; i < 4; ++i) {
             const float v = ex2(sc[n][i] - mu[i & 1]);
             l[n][i & 1] += v;
-            e[i] = v * f;
+            e[i] = v * f[i & 1];
             if (part && j0 + g + 8 * (i >> 1) >= lim[n][i & 1]) e[i] = 0.f;  // (a masked place of a block that holds a NaN)
           }
           pt[n][0] = transpose8x8(pack_half2(e[0], e[1])), pt[n][1] = transpose8x8(pack_half2(e[2], e[3]));
@@ -289,7 +295,7 @@ __global__ void __launch_bounds__(kFewThreads, NT == 1 ? 4 : NT == 2 ? 3 : 2) q8
       for (int i = 0; i < 2; ++i) {
 #pragma unroll
         for (int d = 4; d < 32; d <<= 1) l[n][i] += __shfl_xor_sync(0xffffffffu, l[n][i], d);
-        if (g == 0) wm[warp][8 * n + 2 * t + i] = m[n][i], wl[warp][8 * n + 2 * t + i] = l[n][i];
+        if (g == 0) wm[warp][8 * n + 2 * t + i] = m[n][i], wl[warp][8 * n + 2 * t + i] = l[n][i], wu[warp][8 * n + 2 * t + i] = q8_unit(D[n][i]);
       }
   }
   // ---- the warps' results meet, over the ring
@@ -301,7 +307,7 @@ __global__ void __launch_bounds__(kFewThreads, NT == 1 ? 4 : NT == 2 ? 3 : 2) q8
       for (int i = 0; i < 2; ++i) {
         float M = -INFINITY;
         for (int w = 0; w < kFewWarps; ++w) M = fmaxf(M, wm[w][8 * n + 2 * t + i]);
-        const float weight = m[n][i] == -INFINITY ? 0.f : ex2(m[n][i] - M) * R;
+        const float weight = m[n][i] == -INFINITY ? 0.f : ex2(m[n][i] - M);
 #pragma unroll
         for (int d = 0; d < kSteps; ++d)  // dimensions HD / 8 g + 2 d, + 1
           *reinterpret_cast<float2*>(&os[warp][2 * t + i][(HD / 8) * g + 2 * d]) =
@@ -317,10 +323,11 @@ __global__ void __launch_bounds__(kFewThreads, NT == 1 ? 4 : NT == 2 ? 3 : 2) q8
 #pragma unroll
       for (int w = 0; w < kFewWarps; ++w) {
         if (wm[w][8 * n + row] != -INFINITY || wl[w][8 * n + row] != 0.f) Lr += wl[w][8 * n + row] * (Mr == -INFINITY ? 1.f : ex2(wm[w][8 * n + row] - Mr));
+        const float u = wu[w][8 * n + row];
 #pragma unroll
         for (int i = 0; i < kPer; i += 4) {
           const float4 x = *reinterpret_cast<const float4*>(&os[w][row][d0 + i]);
-          sum[i] += x.x, sum[i + 1] += x.y, sum[i + 2] += x.z, sum[i + 3] += x.w;
+          sum[i] = fmaf(x.x, u, sum[i]), sum[i + 1] = fmaf(x.y, u, sum[i + 1]), sum[i + 2] = fmaf(x.z, u, sum[i + 2]), sum[i + 3] = fmaf(x.w, u, sum[i + 3]);
         }
       }
       if (r < p.rows) {

@@ -81,7 +81,7 @@ def test_later_values_change_nothing_in_earlier_rows(ops, T, H, KV, hd, block, c
 
 @pytest.mark.parametrize("code", [I8, E4], ids=["int8", "e4m3"])
 @pytest.mark.parametrize("where", [0, 3, -2])
-@pytest.mark.parametrize("T,H,KV,hd,slots", [(60, 4, 2, 64, 900), (40, 4, 2, 128, 3000), (2600, 4, 1, 128, 2700)])
+@pytest.mark.parametrize("T,H,KV,hd,slots", [(1, 2, 2, 128, 300), (1, 4, 1, 64, 5000), (5, 4, 2, 128, 700), (8, 4, 1, 128, 400), (60, 4, 2, 64, 900), (40, 4, 2, 128, 3000), (2600, 4, 1, 128, 2700)])
 def test_a_block_of_large_values_and_little_weight(ops, T, H, KV, hd, slots, where, code):
     """Rows of q are positive, the keys of one block as negative as they get: its weights are some 2^-30 to 2^-60, its values 2^10 to 2^50 times the others'.  With the
     largest of these factors the block decides the result, with the smallest it has no part in it."""
