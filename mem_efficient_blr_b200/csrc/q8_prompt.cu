@@ -475,6 +475,7 @@ __global__ void __launch_bounds__(Split<WIDE>::kThreads, 1) q8_prompt_kernel(con
         if (moved) {
           float down = 1.f, corr = 1.f;
           if (ask) move_to(x, fac, factor, part, lim - key0, m, D, down, corr);
+          __syncwarp();  // (what follows in TMEM is the whole warp's)
           l *= down;
           if (u > 0 && __any_sync(0xffffffffu, corr != 1.f)) {
             if (!__all_sync(0xffffffffu, mbar_wait(done + 16 * wg + 8 * ((u - 1) & 1), ((u - 1) >> 1) & 1, abort_flag))) { ok = false; break; }
@@ -512,6 +513,7 @@ __global__ void __launch_bounds__(Split<WIDE>::kThreads, 1) q8_prompt_kernel(con
     float* const to32 = p.part + (((long long)at.bh * p.rows + r) * p.ns + at.split) * (HD + 4);
 #pragma unroll 1
     for (int c = 0; c < HD / 32; ++c) {
+      __syncwarp();  // (rows that are none leave a turn early, and the load is the whole warp's)
       uint32_t x[32];
       if (n > 0 && ok) {
         tmem_ld32(o_at + 32 * c, x);
