@@ -440,6 +440,14 @@ bool records_grad(std::initializer_list<const at::Tensor*> ts) {
   return false;
 }
 
+// The same for operators that no dispatcher knows, which refuse what has a derivative: tangents of forward mode too.
+bool has_derivative(std::initializer_list<const at::Tensor*> ts) {
+  if (c10::AutogradState::get_tls_state().get_fw_grad_mode())
+    for (const at::Tensor* t : ts)
+      if (t->_fw_grad(0).defined()) return true;
+  return records_grad(ts);
+}
+
 // The rest of the function under the operator's name in a profile, as the dispatcher records it (nothing without a profiler)
 #define BLR_RECORD(op, ...) RECORD_FUNCTION("blr_b200_ext::" op, (std::vector<c10::IValue>{__VA_ARGS__}))
 
@@ -917,7 +925,7 @@ PyObject* py_rope_append_q8(PyObject*, PyObject* const* a, Py_ssize_t na) {
   const at::Tensor *cs = d.factor(a[3], at::kFloat), *sn = d.factor(a[4], at::kFloat);
   for (const at::Tensor* t : {cs, sn})
     if (!t || t->dim() != 2 || t->size(0) < c.c.slots || t->size(1) != c.c.head_dim / 2) BLR_NONE();
-  if (!per_sequence(d, c, a[5], false, &start) || !per_sequence(d, c, a[7], true, &n_new) || records_grad({d.x, dk.x, dv.x})) BLR_NONE();
+  if (!per_sequence(d, c, a[5], false, &start) || !per_sequence(d, c, a[7], true, &n_new) || has_derivative({d.x, dk.x, dv.x})) BLR_NONE();
   at::Tensor out = d.output(d.width);
   void* o = out.data_ptr();
   call_library([&] {
@@ -936,7 +944,7 @@ PyObject* py_attention_q8(PyObject*, PyObject* const* a, Py_ssize_t na) {
   const int64_t *start, *n_new;
   float scale;
   if (na != 5 || !d.take_x(a[0]) || !c.take(a[1]) || !c.rows_of(d) || !per_sequence(d, c, a[2], false, &start) || !per_sequence(d, c, a[3], true, &n_new) ||
-      !take_eps(a[4], &scale) || d.width % ((int64_t)c.c.kv_heads * c.c.head_dim) != 0 || records_grad({d.x}))
+      !take_eps(a[4], &scale) || d.width % ((int64_t)c.c.kv_heads * c.c.head_dim) != 0 || has_derivative({d.x}))
     BLR_NONE();
   const int64_t n_tok = d.n / c.c.n_seq;
   const int heads = (int)(d.width / c.c.head_dim);
@@ -985,7 +993,7 @@ PyObject* py_token_logprobs(PyObject*, PyObject* const* a, Py_ssize_t na) {
   const int64_t rows = x->size(0), vocab = x->size(1), ld = rows > 1 ? x->stride(0) : vocab;
   const at::ScalarType dt = x->scalar_type();
   if (rows == 0 || vocab == 0 || ids->size(0) != rows || x->stride(1) != 1 || ld < vocab || x->device().index() != c10::cuda::current_device() ||
-      (dt != at::kHalf && dt != at::kBFloat16 && dt != at::kFloat) || records_grad({x}))
+      (dt != at::kHalf && dt != at::kBFloat16 && dt != at::kFloat) || has_derivative({x}))
     BLR_NONE();
   const cudaStream_t st = at::cuda::getCurrentCUDAStream(x->device().index()).stream();
   auto make = [&](at::IntArrayRef size, at::ScalarType type) { return at::detail::empty_cuda(size, type, x->device(), c10::nullopt); };

@@ -16,6 +16,7 @@ import weakref
 from typing import NamedTuple, Tuple
 
 import torch
+import torch.autograd.forward_ad as _fwd
 
 from . import _lib as L
 
@@ -697,8 +698,16 @@ _Q8_CODE = {torch.int8: 0, torch.float8_e4m3fn: 1}
 
 
 def _no_grad(*ts: torch.Tensor) -> None:
-    if torch.is_grad_enabled() and any(t.requires_grad for t in ts):
-        raise RuntimeError("blr_b200: this operator has no derivative; call it under torch.no_grad() or on detached tensors")
+    if torch.is_grad_enabled() and any(t.requires_grad for t in ts) or \
+            _fwd._current_level >= 0 and torch._C._is_fwd_grad_enabled() and any(_fwd.unpack_dual(t).tangent is not None for t in ts):
+        raise RuntimeError("blr_b200: this operator has no derivative; call it under torch.no_grad() or on detached tensors (no tangents either)")
+
+
+def _not_recorded() -> None:
+    """Refuses a call that torch.jit.trace or make_fx records: they would hold the empty outputs and not the launch that fills them."""
+    from torch.fx.experimental.proxy_tensor import get_proxy_mode
+    if torch.jit.is_tracing() or get_proxy_mode() is not None:
+        raise RuntimeError("blr_b200: the 8-bit cache's operators and token_logprobs cannot be recorded by torch.jit.trace or make_fx; capture them in a CUDA graph")
 
 
 def _q8_desc(c: Q8Cache, x: torch.Tensor) -> "L.Q8CacheDesc":
@@ -728,6 +737,7 @@ def rope_append_q8(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cos_table:
     out = None if dr is None else dr.rope_append_q8(q, k, v, cos_table, sin_table, start, cache, n_new)
     if out is not None:
         return out
+    _not_recorded()
     _no_grad(q, k, v)
     d = _q8_desc(cache, q)
     hd = d.head_dim
@@ -753,6 +763,7 @@ def cache_read_q8(cache: Q8Cache, dtype: torch.dtype, lengths=None) -> Tuple[tor
     out = None if dr is None or dtype not in (torch.float16, torch.bfloat16) else dr.cache_read_q8(cache, int(dtype == torch.bfloat16), lengths)
     if out is not None:
         return out
+    _not_recorded()
     d = _q8_desc(cache, cache.k)
     k, v = (torch.empty(cache.k.shape, dtype=dtype, device=cache.k.device) for _ in range(2))
     L.check(L.load().blr_cache_read_q8(d, None if lengths is None else _per_sequence(lengths, cache.k, d.n_seq, "lengths"), L.dtype_code(dtype), k.data_ptr(),
@@ -768,6 +779,7 @@ def attention_q8(q: torch.Tensor, cache: Q8Cache, start: torch.Tensor, n_new=Non
     out = None if dr is None else dr.attention_q8(q, cache, start, n_new, scale)
     if out is not None:
         return out
+    _not_recorded()
     _no_grad(q)
     d = _q8_desc(cache, q)
     assert q.dim() == 2 and d.n_seq > 0 and q.shape[0] % d.n_seq == 0 and q.shape[1] % (d.kv_heads * d.head_dim) == 0, "q: a row for each token of each sequence"
@@ -791,6 +803,7 @@ def token_logprobs(logits: torch.Tensor, ids: torch.Tensor, top: int = 0) -> Tup
     out = None if dr is None else dr.token_logprobs(logits, ids, top)
     if out is not None:
         return out
+    _not_recorded()
     _no_grad(logits)
     _need_cuda(logits)
     assert logits.dim() >= 1 and ids.shape == logits.shape[:-1] and ids.dtype == torch.int64 and ids.device == logits.device, "ids: one int64 for each row of logits"
