@@ -740,18 +740,18 @@ def rope_append_q8(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cos_table:
     _not_recorded()
     _no_grad(q, k, v)
     d = _q8_desc(cache, q)
-    hd = d.head_dim
+    n_seq, kv_heads, slots, hd = cache.k.shape
     assert all(t.dim() == 2 for t in (q, k, v)) and q.dtype == k.dtype == v.dtype and q.device == k.device == v.device, "q, k, v are rows of one dtype and device"
     rows = q.shape[0]
-    assert d.n_seq > 0 and rows % d.n_seq == 0 and k.shape == v.shape == (rows, d.kv_heads * hd) and q.shape[1] % hd == 0, "q, k, v: a row for each token of each sequence"
+    assert n_seq > 0 and rows % n_seq == 0 and k.shape == v.shape == (rows, kv_heads * hd) and q.shape[1] % hd == 0, "q, k, v: a row for each token of each sequence"
     for t in (cos_table, sin_table):
-        assert t.dtype == torch.float32 and t.is_contiguous() and t.dim() == 2 and t.shape[0] >= d.slots and t.shape[1] == hd // 2 and t.device == q.device, \
+        assert t.dtype == torch.float32 and t.is_contiguous() and t.dim() == 2 and t.shape[0] >= slots and t.shape[1] == hd // 2 and t.device == q.device, \
             "cos / sin tables are packed (slots, head_dim / 2) fp32"
     q2, k2, v2 = (_rows16(t, t.shape[1]) for t in (q, k, v))
     out = torch.empty((rows, q.shape[1]), dtype=q.dtype, device=q.device)
     L.check(L.load().blr_rope_append_q8(q2.data_ptr(), q2.stride(0), k2.data_ptr(), k2.stride(0), v2.data_ptr(), v2.stride(0), cos_table.data_ptr(),
-                                        sin_table.data_ptr(), _per_sequence(start, q, d.n_seq, "start"),
-                                        None if n_new is None else _per_sequence(n_new, q, d.n_seq, "n_new"), rows // d.n_seq, q.shape[1] // hd,
+                                        sin_table.data_ptr(), _per_sequence(start, q, n_seq, "start"),
+                                        None if n_new is None else _per_sequence(n_new, q, n_seq, "n_new"), rows // n_seq, q.shape[1] // hd,
                                         L.dtype_code(q.dtype), d, out.data_ptr(), out.shape[1], L.stream_ptr(q.device)))
     return out
 
@@ -766,7 +766,7 @@ def cache_read_q8(cache: Q8Cache, dtype: torch.dtype, lengths=None) -> Tuple[tor
     _not_recorded()
     d = _q8_desc(cache, cache.k)
     k, v = (torch.empty(cache.k.shape, dtype=dtype, device=cache.k.device) for _ in range(2))
-    L.check(L.load().blr_cache_read_q8(d, None if lengths is None else _per_sequence(lengths, cache.k, d.n_seq, "lengths"), L.dtype_code(dtype), k.data_ptr(),
+    L.check(L.load().blr_cache_read_q8(d, None if lengths is None else _per_sequence(lengths, cache.k, cache.k.shape[0], "lengths"), L.dtype_code(dtype), k.data_ptr(),
                                        v.data_ptr(), L.stream_ptr(cache.k.device)))
     return k, v
 
@@ -782,15 +782,16 @@ def attention_q8(q: torch.Tensor, cache: Q8Cache, start: torch.Tensor, n_new=Non
     _not_recorded()
     _no_grad(q)
     d = _q8_desc(cache, q)
-    assert q.dim() == 2 and d.n_seq > 0 and q.shape[0] % d.n_seq == 0 and q.shape[1] % (d.kv_heads * d.head_dim) == 0, "q: a row for each token of each sequence"
+    n_seq, kv_heads, _, hd = cache.k.shape
+    assert q.dim() == 2 and n_seq > 0 and q.shape[0] % n_seq == 0 and q.shape[1] % (kv_heads * hd) == 0, "q: a row for each token of each sequence"
     q2 = _rows16(q, q.shape[1])
-    lib, n_tok, heads = L.load(), q.shape[0] // d.n_seq, q.shape[1] // d.head_dim
+    lib, n_tok, heads = L.load(), q.shape[0] // n_seq, q.shape[1] // hd
     out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
     nbytes = lib.blr_attention_q8_scratch_bytes(d, n_tok, heads)
     scratch = torch.empty(nbytes, dtype=torch.uint8, device=q.device) if nbytes else None
     ws, st = _ws(q, 1, 0, 0)   # (its status word)
-    L.check(lib.blr_attention_q8(q2.data_ptr(), q2.stride(0), d, _per_sequence(start, q, d.n_seq, "start"),
-                                 None if n_new is None else _per_sequence(n_new, q, d.n_seq, "n_new"), n_tok, heads, float(scale) if scale else d.head_dim ** -0.5,
+    L.check(lib.blr_attention_q8(q2.data_ptr(), q2.stride(0), d, _per_sequence(start, q, n_seq, "start"),
+                                 None if n_new is None else _per_sequence(n_new, q, n_seq, "n_new"), n_tok, heads, float(scale) if scale else hd ** -0.5,
                                  L.dtype_code(q.dtype), out.data_ptr(), out.shape[1], None if scratch is None else scratch.data_ptr(), nbytes, ws.data_ptr(), st))
     return out
 
