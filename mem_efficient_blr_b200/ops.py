@@ -712,6 +712,7 @@ def _not_recorded() -> None:
 
 def _q8_desc(c: Q8Cache, x: torch.Tensor) -> "L.Q8CacheDesc":
     _need_cuda(x, c.k, c.v, c.k_scale, c.v_scale)
+    assert not any(t.is_neg() for t in c[:4]), "a cache is written in place: no lazily negated views"
     assert c.k.dim() == 4 and c.v.shape == c.k.shape and c.v.dtype == c.k.dtype, "keys and values of an 8-bit cache are (n_seq, kv_heads, slots, head_dim) of one type"
     assert c.k.dtype in _Q8_CODE, f"codes are int8 or float8_e4m3fn, got {c.k.dtype}"
     n_seq, kv_heads, slots, hd = c.k.shape
@@ -739,6 +740,7 @@ def rope_append_q8(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cos_table:
         return out
     _not_recorded()
     _no_grad(q, k, v)
+    q, k, v, cos_table, sin_table = (t.resolve_neg() for t in (q, k, v, cos_table, sin_table))
     d = _q8_desc(cache, q)
     n_seq, kv_heads, slots, hd = cache.k.shape
     assert all(t.dim() == 2 for t in (q, k, v)) and q.dtype == k.dtype == v.dtype and q.device == k.device == v.device, "q, k, v are rows of one dtype and device"
@@ -781,6 +783,7 @@ def attention_q8(q: torch.Tensor, cache: Q8Cache, start: torch.Tensor, n_new=Non
         return out
     _not_recorded()
     _no_grad(q)
+    q = q.resolve_neg()
     d = _q8_desc(cache, q)
     n_seq, kv_heads, _, hd = cache.k.shape
     assert q.dim() == 2 and n_seq > 0 and q.shape[0] % n_seq == 0 and q.shape[1] % (kv_heads * hd) == 0, "q: a row for each token of each sequence"
@@ -806,6 +809,7 @@ def token_logprobs(logits: torch.Tensor, ids: torch.Tensor, top: int = 0) -> Tup
         return out
     _not_recorded()
     _no_grad(logits)
+    logits = logits.resolve_neg()
     _need_cuda(logits)
     assert logits.dim() >= 1 and ids.shape == logits.shape[:-1] and ids.dtype == torch.int64 and ids.device == logits.device, "ids: one int64 for each row of logits"
     kind = {torch.float16: 0, torch.bfloat16: 1, torch.float32: 2}.get(logits.dtype)
