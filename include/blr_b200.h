@@ -390,7 +390,8 @@ int blr_attention_decode(const void* q, int64_t ldq, const void* k_cache, const 
  * Codes are (n_seq, kv_heads, slots, head_dim) bytes, int8 in [-127, 127] or e4m3, packed and 16-byte aligned; `block` slots of a head share one fp32
  * scale that is not negative, (n_seq, kv_heads, ceil(slots / block)): value = code * scale.  head_dim 64 or 128, block 16, 32, 64 or 128 (BLR_ERR_UNSUPPORTED else).
  * start, n_new: device int64, one per sequence; a call's tokens of sequence s take slots start[s] .. start[s] + n_new[s] - 1 (n_new NULL: n_tok
- * each).  Rows behind a sequence's n_new, and tokens whose slot is outside the cache, write nothing to it and leave zeros in an output.  16-bit tensors of
+ * each).  Rows behind a sequence's n_new write nothing to it and leave zeros in an output; tokens whose slot is outside the cache, which the host cannot see, are
+ * dropped: they write nothing, their rotated q is zeros, and the attention lets a row behind the last slot see all slots, one ahead of the first none.  16-bit tensors of
  * `dtype`, rows 16-byte aligned, row strides multiples of 8; any of them, start and n_new too, may be written by the kernel directly ahead. */
 #define BLR_Q8_INT8 0
 #define BLR_Q8_E4M3 1

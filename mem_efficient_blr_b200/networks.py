@@ -446,7 +446,13 @@ class LlamaDecoder(nn.Module):
         return x
 
     def _run(self, ids, pos, causal):
-        return self.lm_head(self.norm(self._hidden(ids, pos, causal)[:, -1]))
+        logits = self.lm_head(self.norm(self._hidden(ids, pos, causal)[:, -1]))
+        return logits if self.q8cache is None or causal else self._nan_outside(logits, pos, ids.shape[1])
+
+    def _nan_outside(self, logits, start, n):
+        """NaN for sequences whose n tokens from `start` on do not all lie in the 8-bit cache: those outside are written nowhere, and the host, which does not
+        see the positions, cannot refuse them."""
+        return logits.masked_fill_((start.clamp(min=0).clamp(max=self.cache_len - n) != start)[:, None], float("nan"))
 
     def _hidden(self, ids, pos, causal):
         if self.q8cache is not None:
@@ -476,19 +482,20 @@ class LlamaDecoder(nn.Module):
     def decode_step(self, ids: torch.Tensor, pos: torch.Tensor) -> torch.Tensor:
         """ids (B, 1): one new token per sequence, written to cache slot pos (1,) and attending to the whole cache
         (slots beyond the sequence's length must hold real keys: the benchmark decodes at a full cache).  On an 8-bit cache it attends to the slots up to
-        its own, and pos may be (B,), one for each sequence."""
+        its own, and pos may be (B,), one for each sequence; a position outside the cache gives NaN."""
         return self._run(ids, pos, False)
 
     @torch.no_grad()
     def extend(self, ids: torch.Tensor, start: torch.Tensor, n_new: Optional[torch.Tensor] = None) -> torch.Tensor:
         """The next tokens of sequences at different positions, on an 8-bit cache: ids (B, T) go to slots start[b] .. (start (B,) int64), of each row the
         first n_new[b] ((B,) int64; None: all).  Returns the logits behind each sequence's last new token (B, vocab); those of a sequence without a new
-        token mean nothing."""
+        token mean nothing, and those of one with a token outside the cache are NaN."""
         if self.q8cache is None:
             raise RuntimeError("extend needs a decoder with an 8-bit cache (kv_cache='int8' or 'e4m3')")
         x = self._hidden_q8(ids, start, n_new)
         last = x[:, -1] if n_new is None else x[torch.arange(ids.shape[0], device=ids.device), (n_new - 1).clamp(0, ids.shape[1] - 1)]
-        return self.lm_head(self.norm(last))
+        T = ids.shape[1]
+        return self._nan_outside(self.lm_head(self.norm(last)), start, T if n_new is None else n_new.clamp(0, T))
 
     @torch.no_grad()
     def score(self, ids: torch.Tensor, top: int = 0):

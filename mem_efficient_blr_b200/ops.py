@@ -776,7 +776,7 @@ def cache_read_q8(cache: Q8Cache, dtype: torch.dtype, lengths=None) -> Tuple[tor
 def attention_q8(q: torch.Tensor, cache: Q8Cache, start: torch.Tensor, n_new=None, scale: float = 0.0) -> torch.Tensor:
     """Causal attention of each sequence's newest tokens over an 8-bit cache that holds them already: q (n_seq * n_tok, heads * head_dim) 16-bit rows,
     sequence-major, heads a multiple of the cache's kv_heads; row t of sequence s sits at slot start[s] + t and sees the slots up to its own; rows from
-    n_new[s] on are no tokens and come out as zeros, as does a row that sees no slot.  scale defaults to head_dim ** -0.5.  Returns (rows, heads * head_dim)."""
+    n_new[s] on are no tokens and come out as zeros, as does a row that sees no slot (a row behind the last slot sees all).  scale defaults to head_dim ** -0.5.  Returns (rows, heads * head_dim)."""
     dr = L.direct()
     out = None if dr is None else dr.attention_q8(q, cache, start, n_new, scale)
     if out is not None:
