@@ -370,7 +370,7 @@ int blr_add_layernorm(const void* x, int64_t ldx, const void* y, int64_t ldy, co
  * slot from cos_table / sin_table ((slots, head_dim / 2) fp32; pairs (i, i + head_dim / 2) rotate, as in HF's Llama).
  * Any of the inputs, pos and the tables too, may be written by the kernel directly ahead in the stream.
  * q is rotated in place; rotated k and v are written to k_cache / v_cache [seq][head][pos[t]][:] (caches of
- * (n_seq, heads, slots, head_dim)). */
+ * (n_seq, heads, slots, head_dim)).  A token whose slot is outside them is left out: nothing is written, its q stays as it is. */
 int blr_rope_append(void* q, int64_t ldq, const void* k, int64_t ldk, const void* v, int64_t ldv,
                     const float* cos_table, const float* sin_table, const int64_t* pos,
                     int64_t n_seq, int n_tok, int heads, int head_dim, int slots, int dtype,

@@ -321,6 +321,7 @@ __global__ void __launch_bounds__(256) rope_append_kernel(uint16_t* q, long long
   const uint16_t* vr = v + (long long)r * ldv;
   asm volatile("griddepcontrol.wait;" ::: "memory");  // (slots and angles too: a step's positions are often written right ahead of it)
   const long long slot = pos[t];
+  if (slot < 0 || slot >= slots) return;  // (no such slot: nothing is read or written for it)
   const float* cs = cos_t + slot * half;
   const float* sn = sin_t + slot * half;
   // two values per thread and step: pair index i = 2 u, 2 u + 1 of head h

@@ -438,8 +438,7 @@ class LlamaDecoder(nn.Module):
         return [m for layer in self.layers for m in layer.structured()]
 
     def _hidden_q8(self, ids, start, n_new=None):
-        if ids.shape[1] > self.cache_len:
-            raise ValueError(f"{ids.shape[1]} tokens do not fit a cache of {self.cache_len} slots")
+        self._fit(ids)
         x, B = self.embed_tokens(ids), ids.shape[0]
         for layer, cache in zip(self.layers, self.q8cache):
             x = layer.forward_q8(x, (self.cos, self.sin), cache.first(B), start, n_new, self.fused_decode)
@@ -454,7 +453,12 @@ class LlamaDecoder(nn.Module):
         see the positions, cannot refuse them."""
         return logits.masked_fill_((start.clamp(min=0).clamp(max=self.cache_len - n) != start)[:, None], float("nan"))
 
+    def _fit(self, ids):
+        if ids.shape[1] > self.cache_len:
+            raise ValueError(f"{ids.shape[1]} tokens do not fit a cache of {self.cache_len} slots")
+
     def _hidden(self, ids, pos, causal):
+        self._fit(ids)
         if self.q8cache is not None:
             B = ids.shape[0]
             return self._hidden_q8(ids, pos.new_zeros(B) if causal else pos if pos.numel() == B else pos.expand(B).contiguous())

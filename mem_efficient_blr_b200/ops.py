@@ -641,7 +641,7 @@ def rope_append(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cos_table: to
                 pos: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, n_tok: int) -> torch.Tensor:
     """q, k, v (n_seq * n_tok, heads * head_dim) rows (sequence-major); caches (n_seq, heads, slots, head_dim); cos / sin
     tables (slots, head_dim / 2) fp32; pos (n_tok,) int64 cache slots.  Rotates q in place (returned), writes the
-    rotated k and v into the caches at the tokens' slots."""
+    rotated k and v into the caches at the tokens' slots.  A token whose slot is outside the caches is left out: its q stays as it is."""
     _need_cuda(q, k_cache, v_cache)
     n_seq, heads, slots, hd = k_cache.shape
     assert q.dim() == 2 and q.shape == k.shape == v.shape and q.shape[0] == n_seq * n_tok and q.shape[1] == heads * hd
