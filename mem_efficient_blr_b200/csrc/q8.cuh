@@ -5,7 +5,9 @@
 #include <cuda_runtime.h>
 #include <stdint.h>
 
+#include "../../include/blr_b200.h"
 #include "ptx.cuh"
+#include "tmap.h"
 
 namespace blr {
 
@@ -104,6 +106,22 @@ __device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
 }
 
 // ---- host side
+// A launch that may begin while the kernel ahead of it ends (every kernel here waits before it looks at anything).
+template <typename K, typename... A>
+static int q8_launch(K kernel, dim3 grid, int threads, int smem, cudaStream_t stream, A... args) {
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = grid;
+  cfg.blockDim = dim3((unsigned)threads);
+  cfg.dynamicSmemBytes = (size_t)smem;
+  cfg.stream = stream;
+  cudaLaunchAttribute at[1];
+  at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  at[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = at;
+  cfg.numAttrs = 1;
+  BLR_CUDA_OK(cudaLaunchKernelEx(&cfg, kernel, args...));
+  return BLR_OK;
+}
 int q8_view(const blr_q8_cache* cache, Q8View* out);  // checks the cache's description
 
 }  // namespace blr

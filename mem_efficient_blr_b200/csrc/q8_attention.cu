@@ -433,22 +433,6 @@ static Q8Plan q8_plan(const blr_q8_cache* c, int64_t n_tok, int heads) {
 }
 static size_t q8_wide_bytes(const Q8Plan& a, const blr_q8_cache* c) { return (size_t)(c->n_seq * c->kv_heads * a.wide_tiles) * 512 * c->head_dim; }
 
-template <typename K, typename... A>
-static int launch(K kern, dim3 grid, dim3 block, size_t smem, cudaStream_t st, A... args) {
-  cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = grid;
-  cfg.blockDim = block;
-  cfg.dynamicSmemBytes = smem;
-  cfg.stream = st;
-  cudaLaunchAttribute at[1];
-  at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  at[0].val.programmaticStreamSerializationAllowed = 1;
-  cfg.attrs = at;
-  cfg.numAttrs = 1;
-  BLR_CUDA_OK(cudaLaunchKernelEx(&cfg, kern, args...));
-  return BLR_OK;
-}
-
 template <bool E4M3, int HD, int NT>
 static int launch_few(const Q8AttnParams& p, long long ctas, cudaStream_t st) {
   static bool configured[64] = {};
@@ -460,7 +444,7 @@ static int launch_few(const Q8AttnParams& p, long long ctas, cudaStream_t st) {
     BLR_CUDA_OK(cudaFuncSetAttribute(q8_attention_kernel<E4M3, HD, NT>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
     configured[di.dev] = true;
   }
-  return launch(q8_attention_kernel<E4M3, HD, NT>, dim3((unsigned)ctas), dim3(kFewThreads), smem, st, p);
+  return q8_launch(q8_attention_kernel<E4M3, HD, NT>, dim3((unsigned)ctas), kFewThreads, smem, st, p);
 }
 
 }  // namespace blr
@@ -516,7 +500,7 @@ int blr_attention_q8(const void* q, int64_t ldq, const blr_q8_cache* cache, cons
   if (rc || a.ns == 1) return rc;
   const long long total = cache->n_seq * cache->kv_heads * a.rows;
   const dim3 cgrid((unsigned)((total + 7) / 8));
-  return cache->head_dim == 128 ? launch(q8_combine_kernel<128>, cgrid, dim3(256), 0, st, p, total) : launch(q8_combine_kernel<64>, cgrid, dim3(256), 0, st, p, total);
+  return cache->head_dim == 128 ? q8_launch(q8_combine_kernel<128>, cgrid, 256, 0, st, p, total) : q8_launch(q8_combine_kernel<64>, cgrid, 256, 0, st, p, total);
 }
 
 }  // extern "C"

@@ -253,21 +253,6 @@ __global__ void __launch_bounds__(256) cache_read_q8_kernel(Q8View c, int hd_log
   to[0] = o[0], to[1] = o[1];
 }
 
-template <typename K, typename... A>
-static int launch(K kern, dim3 grid, dim3 block, cudaStream_t st, A... args) {
-  cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = grid;
-  cfg.blockDim = block;
-  cfg.stream = st;
-  cudaLaunchAttribute at[1];
-  at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  at[0].val.programmaticStreamSerializationAllowed = 1;
-  cfg.attrs = at;
-  cfg.numAttrs = 1;
-  BLR_CUDA_OK(cudaLaunchKernelEx(&cfg, kern, args...));
-  return BLR_OK;
-}
-
 }  // namespace blr
 
 using namespace blr;
@@ -309,7 +294,7 @@ int blr_rope_append_q8(const void* q, int64_t ldq, const void* k, int64_t ldk, c
   p.unit_ctas = (unsigned)unit_ctas;
   const cudaStream_t st = static_cast<cudaStream_t>(stream);
   const bool bf = dtype == BLR_DTYPE_BF16, e4 = cache->code == BLR_Q8_E4M3;
-  auto go = [&](auto kernel) { return launch(kernel, dim3((unsigned)ctas), dim3(kAppendThreads), st, p); };
+  auto go = [&](auto kernel) { return q8_launch(kernel, dim3((unsigned)ctas), kAppendThreads, 0, st, p); };
   if (cache->head_dim == 128)
     return bf ? (e4 ? go(rope_append_q8_kernel<true, true, 8>) : go(rope_append_q8_kernel<true, false, 8>))
               : (e4 ? go(rope_append_q8_kernel<false, true, 8>) : go(rope_append_q8_kernel<false, false, 8>));
@@ -332,7 +317,7 @@ int blr_cache_read_q8(const blr_q8_cache* cache, const int64_t* lengths, int dty
   const cudaStream_t st = static_cast<cudaStream_t>(stream);
   const bool bf = dtype == BLR_DTYPE_BF16, e4 = cache->code == BLR_Q8_E4M3;
   auto go = [&](auto kernel) {
-    return launch(kernel, dim3((unsigned)ctas, 2), dim3(256), st, c, hd_log2, reinterpret_cast<const long long*>(lengths), pieces,
+    return q8_launch(kernel, dim3((unsigned)ctas, 2), 256, 0, st, c, hd_log2, reinterpret_cast<const long long*>(lengths), pieces,
                   static_cast<uint16_t*>(k_out), static_cast<uint16_t*>(v_out));
   };
   return bf ? (e4 ? go(cache_read_q8_kernel<true, true>) : go(cache_read_q8_kernel<true, false>))

@@ -589,22 +589,6 @@ __global__ void __launch_bounds__(256) q8_widen_kernel(const __grid_constant__ Q
   }
 }
 
-template <typename K>
-static int launch(K kernel, long long ctas, int threads, int smem, const Q8AttnParams& p, cudaStream_t stream) {
-  cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3((unsigned)ctas);
-  cfg.blockDim = dim3((unsigned)threads);
-  cfg.dynamicSmemBytes = (size_t)smem;
-  cfg.stream = stream;
-  cudaLaunchAttribute at[1];
-  at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  at[0].val.programmaticStreamSerializationAllowed = 1;
-  cfg.attrs = at;
-  cfg.numAttrs = 1;
-  BLR_CUDA_OK(cudaLaunchKernelEx(&cfg, kernel, p));
-  return BLR_OK;
-}
-
 template <bool E4M3, int HD, bool WIDE>
 static int launch_prompt(const Q8AttnParams& p, cudaStream_t stream) {
   static bool configured[64] = {};
@@ -620,7 +604,7 @@ static int launch_prompt(const Q8AttnParams& p, cudaStream_t stream) {
                 Split<WIDE>::kLaunch);
     configured[di.dev] = true;
   }
-  return launch(q8_prompt_kernel<E4M3, HD, WIDE>, (long long)p.n_bh * p.q_tiles * p.ns, Split<WIDE>::kThreads, smem, p, stream);
+  return q8_launch(q8_prompt_kernel<E4M3, HD, WIDE>, dim3((unsigned)p.n_bh * p.q_tiles * p.ns), Split<WIDE>::kThreads, smem, stream, p);
 }
 
 int q8_launch_prompt(const Q8AttnParams& p, int head_dim, int code, cudaStream_t stream) {
@@ -629,10 +613,9 @@ int q8_launch_prompt(const Q8AttnParams& p, int head_dim, int code, cudaStream_t
     if (head_dim == 128) return e4 ? launch_prompt<true, 128, false>(p, stream) : launch_prompt<false, 128, false>(p, stream);
     return e4 ? launch_prompt<true, 64, false>(p, stream) : launch_prompt<false, 64, false>(p, stream);
   }
-  const long long tiles = (long long)p.n_bh * p.wide_tiles;
-  int rc;
-  if (head_dim == 128) rc = e4 ? launch(q8_widen_kernel<true, 128>, tiles, 256, 0, p, stream) : launch(q8_widen_kernel<false, 128>, tiles, 256, 0, p, stream);
-  else rc = e4 ? launch(q8_widen_kernel<true, 64>, tiles, 256, 0, p, stream) : launch(q8_widen_kernel<false, 64>, tiles, 256, 0, p, stream);
+  auto widen = [&](auto kernel) { return q8_launch(kernel, dim3((unsigned)p.n_bh * p.wide_tiles), 256, 0, stream, p); };
+  const int rc = head_dim == 128 ? (e4 ? widen(q8_widen_kernel<true, 128>) : widen(q8_widen_kernel<false, 128>))
+                                 : (e4 ? widen(q8_widen_kernel<true, 64>) : widen(q8_widen_kernel<false, 64>));
   if (rc) return rc;
   return head_dim == 128 ? launch_prompt<false, 128, true>(p, stream) : launch_prompt<false, 64, true>(p, stream);
 }
