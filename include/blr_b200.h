@@ -408,13 +408,13 @@ typedef struct blr_q8_cache {
 /* Rotary embedding and append.  q: n_seq * n_tok rows (sequence-major) of heads * head_dim values, k and v of kv_heads * head_dim.  The angle of a
  * token is its slot's row of cos_table / sin_table ((>= slots, head_dim / 2) fp32, 16-byte aligned; pairs (i, i + head_dim / 2) rotate).  q_out: the
  * rotated q.  Rotated k and v go to the cache as codes round(x (1 / s)), s = max(s_before, max|x| (1 / 127 or 1 / 448)) over the block's tokens, in fp32;
- * s_before = 0 for a block that begins with this call, and where s grows over older tokens of the block their codes become round(code (s_before (1 / s))).  A scale below
- * the smallest normal number is 0.  A block that a NaN or infinity is written to reads back as NaN. */
+ * s_before = 0 for a block that begins with this call, and where s grows over older tokens of the block their codes become round(code (s_before (1 / s))).  A call
+ * ends its sequence: codes behind its last token stay as they are, although the scale of their block may have changed.  A scale below the smallest normal number is 0.  A block that a NaN or infinity is written to reads back as NaN. */
 int blr_rope_append_q8(const void* q, int64_t ldq, const void* k, int64_t ldk, const void* v, int64_t ldv,
                        const float* cos_table, const float* sin_table, const int64_t* start, const int64_t* n_new, int64_t n_tok, int heads,
                        int dtype, const blr_q8_cache* cache, void* q_out, int64_t ldo, void* stream);
 
-/* k_out, v_out (n_seq, kv_heads, slots, head_dim) = code * scale rounded to dtype; zeros from slot lengths[s] on (device int64, NULL: all slots). */
+/* k_out, v_out (n_seq, kv_heads, slots, head_dim) = code * scale, in fp32 and then rounded to dtype; zeros from slot lengths[s] on (device int64, NULL: all slots). */
 int blr_cache_read_q8(const blr_q8_cache* cache, const int64_t* lengths, int dtype, void* k_out, void* v_out, void* stream);
 
 /* Causal attention of the newest tokens: row t < n_new[s] of sequence s sits at slot start[s] + t and sees slots 0 .. start[s] + t;

@@ -9,8 +9,8 @@
 // codes are exact in fp16, q is too (bf16 rows are brought into its range by a power of two; what is 2^-38 of a row's largest value may be lost), so the only rounding to
 // 16 bits is that of p_j vs_j D; sums are fp32.
 // m follows the maximum only where it is more than 2^8 behind, D the heaviest p vs only where it has outgrown 2^15.
-// Bound by HBM on the codes (a key and its value are 2 hd bytes): 64 sequences x 32 heads x 2048 keys of 128, 1.08 GB, 166 us in a graph, 6.5 TB/s; by latency where they are
-// few (1 sequence: 12.6 us for 17 MB: positions, codes, a few groups a warp, the second kernel).  The keys of a row are shared out over the warps of a CTA and
+// Bound by HBM on the codes (a key and its value are 2 hd bytes): 64 sequences x 32 heads x 2048 keys of 128, 1.08 GB, 163 us in a graph, 6.6 TB/s (194 among calls
+// from Python); by latency where they are few (1 sequence: 13 us for 17 MB: positions, codes, a few groups a warp, the second kernel).  The keys of a row are shared out over the warps of a CTA and
 // over up to kMaxSplits CTAs.  A first version that loaded the groups into registers took 280 us for the former: 8 warps an SM instead of 16.
 #include "../../include/blr_b200.h"
 #include "q8_attention.h"
@@ -152,7 +152,7 @@ __global__ void __launch_bounds__(kFewThreads, NT == 1 ? 4 : NT == 2 ? 3 : 2) q8
       m[n][0] = m[n][1] = -INFINITY, D[n][0] = D[n][1] = 1.f;
     }
     if constexpr (kQShared) __syncthreads();
-    int lim_all = 0x7fffffff;  // keys below it are masked for no row of the warp
+    int lim_all = 0x7fffffff;  // keys below it are masked for no row of the warp (0 where its tiles have places without a row: leaving those out gained nothing for 20 rows of 32)
 #pragma unroll
     for (int n = 0; n < NT; ++n) lim_all = min(lim_all, min(lim[n][0], lim[n][1]));
     lim_all = __reduce_min_sync(0xffffffffu, lim_all);
@@ -406,8 +406,13 @@ struct Q8Plan {
   int nt, q_tiles, ns, room;  // nt: column tiles of 8 rows of the kernel here, 0: the prompt kernel; ns: CTAs that may share a row tile's keys
   long long rows, tiles, wide_tiles;  // wide_tiles: of 128 slots of a head, whose codes are widened ahead (0: not)
 };
-// Row tiles of a kv head from which its codes are widened ahead of the prompt kernel (us without | with, 32 heads on 8: 32 tiles, 2048 tokens 59 | 68, 40 tiles, 2560 tokens
-// 93 | 91, 64 tiles, 4096 tokens 187 | 180, 128 tiles, 8192 tokens 637 | 557), and the room that they may take.
+// Row tiles of a kv head from which its codes are widened ahead of the prompt kernel, and the room that they may take.  us without | with, prompts from slot 0, heads of 128:
+//   32 heads on 8   24 tiles, 1536 tokens 43 | 52   32, 2048: 60 | 67    40, 2560: 91 | 88    64, 4096: 184 | 179   128, 8192: 637 | 557
+//   32 on 32        16 tiles, 4096 tokens 190 | 193  24, 6144: 381 | 368  32, 8192: 649 | 590  40, 10240: 972 | 914
+//   8 on 1          40 tiles, 1280 tokens 31 | 34    64, 2048: 42 | 42
+// of 64: 32 on 8, 40 tiles 74 | 74, 64 tiles 151 | 155; 32 on 32, 40 tiles 817 | 806.  With four times as many older keys, 40 tiles: 32 on 8 672 | 609 (of 64: 580 | 564), 8 on 1
+// 64 | 64.  The launch and the pass cost 3 to 9 us, and the gain grows with the steps of an SM, which the host knows from the tokens alone: tiles are the simple measure, off by up
+// to 9 % for long unshared prompts below it and for short ones of few heads above it.
 static constexpr int kWideFrom = 40;
 static constexpr long long kWideBytes = 256ll << 20;
 // Few row tiles share their keys out over more CTAs, as many as the SMs hold at a time (4, 3, 2 or 1 of a kind); a second kernel sums the parts.  The host does not

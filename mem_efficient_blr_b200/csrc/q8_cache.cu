@@ -4,8 +4,8 @@
 //   s = max(s_before, max|x| (1 / top))  (top = 127 for int8, 448 for e4m3; s_before = 0 where the block begins with this call)
 // and codes round(x (1 / s)); where s has grown, the codes that were there become round(code (s_before (1 / s))).  So a block's scale only ever grows while the
 // block fills, a value is off by half a step of its block's final scale, and by half a step more for each time that the scale grew over it.  Nothing
-// else of the cache is touched.  All of it is fp32 with every product and sum rounded by itself (no fused multiply-add), so that the codes are a matter of
-// the formula alone.
+// else of the cache is touched: codes behind a call's last token stay, although their block's scale may change, since a call ends its sequence there.
+// All of it is fp32 with every product and sum rounded by itself (no fused multiply-add), so that the codes are a matter of the formula alone.
 #include "../../include/blr_b200.h"
 #include "q8.cuh"
 #include "tmap.h"
@@ -225,8 +225,8 @@ __global__ void __launch_bounds__(kAppendThreads, 2) rope_append_q8_kernel(const
   if (w == 0 && lane == 0) *scale = after;
 }
 
-// value = code * scale, rounded once; 16 codes a thread; zeros behind a sequence's length.  Bound by HBM, 1 byte in, 2 out: 16 x 8 x 4099 slots of 64, 186 MB, 33 us,
-// 5.6 TB/s.
+// value = code * scale, the product in fp32 and then rounded to 16 bits; 16 codes a thread; zeros behind a sequence's length.  Bound by HBM, 1 byte in, 2 out: 16 x 8 x 4099 slots of 64, 186 MB, 34 us,
+// 5.4 TB/s.
 template <bool BF16, bool E4M3>
 __global__ void __launch_bounds__(256) cache_read_q8_kernel(Q8View c, int hd_log2, const long long* lengths, long long pieces, uint16_t* k_out, uint16_t* v_out) {
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");

@@ -9,8 +9,9 @@
 // the place that the PV's P has left (P lies over the S that it was made of; one queue, so in order).  Neither half waits for the other's softmax, or for its own scores.
 // O is rescaled, seldom, when the last PV is known to be done.
 // Bounds, a step of 256 x 64 scores of heads of 128: 1280 cycles of tensor core (2 x 256 for PV, 2 x 384 for S, which reads both operands from shared memory for 64 columns)
-// and 1024 of ex2 (16 a cycle).  It takes 2150: the softmaxes of both halves share the schedulers for 1520 from scores in registers to P in TMEM, and spend 640 on barriers,
-// factors and TMEM's latency.  8192 tokens, 32 heads on 8: 592 us, 928 TFLOP/s.  (Steps of 128 keys, which leave no room for a second S: 600; back to back 571 against 561; and 3 x 257 tokens over up to 6001
+// and 1024 of ex2 (16 a cycle).  It takes 2140: the softmaxes of both halves share the schedulers for 1270 from scores in registers to P in TMEM, and spend 870 on barriers,
+// factors and TMEM's latency.  8192 tokens, 32 heads on 8: 565 us in a graph, 608 among calls from Python, 904 TFLOP/s.  (One reference of value scales for all rows of a CTA, which
+// later keys decided, took 1 % less.  What follows was measured on that form.  Steps of 128 keys, which leave no room for a second S: 600; back to back 571 against 561; and 3 x 257 tokens over up to 6001
 // keys of heads of 64 71 instead of 67.  All ex2 left out: 12 % less time.  With the next scores loaded between the two halves of a step's: 610.)  Tried on steps of 128 without
 // gain: part of ex2 as a polynomial on the FMA pipe (1/8: 617 us, 3/8: 623), four softmax warpgroups of half a tile's width each (771), vs / R in the exponent instead of a
 // multiplication (610), scores read twice instead of held (697).
@@ -320,7 +321,7 @@ __global__ void __launch_bounds__(Split<WIDE>::kThreads, 1) q8_prompt_kernel(con
   const uint32_t tmem = tmem_slot;
   const int halves = max(n0, n1), steps = (halves + 1) / 2;  // (n0, n1, halves: of 64 keys; steps: tiles of 128)
 
-  // (No spills in any of these: what shared memory leaves of L1 does not keep them, and a reload from L2 inside a loop costs more than anything that it saves.)
+  // (Few spills, 4 to 20 bytes in four of the six instances: what shared memory leaves of L1 does not keep them, and a reload from L2 inside a loop costs more than it saves.)
   // A step's factors: ks and vs of 8 groups of 16 keys (an infinite vs as a NaN).  One warp brings them, four steps deep (a step's are free when the S of the step after it
   // is done, and that warp is two steps ahead of that at most).
   float next_scale = 0.f;

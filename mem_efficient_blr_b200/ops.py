@@ -733,7 +733,8 @@ def rope_append_q8(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cos_table:
     sequence-major; start (n_seq,) int64: the slot of each sequence's first token, n_new (n_seq,) int64 (None: all n_tok): how many of its rows are
     tokens.  cos / sin tables (>= slots, head_dim / 2) fp32.  Returns the rotated q (zeros in rows that are no token) and writes codes and scales of the
     rotated k and of v: a block's scale is the largest its tokens asked for since it was begun, and where it grows the codes that were there follow.
-    Tokens whose slot lies outside the cache write nothing."""
+    A call ends its sequence: codes behind its last token stay, although the scale of their block may have changed.  Tokens whose slot lies outside the cache
+    write nothing."""
     dr = L.direct()
     out = None if dr is None else dr.rope_append_q8(q, k, v, cos_table, sin_table, start, cache, n_new)
     if out is not None:
@@ -759,7 +760,7 @@ def rope_append_q8(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cos_table:
 
 
 def cache_read_q8(cache: Q8Cache, dtype: torch.dtype, lengths=None) -> Tuple[torch.Tensor, torch.Tensor]:
-    """(keys, values) of an 8-bit cache in 16 bits, (n_seq, kv_heads, slots, head_dim): code * scale rounded once; zeros from slot lengths[s] of a sequence
+    """(keys, values) of an 8-bit cache in 16 bits, (n_seq, kv_heads, slots, head_dim): code * scale in fp32, rounded to dtype; zeros from slot lengths[s] of a sequence
     on ((n_seq,) int64; None: all slots)."""
     dr = L.direct()
     out = None if dr is None or dtype not in (torch.float16, torch.bfloat16) else dr.cache_read_q8(cache, int(dtype == torch.bfloat16), lengths)
