@@ -433,6 +433,56 @@ int blr_attention_q8(const void* q, int64_t ldq, const blr_q8_cache* cache, cons
 int blr_token_logprobs(const void* logits, int64_t ld, int64_t rows, int64_t vocab, int kind, const int64_t* ids, int top,
                        float* logprob, float* entropy, float* top_logprob, int64_t* top_ids, void* stream);
 
+/* ---- A key / value cache in pages, and the attention over it.  No counterpart in the reference.
+ * k and v are pools of pages in 16 bits, (pages, kv_heads, page, head_dim), head_dim values packed, the other strides as given (k_strides, v_strides: of a page, a head, a slot, in
+ * values; positive multiples of 8), 16-byte aligned.  Slot s of a sequence lies in page table[seq][s / page] (device int32, rows of pages_per_seq, ld_table apart); any
+ * number that is no page of the pool stands for "no page".  head_dim 64 or 128, page 16, 32, 64 or 128 (BLR_ERR_UNSUPPORTED else).
+ * start, n_new: device int64, one per sequence; a call's tokens of sequence s take slots start[s] .. start[s] + n_new[s] - 1 (n_new NULL: n_tok each).  Tokens without a place
+ * (outside the table's slots, or without a page), which the host cannot see, are dropped: they write nothing, and their rotated q is zeros.  Sequences may share pages that no call
+ * writes to; two tokens of a call in one place are the caller's mistake.  16-bit tensors of `dtype`, rows 16-byte aligned, row strides multiples of 8; any of them, the
+ * table, start and n_new too, may be written by the kernel directly ahead. */
+typedef struct blr_paged_cache {
+  void* k;
+  void* v;
+  int64_t k_strides[3], v_strides[3];
+  const int32_t* table;
+  int64_t ld_table, n_seq, pages, pages_per_seq;
+  int kv_heads, page, head_dim;
+} blr_paged_cache;
+
+/* Rotary embedding and append.  q: n_seq * n_tok rows (sequence-major) of heads * head_dim values, k and v of kv_heads * head_dim.  The angle of a
+ * token is its slot's row of cos_table / sin_table ((positions, head_dim / 2) fp32, 16-byte aligned; pairs (i, i + head_dim / 2) rotate); a slot from `positions` on counts as
+ * outside the cache.  q_out: the rotated q, zeros in rows that are no token.  fp32, one rounding.  Only the slots of the call's tokens are written. */
+int blr_rope_append_paged(const void* q, int64_t ldq, const void* k, int64_t ldk, const void* v, int64_t ldv,
+                          const float* cos_table, const float* sin_table, int64_t positions, const int64_t* start, const int64_t* n_new, int64_t n_tok, int heads,
+                          int dtype, const blr_paged_cache* cache, void* q_out, int64_t ldo, void* stream);
+
+/* Causal attention of the newest tokens: row t < n_new[s] of sequence s sits at slot start[s] + t and sees slots 0 .. start[s] + t as far as they have a page;
+ * out = softmax(scale * q . K^T) V, zeros for a row that is no token or sees nothing.  heads a multiple of kv_heads: head h reads kv head h / (heads / kv_heads).  What a row does
+ * not see has no part in it, whatever bits lie there.  scratch: blr_attention_paged_scratch_bytes (may be 0), 16-byte aligned, nothing kept in it between calls.  scale: a positive
+ * number.  ws: a workspace (NULL: none) whose status word tells of a device-side wait that ran out (blr_workspace_status); the rows concerned come out as NaN. */
+size_t blr_attention_paged_scratch_bytes(const blr_paged_cache* cache, int64_t n_tok, int heads);
+int blr_attention_paged(const void* q, int64_t ldq, const blr_paged_cache* cache, const int64_t* start, const int64_t* n_new, int64_t n_tok, int heads,
+                        float scale, int dtype, void* out, int64_t ldo, void* scratch, size_t scratch_bytes, void* ws, void* stream);
+
+/* ---- The next token of rows of logits (row stride ld; kind 0 fp16, 1 bf16, 2 fp32) from one uniform number a row (device fp32, in [0, 1)).
+ * With M the row's largest logit and T its temperature a token weighs w = exp((x - M) / T); T = 0: the first of the largest alone.  In the order of falling logits, equal
+ * ones by rising id, are kept: the first top_k (<= 0: all); of those the fewest first ones whose weights reach top_p times their sum (>= 1: all, <= 0: the first); of those the ones with
+ * w >= min(min_p, 1).  ids[r] is the least kept id for which the weights of the kept ids up to it exceed uniform[r] times the sum of all kept; logprob[r] = log(its weight / that
+ * sum).  Weights and sums in 64 bits.  uniform >= 1: the last kept id, < 0: as 0.  A row with a NaN (logit or setting), of -inf alone, or with a negative temperature has id -1
+ * and NaN; logits of -inf are never chosen, +inf ones share the row.  Settings: one for each row (device pointers, fp32, top_k int64), or, where the pointer is NULL, the number
+ * behind it for all.  A row is at most 1536 KB (BLR_ERR_UNSUPPORTED above).  No reference counterpart. */
+typedef struct blr_sampling {
+  const float* temperature;
+  const int64_t* top_k;
+  const float* top_p;
+  const float* min_p;
+  int64_t top_k_all;
+  float temperature_all, top_p_all, min_p_all;
+} blr_sampling;
+int blr_sample(const void* logits, int64_t ld, int64_t rows, int64_t vocab, int kind, const float* uniform, const blr_sampling* settings, int64_t* ids,
+               float* logprob, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

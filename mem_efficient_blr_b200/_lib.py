@@ -37,6 +37,18 @@ class Q8CacheDesc(C.Structure):
                 ("head_dim", _int), ("block", _int), ("code", _int)]
 
 
+class PagedCacheDesc(C.Structure):
+    """blr_paged_cache of include/blr_b200.h."""
+    _fields_ = [("k", _vp), ("v", _vp), ("k_strides", _i64 * 3), ("v_strides", _i64 * 3), ("table", _vp), ("ld_table", _i64), ("n_seq", _i64), ("pages", _i64),
+                ("pages_per_seq", _i64), ("kv_heads", _int), ("page", _int), ("head_dim", _int)]
+
+
+class Sampling(C.Structure):
+    """blr_sampling of include/blr_b200.h."""
+    _fields_ = [("temperature", _vp), ("top_k", _vp), ("top_p", _vp), ("min_p", _vp), ("top_k_all", _i64), ("temperature_all", C.c_float), ("top_p_all", C.c_float),
+                ("min_p_all", C.c_float)]
+
+
 ACT_NONE, ACT_SILU_MUL = 0, 1
 ACT_OUT = {None: 0, "gelu": 0x10, "gelu_tanh": 0x20}   # output activations of the fused call above 16 tokens
 
@@ -101,6 +113,10 @@ SIGNATURES = {
     "blr_attention_q8_scratch_bytes": (_sz, [C.POINTER(Q8CacheDesc), _i64, _int]),
     "blr_attention_q8": (_int, [_vp, _i64, C.POINTER(Q8CacheDesc), _vp, _vp, _i64, _int, C.c_float, _int, _vp, _i64, _vp, _sz, _vp, _vp]),
     "blr_token_logprobs": (_int, [_vp, _i64, _i64, _i64, _int, _vp, _int, _vp, _vp, _vp, _vp, _vp]),
+    "blr_rope_append_paged": (_int, [_vp, _i64, _vp, _i64, _vp, _i64, _vp, _vp, _i64, _vp, _vp, _i64, _int, _int, C.POINTER(PagedCacheDesc), _vp, _i64, _vp]),
+    "blr_attention_paged_scratch_bytes": (_sz, [C.POINTER(PagedCacheDesc), _i64, _int]),
+    "blr_attention_paged": (_int, [_vp, _i64, C.POINTER(PagedCacheDesc), _vp, _vp, _i64, _int, C.c_float, _int, _vp, _i64, _vp, _sz, _vp, _vp]),
+    "blr_sample": (_int, [_vp, _i64, _i64, _i64, _int, _vp, C.POINTER(Sampling), _vp, _vp, _vp]),
     "blr_quantize_sym": (_int, [_vp, _int, _i64, _i64, _int, _vp, _vp, _vp]),
     "blr_dequantize_sym": (_int, [_vp, _vp, _i64, _i64, _int, _i64, _int, _vp, _vp]),
 }

@@ -1,0 +1,45 @@
+// What the kernels around a key / value cache in pages share: its layout.
+#pragma once
+#include "q8.cuh"
+
+namespace blr {
+
+// Slot s of a sequence lies in page table[seq][s / page] of the pool, at place s % page; a number that is no page of the pool: nowhere.  Strides count 16-bit values.
+struct PagedView {
+  uint16_t *k, *v;
+  long long k_page, k_head, k_slot, v_page, v_head, v_slot;
+  const int* table;
+  long long ld_table;
+  int kv_heads, pages, page_log2, slots;  // slots of a sequence: those that its row of the table has pages for
+};
+
+int paged_view(const blr_paged_cache* cache, PagedView* out);  // checks the cache's description
+
+// ---- attention: what the kernels share
+struct PagedAttnParams {
+  PagedView c;
+  const uint16_t* q;
+  uint16_t* out;
+  long long ldq, ldo;
+  const long long *start, *n_new;
+  float* part;       // ns > 1: of each (sequence, kv head, row, split) hd sums, the maximum that they are taken against, the sum of the weights, 2 free
+  unsigned* status;  // NULL, or where a wait that gave up is noted
+  float scale_log2;
+  int T, H, G, rows, q_tiles, ns, n_bh, n_seq;
+  int room;  // CTAs that the SMs hold
+};
+
+// Slots that a row of token t sees.
+__device__ __forceinline__ int paged_seen(long long start, long long count, long long t, int slots) {
+  if (t >= count) return 0;
+  const long long n = min(start, (long long)slots) + t + 1;
+  return n <= 0 ? 0 : n > slots ? slots : (int)n;
+}
+// The slots that the last of rows [r0, r1) of a kv head sees: 0 where none of them is a token.
+__device__ __forceinline__ int paged_seen_by(const PagedAttnParams& p, long long start, long long count, int r0, int r1) {
+  r1 = min(r1, p.rows);
+  if (r0 >= r1 || r0 / p.G >= count) return 0;
+  return paged_seen(start, count, min((long long)((r1 - 1) / p.G), count - 1), p.c.slots);
+}
+
+}  // namespace blr

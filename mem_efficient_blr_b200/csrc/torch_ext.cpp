@@ -903,11 +903,11 @@ struct Cache8 {
 };
 
 // A number for each sequence, or (none_too) None: false when it is neither.
-bool per_sequence(const Direct& d, const Cache8& c, PyObject* o, bool none_too, const int64_t** p) {
+bool per_sequence(const Direct& d, int64_t n_seq, PyObject* o, bool none_too, const int64_t** p) {
   *p = nullptr;
   if (o == Py_None) return none_too;
   const at::Tensor* t = d.factor(o, at::kLong);
-  if (!t || t->numel() != c.c.n_seq) return false;
+  if (!t || t->numel() != n_seq) return false;
   *p = t->data_ptr<int64_t>();
   return true;
 }
@@ -925,7 +925,7 @@ PyObject* py_rope_append_q8(PyObject*, PyObject* const* a, Py_ssize_t na) {
   const at::Tensor *cs = d.factor(a[3], at::kFloat), *sn = d.factor(a[4], at::kFloat);
   for (const at::Tensor* t : {cs, sn})
     if (!t || t->dim() != 2 || t->size(0) < c.c.slots || t->size(1) != c.c.head_dim / 2) BLR_NONE();
-  if (!per_sequence(d, c, a[5], false, &start) || !per_sequence(d, c, a[7], true, &n_new) || has_derivative({d.x, dk.x, dv.x})) BLR_NONE();
+  if (!per_sequence(d, c.c.n_seq, a[5], false, &start) || !per_sequence(d, c.c.n_seq, a[7], true, &n_new) || has_derivative({d.x, dk.x, dv.x})) BLR_NONE();
   at::Tensor out = d.output(d.width);
   void* o = out.data_ptr();
   call_library([&] {
@@ -943,7 +943,7 @@ PyObject* py_attention_q8(PyObject*, PyObject* const* a, Py_ssize_t na) {
   Cache8 c;
   const int64_t *start, *n_new;
   float scale;
-  if (na != 5 || !d.take_x(a[0]) || !c.take(a[1]) || !c.rows_of(d) || !per_sequence(d, c, a[2], false, &start) || !per_sequence(d, c, a[3], true, &n_new) ||
+  if (na != 5 || !d.take_x(a[0]) || !c.take(a[1]) || !c.rows_of(d) || !per_sequence(d, c.c.n_seq, a[2], false, &start) || !per_sequence(d, c.c.n_seq, a[3], true, &n_new) ||
       !take_eps(a[4], &scale) || d.width % ((int64_t)c.c.kv_heads * c.c.head_dim) != 0 || has_derivative({d.x}))
     BLR_NONE();
   const int64_t n_tok = d.n / c.c.n_seq;
@@ -969,7 +969,7 @@ PyObject* py_cache_read_q8(PyObject*, PyObject* const* a, Py_ssize_t na) {
   const int64_t* lengths;
   if (na != 3 || !c.take(a[0]) || !take_ints(a + 1, 1, &bf16) || c10::impl::dispatch_mode_enabled() || at::impl::torch_function_mode_enabled()) BLR_NONE();
   d.dev = c.k->device().index();
-  if (d.dev != c10::cuda::current_device() || !per_sequence(d, c, a[2], true, &lengths)) BLR_NONE();
+  if (d.dev != c10::cuda::current_device() || !per_sequence(d, c.c.n_seq, a[2], true, &lengths)) BLR_NONE();
   d.st = at::cuda::getCurrentCUDAStream(d.dev).stream();
   const at::ScalarType dt = bf16 ? at::kBFloat16 : at::kHalf;
   at::Tensor k = at::detail::empty_cuda(c.k->sizes(), dt, c.k->device(), c10::nullopt), v = at::detail::empty_cuda(c.k->sizes(), dt, c.k->device(), c10::nullopt);
@@ -1010,7 +1010,138 @@ PyObject* py_token_logprobs(PyObject*, PyObject* const* a, Py_ssize_t na) {
   END_HANDLE_TH_ERRORS
 }
 
+// ops.PagedCache, a tuple (k, v, table) of tensors on one device: what the library calls a paged cache.
+struct CachePaged {
+  blr_paged_cache c = {};
+  const at::Tensor* k = nullptr;
+  bool take(PyObject* o) {
+    if (!PyTuple_Check(o) || PyTuple_GET_SIZE(o) != 3) return false;
+    const at::Tensor* t[3];
+    for (int i = 0; i < 3; ++i) {
+      t[i] = plain(PyTuple_GET_ITEM(o, i));
+      if (!t[i] || !t[i]->is_cuda() || t[i]->device() != t[0]->device()) return false;
+    }
+    k = t[0];
+    if (k->dim() != 4 || t[1]->sizes() != k->sizes() || t[1]->scalar_type() != k->scalar_type() || k->stride(3) != 1 || t[1]->stride(3) != 1) return false;
+    if (t[2]->dim() != 2 || t[2]->scalar_type() != at::kInt || t[2]->stride(1) != 1 || k->size(1) > INT_MAX || k->size(2) > INT_MAX || k->size(3) > INT_MAX) return false;
+    c.k = t[0]->data_ptr(), c.v = t[1]->data_ptr();
+    for (int i = 0; i < 3; ++i) {  // (the stride of a dimension of one means nothing)
+      c.k_strides[i] = k->size(i) > 1 ? k->stride(i) : k->size(3);
+      c.v_strides[i] = k->size(i) > 1 ? t[1]->stride(i) : k->size(3);
+    }
+    c.table = static_cast<const int32_t*>(t[2]->data_ptr());
+    c.n_seq = t[2]->size(0), c.pages = k->size(0), c.pages_per_seq = t[2]->size(1);
+    c.ld_table = c.n_seq > 1 ? t[2]->stride(0) : c.pages_per_seq;
+    c.kv_heads = (int)k->size(1), c.page = (int)k->size(2), c.head_dim = (int)k->size(3);
+    return c.n_seq > 0 && c.kv_heads > 0 && c.head_dim > 0;
+  }
+  // rows of q, of the cache's type and of whole heads, for each of its sequences
+  bool rows_of(const Direct& d) const {
+    return d.x->dim() == 2 && k->device() == d.x->device() && k->scalar_type() == d.dt && d.n % c.n_seq == 0 && d.width % c.head_dim == 0;
+  }
+};
+
+// rope_append_paged(q, k, v, cos, sin, start, cache, n_new | None)
+PyObject* py_rope_append_paged(PyObject*, PyObject* const* a, Py_ssize_t na) {
+  HANDLE_TH_ERRORS
+  Direct d, dk, dv;
+  CachePaged c;
+  const int64_t *start, *n_new;
+  if (na != 8 || !d.take_x(a[0]) || !dk.take_x(a[1]) || !dv.take_x(a[2]) || !c.take(a[6]) || !c.rows_of(d)) BLR_NONE();
+  if (dk.dt != d.dt || dv.dt != d.dt || dk.dev != d.dev || dv.dev != d.dev || dk.x->dim() != 2 || dv.x->dim() != 2 || dk.n != d.n || dv.n != d.n ||
+      dk.width != (int64_t)c.c.kv_heads * c.c.head_dim || dv.width != dk.width)
+    BLR_NONE();
+  const at::Tensor *cs = d.factor(a[3], at::kFloat), *sn = d.factor(a[4], at::kFloat);
+  for (const at::Tensor* t : {cs, sn})
+    if (!t || t->dim() != 2 || t->size(0) != cs->size(0) || t->size(1) != c.c.head_dim / 2) BLR_NONE();
+  if (!per_sequence(d, c.c.n_seq, a[5], false, &start) || !per_sequence(d, c.c.n_seq, a[7], true, &n_new) || has_derivative({d.x, dk.x, dv.x})) BLR_NONE();
+  at::Tensor out = d.output(d.width);
+  void* o = out.data_ptr();
+  call_library([&] {
+    return blr_rope_append_paged(d.x->data_ptr(), d.ldx, dk.x->data_ptr(), dk.ldx, dv.x->data_ptr(), dv.ldx, cs->data_ptr<float>(), sn->data_ptr<float>(), cs->size(0), start,
+                                 n_new, d.n / c.c.n_seq, (int)(d.width / c.c.head_dim), d.code(), &c.c, o, d.width, d.st);
+  });
+  return THPVariable_Wrap(std::move(out));
+  END_HANDLE_TH_ERRORS
+}
+
+// attention_paged(q, cache, start, n_new | None, scale)
+PyObject* py_attention_paged(PyObject*, PyObject* const* a, Py_ssize_t na) {
+  HANDLE_TH_ERRORS
+  Direct d;
+  CachePaged c;
+  const int64_t *start, *n_new;
+  float scale;
+  if (na != 5 || !d.take_x(a[0]) || !c.take(a[1]) || !c.rows_of(d) || !per_sequence(d, c.c.n_seq, a[2], false, &start) || !per_sequence(d, c.c.n_seq, a[3], true, &n_new) ||
+      !take_eps(a[4], &scale) || d.width % ((int64_t)c.c.kv_heads * c.c.head_dim) != 0 || has_derivative({d.x}))
+    BLR_NONE();
+  const int64_t n_tok = d.n / c.c.n_seq;
+  const int heads = (int)(d.width / c.c.head_dim);
+  if (scale == 0.f) scale = 1.f / std::sqrt((float)c.c.head_dim);
+  const size_t bytes = blr_attention_paged_scratch_bytes(&c.c, n_tok, heads);
+  at::Tensor out = d.output(d.width), part;
+  if (bytes > 0) part = at::detail::empty_cuda({(int64_t)bytes}, at::kByte, d.x->device(), c10::nullopt);
+  void *o = out.data_ptr(), *sp = bytes > 0 ? part.data_ptr() : nullptr;
+  call_library([&] {
+    return blr_attention_paged(d.x->data_ptr(), d.ldx, &c.c, start, n_new, n_tok, heads, scale, d.code(), o, d.width, sp, bytes, d.ws(0, 0).ptr, d.st);
+  });
+  return THPVariable_Wrap(std::move(out));
+  END_HANDLE_TH_ERRORS
+}
+
+// A setting of `sample`: a number, or one for each row; false where it is neither.
+template <typename N>
+bool setting(PyObject* o, const at::Tensor& like, at::ScalarType type, const N** each, N* all) {
+  *each = nullptr;
+  if (THPVariable_Check(o)) {
+    const at::Tensor* t = plain(o);
+    if (!t || !t->is_cuda() || t->device() != like.device() || t->scalar_type() != type || t->sizes() != like.sizes() || !t->is_contiguous() || has_derivative({t})) return false;
+    *each = t->data_ptr<N>();
+    return true;
+  }
+  if constexpr (std::is_same_v<N, float>) {
+    return take_eps(o, all);
+  } else {
+    long v;
+    if (!take_ints(&o, 1, &v)) return false;
+    *all = v;
+    return true;
+  }
+}
+
+// sample(logits (rows, vocab), uniform (rows), temperature, top_k, top_p, min_p) -> (ids, log probabilities)
+PyObject* py_sample(PyObject*, PyObject* const* a, Py_ssize_t na) {
+  HANDLE_TH_ERRORS
+  if (na != 6 || c10::impl::dispatch_mode_enabled() || at::impl::torch_function_mode_enabled()) BLR_NONE();
+  const at::Tensor *x = plain(a[0]), *u = plain(a[1]);
+  if (!x || !u || !x->is_cuda() || x->dim() != 2 || u->dim() != 1 || u->device() != x->device() || u->scalar_type() != at::kFloat || !u->is_contiguous()) BLR_NONE();
+  const int64_t rows = x->size(0), vocab = x->size(1), ld = rows > 1 ? x->stride(0) : vocab;
+  const at::ScalarType dt = x->scalar_type();
+  if (rows == 0 || vocab == 0 || u->size(0) != rows || x->stride(1) != 1 || ld < vocab || x->device().index() != c10::cuda::current_device() ||
+      (dt != at::kHalf && dt != at::kBFloat16 && dt != at::kFloat) || has_derivative({x, u}))
+    BLR_NONE();
+  blr_sampling s = {};
+  if (!setting(a[2], *u, at::kFloat, &s.temperature, &s.temperature_all) || !setting(a[3], *u, at::kLong, &s.top_k, &s.top_k_all) ||
+      !setting(a[4], *u, at::kFloat, &s.top_p, &s.top_p_all) || !setting(a[5], *u, at::kFloat, &s.min_p, &s.min_p_all) ||
+      (s.temperature == nullptr && !(s.temperature_all >= 0.f)))
+    BLR_NONE();
+  const cudaStream_t st = at::cuda::getCurrentCUDAStream(x->device().index()).stream();
+  at::Tensor ids = at::detail::empty_cuda({rows}, at::kLong, x->device(), c10::nullopt), lp = at::detail::empty_cuda({rows}, at::kFloat, x->device(), c10::nullopt);
+  int64_t* ip = ids.data_ptr<int64_t>();
+  float* pp = lp.data_ptr<float>();
+  call_library([&] { return blr_sample(x->data_ptr(), ld, rows, vocab, dt == at::kHalf ? 0 : dt == at::kBFloat16 ? 1 : 2, u->data_ptr<float>(), &s, ip, pp, st); });
+  PyObject* t = PyTuple_New(2);
+  if (t == nullptr) return nullptr;
+  PyTuple_SET_ITEM(t, 0, THPVariable_Wrap(std::move(ids)));
+  PyTuple_SET_ITEM(t, 1, THPVariable_Wrap(std::move(lp)));
+  return t;
+  END_HANDLE_TH_ERRORS
+}
+
 PyMethodDef g_methods[] = {
+    {"rope_append_paged", (PyCFunction)(void*)py_rope_append_paged, METH_FASTCALL, nullptr},
+    {"attention_paged", (PyCFunction)(void*)py_attention_paged, METH_FASTCALL, nullptr},
+    {"sample", (PyCFunction)(void*)py_sample, METH_FASTCALL, nullptr},
     {"rope_append_q8", (PyCFunction)(void*)py_rope_append_q8, METH_FASTCALL, nullptr},
     {"attention_q8", (PyCFunction)(void*)py_attention_q8, METH_FASTCALL, nullptr},
     {"cache_read_q8", (PyCFunction)(void*)py_cache_read_q8, METH_FASTCALL, nullptr},

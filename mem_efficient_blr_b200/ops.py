@@ -707,7 +707,7 @@ def _not_recorded() -> None:
     """Refuses a call that torch.jit.trace or make_fx records: they would hold the empty outputs and not the launch that fills them."""
     from torch.fx.experimental.proxy_tensor import get_proxy_mode
     if torch.jit.is_tracing() or get_proxy_mode() is not None:
-        raise RuntimeError("blr_b200: the 8-bit cache's operators and token_logprobs cannot be recorded by torch.jit.trace or make_fx; capture them in a CUDA graph")
+        raise RuntimeError("blr_b200: the operators around a cache and those on logits cannot be recorded by torch.jit.trace or make_fx; capture them in a CUDA graph")
 
 
 def _q8_desc(c: Q8Cache, x: torch.Tensor) -> "L.Q8CacheDesc":
@@ -826,3 +826,140 @@ def token_logprobs(logits: torch.Tensor, ids: torch.Tensor, top: int = 0) -> Tup
     L.check(L.load().blr_token_logprobs(x.data_ptr(), x.stride(0), rows, vocab, kind, ids.data_ptr(), top, lp.data_ptr(), ent.data_ptr(), tlp.data_ptr(),
                                         tid.data_ptr(), L.stream_ptr(dev)))
     return lp.view(lead), ent.view(lead), tlp.view(*lead, top), tid.view(*lead, top)
+
+
+# ----------------------------------------------------------------------------- key / value cache in pages, choice of the next token
+class PagedCache(NamedTuple):
+    """A layer's keys and values in pages of a common pool: k, v (pages, kv_heads, page, head_dim), fp16 or bf16, head_dim values packed, the other strides any
+    multiples of 8 (so keys and values may be parts of one tensor, or heads lie within slots); table (n_seq, pages of a sequence) int32: slot s of sequence b lies in
+    page table[b, s // page], and nowhere where that is no page of the pool.  head_dim 64 or 128, page 16, 32, 64 or 128."""
+    k: torch.Tensor
+    v: torch.Tensor
+    table: torch.Tensor
+
+    def first(self, n_seq: int) -> "PagedCache":
+        """The first n_seq sequences of the cache (views)."""
+        return PagedCache(self.k, self.v, self.table[:n_seq])
+
+
+def paged_cache(n_seq: int, kv_heads: int, pages: int, pages_per_seq: int, head_dim: int, page: int = 16, dtype: torch.dtype = torch.float16, device="cuda") -> PagedCache:
+    """An empty cache in pages (zeros), its table without a page."""
+    assert dtype in (torch.float16, torch.bfloat16) and head_dim in (64, 128) and page in (16, 32, 64, 128), "paged caches: float16 or bfloat16, heads of 64 or 128, pages of 16 to 128"
+    pool = lambda: torch.zeros(pages, kv_heads, page, head_dim, dtype=dtype, device=device)   # noqa: E731
+    return PagedCache(pool(), pool(), torch.full((n_seq, pages_per_seq), -1, dtype=torch.int32, device=device))
+
+
+def _paged_desc(c: PagedCache, x: torch.Tensor) -> "L.PagedCacheDesc":
+    _need_cuda(x)
+    for t in c[:3]:
+        if not t.is_cuda:
+            raise RuntimeError("blr_b200 operators need CUDA tensors: there is no CPU implementation in this package")
+        assert t.device == x.device, "x and the cache must live on one device"
+        assert not t.is_neg(), "a cache is written in place: no lazily negated views"
+    k, v, table = c
+    assert k.dim() == 4 and v.shape == k.shape and k.dtype == v.dtype == x.dtype, "keys and values of a paged cache are (pages, kv_heads, page, head_dim) of the rows' type"
+    assert table.dim() == 2 and table.dtype == torch.int32 and table.stride(1) == 1, "the table of a paged cache is (n_seq, pages of a sequence) int32, rows packed"
+    assert k.stride(3) == v.stride(3) == 1, "values of a head are packed"
+    pages, kv_heads, page, hd = k.shape
+    # (the stride of a dimension of one means nothing)
+    ks, vs = ([t.stride(i) if t.shape[i] > 1 else hd for i in range(3)] for t in (k, v))
+    ld = table.stride(0) if table.shape[0] > 1 else table.shape[1]
+    return L.PagedCacheDesc(k.data_ptr(), v.data_ptr(), (L.C.c_int64 * 3)(*ks), (L.C.c_int64 * 3)(*vs), table.data_ptr(), ld, table.shape[0], pages, table.shape[1],
+                            kv_heads, page, hd)
+
+
+def rope_append_paged(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cos_table: torch.Tensor, sin_table: torch.Tensor, start: torch.Tensor,
+                      cache: PagedCache, n_new=None) -> torch.Tensor:
+    """Rotary embedding and append to a cache in pages.  q (n_seq * n_tok, heads * head_dim), k and v (n_seq * n_tok, kv_heads * head_dim) rows of the cache's type,
+    sequence-major; start (n_seq,) int64: the slot of each sequence's first token, n_new (n_seq,) int64 (None: all n_tok): how many of its rows are tokens.  cos / sin tables
+    (positions, head_dim / 2) fp32.  Returns the rotated q and writes the rotated k and v to the tokens' slots, and nothing else.  Rows that are no token, and tokens whose slot has
+    no page or no angle, have zeros for q and write nothing."""
+    dr = L.direct()
+    out = None if dr is None else dr.rope_append_paged(q, k, v, cos_table, sin_table, start, cache, n_new)
+    if out is not None:
+        return out
+    _not_recorded()
+    _no_grad(q, k, v)
+    q, k, v, cos_table, sin_table = (t.resolve_neg() for t in (q, k, v, cos_table, sin_table))
+    d = _paged_desc(cache, q)
+    n_seq, kv_heads, hd = cache.table.shape[0], cache.k.shape[1], cache.k.shape[3]
+    assert all(t.dim() == 2 for t in (q, k, v)) and q.dtype == k.dtype == v.dtype and q.device == k.device == v.device, "q, k, v are rows of one dtype and device"
+    rows = q.shape[0]
+    assert n_seq > 0 and rows % n_seq == 0 and k.shape == v.shape == (rows, kv_heads * hd) and q.shape[1] % hd == 0, "q, k, v: a row for each token of each sequence"
+    for t in (cos_table, sin_table):
+        assert t.dtype == torch.float32 and t.is_contiguous() and t.dim() == 2 and t.shape[1] == hd // 2 and t.device == q.device and t.shape[0] == cos_table.shape[0], \
+            "cos / sin tables are packed (positions, head_dim / 2) fp32"
+    q2, k2, v2 = (_rows16(t, t.shape[1]) for t in (q, k, v))
+    out = torch.empty((rows, q.shape[1]), dtype=q.dtype, device=q.device)
+    L.check(L.load().blr_rope_append_paged(q2.data_ptr(), q2.stride(0), k2.data_ptr(), k2.stride(0), v2.data_ptr(), v2.stride(0), cos_table.data_ptr(),
+                                           sin_table.data_ptr(), cos_table.shape[0], _per_sequence(start, q, n_seq, "start"),
+                                           None if n_new is None else _per_sequence(n_new, q, n_seq, "n_new"), rows // n_seq, q.shape[1] // hd,
+                                           L.dtype_code(q.dtype), d, out.data_ptr(), out.shape[1], L.stream_ptr(q.device)))
+    return out
+
+
+def attention_paged(q: torch.Tensor, cache: PagedCache, start: torch.Tensor, n_new=None, scale: float = 0.0) -> torch.Tensor:
+    """Causal attention of each sequence's newest tokens over a cache in pages that holds them already: q (n_seq * n_tok, heads * head_dim) rows of the cache's type,
+    sequence-major, heads a multiple of the cache's kv_heads; row t of sequence s sits at slot start[s] + t and sees the slots up to its own that have a page; rows from n_new[s] on are
+    no tokens and come out as zeros, as does a row that sees no slot (a row behind the last slot sees all).  scale defaults to head_dim ** -0.5.  Returns
+    (rows, heads * head_dim)."""
+    dr = L.direct()
+    out = None if dr is None else dr.attention_paged(q, cache, start, n_new, scale)
+    if out is not None:
+        return out
+    _not_recorded()
+    _no_grad(q)
+    q = q.resolve_neg()
+    d = _paged_desc(cache, q)
+    n_seq, kv_heads, hd = cache.table.shape[0], cache.k.shape[1], cache.k.shape[3]
+    assert q.dim() == 2 and n_seq > 0 and q.shape[0] % n_seq == 0 and q.shape[1] % (kv_heads * hd) == 0, "q: a row for each token of each sequence"
+    q2 = _rows16(q, q.shape[1])
+    lib, n_tok, heads = L.load(), q.shape[0] // n_seq, q.shape[1] // hd
+    out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+    nbytes = lib.blr_attention_paged_scratch_bytes(d, n_tok, heads)
+    scratch = torch.empty(nbytes, dtype=torch.uint8, device=q.device) if nbytes else None
+    ws, st = _ws(q, 1, 0, 0)   # (its status word)
+    L.check(lib.blr_attention_paged(q2.data_ptr(), q2.stride(0), d, _per_sequence(start, q, n_seq, "start"),
+                                    None if n_new is None else _per_sequence(n_new, q, n_seq, "n_new"), n_tok, heads, float(scale) if scale else hd ** -0.5,
+                                    L.dtype_code(q.dtype), out.data_ptr(), out.shape[1], None if scratch is None else scratch.data_ptr(), nbytes, ws.data_ptr(), st))
+    return out
+
+
+def sample(logits: torch.Tensor, uniform: torch.Tensor, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0) -> Tuple[torch.Tensor, torch.Tensor]:
+    """The next token of each row of logits (..., vocab), fp16, bf16 or fp32, from uniform numbers in [0, 1) (...) fp32 (torch.rand): (ids, their log probabilities among what
+    was kept), int64 and fp32.  A token weighs w = exp((logit - largest) / temperature); temperature 0: the first of the largest.  In the order of falling logits, ties by rising
+    id, are kept the first top_k (0: all), of those the fewest first ones that hold top_p of their weight, of those the ones with w >= min_p; the kept tokens then share [0, 1) by
+    rising id.  Each setting is a number or a tensor of one for each row (fp32; top_k int64).  A row with a NaN, of -inf alone, or with a negative temperature has id -1 and NaN."""
+    dr = L.direct()
+    out = None if dr is None else dr.sample(logits, uniform, temperature, top_k, top_p, min_p)
+    if out is not None:
+        return out
+    _not_recorded()
+    settings = dict(temperature=temperature, top_k=top_k, top_p=top_p, min_p=min_p)
+    given = {n: t for n, t in settings.items() if torch.is_tensor(t)}
+    _no_grad(logits, uniform, *given.values())
+    logits, uniform = logits.resolve_neg(), uniform.resolve_neg()
+    _need_cuda(logits)
+    lead, dev = logits.shape[:-1], logits.device
+    assert logits.dim() >= 1 and uniform.shape == lead and uniform.dtype == torch.float32 and uniform.device == dev, "uniform: one fp32 number for each row of logits"
+    kind = {torch.float16: 0, torch.bfloat16: 1, torch.float32: 2}.get(logits.dtype)
+    assert kind is not None, f"expected float16, bfloat16 or float32 logits, got {logits.dtype}"
+    held = {}
+    for n, t in given.items():
+        want = torch.int64 if n == "top_k" else torch.float32
+        assert t.dtype == want and t.device == dev and (t.shape == lead or t.dim() == 0), f"{n}: a number, or one {want} for each row of logits on its device"
+        held[n] = t.resolve_neg().expand(lead).reshape(-1).contiguous()
+    number = lambda n, other: other if n in held else settings[n]   # noqa: E731
+    assert float(number("temperature", 0.0)) >= 0.0, "the temperature must not be negative"
+    vocab = logits.shape[-1]
+    x = logits if logits.dim() == 2 else logits.reshape(-1, vocab)
+    if x.stride(1) != 1 or (x.shape[0] > 1 and x.stride(0) < vocab):
+        x = x.contiguous()
+    rows = x.shape[0]
+    u = uniform.reshape(-1).contiguous()
+    ids, lp = torch.empty(rows, dtype=torch.int64, device=dev), torch.empty(rows, dtype=torch.float32, device=dev)
+    at = lambda n: held[n].data_ptr() if n in held else None   # noqa: E731
+    s = L.Sampling(at("temperature"), at("top_k"), at("top_p"), at("min_p"), int(number("top_k", 0)), float(number("temperature", 0.0)), float(number("top_p", 1.0)),
+                   float(number("min_p", 0.0)))
+    L.check(L.load().blr_sample(x.data_ptr(), x.stride(0), rows, vocab, kind, u.data_ptr(), s, ids.data_ptr(), lp.data_ptr(), L.stream_ptr(dev)))
+    return ids.view(lead), lp.view(lead)
