@@ -42,4 +42,8 @@ __device__ __forceinline__ int paged_seen_by(const PagedAttnParams& p, long long
   return paged_seen(start, count, min((long long)((r1 - 1) / p.G), count - 1), p.c.slots);
 }
 
+static constexpr int kPagedPromptRows = 256;  // rows of a CTA of the kernel for many
+bool paged_prompt_fits(const blr_paged_cache* cache);
+int paged_launch_prompt(const PagedAttnParams& p, const blr_paged_cache* cache, bool bf16, cudaStream_t stream);
+
 }  // namespace blr

@@ -400,7 +400,7 @@ __global__ void __launch_bounds__(256) paged_combine_kernel(const __grid_constan
 }
 
 struct PagedPlan {
-  int nt, q_tiles, ns, room;  // nt: column tiles of 8 rows; ns: CTAs that may share a row tile's keys
+  int nt, q_tiles, ns, room;  // nt: column tiles of 8 rows of the kernel here, 0: the prompt kernel; ns: CTAs that may share a row tile's keys
   long long rows, tiles;
 };
 // Few row tiles share their keys out over more CTAs, as many as the SMs hold at a time; a second kernel sums the parts.  The host does not know the sequences' lengths: a
@@ -409,14 +409,14 @@ static PagedPlan paged_plan(const blr_paged_cache* c, int64_t n_tok, int heads) 
   PagedPlan a = {};
   const int64_t slots = c->pages_per_seq * c->page;
   a.rows = n_tok * (heads / c->kv_heads);
-  a.nt = a.rows <= 8 ? 1 : a.rows <= 16 ? 2 : 4;
-  const int per = 8 * a.nt;
+  a.nt = a.rows <= 8 ? 1 : a.rows <= 16 ? 2 : a.rows <= 32 || !paged_prompt_fits(c) ? 4 : 0;
+  const int per = a.nt ? 8 * a.nt : kPagedPromptRows;
   a.q_tiles = (int)((a.rows + per - 1) / per);
   a.tiles = c->n_seq * c->kv_heads * a.q_tiles;
-  a.room = (c->head_dim == 64 && a.nt < 4 ? 4 : 2) * sm_count();
+  a.room = (a.nt == 0 ? 1 : c->head_dim == 64 && a.nt < 4 ? 4 : 2) * sm_count();
   long long ns = a.tiles > 0 ? a.room / a.tiles : 1;
-  const long long most = (slots + 127) / 128;  // at least 128 keys for a CTA
-  if (ns > 1 && c->n_seq > 1) ns += ns / 2;
+  const long long least = a.nt ? 128 : 512, most = (slots + least - 1) / least;  // keys of a CTA
+  if (a.nt && ns > 1 && c->n_seq > 1) ns += ns / 2;
   if (slots <= 512) ns = 1;
   if (ns > most) ns = most;
   a.ns = ns < 1 ? 1 : ns > kPagedMaxSplits ? kPagedMaxSplits : (int)ns;
@@ -478,11 +478,15 @@ int blr_attention_paged(const void* q, int64_t ldq, const blr_paged_cache* cache
   const cudaStream_t st = static_cast<cudaStream_t>(stream);
   const bool bf = dtype == BLR_DTYPE_BF16;
   const long long ctas = a.tiles * a.ns;
+  if (a.nt == 0) {
+    rc = paged_launch_prompt(p, cache, bf, st);
+  } else {
 #define BLR_PAGED(BF, HD) \
   (a.nt == 1 ? launch_paged_few<BF, HD, 1>(p, ctas, st) : a.nt == 2 ? launch_paged_few<BF, HD, 2>(p, ctas, st) : launch_paged_few<BF, HD, 4>(p, ctas, st))
-  if (cache->head_dim == 128) rc = bf ? BLR_PAGED(true, 128) : BLR_PAGED(false, 128);
-  else rc = bf ? BLR_PAGED(true, 64) : BLR_PAGED(false, 64);
+    if (cache->head_dim == 128) rc = bf ? BLR_PAGED(true, 128) : BLR_PAGED(false, 128);
+    else rc = bf ? BLR_PAGED(true, 64) : BLR_PAGED(false, 64);
 #undef BLR_PAGED
+  }
   if (rc || a.ns == 1) return rc;
   const long long total = cache->n_seq * cache->kv_heads * a.rows;
   const dim3 cgrid((unsigned)((total + 7) / 8));

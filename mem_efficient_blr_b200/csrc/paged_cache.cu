@@ -13,7 +13,7 @@ int paged_view(const blr_paged_cache* c, PagedView* out) {
   BLR_REQUIRE(c->n_seq >= 0 && c->pages >= 0 && c->kv_heads > 0 && c->pages_per_seq > 0, BLR_ERR_ARG, "a paged cache needs kv_heads and a table of pages");
   BLR_REQUIRE(c->head_dim == 64 || c->head_dim == 128, BLR_ERR_UNSUPPORTED, "paged caches have heads of 64 or 128 values, got %d", c->head_dim);
   BLR_REQUIRE(c->page == 16 || c->page == 32 || c->page == 64 || c->page == 128, BLR_ERR_UNSUPPORTED, "a paged cache has pages of 16, 32, 64 or 128 slots, got %d", c->page);
-  BLR_REQUIRE(c->n_seq * c->kv_heads < (1ll << 31) && c->pages < (1ll << 31) && c->pages_per_seq < (1ll << 31) / c->page, BLR_ERR_SHAPE, "a paged cache of too many pages or sequences");
+  BLR_REQUIRE(c->n_seq * c->kv_heads < (1ll << 31) && c->pages < (1ll << 31) && c->pages_per_seq <= (1ll << 30) / c->page, BLR_ERR_SHAPE, "a paged cache of too many pages or sequences");
   BLR_REQUIRE(c->n_seq <= 1 || c->ld_table >= c->pages_per_seq, BLR_ERR_ARG, "the table's rows overlap");
   for (const int64_t* s : {c->k_strides, c->v_strides})
     for (int i = 0; i < 3; ++i) BLR_REQUIRE(s[i] > 0 && s[i] % 8 == 0, BLR_ERR_ARG, "a paged cache's strides are positive multiples of 8 values");
