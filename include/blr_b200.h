@@ -471,7 +471,7 @@ int blr_attention_paged(const void* q, int64_t ldq, const blr_paged_cache* cache
  * w >= min(min_p, 1).  ids[r] is the least kept id for which the weights of the kept ids up to it exceed uniform[r] times the sum of all kept; logprob[r] = log(its weight / that
  * sum).  Weights and sums in 64 bits.  uniform >= 1: the last kept id, < 0: as 0.  A row with a NaN (logit or setting), of -inf alone, or with a negative temperature has id -1
  * and NaN; logits of -inf are never chosen, +inf ones share the row.  Settings: one for each row (device pointers, fp32, top_k int64), or, where the pointer is NULL, the number
- * behind it for all.  A row is at most 1536 KB (BLR_ERR_UNSUPPORTED above).  No reference counterpart. */
+ * behind it for all.  A row is at most 4 MB (BLR_ERR_UNSUPPORTED above).  No reference counterpart. */
 typedef struct blr_sampling {
   const float* temperature;
   const int64_t* top_k;

@@ -67,7 +67,7 @@ def test_arguments_of_the_choice(L):
         return f(logits, ld, rows, vocab, kind, u, L.Sampling(*s.values()), ids, P, None)
 
     assert call(kind=3) == ARG and call(ld=99) == ARG and call(vocab=0) == ARG and call(rows=-1) == ARG
-    assert call(vocab=800000, ld=800000) == UNSUPPORTED and call(vocab=400000, ld=400000, kind=2) == UNSUPPORTED and call(logits=P + 1) == ARG
+    assert call(vocab=2097153, ld=2097153) == UNSUPPORTED and call(vocab=1048577, ld=1048577, kind=2) == UNSUPPORTED and call(logits=P + 1) == ARG
     assert call(logits=None) == ARG and call(ids=None) == ARG and call(u=None) == ARG and f(P, 100, 2, 100, 0, P, None, P, P, None) == ARG
     assert call(temperature_all=-1.0) == ARG and call(temperature_all=math.nan) == ARG and call(top_p_all=math.nan) == ARG and call(min_p_all=math.nan) == ARG
     assert call(rows=0, logits=None) == 0
