@@ -348,20 +348,29 @@ class LlamaLayer(nn.Module):
         return x
 
     def forward_q8(self, x, tables, cache, start, n_new=None, kernels: bool = True):
-        """The layer on an 8-bit cache (ops.Q8Cache): x (B, T, d), the next T tokens of each sequence from slot start[b] on, of which the first n_new[b]
-        (None: all) are tokens.  kernels = False reads the cache back and leaves the attention to torch."""
+        """The layer on an 8-bit cache (ops.Q8Cache) or one in pages (ops.PagedCache): x (B, T, d), the next T tokens of each sequence from slot start[b] on, of which the
+        first n_new[b] (None: all) are tokens.  kernels = False reads the cache back and leaves the attention to torch."""
         from . import ops
         B, T, d = x.shape
+        paged = isinstance(cache, ops.PagedCache)
         h = self.input_layernorm(x)
         q, k, v = (t.view(B * T, d) for t in structured_multi([self.q_proj, self.k_proj, self.v_proj], h))
-        q = ops.rope_append_q8(q, k, v, tables[0], tables[1], start, cache, n_new)
+        q = (ops.rope_append_paged if paged else ops.rope_append_q8)(q, k, v, tables[0], tables[1], start, cache, n_new)
         if kernels:
-            a = ops.attention_q8(q, cache, start, n_new)
+            a = (ops.attention_paged if paged else ops.attention_q8)(q, cache, start, n_new)
         else:
-            slots = cache.k.shape[2]
             last = start[:, None] + torch.arange(T, device=x.device)   # (slots behind a row's own are masked, and zeros where nobody wrote)
-            kc, vc = ops.cache_read_q8(cache, x.dtype, start + (T if n_new is None else n_new))
-            seen = torch.arange(slots, device=x.device) <= last[..., None]
+            if paged:
+                there = cache.table >= 0
+                kc, vc = (t[cache.table.clamp(min=0).long()].transpose(1, 2).reshape(B, self.heads, -1, self.hd) for t in cache[:2])
+                written = torch.arange(kc.shape[2], device=x.device) < (start + (T if n_new is None else n_new))[:, None]
+                written &= there.repeat_interleave(cache.k.shape[2], 1)
+                kc, vc = (t.masked_fill(~written[:, None, :, None], 0) for t in (kc, vc))
+            else:
+                kc, vc = ops.cache_read_q8(cache, x.dtype, start + (T if n_new is None else n_new))
+            seen = torch.arange(kc.shape[2], device=x.device) <= last[..., None]
+            if paged:
+                seen = seen & written[:, None]
             a = F.scaled_dot_product_attention(q.view(B, T, self.heads, self.hd).transpose(1, 2), kc, vc, attn_mask=seen[:, None]).transpose(1, 2)
         (x,) = structured_multi([self.o_proj], a.reshape(B, T, d), residual=x)
         h = self.post_attention_layernorm(x)
@@ -402,10 +411,12 @@ class LlamaLayer(nn.Module):
 class LlamaDecoder(nn.Module):
     """Decoder of the shape above with a static cache for `cache_len` positions and `batch` sequences.  kv_cache "int8" or "e4m3": the cache in 8 bits with
     a scale for each kv_block slots and head (ops.Q8Cache; CUDA, heads of 64 or 128), which a token attends to up to its own slot; sequences may then be
-    at different positions (`extend`).  None: in the activations' 16-bit type."""
+    at different positions (`extend`, `generate`).  "paged": the same in the activations' 16-bit type, in pages of kv_block slots out of kv_pages for all sequences
+    (ops.PagedCache), which `reserve` gives to sequences and `release` takes back; kv_pages None: every sequence has its pages from the beginning.  None: a static cache in the
+    activations' 16-bit type."""
 
     def __init__(self, shape: LlamaShape, method: str, batch: int, cache_len: int, device="cuda", dtype=torch.float16, seed=0,
-                 init_on_device: bool = False, kv_cache: Optional[str] = None, kv_block: int = 16):
+                 init_on_device: bool = False, kv_cache: Optional[str] = None, kv_block: int = 16, kv_pages: Optional[int] = None):
         super().__init__()
         g = torch.Generator(device=device if init_on_device else "cpu").manual_seed(seed)
         self.shape, self.method, self.batch, self.cache_len = shape, method, batch, cache_len
@@ -424,7 +435,19 @@ class LlamaDecoder(nn.Module):
         self.register_buffer("cos", ang.cos().to(device), persistent=False)
         self.register_buffer("sin", ang.sin().to(device), persistent=False)
         self.q8cache = None
-        if kv_cache is not None:
+        self.paged = None
+        if kv_pages is not None and kv_cache != "paged":
+            raise ValueError("kv_pages is for a cache in pages (kv_cache='paged')")
+        if kv_cache == "paged":
+            from . import ops
+            each = -(-cache_len // kv_block)
+            self.kv_pages, self.kv_page = batch * each if kv_pages is None else kv_pages, kv_block
+            self.page_table = torch.full((batch, each), -1, dtype=torch.int32, device=device)   # (the layers' caches share it)
+            self.paged = [ops.paged_cache(batch, shape.heads, self.kv_pages, each, hd, kv_block, dtype, device)._replace(table=self.page_table) for _ in range(shape.layers)]
+            self._pages, self._free = [[] for _ in range(batch)], list(range(self.kv_pages))[::-1]
+            if kv_pages is None:
+                self.reserve([cache_len] * batch)
+        elif kv_cache is not None:
             from . import ops
             codes = {"int8": torch.int8, "e4m3": torch.float8_e4m3fn}.get(kv_cache)
             if codes is None:
@@ -437,21 +460,60 @@ class LlamaDecoder(nn.Module):
     def structured_linears(self):
         return [m for layer in self.layers for m in layer.structured()]
 
+    def reserve(self, lengths) -> None:
+        """Pages for the first lengths[b] slots of sequence b (one number for each of the first sequences), out of those that are free; what a sequence has stays.  Raises
+        where there are too few, and then nothing has changed.  The table is written behind what the current stream has been given so far."""
+        if self.paged is None:
+            raise RuntimeError("reserve needs a decoder with a cache in pages (kv_cache='paged')")
+        lengths = [int(n) for n in lengths]
+        if len(lengths) > self.batch or any(n < 0 or n > self.cache_len for n in lengths):
+            raise ValueError(f"lengths of at most {self.batch} sequences, up to {self.cache_len} slots each")
+        more = [max(0, -(-n // self.kv_page) - len(have)) for n, have in zip(lengths, self._pages)]
+        if sum(more) > len(self._free):
+            raise RuntimeError(f"{sum(more)} more pages are needed, {len(self._free)} are free")
+        for b, n in enumerate(more):
+            if n:
+                have = self._pages[b]
+                new = [self._free.pop() for _ in range(n)]
+                self.page_table[b, len(have):len(have) + n] = torch.tensor(new, dtype=torch.int32).to(self.page_table.device)
+                have.extend(new)
+
+    def release(self, sequences) -> None:
+        """Takes back the pages of these sequences (their numbers in the batch)."""
+        if self.paged is None:
+            raise RuntimeError("release needs a decoder with a cache in pages (kv_cache='paged')")
+        for b in sequences:
+            if not 0 <= b < self.batch:
+                raise ValueError(f"there is no sequence {b}")
+            self._free.extend(reversed(self._pages[b]))
+            self._pages[b] = []
+            self.page_table[b].fill_(-1)
+
+    def _caches(self):
+        """The caches of sequences at positions of their own, one for each layer; None: the static cache."""
+        return self.paged if self.paged is not None else self.q8cache
+
     def _hidden_q8(self, ids, start, n_new=None):
         self._fit(ids)
         x, B = self.embed_tokens(ids), ids.shape[0]
-        for layer, cache in zip(self.layers, self.q8cache):
+        for layer, cache in zip(self.layers, self._caches()):
             x = layer.forward_q8(x, (self.cos, self.sin), cache.first(B), start, n_new, self.fused_decode)
         return x
 
     def _run(self, ids, pos, causal):
         logits = self.lm_head(self.norm(self._hidden(ids, pos, causal)[:, -1]))
-        return logits if self.q8cache is None or causal else self._nan_outside(logits, pos, ids.shape[1])
+        return logits if self._caches() is None or causal else self._nan_outside(logits, pos, ids.shape[1])
 
     def _nan_outside(self, logits, start, n):
-        """NaN for sequences whose n tokens from `start` on do not all lie in the 8-bit cache: those outside are written nowhere, and the host, which does not
+        """NaN for sequences whose n tokens from `start` on do not all have a place in the cache: those outside are written nowhere, and the host, which does not
         see the positions, cannot refuse them."""
-        return logits.masked_fill_((start.clamp(min=0).clamp(max=self.cache_len - n) != start)[:, None], float("nan"))
+        outside = start.clamp(min=0).clamp(max=self.cache_len - n) != start
+        if self.paged is not None:
+            table = self.page_table[:logits.shape[0]]
+            at = torch.arange(table.shape[1], device=start.device) * self.kv_page
+            first, end = start.clamp(0, self.cache_len), (start.clamp(0, self.cache_len) + n).clamp(max=self.cache_len)
+            outside = outside | ((table < 0) & (at + self.kv_page > first[:, None]) & (at < end[:, None])).any(1)
+        return logits.masked_fill_(outside[:, None], float("nan"))
 
     def _fit(self, ids):
         if ids.shape[1] > self.cache_len:
@@ -459,8 +521,10 @@ class LlamaDecoder(nn.Module):
 
     def _hidden(self, ids, pos, causal):
         self._fit(ids)
-        if self.q8cache is not None:
+        if self._caches() is not None:
             B = ids.shape[0]
+            if self.paged is not None and causal:
+                self.reserve([ids.shape[1]] * B)
             return self._hidden_q8(ids, pos.new_zeros(B) if causal else pos if pos.numel() == B else pos.expand(B).contiguous())
         x = self.embed_tokens(ids)
         B = ids.shape[0]   # a smaller batch than the cache was built for uses the first B sequences' slots
@@ -491,15 +555,48 @@ class LlamaDecoder(nn.Module):
 
     @torch.no_grad()
     def extend(self, ids: torch.Tensor, start: torch.Tensor, n_new: Optional[torch.Tensor] = None) -> torch.Tensor:
-        """The next tokens of sequences at different positions, on an 8-bit cache: ids (B, T) go to slots start[b] .. (start (B,) int64), of each row the
+        """The next tokens of sequences at different positions, on an 8-bit cache or one in pages: ids (B, T) go to slots start[b] .. (start (B,) int64), of each row the
         first n_new[b] ((B,) int64; None: all).  Returns the logits behind each sequence's last new token (B, vocab); those of a sequence without a new
         token mean nothing, and those of one with a token outside the cache are NaN."""
-        if self.q8cache is None:
-            raise RuntimeError("extend needs a decoder with an 8-bit cache (kv_cache='int8' or 'e4m3')")
+        if self._caches() is None:
+            raise RuntimeError("extend needs a decoder with an 8-bit cache or one in pages (kv_cache='int8', 'e4m3' or 'paged')")
         x = self._hidden_q8(ids, start, n_new)
         last = x[:, -1] if n_new is None else x[torch.arange(ids.shape[0], device=ids.device), (n_new - 1).clamp(0, ids.shape[1] - 1)]
         T = ids.shape[1]
         return self._nan_outside(self.lm_head(self.norm(last)), start, T if n_new is None else n_new.clamp(0, T))
+
+    @torch.no_grad()
+    def generate(self, ids: torch.Tensor, new_tokens: int, uniform: Optional[torch.Tensor] = None, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0,
+                 n_new: Optional[torch.Tensor] = None):
+        """Goes on from prompts ids (B, T), of each row the first n_new[b] ((B,) int64; None: all), by new_tokens tokens, each chosen as ops.sample does from its
+        uniform number (B, new_tokens) fp32 (None: torch.rand) with these settings.  On an 8-bit cache or one in pages, whose first B sequences it begins anew.  Returns (ids, log probabilities),
+        (B, new_tokens) each; a sequence that does not fit the cache has id -1 and NaN from there on."""
+        from . import ops
+        if self._caches() is None:
+            raise RuntimeError("generate needs a decoder with an 8-bit cache or one in pages (kv_cache='int8', 'e4m3' or 'paged')")
+        B, T = ids.shape
+        if uniform is None:
+            uniform = torch.rand(B, new_tokens, device=ids.device)
+        if uniform.shape != (B, new_tokens):
+            raise ValueError(f"uniform: a number for each of {new_tokens} tokens of {B} sequences")
+        if self.paged is not None:
+            self.reserve([min(T + new_tokens, self.cache_len)] * B)
+        pos = ids.new_zeros(B) if n_new is None else n_new
+        pos = pos + T if n_new is None else pos.clamp(0, T)
+        chosen, logprobs, each = [], [], uniform.t().contiguous()
+        logits = self.extend(ids, torch.zeros_like(pos), n_new)
+        for i in range(new_tokens):
+            token, lp = ops.sample(logits, each[i], temperature, top_k, top_p, min_p)
+            chosen.append(token)
+            logprobs.append(lp)
+            if i + 1 < new_tokens:
+                # (a sequence without a token has NaN for its logits from here on: the position that its next one would have is outside the cache)
+                pos = torch.where(token < 0, -1, pos)
+                logits = self.decode_step(token.clamp(min=0)[:, None], pos)
+                pos = torch.where(pos < 0, pos, pos + 1)
+        if not chosen:
+            return ids.new_zeros(B, 0), uniform
+        return torch.stack(chosen, 1), torch.stack(logprobs, 1)
 
     @torch.no_grad()
     def score(self, ids: torch.Tensor, top: int = 0):
