@@ -48,7 +48,7 @@ __device__ __forceinline__ bool no_number2(uint32_t w) {  // either half of the 
 }
 
 template <bool BF16, int HD, int NT>
-__global__ void __launch_bounds__(kFewThreads, HD == 64 && NT < 4 ? 4 : 2) paged_attention_kernel(const __grid_constant__ PagedAttnParams p) {
+__global__ void __launch_bounds__(kFewThreads, HD == 64 && NT < 3 ? 4 : 2) paged_attention_kernel(const __grid_constant__ PagedAttnParams p) {
   constexpr int kSteps = HD / 16, kRows = 8 * NT, kPitch = HD + 4, kPieces = HD / 8, kGroup = 64 * HD, kHalf = 32 * HD;  // bytes of a group, of its keys
   constexpr bool kQShared = NT > 2;
   extern __shared__ __align__(128) uint8_t ring[];
@@ -62,25 +62,10 @@ __global__ void __launch_bounds__(kFewThreads, HD == 64 && NT < 4 ? 4 : 2) paged
   asm volatile("griddepcontrol.wait;" ::: "memory");
   const long long start = p.start[b], count = p.n_new == nullptr ? p.T : min((long long)p.T, p.n_new[b]);
   const int keys = paged_seen_by(p, start, count, r0, r0 + kRows);
-  int share = keys;
-  if (p.ns > 1 && p.n_seq == 1) {
-    share = ((keys + p.ns - 1) / p.ns + 16 * kFewWarps - 1) / (16 * kFewWarps) * (16 * kFewWarps);
-  } else if (p.ns > 1) {
-    // as many keys for every CTA, whatever its sequence's length: all of them over the CTAs that the SMs hold, but a sequence has no more than ns CTAs
-    float total = 0.f;
-    for (int i = lane; i < p.n_seq; i += 32) {
-      const long long n = p.n_new == nullptr ? p.T : min((long long)p.T, p.n_new[i]);
-      total += (float)paged_seen_by(p, p.start[i], n, 0, p.rows);
-    }
-#pragma unroll
-    for (int d = 16; d > 0; d >>= 1) total += __shfl_xor_sync(0xffffffffu, total, d);
-    const float even = total * (float)(p.c.kv_heads * p.q_tiles) / (float)p.room;
-    const int n = max(1, min(p.ns, (int)((float)keys / fmaxf(even, 1.f))));  // (rounded down: all of them together are no more than the SMs hold)
-    share = ((keys + n - 1) / n + 16 * kFewWarps - 1) / (16 * kFewWarps) * (16 * kFewWarps);
-  }
+  const int share = p.ns > 1 ? paged_share(p, keys, kRows, kRows, 0, 16 * kFewWarps, lane) : max(keys, 1);
   const int k0 = (int)min((long long)keys, (long long)split * share), k1 = min(keys, k0 + min(share, keys - k0));
   if (p.ns > 1 && k0 >= k1) {  // no keys for this CTA: its rows say so
-    if (threadIdx.x < kRows && r0 + threadIdx.x < p.rows)
+    if (threadIdx.x < kRows && r0 + (int)threadIdx.x < p.rows)
       *reinterpret_cast<float2*>(p.part + (((long long)bh * p.rows + r0 + threadIdx.x) * p.ns + split) * (HD + 4) + HD) = make_float2(-INFINITY, 0.f);
     return;
   }
@@ -381,6 +366,7 @@ __global__ void __launch_bounds__(256) paged_combine_kernel(const __grid_constan
 #pragma unroll 8
   for (int s = 0; s < p.ns; ++s) {
     const float ws = __shfl_sync(0xffffffffu, s < 32 ? w[0] : w[1], s & 31);
+    if (ws < 0.f) continue;
     float x[HD / 32];
     if constexpr (HD == 128) {
       const float4 v = *reinterpret_cast<const float4*>(from + s * (HD + 4) + 4 * lane);
@@ -390,7 +376,7 @@ __global__ void __launch_bounds__(256) paged_combine_kernel(const __grid_constan
       x[0] = v.x, x[1] = v.y;
     }
 #pragma unroll
-    for (int i = 0; i < HD / 32; ++i) sum[i] += ws < 0.f ? 0.f : x[i] * ws;
+    for (int i = 0; i < HD / 32; ++i) sum[i] += x[i] * ws;
   }
   const float inv = 1.f / L;
   const long long bh = row / p.rows, r = row - bh * p.rows, b = bh / p.c.kv_heads, h = bh - b * p.c.kv_heads, tok = r / p.G;
@@ -404,19 +390,19 @@ struct PagedPlan {
   long long rows, tiles;
 };
 // Few row tiles share their keys out over more CTAs, as many as the SMs hold at a time; a second kernel sums the parts.  The host does not know the sequences' lengths: a
-// tile may have half as many CTAs again as its even share, and the kernel shares by the lengths.
+// tile may have twice its even share of CTAs and one, and the kernels share by the lengths (paged_share); CTAs that are left over say so and end.
 static PagedPlan paged_plan(const blr_paged_cache* c, int64_t n_tok, int heads) {
   PagedPlan a = {};
   const int64_t slots = c->pages_per_seq * c->page;
   a.rows = n_tok * (heads / c->kv_heads);
-  a.nt = a.rows <= 8 ? 1 : a.rows <= 16 ? 2 : a.rows <= 32 || !paged_prompt_fits(c) ? 4 : 0;
+  a.nt = a.rows <= 8 ? 1 : a.rows <= 16 ? 2 : a.rows <= 24 ? 3 : a.rows <= 32 || !paged_prompt_fits(c) ? 4 : 0;
   const int per = a.nt ? 8 * a.nt : kPagedPromptRows;
   a.q_tiles = (int)((a.rows + per - 1) / per);
   a.tiles = c->n_seq * c->kv_heads * a.q_tiles;
-  a.room = (a.nt == 0 ? 1 : c->head_dim == 64 && a.nt < 4 ? 4 : 2) * sm_count();
+  a.room = (a.nt == 0 ? 1 : c->head_dim == 64 && a.nt < 3 ? 4 : 2) * sm_count();
   long long ns = a.tiles > 0 ? a.room / a.tiles : 1;
   const long long least = a.nt ? 128 : 512, most = (slots + least - 1) / least;  // keys of a CTA
-  if (a.nt && ns > 1 && c->n_seq > 1) ns += ns / 2;
+  if (ns > 1 && (c->n_seq > 1 || a.q_tiles > 1)) ns = 2 * ns + 1;
   if (slots <= 512) ns = 1;
   if (ns > most) ns = most;
   a.ns = ns < 1 ? 1 : ns > kPagedMaxSplits ? kPagedMaxSplits : (int)ns;
@@ -482,7 +468,7 @@ int blr_attention_paged(const void* q, int64_t ldq, const blr_paged_cache* cache
     rc = paged_launch_prompt(p, cache, bf, st);
   } else {
 #define BLR_PAGED(BF, HD) \
-  (a.nt == 1 ? launch_paged_few<BF, HD, 1>(p, ctas, st) : a.nt == 2 ? launch_paged_few<BF, HD, 2>(p, ctas, st) : launch_paged_few<BF, HD, 4>(p, ctas, st))
+  (a.nt == 1 ? launch_paged_few<BF, HD, 1>(p, ctas, st) : a.nt == 2 ? launch_paged_few<BF, HD, 2>(p, ctas, st) : a.nt == 3 ? launch_paged_few<BF, HD, 3>(p, ctas, st) : launch_paged_few<BF, HD, 4>(p, ctas, st))
     if (cache->head_dim == 128) rc = bf ? BLR_PAGED(true, 128) : BLR_PAGED(false, 128);
     else rc = bf ? BLR_PAGED(true, 64) : BLR_PAGED(false, 64);
 #undef BLR_PAGED

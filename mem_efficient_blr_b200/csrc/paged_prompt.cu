@@ -97,8 +97,9 @@ __device__ __forceinline__ Place place_of(const PagedAttnParams& p) {
   int cta;
   asm volatile("mov.u32 %0, %%ctaid.x;" : "=r"(cta));
   Place a;
-  const int tile = cta / p.ns;
-  a.split = cta - tile * p.ns;
+  const int tiles = p.n_bh * p.q_tiles;
+  a.split = cta / tiles;
+  const int tile = cta - a.split * tiles;
   a.bh = tile % p.n_bh;
   a.r0 = (p.q_tiles - 1 - tile / p.n_bh) * kRows;  // the last rows have the most keys: their CTAs come first
   a.b = a.bh / p.c.kv_heads;
@@ -139,21 +140,13 @@ __global__ void __launch_bounds__(kPromptThreads, 1) paged_prompt_kernel(const _
     }
     mbar_init_fence();
   }
-  if (warp == 8) tmem_alloc(smem_u32(&tmem_slot), 512);
-
+  __syncthreads();  // (the barriers are there)
   asm volatile("griddepcontrol.wait;" ::: "memory");
   int k0, k1, n0, n1, lim = 0, clean0;  // clean0: the first tile that not all rows see
   const int wg = warp >> 2;
   {
     const Place at = place_of(p);
     const long long start = p.start[at.b], count = p.n_new == nullptr ? p.T : min((long long)p.T, p.n_new[at.b]);
-    const int keys0 = paged_seen_by(p, start, count, at.r0, at.r0 + 128), keys1 = paged_seen_by(p, start, count, at.r0 + 128, at.r0 + 256);
-    const int keys = max(keys0, keys1), share = ((keys + p.ns - 1) / p.ns + kKeys - 1) / kKeys * kKeys;
-    k0 = (int)min((long long)keys, (long long)at.split * share), k1 = min(keys, k0 + min(share, keys - k0));
-    n0 = max(0, min(keys0, k1) - k0 + kStepKeys - 1) / kStepKeys;
-    n1 = max(0, min(keys1, k1) - k0 + kStepKeys - 1) / kStepKeys;
-    clean0 = max(0, max(1, paged_seen(start, count, at.r0 / p.G, p.c.slots)) - k0) / kKeys;
-
     // ---- a softmax thread's row of q
     const int row_i = (int)threadIdx.x & 127, r = at.r0 + (int)threadIdx.x;
     if (warp < 8) {
@@ -169,10 +162,24 @@ __global__ void __launch_bounds__(kPromptThreads, 1) paged_prompt_kernel(const _
       }
       fence_proxy_async_smem();
     }
+    const int keys0 = paged_seen_by(p, start, count, at.r0, at.r0 + 128), keys1 = paged_seen_by(p, start, count, at.r0 + 128, at.r0 + 256);
+    const int keys = max(keys0, keys1), share = p.ns > 1 ? paged_share(p, keys, p.rows - at.r0, kRows, kRows / 2, kKeys, lane) : max(keys, 1);
+    k0 = (int)min((long long)keys, (long long)at.split * share), k1 = min(keys, k0 + min(share, keys - k0));
+    if (p.ns > 1 && k0 >= k1) {  // no keys for this CTA: its rows say so
+      const int r = at.r0 + (int)threadIdx.x;
+      if ((int)threadIdx.x < kRows && r < p.rows) *reinterpret_cast<float2*>(p.part + (((long long)at.bh * p.rows + r) * p.ns + at.split) * (HD + 4) + HD) = make_float2(-INFINITY, 0.f);
+      return;
+    }
+    n0 = max(0, min(keys0, k1) - k0 + kStepKeys - 1) / kStepKeys;
+    n1 = max(0, min(keys1, k1) - k0 + kStepKeys - 1) / kStepKeys;
+    clean0 = max(0, max(1, paged_seen(start, count, at.r0 / p.G, p.c.slots)) - k0) / kKeys;
   }
-  tc_fence_before();
-  __syncthreads();
-  tc_fence_after();
+  if (warp == 8) tmem_alloc(smem_u32(&tmem_slot), 512);
+  if (warp < 9) {  // (q and the room in TMEM; the copies begin meanwhile)
+    tc_fence_before();
+    asm volatile("bar.sync 2, 288;" ::: "memory");
+    tc_fence_after();
+  }
   const uint32_t tmem = tmem_slot;
   const int halves = max(n0, n1), steps = (halves + 1) / 2;  // (n0, n1, halves: of 64 keys; steps: tiles of 128)
 
