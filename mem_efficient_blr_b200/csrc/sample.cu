@@ -37,6 +37,7 @@ struct SampleParams {
   long long* ids;
   float* logprob;
   int vocab, chunks;  // chunks: of 32 vectors of 16 bytes, that a row can have
+  double series[5];   // log(2) / 32 to the powers 1 to 4 over their factorials; 1.5 2^52
 };
 
 struct SampleSum {
@@ -53,7 +54,7 @@ struct SampleShared {
       double upto[kListed];  // sums over what is sorted
     };
     int hist[kBins];
-    uint32_t groups[THREADS];
+    uint32_t groups[33 * kWarps];  // (a warp's 32 a word apart from the next one's: lane i reads warp i's)
   };
   double table[32];  // 2^(j / 32)
   SampleSum warp[2][kWarps];
@@ -64,18 +65,18 @@ struct SampleShared {
 
 // e^((x - M) / T) in 64 bits to 2^-39 of itself: 2^(n / 32) from the table times the Taylor series of 2^(r / 32), |r| <= 1/2, up to the fourth power.  Exactly 1 at M; for x above `low`,
 // which is next below M, or where e^-700 is.  (A call of exp has three times the instructions, and they are what bounds a row that is summed as a whole.)
+// (The series' numbers come as the kernel's parameters, where an instruction reads them: as literals each takes two more.)
 struct Weight {
   float low;
   double most, c;  // 32 log2(e) / T
-  const double* table;
+  const double *table, *series;
   __device__ __forceinline__ double operator()(float x) const {
-    const double d = (double)x - most, s = fma(d, c, 6755399441055744.0);  // 1.5 2^52: whole numbers end in the last bits
+    const double d = (double)x - most, s = fma(d, c, series[4]);  // 1.5 2^52: whole numbers end in the last bits
     const int n = __double2loint(s);
-    const double r = fma(d, c, -(s - 6755399441055744.0));
-    constexpr double q = 0.69314718055994530942 / 32.0;
-    double e = fma(r, q * q * q * q / 24.0, q * q * q / 6.0);
-    e = fma(r, e, q * q / 2.0);
-    e = fma(r, e, q);
+    const double r = fma(d, c, -(s - series[4]));
+    double e = fma(r, series[3], series[2]);
+    e = fma(r, e, series[1]);
+    e = fma(r, e, series[0]);
     e = fma(r, e, 1.0) * table[n & 31];
     return __hiloint2double(__double2hiint(e) + ((n & ~31) << 15), __double2loint(e));
   }
@@ -144,21 +145,27 @@ struct SampleRow {
     }
     return make_uint4(x[0], x[1], x[2], x[3]);
   }
-  __device__ __forceinline__ uint4 vec(int i) const {
+  // inner: known not to be the first or the last
+  __device__ __forceinline__ uint4 load_inner(int i) const { return reinterpret_cast<const uint4*>(row + (long long)id0 * kSize)[i]; }
+  __device__ __forceinline__ uint4 vec(int i, bool inner = false) const {
     if constexpr (STAGED) return part[i];
-    else return load(i);
+    else return inner ? load_inner(i) : load(i);
   }
   // f(vector, its number) of this thread's vectors, AHEAD of them loaded at a time
   template <int AHEAD, typename F>
   __device__ __forceinline__ void each_vector(F f) const {
-    for (int i = tid; i < vecs; i += AHEAD * THREADS) {
+    for (int i0 = 0; i0 < vecs; i0 += AHEAD * THREADS) {
+      const int i = i0 + tid;
       uint4 w[AHEAD];
+      if (i0 > 0 && i0 + AHEAD * THREADS < vecs) {
 #pragma unroll
-      for (int a = 0; a < AHEAD; ++a)
-        if (i + a * THREADS < vecs) w[a] = vec(i + a * THREADS);
+        for (int a = 0; a < AHEAD; ++a) w[a] = vec(i + a * THREADS, true);
 #pragma unroll
-      for (int a = 0; a < AHEAD; ++a)
-        if (i + a * THREADS < vecs) f(w[a], i + a * THREADS);
+        for (int a = 0; a < AHEAD; ++a) f(w[a], i + a * THREADS);
+      } else {
+#pragma unroll 1
+        for (int k = i; k < min(vecs, i0 + AHEAD * THREADS); k += THREADS) f(vec(k), k);
+      }
     }
   }
   // f(value) of this thread's values, in few instructions: what few rows come to is not to push the rest out of the instruction cache
@@ -241,20 +248,41 @@ struct SampleRow {
       sh.kept = n, sh.ties = 0;
     }
     __syncthreads();
-    // each value's place: how many come before it; as many threads to a value as there are
-    int by = 1;
-    while (by < 32 && 2 * by * n <= THREADS) by *= 2;
-    for (int i0 = 0; i0 < n; i0 += THREADS / by) {
-      const int i = i0 + tid / by, end = i < n ? (n + 1) / 2 : 0;
-      const Listed v = i < n ? sh.list[i] : 0;
-      int before = 0;
+    if (THREADS < kListed || 16 * n <= 5 * THREADS) {
+      // each value's place: how many come before it; as many threads to a value as there are
+      int by = 1;
+      while (by < 32 && 2 * by * n <= THREADS) by *= 2;
+      for (int i0 = 0; i0 < n; i0 += THREADS / by) {
+        const int i = i0 + tid / by, end = i < n ? (n + 1) / 2 : 0;
+        const Listed v = i < n ? sh.list[i] : 0;
+        int before = 0;
 #pragma unroll 4
-      for (int q = tid % by; q < end; q += by) {
-        const ulonglong2 o = reinterpret_cast<const ulonglong2*>(sh.list)[q];
-        before += (o.x > v) + (o.y > v);
+        for (int q = tid % by; q < end; q += by) {
+          const ulonglong2 o = reinterpret_cast<const ulonglong2*>(sh.list)[q];
+          before += (o.x > v) + (o.y > v);
+        }
+        for (int d = 1; d < by; d <<= 1) before += __shfl_xor_sync(0xffffffffu, before, d);
+        if (i < n && tid % by == 0) sh.sorted[before] = v;
       }
-      for (int d = 1; d < by; d <<= 1) before += __shfl_xor_sync(0xffffffffu, before, d);
-      if (i < n && tid % by == 0) sh.sorted[before] = v;
+    } else {
+      // a value for each thread, sorted by comparisons in pairs (cycles by places | like this: 60 values 1900 | 2900, 250 by 1024 threads 4500 | 7400, 300 by 512 14800 | 8900)
+      Listed v = tid < n ? sh.list[tid] : 0, *at = sh.sorted;
+      __syncthreads();
+      for (int k = 2; k <= kListed; k <<= 1)
+        for (int j = k >> 1; j > 0; j >>= 1) {
+          Listed o;
+          if (j >= 32) {
+            if (tid < kListed) at[tid] = v;
+            __syncthreads();
+            o = tid < kListed ? at[tid ^ j] : 0;
+            at = at == sh.sorted ? sh.list : sh.sorted;  // (what has been written here two steps ago has been read by everybody)
+          } else {
+            o = __shfl_xor_sync(0xffffffffu, v, j);
+          }
+          if ((o > v) == (((tid & j) == 0) == ((tid & k) == 0))) v = o;
+        }
+      __syncthreads();
+      if (tid < n) sh.sorted[tid] = v;
     }
     __syncthreads();
     bool reaches = left <= n;
@@ -517,14 +545,16 @@ __global__ void __launch_bounds__(THREADS, THREADS == 1024 ? 1 : THREADS == 512 
   {
     uint32_t top = Vec<KIND>::kLowest;
     constexpr int kAhead = 4;
-    for (int i = tid; i < vecs; i += kAhead * THREADS) {
+    for (int i0 = 0; i0 < vecs; i0 += kAhead * THREADS) {
+      const int i = i0 + tid;
+      const bool inner = i0 > 0 && i0 + kAhead * THREADS < vecs;
       uint4 w[kAhead];
 #pragma unroll
       for (int a = 0; a < kAhead; ++a)
-        if (i + a * THREADS < vecs) w[a] = R.load(i + a * THREADS);
+        if (inner || i + a * THREADS < vecs) w[a] = inner ? R.load_inner(i + a * THREADS) : R.load(i + a * THREADS);
 #pragma unroll
       for (int a = 0; a < kAhead; ++a)
-        if (i + a * THREADS < vecs) {
+        if (inner || i + a * THREADS < vecs) {
           if constexpr (STAGED) part[i + a * THREADS] = w[a];
           top = Vec<KIND>::larger(top, Vec<KIND>::largest(w[a]));
         }
@@ -538,7 +568,7 @@ __global__ void __launch_bounds__(THREADS, THREADS == 1024 ? 1 : THREADS == 512 
   uint32_t ranked = 0;
   if (listing) {
     ranked = sort_falling(seen, lane);
-    sh.groups[tid] = ranked;
+    sh.groups[33 * warp + lane] = ranked;
   }
   const uint32_t warp_most = __reduce_max_sync(0xffffffffu, seen);
   if (lane == 0) sh.most[warp] = warp_most;
@@ -552,8 +582,8 @@ __global__ void __launch_bounds__(THREADS, THREADS == 1024 ? 1 : THREADS == 512 
     if (lane < kWarps) {
 #pragma unroll
       for (int step = 16; step > 0; step >>= 1)
-        if (sh.groups[32 * lane + n + step - 1] >= v) n += step;
-      n += sh.groups[32 * lane + n] >= v;
+        if (sh.groups[33 * lane + n + step - 1] >= v) n += step;
+      n += sh.groups[33 * lane + n] >= v;
     }
     n = __reduce_add_sync(0xffffffffu, n);
     if (lane == 0) sh.reach[warp] = n >= want_listed ? v : 0u;
@@ -568,8 +598,9 @@ __global__ void __launch_bounds__(THREADS, THREADS == 1024 ? 1 : THREADS == 512 
     return;
   }
   const double least = fmin((double)min_p, 1.0);
-  const Weight weight = {fminf(M - 700.f * T, value_of(most - 1)), (double)M, T > 0.f ? 32.0 * 1.4426950408889634074 / (double)T : 0.0, sh.table};
+  const Weight weight = {fminf(M - 700.f * T, value_of(most - 1)), (double)M, T > 0.f ? 32.0 * 1.4426950408889634074 / (double)T : 0.0, sh.table, p.series};
   R.M = M, R.weight = weight;
+  const float low_p = least > 0.0 ? M + T * 1.0001f * (logf((float)least) - 1e-3f) - 1e-6f * fabsf(M) : -CUDART_INF_F;  // what lies below weighs less than min_p
 
   // ---- the edge: values above it are kept, and the first `ties` of those that equal it
   const uint32_t edge_most = most >> kDrop, edge_least = order_of(-CUDART_INF_F) >> kDrop;
@@ -656,11 +687,11 @@ __global__ void __launch_bounds__(THREADS, THREADS == 1024 ? 1 : THREADS == 512 
           const float x = Vec<KIND>::value(w, k);
           const double v = weight(x), c = x > over_k ? v : 0.0;
           mass[k & 1] += c;
-          if (c >= least) likely += c;
+          if (x >= low_p) likely += c;  // (or a little less than min_p)
         }
       });
       SampleSum whole = R.template total<true>(mass[0] + mass[1], likely, 0);
-      if (tie >= least) whole.likely += k_ties * tie;
+      if (k_value >= low_p) whole.likely += k_ties * tie;
       whole.mass += k_ties * tie;
       const double want = (double)top_p * whole.mass;
       if (!(least > 0.0 && whole.likely < want)) {  // (where what min-p keeps does not reach the share, the nucleus has no part in it)
@@ -705,8 +736,7 @@ __global__ void __launch_bounds__(THREADS, THREADS == 1024 ? 1 : THREADS == 512 
   // ---- what is kept, chunk by chunk (of 32 vectors: neighbouring ids)
   const float edge_value = edge == 0 ? -CUDART_INF_F : Row::value_of_key(edge), over_edge = first ? CUDART_INF_F : fmaxf(edge_value, weight.low);
   const double edge_alone = edge == 0 ? 0.0 : first ? 1.0 : weight.or_zero(edge_value), edge_weight = edge_alone >= least ? edge_alone : 0.0;
-  // (what lies clearly below the edge or min-p is passed over by the vector)
-  const float pass = fmaxf(edge_value, least > 0.0 && !first ? M + T * 1.0001f * (logf((float)least) - 1e-3f) - 1e-6f * fabsf(M) : -CUDART_INF_F);
+  const float pass = fmaxf(edge_value, first ? -CUDART_INF_F : low_p);  // (what lies clearly below the edge or min-p is passed over by the vector)
   auto above_edge = [&](float x) {  // its weight, if it counts
     const double w = weight(x);
     return x > over_edge && w >= least ? w : 0.0;
@@ -715,17 +745,17 @@ __global__ void __launch_bounds__(THREADS, THREADS == 1024 ? 1 : THREADS == 512 
   int count = 0;
   auto sum_chunks = [&](auto all_of_it) {  // all_of_it: no edge, no min-p
     constexpr bool kAll = decltype(all_of_it)::value;
-    constexpr int kAhead = 2;  // chunks of a warp at a time
-    for (int c0 = warp; c0 < chunks; c0 += kAhead * kWarps) {
-      double m[kAhead] = {};
-      int n[kAhead] = {};
-      uint4 w[kAhead];
+    for (int c0 = warp; c0 < chunks; c0 += 4 * kWarps) {  // four chunks of a warp at a time
+      double m[4] = {};
+      uint32_t n[2] = {};  // a half for each chunk
+      uint4 w[4];
       bool any = false;
 #pragma unroll
-      for (int a = 0; a < kAhead; ++a) {
+      for (int a = 0; a < 4; ++a) {
         const int i = (c0 + a * kWarps) * 32 + lane;
         constexpr uint32_t low = Vec<KIND>::kLowest;
-        w[a] = i < vecs ? R.vec(i) : make_uint4(low, low, low, low);
+        if (c0 > 0 && c0 + 3 * kWarps < chunks - 1) w[a] = R.vec(i, true);
+        else w[a] = i < vecs ? R.vec(i) : make_uint4(low, low, low, low);
         if constexpr (!kAll) {
           if (i < vecs && Vec<KIND>::most(Vec<KIND>::largest(w[a])) >= pass) any = true;
           else w[a] = make_uint4(low, low, low, low);
@@ -734,34 +764,38 @@ __global__ void __launch_bounds__(THREADS, THREADS == 1024 ? 1 : THREADS == 512 
       if (kAll || __any_sync(0xffffffffu, any)) {
         if (kAll || any) {
 #pragma unroll
-          for (int k = 0; k < kPer; ++k)
+          for (int a = 0; a < 4; ++a)
 #pragma unroll
-            for (int a = 0; a < kAhead; ++a) {
+            for (int k = 0; k < kPer; ++k) {
               const float x = Vec<KIND>::value(w[a], k);
               if constexpr (kAll) {
                 m[a] += weight.or_zero(x);
               } else {
                 m[a] += above_edge(x);
-                n[a] += x == edge_value;
+                n[a >> 1] += x == edge_value ? 1u << 16 * (a & 1) : 0u;
               }
             }
         }
+        // each lane goes on with half of what it has: eight lanes have a chunk in the end
+        const bool high = lane & 16, odd = lane & 8;
+        double e = high ? m[2] : m[0], o = high ? m[3] : m[1];
+        e += __shfl_xor_sync(0xffffffffu, high ? m[0] : m[2], 16);
+        o += __shfl_xor_sync(0xffffffffu, high ? m[1] : m[3], 16);
+        m[0] = (odd ? o : e) + __shfl_xor_sync(0xffffffffu, odd ? e : o, 8);
 #pragma unroll
-        for (int d = 16; d > 0; d >>= 1)
-#pragma unroll
-          for (int a = 0; a < kAhead; ++a) m[a] += __shfl_xor_sync(0xffffffffu, m[a], d);
-        if constexpr (!kAll)
-#pragma unroll
-          for (int a = 0; a < kAhead; ++a) n[a] = __reduce_add_sync(0xffffffffu, n[a]);
+        for (int d = 4; d > 0; d >>= 1) m[0] += __shfl_xor_sync(0xffffffffu, m[0], d);
+        if constexpr (!kAll) {
+          n[0] = __reduce_add_sync(0xffffffffu, n[0]), n[1] = __reduce_add_sync(0xffffffffu, n[1]);
+          n[0] = (high ? n[1] : n[0]) >> (odd ? 16 : 0) & 0xffffu;
+        }
       }
-#pragma unroll
-      for (int a = 0; a < kAhead; ++a)
-        if (lane == 0 && c0 + a * kWarps < chunks) chunk_mass[c0 + a * kWarps] = m[a], chunk_ties[c0 + a * kWarps] = n[a], mass += m[a], count += n[a];
+      const int c = c0 + (lane >> 3) * kWarps;
+      if ((lane & 7) == 0 && c < chunks) chunk_mass[c] = m[0], chunk_ties[c] = (int)n[0], mass += m[0], count += (int)n[0];
     }
   };
   if (edge == 0 && !(least > 0.0)) sum_chunks(std::true_type());
   else sum_chunks(std::false_type());
-  const SampleSum kept = R.total(mass, 0.0, lane == 0 ? count : 0);
+  const SampleSum kept = R.total(mass, 0.0, count);
   const double all = kept.mass + min(kept.count, ties) * edge_weight, want = (double)fmaxf(u, 0.f) * all;
   const bool to_end = u >= 1.f;
 
@@ -896,6 +930,8 @@ int blr_sample(const void* logits, int64_t ld, int64_t rows, int64_t vocab, int 
   p.ids = reinterpret_cast<long long*>(ids), p.logprob = logprob;
   const int64_t per = 16 / size, vecs = (vocab + 2 * per - 2) / per;  // (as many vectors as a row can have, however it is aligned)
   p.vocab = (int)vocab, p.chunks = (int)((vecs + 31) / 32);
+  for (int i = 0; i < 4; ++i) p.series[i] = (i > 0 ? p.series[i - 1] : 1.0) * (0.69314718055994530942 / 32.0) / (i + 1);
+  p.series[4] = 6755399441055744.0;
   const cudaStream_t st = static_cast<cudaStream_t>(stream);
 #define BLR_SAMPLE(THREADS, STAGED) \
   (kind == 0 ? launch_sample<0, THREADS, STAGED>(p, rows, st) : kind == 1 ? launch_sample<1, THREADS, STAGED>(p, rows, st) : launch_sample<2, THREADS, STAGED>(p, rows, st))
