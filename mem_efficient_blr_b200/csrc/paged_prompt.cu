@@ -60,27 +60,25 @@ __device__ __forceinline__ float prompt_move(const uint32_t (&x)[2][32], float f
   m = to;
   return down;
 }
-// p = 2^(s - mu) as 16-bit pairs over the scores in TMEM; returns their sum.
+// p = 2^(s - mu) as 16-bit pairs over the scores in TMEM; returns their sum.  (One number at a time: a warp alone takes 605 cycles for its 64, of which ex2 512, and with the instructions for pairs of
+// floats, through which ex2 has to wait for its register pairs, 1003.)
 template <bool BF16>
 __device__ __forceinline__ float prompt_weights(uint32_t s_at, const uint32_t (&x)[2][32], float factor, float mu) {
-  uint64_t sum[2] = {0, 0};
-  const uint64_t neg = pair(-mu, -mu), mul = pair(factor, factor);
+  float sum[4] = {};
+  uint32_t yy[2][16];
 #pragma unroll
   for (int c = 0; c < 2; ++c) {
-    uint32_t y[16];
+    uint32_t (&y)[16] = yy[c];
 #pragma unroll
     for (int i = 0; i < 32; i += 2) {
-      float a, b;
-      unpair(fma2(pair(__uint_as_float(x[c][i]), __uint_as_float(x[c][i + 1])), mul, neg), a, b);
-      a = ex2(a), b = ex2(b);
-      sum[i / 2 & 1] = add2(sum[i / 2 & 1], pair(a, b));
+      const float a = ex2(fmaf(__uint_as_float(x[c][i]), factor, -mu)), b = ex2(fmaf(__uint_as_float(x[c][i + 1]), factor, -mu));
+      sum[i & 2] += a, sum[(i & 2) + 1] += b;
       y[i / 2] = q8_down2<BF16>(a, b);
     }
-    tmem_st16(s_at + 16 * c, y);
   }
-  float a, b;
-  unpair(add2(sum[0], sum[1]), a, b);
-  return a + b;
+  tmem_st16(s_at, yy[0]);
+  tmem_st16(s_at + 16, yy[1]);
+  return (sum[0] + sum[2]) + (sum[1] + sum[3]);
 }
 
 template <bool BF16>
@@ -114,9 +112,9 @@ __global__ void __launch_bounds__(kPromptThreads, 1) paged_prompt_kernel(const _
   constexpr uint32_t kTile = 128 * HD * 2;
   const uint32_t base = (smem_u32(prompt_raw) + 1023u) & ~1023u;
   const uint32_t qs = base, ks = base + 2 * kTile, vs = base + 4 * kTile, bars = base + 6 * kTile;
-  // sfull, pfull, done: [half][place]; mfull: [4], the tiles' pages are known; zfull: the values of a tile that not all rows see are there (its own count: those who wait for it
+  // sfull, pfull, done: [half][place]; zfull: the values of a tile that not all rows see are there (its own count: those who wait for it
   // begin with the first such tile), vclean: they have been looked through
-  const uint32_t kfull = bars, vfull = bars + 16, kempty = bars + 32, vempty = bars + 48, sfull = bars + 64, pfull = bars + 96, done = bars + 128, mfull = bars + 160, vclean = bars + 192, zfull = bars + 208;
+  const uint32_t kfull = bars, vfull = bars + 16, kempty = bars + 32, vempty = bars + 48, sfull = bars + 64, pfull = bars + 96, done = bars + 128, vclean = bars + 192, zfull = bars + 208;
   __shared__ uint32_t tmem_slot, there[4], any_bad;
   __shared__ volatile int aborted;
   volatile int* const abort_flag = &aborted;
@@ -136,7 +134,6 @@ __global__ void __launch_bounds__(kPromptThreads, 1) paged_prompt_kernel(const _
       mbar_init(sfull + 8 * i, 1);
       mbar_init(pfull + 8 * i, 4);
       mbar_init(done + 8 * i, 1);
-      mbar_init(mfull + 8 * i, 1);
     }
     mbar_init_fence();
   }
@@ -222,7 +219,6 @@ __global__ void __launch_bounds__(kPromptThreads, 1) paged_prompt_kernel(const _
           uint32_t groups = 0;
           for (int g = 0; g < 8; ++g) groups |= (parts_there >> (g * 16 >> p.c.page_log2) & 1u) << g;
           there[j & 3] = groups;
-          mbar_arrive(mfull + 8 * (j & 3));
         }
         copy(ks + s * kTile, &pp.k, page, pp.k_head_at, pp.k_page_at, kfull + 8 * s);
         if (j >= 2 && !__all_sync(0xffffffffu, mbar_wait(vempty + 8 * s, parity, abort_flag))) break;
@@ -323,17 +319,14 @@ __global__ void __launch_bounds__(kPromptThreads, 1) paged_prompt_kernel(const _
     float m = -INFINITY, l = 0.f;
     const int lim_all = __reduce_min_sync(0xffffffffu, lim);
     uint32_t groups = 0xffu;  // of the tile's keys by 16: which have a page
-    bool ok = true;
+    bool ok = true, fresh = true;  // fresh: a row of the warp has yet to see its first keys
 #pragma unroll 1
     for (int u = 0; u < n; ++u) {
       const int j = u >> 1, key0 = k0 + u * kStepKeys;
       const uint32_t s_at = tmem + lanes + 128 * wg + 64 * (u & 1);
       const bool part = key0 + kStepKeys > lim_all;  // some of these keys are masked for a row of the warp
-      if ((u & 1) == 0) {
-        if (!__all_sync(0xffffffffu, mbar_wait(mfull + 8 * (j & 3), (j >> 2) & 1, abort_flag))) { ok = false; break; }
-        groups = *(volatile uint32_t*)&there[j & 3];
-      }
       if (!__all_sync(0xffffffffu, mbar_wait(sfull + 16 * wg + 8 * (u & 1), j & 1, abort_flag))) { ok = false; break; }
+      if ((u & 1) == 0) groups = *(volatile uint32_t*)&there[j & 3];  // (written ahead of the copy of the keys that these scores are of)
       tc_fence_after();
       uint32_t x[2][32];
       tmem_ld32(s_at, x[0]);
@@ -352,9 +345,10 @@ __global__ void __launch_bounds__(kPromptThreads, 1) paged_prompt_kernel(const _
       // against the m so far, which is seldom left behind: a sum above 2^11 tells of it, and all is done once more.  The rows that ask for it move theirs, the others come out as
       // they were.
       float total = 0.f;
-      bool ask = m == -INFINITY && lim > key0;  // (a row's first keys)
+      bool ask = fresh && m == -INFINITY && lim > key0;  // (a row's first keys)
+      if (fresh) fresh = __any_sync(0xffffffffu, m == -INFINITY && lim > 0);
 #pragma unroll 1
-      for (bool moved = __any_sync(0xffffffffu, ask);; moved = true) {
+      for (bool moved = fresh && __any_sync(0xffffffffu, ask);; moved = true) {
         if (moved) {
           float down = 1.f;
           if (ask) down = prompt_move(x, factor, m);
