@@ -553,6 +553,8 @@ def _rows16(t: torch.Tensor, d: int) -> torch.Tensor:
         t2 = t2.contiguous()
         if t2.data_ptr() % 16 != 0:   # (was contiguous already, from an odd place on)
             t2 = t2.clone()
+    if t2.shape[0] == 1:   # (counts as contiguous with any row stride)
+        t2 = t2.reshape(-1).view(1, -1)
     return t2
 
 

@@ -311,6 +311,77 @@ def test_strides_and_streams(ops):
             assert torch.equal(a, b)
 
 
+@pytest.mark.parametrize("dtype", [F16, BF16])
+@pytest.mark.parametrize("T,hd", [(90, 128), (300, 64)])
+@pytest.mark.parametrize("layout", ["slots", "turns", "heads", "odd"])
+def test_many_rows_on_other_layouts(ops, T, hd, dtype, layout):
+    """Prompts over pools whose strides rise in other orders, and over one (odd) that the copy engine cannot describe, where a head's stride is no multiple of a slot's."""
+    B, H, KV, page, per = 2, 4, 2, 32, 12
+    g = torch.Generator().manual_seed(T)
+    pk, pv, table = _pool(B, KV, hd, page, per, dtype, g, [(1, 3)])
+    n = len(pk)
+
+    def pools():
+        if layout == "slots":
+            one = torch.zeros(n, page, 2, KV, hd, dtype=dtype, device=DEV)
+            return one[:, :, 0].transpose(1, 2), one[:, :, 1].transpose(1, 2)
+        if layout == "turns":
+            one = torch.zeros(n, KV, page, 2, hd + 8, dtype=dtype, device=DEV)
+            return one[..., 0, :hd], one[..., 1, :hd]
+        if layout == "heads":
+            return tuple(torch.zeros(KV, n, page, hd, dtype=dtype, device=DEV).transpose(0, 1) for _ in range(2))
+        sizes = (KV * (page * (hd + 8) + 8) + 16, page * (hd + 8) + 8, hd + 8, 1)
+        return tuple(torch.zeros(n * sizes[0], dtype=dtype, device=DEV).as_strided((n, KV, page, hd), sizes) for _ in range(2))
+
+    k, v = pools()
+    k.copy_(pk), v.copy_(pv)
+    q = (torch.randn(B, T, H, hd, generator=g) * 2).to(dtype)
+    starts = [page * per - T, 11]
+    got = ops.attention_paged(q.view(B * T, -1).to(DEV), ops.PagedCache(k, v, table.to(DEV)), _dev(starts)).cpu().double().view(B, T, H, hd)
+    want, room = _attention(q, pk, pv, table, starts, None, hd ** -0.5)
+    assert ((got - want).abs() <= _half(dtype) * want.abs() * 1.001 + room + _subnormal(dtype)).all()
+    if layout != "odd":   # (there the rows go through the kernel for few, which sums in another order)
+        assert torch.equal(ops.attention_paged(q.view(B * T, -1).to(DEV), _on(ops, pk, pv, table), _dev(starts)).cpu().double().view(B, T, H, hd), got)
+
+
+@pytest.mark.parametrize("T", [1, 70])
+def test_lazily_negated_rows_and_odd_columns(ops, T):
+    """Views that the kernels do not take as they are give what their copies give."""
+    H, KV, hd, page, per = 4, 2, 64, 16, 8
+    g = torch.Generator().manual_seed(9)
+    pk, pv, table = _pool(1, KV, hd, page, per, F16, g)
+    cos, sin = (t.to(DEV) for t in _tables(page * per, hd))
+    q, k, v = (torch.randn(T, h * hd, generator=g).half().to(DEV) for h in (H, KV, KV))
+    start = _dev([50])
+    a, b = _on(ops, pk, pv, table), _on(ops, pk, pv, table)
+    x = ops.rope_append_paged(-q, -k, -v, cos, sin, start, a)
+    y = ops.rope_append_paged(*(torch._neg_view(t) for t in (q, k, v)), cos, sin, start, b)
+    assert torch.equal(x, y) and torch.equal(a.k, b.k) and torch.equal(a.v, b.v)
+    odd = torch.empty(T, H * hd + 1, dtype=F16, device=DEV)[:, 1:]
+    odd.copy_(-x)
+    assert torch.equal(ops.attention_paged(x, a, start), ops.attention_paged(torch._neg_view(odd), a, start))
+
+
+def test_two_streams_at_once(ops):
+    """Calls on two streams that share a pool and q, but neither scratch nor results."""
+    B, H, KV, hd, page, per = 2, 8, 2, 128, 16, 64
+    g = torch.Generator().manual_seed(12)
+    c = _on(ops, *_pool(B, KV, hd, page, per, BF16, g))
+    calls = [(torch.randn(B * T, H * hd, generator=g).bfloat16().to(DEV), _dev([1024 - T, 700])) for T in (1, 3, 200)]
+    want = [ops.attention_paged(q, c, start) for q, start in calls]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    got = [[], []]
+    for _ in range(10):
+        for st, to in zip(streams, got):
+            with torch.cuda.stream(st):
+                to.extend(ops.attention_paged(q, c, start) for q, start in calls)
+    torch.cuda.synchronize()
+    for to in got:
+        for i, o in enumerate(to):
+            assert torch.equal(o, want[i % 3])
+
+
 def test_sequences_that_share_pages(ops):
     """Two sequences on the pages of one prompt, each with a last page of its own."""
     KV, H, hd, page = 2, 4, 128, 16
