@@ -8,7 +8,9 @@
 // transposed; P^T comes out of S^T by movmatrix.  The products' operands have 16 bits: q, k and v as they are, p rounded to fp16 for fp16 values (2^-11 of itself, or 2^-25
 // below 2^-14 of the heaviest); for bf16 values, where that would be 2^-8, as the sum of two bf16 numbers (2^-15), by a second product.
 // What a row does not see has no part in any bit of its result, whatever lies there: see "values that are no numbers" below.
-// Bound by HBM: a key and its value are 4 hd bytes, read once for 8 to 32 rows.
+// Bound by HBM: a key and its value are 4 hd bytes, read once for 8 to 32 rows.  64 sequences x 2048 keys, 32 heads of 128, fp16: 299 us, 7.2 TB/s; 7 x 16 to 32 k keys, 32 heads on 8,
+// bf16: 107 us, 6.2 TB/s.  1 x 2048 keys, 10.2 us for 34 MB: launch, table, pages, four groups a warp and the second kernel follow each other.  8 x 5 tokens, 30 us where the bytes take
+// 15.8: eight warps an SM (247 registers hold three tiles' sums) issue in 31 % of the cycles and wait for their products; bf16 weights are multiplied twice.
 #include "../../include/blr_b200.h"
 #include "paged.cuh"
 #include "tmap.h"
@@ -391,6 +393,13 @@ struct PagedPlan {
 };
 // Few row tiles share their keys out over more CTAs, as many as the SMs hold at a time; a second kernel sums the parts.  The host does not know the sequences' lengths: a
 // tile may have twice its even share of CTAs and one, and the kernels share by the lengths (paged_share); CTAs that are left over say so and end.
+// Both sides of each rule, us from a graph, 32 heads of 128 on 8 unless said otherwise, fp16, pages of 16:
+//   24 rows in three column tiles: 8 sequences x 6 tokens, 4096 keys at most, 29.4; in four 32.0; in the prompt kernel 45.9 (one sequence x 6: 18.5 | 20.0 | 20.1; x 8 tokens, 8192 keys,
+//     32 rows: 24.8 here, 21.9 there, but 8 sequences x 8 33.5 | 46.2).
+//   No CTA has fewer keys than `least`: with one column tile 128 (1 x 1000 keys 8.4; 64: 9.2, 256: 9.3), with more 256 (1 x 6 tokens, 4096 keys 15.5; 128: 18.5), in the prompt kernel 256 (1 x 40
+//     tokens, 2048 keys 21.4; 512: 25.3, 1024: 32.7).
+//   Up to 512 slots are not split: 8 x 500 keys 8.6, split 10.5; up to 1024: 1 x 1000 keys 11.9, split 8.4.
+//   Twice the even share: 8 x 5 tokens over 2000 to 4001 keys 30.2, without 33.0; 3 x 257 tokens, 16 heads of 64 on 4, 50.7 | 65.8; but 8 x 1 over 500 to 1000 keys 13.2 | 11.9.
 static PagedPlan paged_plan(const blr_paged_cache* c, int64_t n_tok, int heads) {
   PagedPlan a = {};
   const int64_t slots = c->pages_per_seq * c->page;
@@ -401,7 +410,7 @@ static PagedPlan paged_plan(const blr_paged_cache* c, int64_t n_tok, int heads) 
   a.tiles = c->n_seq * c->kv_heads * a.q_tiles;
   a.room = (a.nt == 0 ? 1 : c->head_dim == 64 && a.nt < 3 ? 4 : 2) * sm_count();
   long long ns = a.tiles > 0 ? a.room / a.tiles : 1;
-  const long long least = a.nt ? 128 : 512, most = (slots + least - 1) / least;  // keys of a CTA
+  const long long least = a.nt == 1 ? 128 : 256, most = (slots + least - 1) / least;  // keys of a CTA
   if (ns > 1 && (c->n_seq > 1 || a.q_tiles > 1)) ns = 2 * ns + 1;
   if (slots <= 512) ns = 1;
   if (ns > most) ns = most;
