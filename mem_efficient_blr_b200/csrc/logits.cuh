@@ -13,6 +13,8 @@ __device__ __forceinline__ uint32_t order_of(float x) {
 __device__ __forceinline__ float value_of(uint32_t o) {
   return __uint_as_float(o == kOrderOfNan ? 0x7fffffffu : o & 0x80000000u ? o & 0x7fffffffu : ~o);
 }
+// The largest number below the one of order o.  (0x7fffffff is the order of none: it lies between 0 and the number below it, and would be -0, which equals 0.)
+__device__ __forceinline__ float value_below(uint32_t o) { return value_of(o == 0x80000000u ? 0x7ffffffeu : o - 1); }
 
 // 16 bytes of logits: kPer values.
 template <int KIND>

@@ -501,7 +501,7 @@ struct SampleRow {
       if (below) {
         if (single) return false;
         b.over.mass += s.likely, b.over.count += in;
-        b.hi = value_of(order_of(lo) - 1);
+        b.hi = value_below(order_of(lo));
         if (!(b.hi >= b.lo)) return false;
         continue;
       }
@@ -601,7 +601,7 @@ __global__ void __launch_bounds__(THREADS, THREADS == 1024 ? 1 : THREADS == 512 
     return;
   }
   const double least = fmin((double)min_p, 1.0);
-  const Weight weight = {fminf(M - 700.f * T, value_of(most - 1)), (double)M, T > 0.f ? 32.0 * 1.4426950408889634074 / (double)T : 0.0, sh.table, p.series};
+  const Weight weight = {fminf(M - 700.f * T, value_below(most)), (double)M, T > 0.f ? 32.0 * 1.4426950408889634074 / (double)T : 0.0, sh.table, p.series};
   R.M = M, R.weight = weight;
   const float low_p = least > 0.0 ? M + T * 1.0001f * (logf((float)least) - 1e-3f) - 1e-6f * fabsf(M) : -CUDART_INF_F;  // what lies below weighs less than min_p
 
@@ -705,7 +705,7 @@ __global__ void __launch_bounds__(THREADS, THREADS == 1024 ? 1 : THREADS == 512 
         if (!k_mode) {
           found = R.cut(listed, listed, over.mass, top_p, whole.mass, edge, ties);
           if (found) return R.pick(least, u, p.ids + r, p.logprob + r);
-          if (over.mass > 0.0) over.count = listed, below = value_of(reached - 1);  // (it goes on below what was listed)
+          if (over.mass > 0.0) over.count = listed, below = value_below(reached);  // (it goes on below what was listed)
         }
         const float from = fmaxf(fmaxf(k_value, M - kSpan * T), -3.402823466e38f);
         if (!found && below >= from) found = R.search({from, below, over}, false, 0, want, top_p, whole.mass, log2_per, edge, ties);
