@@ -350,13 +350,14 @@ __global__ void __launch_bounds__(kPromptThreads, 1) paged_prompt_kernel(const _
         mask_groups(x[1], groups >> (4 * (u & 1) + 2));
       }
       // against the m so far, which is seldom left behind: a sum above 2^11 tells of it, and all is done once more.  The rows that ask for it move theirs, the others come out as
-      // they were.
+      // they were.  The first keys of a row are a pass of their own, ahead of that: a row without a number among its scores takes all of its keys for the first, and the rows beside it are not
+      // to wait for it.
       float total = 0.f;
       bool ask = fresh && m == -INFINITY && lim > key0;  // (a row's first keys)
       if (fresh) fresh = __any_sync(0xffffffffu, m == -INFINITY && lim > 0);
 #pragma unroll 1
-      for (bool moved = fresh && __any_sync(0xffffffffu, ask);; moved = true) {
-        if (moved) {
+      for (int pass = fresh && __any_sync(0xffffffffu, ask) ? 1 : 0;; pass = 2) {  // 0: nothing moves, 1: a row's first keys, 2: what is behind
+        if (pass != 0) {
           float down = 1.f;
           if (ask) down = prompt_move(x, factor, m);
           __syncwarp();  // (what follows in TMEM is the whole warp's)
@@ -376,7 +377,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1) paged_prompt_kernel(const _
         }
         total = prompt_weights<BF16>(s_at, x, factor, m == -INFINITY ? 0.f : m);
         ask = total > 2048.f;
-        if (moved || !__any_sync(0xffffffffu, ask)) break;
+        if (pass == 2 || !__any_sync(0xffffffffu, ask)) break;
       }
       if (!ok) break;
       l += total;
