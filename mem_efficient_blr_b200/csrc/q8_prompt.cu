@@ -74,7 +74,12 @@ __device__ __forceinline__ void move_to(const uint32_t (&x)[2][32], uint32_t fac
       to = fmaxf(to, peak[2 * c + g]);
     }
   }
-  if (to == -INFINITY) return;
+  if (to == -INFINITY) {
+    // (no number among the row's first keys.  It counts as begun, or it would ask for a move at every step, and the rows beside it would not come to theirs; a number that follows is above
+    // this by more than any sum has room for, and moves it)
+    m = -3.402823466e38f;
+    return;
+  }
   uint32_t vs[4];
   lds128(fac + 32, vs[0], vs[1], vs[2], vs[3]);
   float heavy = -INFINITY;
