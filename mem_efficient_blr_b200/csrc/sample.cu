@@ -40,7 +40,7 @@ struct SampleParams {
   long long* ids;
   float* logprob;
   int vocab, chunks;  // chunks: of 32 vectors of 16 bytes, that a row can have
-  double series[5];   // log(2) / 32 to the powers 1 to 4 over their factorials; 1.5 2^52
+  double series[5];   // log(2) / 256 to the powers 1 to 4 over their factorials; 1.5 2^52
 };
 
 struct SampleSum {
@@ -59,19 +59,20 @@ struct SampleShared {
     int hist[kBins];
     uint32_t groups[33 * kWarps];  // (a warp's 32 a word apart from the next one's: lane i reads warp i's)
   };
-  double table[32];  // 2^(j / 32)
+  double table[256];  // 2^(j / 256)
   SampleSum warp[2][kWarps];
   uint32_t most[kWarps], reach[kWarps], listed;
   float estimate[kWarps];
   int ties, kept, bin, inside, at[2];
 };
 
-// e^((x - M) / T) in 64 bits to 2^-39 of itself: 2^(n / 32) from the table times the Taylor series of 2^(r / 32), |r| <= 1/2, up to the fourth power.  Exactly 1 at M; for x above `low`,
-// which is next below M, or where e^-700 is.  (A call of exp has three times the instructions, and they are what bounds a row that is summed as a whole.)
+// e^((x - M) / T) in 64 bits, to 2^-50 of itself and 2^-52 for each unit of (M - x) / T: 2^(n / 256) from the table times the Taylor series of 2^(r / 256), |r| <= 1/2, up to the fourth power,
+// which leaves 2^-54 (of 2^(r / 32), with a table of 32 numbers, it left 2^-39, and one more power to 2^-48 cost 1 % of a row that is summed as a whole: 113.8 us for 112.7).  Exactly 1
+// at M; for x above `low`, which is next below M, or where e^-700 is.  (A call of exp has three times the instructions, and they are what bounds such a row.)
 // (The series' numbers come as the kernel's parameters, where an instruction reads them: as literals each takes two more.)
 struct Weight {
   float low;
-  double most, c;  // 32 log2(e) / T
+  double most, c;  // 256 log2(e) / T
   const double *table, *series;
   __device__ __forceinline__ double operator()(float x) const {
     const double d = (double)x - most, s = fma(d, c, series[4]);  // 1.5 2^52: whole numbers end in the last bits
@@ -80,8 +81,8 @@ struct Weight {
     double e = fma(r, series[3], series[2]);
     e = fma(r, e, series[1]);
     e = fma(r, e, series[0]);
-    e = fma(r, e, 1.0) * table[n & 31];
-    return __hiloint2double(__double2hiint(e) + ((n & ~31) << 15), __double2loint(e));
+    e = fma(r, e, 1.0) * table[n & 255];
+    return __hiloint2double(__double2hiint(e) + ((n & ~255) << 12), __double2loint(e));
   }
   __device__ __forceinline__ double or_zero(float x) const { return x > low ? (*this)(x) : 0.0; }
 };
@@ -92,9 +93,9 @@ constexpr double power_of_two(double x) {  // its Taylor series, 0 <= x < 1
   return sum;
 }
 struct Powers {
-  double of[32];
+  double of[256];
   constexpr Powers() : of() {
-    for (int j = 0; j < 32; ++j) of[j] = power_of_two(j / 32.0);
+    for (int j = 0; j < 256; ++j) of[j] = power_of_two(j / 256.0);
   }
 };
 __device__ const Powers kPowers = Powers();
@@ -536,7 +537,7 @@ __global__ void __launch_bounds__(THREADS, THREADS == 1024 ? 1 : THREADS == 512 
   int* const chunk_ties = reinterpret_cast<int*>(chunk_mass + p.chunks);
   uint4* const part = dynamic + (p.chunks * 12 + 15) / 16;
   Row R = {sh, part, row, tid, warp, lane, vecs, -shift, p.vocab, 0, 0.f, {}};
-  if (tid < 32) sh.table[tid] = kPowers.of[tid];
+  for (int i = tid; i < 256; i += THREADS) sh.table[i] = kPowers.of[i];
   if (tid == 0) sh.listed = 0;
   asm volatile("griddepcontrol.wait;" ::: "memory");
   const float T = p.s.temperature ? p.s.temperature[r] : p.s.temperature_all, top_p = p.s.top_p ? p.s.top_p[r] : p.s.top_p_all;
@@ -601,7 +602,7 @@ __global__ void __launch_bounds__(THREADS, THREADS == 1024 ? 1 : THREADS == 512 
     return;
   }
   const double least = fmin((double)min_p, 1.0);
-  const Weight weight = {fminf(M - 700.f * T, value_below(most)), (double)M, T > 0.f ? 32.0 * 1.4426950408889634074 / (double)T : 0.0, sh.table, p.series};
+  const Weight weight = {fminf(M - 700.f * T, value_below(most)), (double)M, T > 0.f ? 256.0 * 1.4426950408889634074 / (double)T : 0.0, sh.table, p.series};
   R.M = M, R.weight = weight;
   const float low_p = least > 0.0 ? M + T * 1.0001f * (logf((float)least) - 1e-3f) - 1e-6f * fabsf(M) : -CUDART_INF_F;  // what lies below weighs less than min_p
 
@@ -933,7 +934,7 @@ int blr_sample(const void* logits, int64_t ld, int64_t rows, int64_t vocab, int 
   p.ids = reinterpret_cast<long long*>(ids), p.logprob = logprob;
   const int64_t per = 16 / size, vecs = (vocab + 2 * per - 2) / per;  // (as many vectors as a row can have, however it is aligned)
   p.vocab = (int)vocab, p.chunks = (int)((vecs + 31) / 32);
-  for (int i = 0; i < 4; ++i) p.series[i] = (i > 0 ? p.series[i - 1] : 1.0) * (0.69314718055994530942 / 32.0) / (i + 1);
+  for (int i = 0; i < 4; ++i) p.series[i] = (i > 0 ? p.series[i - 1] : 1.0) * (0.69314718055994530942 / 256.0) / (i + 1);
   p.series[4] = 6755399441055744.0;
   const cudaStream_t st = static_cast<cudaStream_t>(stream);
 #define BLR_SAMPLE(THREADS, STAGED) \
