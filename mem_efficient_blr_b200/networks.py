@@ -570,7 +570,7 @@ class LlamaDecoder(nn.Module):
                  n_new: Optional[torch.Tensor] = None):
         """Goes on from prompts ids (B, T), of each row the first n_new[b] ((B,) int64; None: all), by new_tokens tokens, each chosen as ops.sample does from its
         uniform number (B, new_tokens) fp32 (None: torch.rand) with these settings.  On an 8-bit cache or one in pages, whose first B sequences it begins anew.  Returns (ids, log probabilities),
-        (B, new_tokens) each; a sequence that does not fit the cache has id -1 and NaN from there on."""
+        (B, new_tokens) each; a sequence without a token has ids -1 and NaN, and so has one that does not fit the cache from there on."""
         from . import ops
         if self._caches() is None:
             raise RuntimeError("generate needs a decoder with an 8-bit cache or one in pages (kv_cache='int8', 'e4m3' or 'paged')")
@@ -585,6 +585,8 @@ class LlamaDecoder(nn.Module):
         pos = pos + T if n_new is None else pos.clamp(0, T)
         chosen, logprobs, each = [], [], uniform.t().contiguous()
         logits = self.extend(ids, torch.zeros_like(pos), n_new)
+        if n_new is not None:
+            logits = logits.masked_fill_((pos == 0)[:, None], float("nan"))
         for i in range(new_tokens):
             token, lp = ops.sample(logits, each[i], temperature, top_k, top_p, min_p)
             chosen.append(token)
