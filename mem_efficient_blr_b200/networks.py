@@ -569,8 +569,9 @@ class LlamaDecoder(nn.Module):
     def generate(self, ids: torch.Tensor, new_tokens: int, uniform: Optional[torch.Tensor] = None, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0,
                  n_new: Optional[torch.Tensor] = None):
         """Goes on from prompts ids (B, T), of each row the first n_new[b] ((B,) int64; None: all), by new_tokens tokens, each chosen as ops.sample does from its
-        uniform number (B, new_tokens) fp32 (None: torch.rand) with these settings.  On an 8-bit cache or one in pages, whose first B sequences it begins anew.  Returns (ids, log probabilities),
-        (B, new_tokens) each; a sequence without a token has ids -1 and NaN, and so has one that does not fit the cache from there on."""
+        uniform number (B, new_tokens) fp32 (None: torch.rand) with these settings.  On an 8-bit cache or one in pages, whose first B sequences it begins anew; in pages it reserves
+        each sequence's prompt and what it appends, n_new[b] + new_tokens - 1 slots (the last token is the caller's to append, and to reserve for).  Returns (ids, log probabilities), (B, new_tokens) each; a
+        sequence without a token has ids -1 and NaN, and so has one that does not fit the cache from there on."""
         from . import ops
         if self._caches() is None:
             raise RuntimeError("generate needs a decoder with an 8-bit cache or one in pages (kv_cache='int8', 'e4m3' or 'paged')")
@@ -580,7 +581,12 @@ class LlamaDecoder(nn.Module):
         if uniform.shape != (B, new_tokens):
             raise ValueError(f"uniform: a number for each of {new_tokens} tokens of {B} sequences")
         if self.paged is not None:
-            self.reserve([min(T + new_tokens, self.cache_len)] * B)
+            # the last token that is chosen is not appended.  n_new is read back only where not everybody has the pages of a whole row already
+            slots = lambda n: min(n + max(new_tokens - 1, 0), self.cache_len) if n > 0 else 0   # noqa: E731
+            lengths = [slots(T)] * B
+            if n_new is not None and B <= self.batch and any(len(have) * self.kv_page < lengths[0] for have in self._pages[:B]):
+                lengths = [slots(n) for n in n_new.clamp(0, T).tolist()]
+            self.reserve(lengths)
         pos = ids.new_zeros(B) if n_new is None else n_new
         pos = pos + T if n_new is None else pos.clamp(0, T)
         chosen, logprobs, each = [], [], uniform.t().contiguous()
