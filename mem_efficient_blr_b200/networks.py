@@ -462,7 +462,7 @@ class LlamaDecoder(nn.Module):
 
     def reserve(self, lengths) -> None:
         """Pages for the first lengths[b] slots of sequence b (one number for each of the first sequences), out of those that are free; what a sequence has stays.  Raises
-        where there are too few, and then nothing has changed.  The table is written behind what the current stream has been given so far."""
+        where there are too few, or where the table cannot be written (inside a stream capture), and then nothing has changed.  The table is written behind what the current stream has been given so far."""
         if self.paged is None:
             raise RuntimeError("reserve needs a decoder with a cache in pages (kv_cache='paged')")
         lengths = [int(n) for n in lengths]
@@ -471,20 +471,25 @@ class LlamaDecoder(nn.Module):
         more = [max(0, -(-n // self.kv_page) - len(have)) for n, have in zip(lengths, self._pages)]
         if sum(more) > len(self._free):
             raise RuntimeError(f"{sum(more)} more pages are needed, {len(self._free)} are free")
-        for b, n in enumerate(more):
-            if n:
-                have = self._pages[b]
-                new = [self._free.pop() for _ in range(n)]
-                self.page_table[b, len(have):len(have) + n] = torch.tensor(new, dtype=torch.int32).to(self.page_table.device)
-                have.extend(new)
+        if sum(more) == 0:
+            return
+        new = self._free[::-1][:sum(more)]
+        dev = torch.tensor(new, dtype=torch.int32).to(self.page_table.device)   # (what a stream capture refuses comes first)
+        del self._free[-len(new):]
+        for have, row, n in zip(self._pages, self.page_table, more):
+            row[len(have):len(have) + n] = dev[:n]
+            have.extend(new[:n])
+            new, dev = new[n:], dev[n:]
 
     def release(self, sequences) -> None:
-        """Takes back the pages of these sequences (their numbers in the batch)."""
+        """Takes back the pages of these sequences (their numbers in the batch); of none where one of them does not exist."""
         if self.paged is None:
             raise RuntimeError("release needs a decoder with a cache in pages (kv_cache='paged')")
+        sequences = list(sequences)
         for b in sequences:
             if not 0 <= b < self.batch:
                 raise ValueError(f"there is no sequence {b}")
+        for b in sequences:
             self._free.extend(reversed(self._pages[b]))
             self._pages[b] = []
             self.page_table[b].fill_(-1)
