@@ -6,11 +6,12 @@
 //   warps 10, 11    look through the values of the tiles that not all rows see: what is no number there, and what lies behind the last key, becomes 0 for the product
 //                   (which would multiply it with 0 for the rows that must not see it), and is added by the rows that do see it in the end
 // p = 2^(s - m): m, a whole number, is the row's own and moves when a step's sum of p has outgrown 2^11, so that nothing but P is rounded (fp16: 2^-11 of itself, or
-// 2^-25 below 2^-14 of the heaviest; bf16: 2^-8), and no bit of a row depends on what it does not see.
+// 2^-25 below 2^-14 of the heaviest; bf16: 2^-8), and no bit of a row depends on what it does not see.  P has the values' type because the product's operands must have one type; what bf16
+// leaves of it (2^-15, as the kernel for few rows has it) would be a second product, 524 cycles to a step's 1440, and as many conversions again in the softmax, which is what a step waits for.
 // A step is half a tile, 64 keys, and a half's S alternates between two places of TMEM: S0 S0 S1 S1 first, then PV0 S0 | PV1 S1 | ... with the S two steps ahead of the PV, into
 // the place that the PV's P has left (P lies over the S that it was made of; one queue, so in order).  Neither half waits for the other's softmax, or for its own scores.
 // O is rescaled, seldom, when the last PV is known to be done.
-// 8192 tokens, 32 heads of 128 on 8, fp16: 530 us, 1037 TFLOP/s, for some 10 ms; 600 us when it goes on and the power limit lowers the clock.  A step's products take 1440 cycles (S has 64
+// 8192 tokens, 32 heads of 128 on 8, fp16: 530 us, 1037 TFLOP/s, for some 10 ms; 600 to 615 us when it goes on and the power limit lowers the clock.  A step's products take 1440 cycles (S has 64
 // columns, whose Q and K come out of shared memory: 476 of a half's 720) and a step 2000: the two halves' softmaxes, which run side by side (1470 for the weights of both, 500 from their
 // scores to the weights and from the weights to the products).  Tried: the halves by turns 713 us; S of 128 keys in one place 583; fewer registers in the softmax 532; a polynomial for ex2, below.
 // 3 x 257 tokens over up to 6001 keys, 16 heads of 64 on 4: 50 us; the longest of 136 shares has 16 tiles of keys where even ones would have 13, and a sequence's fifth row tile has 4 rows.
@@ -65,7 +66,7 @@ __device__ __forceinline__ float prompt_move(const uint32_t (&x)[2][32], float f
   return down;
 }
 // p = 2^(s - mu) as 16-bit pairs over the scores in TMEM; returns their sum.  The arguments one number at a time: with the instruction for pairs of floats ex2 has to wait for
-// its register pairs (1003 cycles for a warp's 64 numbers, and 605 without; 562 us for a prompt of 8192 tokens with 8 heads, and 534 without); the sums, whose operands come out of
+// its register pairs (1003 cycles for a warp's 64 numbers, and 605 without; 562 us for a prompt of 8192 tokens with 32 heads on 8, and 534 without); the sums, whose operands come out of
 // ex2, by pairs (531 us).  A polynomial in place of ex2 for a sixteenth, an eighth and a quarter of the numbers: 538, 554 and 567 us, the warps are short of turns, not of ex2.
 template <bool BF16>
 __device__ __forceinline__ float prompt_weights(uint32_t s_at, const uint32_t (&x)[2][32], float factor, float mu) {

@@ -7,12 +7,16 @@
 // row's length and place alone.
 //
 // One CTA takes a row and keeps it in shared memory, where it fits, or reads it again from L2.
-//   The edge of small k, or of most nuclei, is among the few hundred values that reach a number which enough groups of threads have seen reached: they are put in order.
-//   Where it is not (long nuclei, large k), a histogram of the row says between which values the edge lies, those above are summed, and so on with those between until they can be
+//   The edge of small k, or of short nuclei, is among the few hundred values that reach a number which enough groups of threads have seen reached: they are put in order.  (128 threads, which
+//   rows of up to 512 vectors have, are too few groups for a nucleus or k above 128.)
+//   Where it is not (long nuclei), a histogram of the row says between which values the edge lies, those above are summed, and so on with those between until they can be
 //   put in order or are one value.
-//   Where that does not end in a few rounds, the edge is searched for bit by bit.
+//   Where that does not end in a few rounds, the edge is searched for bit by bit, a pass over the row each.  That is every row whose k is more than its threads (the histogram then begins at the
+//   lowest number there is, and its bins are even in value), or more than a mask leaves: 4 | 256 rows of 32000 bf16 numbers, k = 1000, 96 | 136 us, k = 50 of 20 that are left 44 | 68 (of 32000:
+//   8 | 12), k = 200 of 2000 40 | 47; 256 rows of 150000 fp32 numbers, which do not stay on the chip, k = 1000, 1.9 ms.
 // Bound by instructions, not by HBM: 1024 rows of 50001 fp32 numbers drawn from as a whole take 112 us for 31.5 of bytes, 42 instructions a value, 10 of them in 64 bits, at 2.3 a cycle and SM;
-// 256 nuclei of 0.9 of 32000 bf16 numbers 37 to 56 us by the inputs, the slowest row counts (2.5): rounds behind barriers, each over the row (256 rows are one wave).  4 rows, k = 50 and p = 0.95: 8.6 us, launch, row, list, order, sums.
+// 256 nuclei of 0.9 of 32000 bf16 numbers 36 to 86 us by the inputs, 52 on average, the slowest row counts (2.5): rounds behind barriers, each over the row (256 rows are one wave).  4 rows, k = 50 and p = 0.95: 8.8 us, launch, row, list, order, sums.
+// The likeliest alone, 600 rows of 32000: 26 us (5.9 of bytes): behind the row's maximum a second pass over it with the sums' chunks, scans and barriers finds the id.
 // A row on a cluster of CTAs: 13 to 22 us for 4 rows, 72 to 150 for the nuclei, 200 to 220 for the whole.
 #include <math_constants.h>
 
@@ -943,7 +947,7 @@ int blr_sample(const void* logits, int64_t ld, int64_t rows, int64_t vocab, int 
   // rows of up to 512 vectors have 128, eight to an SM (1000 values, k: 4 rows 7.5, with 512 threads 25.9; 600 rows 12 | 69; 600 nuclei 46 | 56);
   // what is kept in shared memory 512, two to an SM, although there is an SM for each (32000 values, 4 rows: k 8.6, with 1024 threads 9.9; the whole row 12.2 | 11.7, nucleus 37 | 36);
   // what is not 1024 where there is an SM for each row (150000 values, 4 rows: k 14.1, with 512 threads 16.6; the whole row 33 | 40).
-  // Keeping a row saves what L2 takes to give it again (32000 values, 600 rows: greedy 25.8, read again 27.4; nucleus 112 | 115).
+  // Keeping a row saves what L2 takes to give it again (32000 values, 600 rows: greedy 25.8, read again 27.4; nucleus 112 | 115).  None of these was measured with a k beyond the list.
   if (vecs <= 512) return BLR_SAMPLE(128, true);
   if (p.chunks * 512ll <= kStaged) return BLR_SAMPLE(512, true);
   return rows <= sm_count() ? BLR_SAMPLE(1024, false) : BLR_SAMPLE(512, false);
