@@ -470,7 +470,7 @@ int blr_attention_paged(const void* q, int64_t ldq, const blr_paged_cache* cache
  * ones by rising id, are kept: the first top_k (<= 0: all); of those the fewest first ones whose weights reach top_p times their sum (>= 1: all, <= 0: the first); of those the ones with
  * w >= min(min_p, 1).  ids[r] is the least kept id for which the weights of the kept ids up to it exceed uniform[r] times the sum of all kept; logprob[r] = log(its weight / that
  * sum).  Weights and sums in 64 bits, weights to 2^-50 of themselves and 2^-52 for each unit of
- * (M - x) / T.  uniform >= 1: the last kept id, < 0: as 0.  A row with a NaN (logit or setting), of -inf alone, or with a negative temperature has id -1
+ * (M - x) / T; below e^-700 they count as 0.  uniform >= 1: the last kept id, < 0: as 0.  A row with a NaN (logit or setting), of -inf alone, or with a negative temperature has id -1
  * and NaN; logits of -inf are never chosen, +inf ones share the row.  Settings: one for each row (device pointers, fp32, top_k int64), or, where the pointer is NULL, the number
  * behind it for all.  A row is at most 4 MB (BLR_ERR_UNSUPPORTED above).  No reference counterpart. */
 typedef struct blr_sampling {
